@@ -7,11 +7,23 @@ hand-written HIP kernels behind the C ABI of ``include/harp_ring_attn.h``
 rotary embedding, runs on the GPU too (``include/harp_qk_norm_rope.h``,
 ``kernels/libharp_async_op.so``, namespace ``async_op``), and
 :class:`RingZAttention` wires projections, QK norm, RoPE, ring attention and
-the output projection as the model's attention block does.  Build with
-``python -m harp_amd.build``.
+the output projection as the model's attention block does.  Around it
+(``include/harp_block_ops.h``, ``kernels/libharp_block_ops.so``):
+:func:`add_rms_norm`, the residual addition with its RMSNorm, and the Linear
+layers in 8-bit integers for forward-only use (:class:`Int8Linear`,
+:func:`quantize_attention`).  Build with ``python -m harp_amd.build``.
 """
 
-from ._lib import ABI_LIB, ASYNC_OPS_LIB, OPS_LIB, load_abi, load_async_ops, load_ops  # noqa: F401
+from ._lib import (  # noqa: F401
+    ABI_LIB,
+    ASYNC_OPS_LIB,
+    BLOCK_OPS_LIB,
+    OPS_LIB,
+    load_abi,
+    load_async_ops,
+    load_block_ops,
+    load_ops,
+)
 from .ops import (  # noqa: F401
     RingAttention,
     abi_backward,
@@ -23,6 +35,8 @@ from .ops import (  # noqa: F401
     ring_attention,
 )
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn  # noqa: F401
+from .residual_norm import AddRMSNormFn, add_rms_norm, add_rms_norm_int8  # noqa: F401
+from .int8 import Int8Linear, Int8Rows, int8_linear, quantize_attention, quantize_int8  # noqa: F401
 from .attention import RingZAttention, project_qkv  # noqa: F401
 from .wait_engine import CommWork, WaitEngine  # noqa: F401
 from .gemm import xhblas_gemm  # noqa: F401

@@ -21,6 +21,7 @@ KERNELS = ROOT / "kernels"
 ABI_LIB = KERNELS / "libharp_ra.so"
 OPS_LIB = KERNELS / "libring_attention_ops.so"
 ASYNC_OPS_LIB = KERNELS / "libharp_async_op.so"
+BLOCK_OPS_LIB = KERNELS / "libharp_block_ops.so"
 
 HARP_RA_OK = 0
 HARP_RA_EINVAL = 1
@@ -36,6 +37,7 @@ _lock = threading.Lock()
 _abi: ctypes.CDLL | None = None
 _ops_loaded = False
 _async_ops_loaded = False
+_block_ops_loaded = False
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -119,6 +121,41 @@ QK_PROTOTYPES = {
 }
 
 
+HARP_BLK_OK = 0
+HARP_BLK_F32 = 0
+HARP_BLK_BF16 = 1
+
+
+class BlkQkvOut(ctypes.Structure):
+    """harp_blk_qkv_out_t of include/harp_block_ops.h (one projection of harp_blk_qkv_int8)."""
+
+    _fields_ = [
+        ("weight", _p),
+        ("ld_weight", _i64),
+        ("weight_scales", _p),
+        ("y", _p),
+        ("ld_y", _i64),
+        ("norm_weight", _p),
+        ("norm_weight_dtype", _i),
+        ("eps", _f),
+    ]
+
+
+# (restype, argtypes) of every symbol include/harp_block_ops.h declares
+BLK_PROTOTYPES = {
+    "harp_blk_add_rms_norm_forward": (_i, [_p, _i64, _i, _p, _i64, _i, _p, _i, _f, _p, _i64, _p, _i64, _p, _i, _i, _p]),
+    "harp_blk_add_rms_norm_backward": (_i, [_p, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i, _p, _p, _i64, _p, _i64,
+                                            _p, _i, _i, _i, _p, _sz, _p]),
+    "harp_blk_backward_workspace_bytes": (_sz, [_i, _i]),
+    "harp_blk_add_rms_norm_int8": (_i, [_p, _i64, _i, _p, _i64, _i, _p, _i, _f, _p, _i64, _p, _i64, _p, _i, _i, _p]),
+    "harp_blk_quantize_int8": (_i, [_p, _i64, _i, _p, _i64, _p, _i, _i, _p]),
+    "harp_blk_dequantize_int8": (_i, [_p, _i64, _p, _p, _i64, _i, _i, _i, _p]),
+    "harp_blk_linear_int8": (_i, [_p, _i64, _p, _p, _i64, _p, _p, _i, _p, _i64, _i, _i, _i, _i, _p]),
+    "harp_blk_qkv_int8": (_i, [_p, _i64, _p, _i, _i, _i, _i, _p, _i64, _i64, ctypes.POINTER(BlkQkvOut), _i, _p]),
+    "harp_blk_last_error": (ctypes.c_char_p, []),
+}
+
+
 def _missing(path: Path) -> RuntimeError:
     return RuntimeError(
         f"{path} is not built; run `python -m harp_amd.build` (or __graft_entry__.build()). "
@@ -134,7 +171,7 @@ def load_abi() -> ctypes.CDLL:
             if not ABI_LIB.exists():
                 raise _missing(ABI_LIB)
             lib = ctypes.CDLL(str(ABI_LIB))
-            for name, (res, args) in {**ABI_PROTOTYPES, **QK_PROTOTYPES}.items():
+            for name, (res, args) in {**ABI_PROTOTYPES, **QK_PROTOTYPES, **BLK_PROTOTYPES}.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args
@@ -164,6 +201,18 @@ def load_async_ops() -> None:
             raise _missing(ASYNC_OPS_LIB)
         torch.ops.load_library(str(ASYNC_OPS_LIB))
         _async_ops_loaded = True
+
+
+def load_block_ops() -> None:
+    """Register torch.ops.harp_block (residual RMSNorm, 8-bit rows) from kernels/libharp_block_ops.so."""
+    global _block_ops_loaded
+    with _lock:
+        if _block_ops_loaded:
+            return
+        if not BLOCK_OPS_LIB.exists():
+            raise _missing(BLOCK_OPS_LIB)
+        torch.ops.load_library(str(BLOCK_OPS_LIB))
+        _block_ops_loaded = True
 
 
 def qk_check(rc: int, what: str) -> None:

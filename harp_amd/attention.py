@@ -17,17 +17,23 @@ runs, for ``hidden_states`` [B, S, dim]:
    this GPU), then ``transpose(1, 2).flatten(2, 3)`` and ``to_out``
    (attn.py:99-103).
 
+A module whose projections are :class:`harp_amd.Int8Linear`
+(:func:`harp_amd.quantize_attention`) runs them in 8-bit integers, forward
+only; ``hidden_states`` may then be 8-bit rows (:class:`harp_amd.Int8Rows`),
+as :func:`harp_amd.add_rms_norm_int8` writes them.
+
 ``attn_mask`` is accepted and ignored, as in the reference (attn.py:91-97).
 :func:`project_qkv` is steps 1-2 on their own (the producer of q, k, v).
 """
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch import nn
 
+from .int8 import Int8Rows, fused_int8_supported, is_int8, project_qkv_int8, quantize_int8
 from .ops import RingAttention
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn
 from .qkv import ProjectQKVFn, fused_supported, qkv_project
@@ -47,14 +53,23 @@ def _norm_rope(x: torch.Tensor, norm: Optional[nn.Module], freqs_cis: Optional[t
     return x
 
 
-def project_qkv(attn: nn.Module, hidden_states: torch.Tensor, freqs_cis: Optional[torch.Tensor],
+def project_qkv(attn: nn.Module, hidden_states: Union[torch.Tensor, Int8Rows], freqs_cis: Optional[torch.Tensor],
                 fused: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """q, k, v as token-major [B, H, S, D] views: projections, then QK RMSNorm
     and RoPE (attn.py:69-89).  With ``fused`` (default) and a module and input
     the fused kernel takes (:func:`harp_amd.qkv.fused_supported`: head dim
     128, no bias), all of it is one launch (:class:`ProjectQKVFn`); otherwise
-    three library GEMMs and the separate norm + RoPE kernels."""
-    if fused and fused_supported(attn, hidden_states, freqs_cis):
+    three library GEMMs and the separate norm + RoPE kernels.  With 8-bit
+    projections the one launch is :func:`harp_amd.int8.project_qkv_int8` where
+    it applies, else three 8-bit products and the separate kernels."""
+    if is_int8(attn):
+        if not isinstance(hidden_states, Int8Rows):
+            hidden_states = quantize_int8(hidden_states)  # once for all three
+        if fused and fused_int8_supported(attn, freqs_cis):
+            return project_qkv_int8(attn, hidden_states, freqs_cis)
+    elif isinstance(hidden_states, Int8Rows):
+        raise ValueError("8-bit hidden states need 8-bit projections (harp_amd.quantize_attention)")
+    elif fused and fused_supported(attn, hidden_states, freqs_cis):
         nq, nk = getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)
         args = (hidden_states, attn.to_q.weight, attn.to_k.weight, attn.to_v.weight,
                 None if nq is None else nq.weight, None if nk is None else nk.weight, freqs_cis,
@@ -89,11 +104,12 @@ class RingZAttention(nn.Module):
         self.attn = pretrained_attn
         self.sp_size = sp_size
 
-    def forward(self, hidden_states: torch.Tensor, RoPE_embeds: Optional[torch.Tensor],
+    def forward(self, hidden_states: Union[torch.Tensor, Int8Rows], RoPE_embeds: Optional[torch.Tensor],
                 attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         attn = self.attn
-        if hidden_states.size(1) % self.sp_size:
-            raise ValueError(f"sequence length {hidden_states.size(1)} is not a multiple of sp_size {self.sp_size}")
+        tokens = (hidden_states.values if isinstance(hidden_states, Int8Rows) else hidden_states).size(1)
+        if tokens % self.sp_size:
+            raise ValueError(f"sequence length {tokens} is not a multiple of sp_size {self.sp_size}")
         query, key, value = project_qkv(attn, hidden_states, RoPE_embeds)
         out = RingAttention.apply(query, key, value, self.sp_size).transpose(1, 2).flatten(2, 3)
         out = attn.to_out[0](out)

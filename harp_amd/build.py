@@ -3,8 +3,8 @@
 Outputs (all under ``kernels/`` at the repository root, next to each other
 so the operator libraries find the C-ABI library through ``$ORIGIN``):
 
-* ``libharp_ra.so``              HIP kernels + the C ABIs of include/harp_ring_attn.h
-                                 and include/harp_qk_norm_rope.h
+* ``libharp_ra.so``              HIP kernels + the C ABIs of include/harp_ring_attn.h,
+                                 include/harp_qk_norm_rope.h and include/harp_block_ops.h
                                  (hipcc, --offload-arch=gfx950).
 * ``libring_attention_ops.so``   the PyTorch operator library (namespace
                                  ``ring_attention_ops``), the drop-in for the
@@ -13,6 +13,9 @@ so the operator libraries find the C-ABI library through ``$ORIGIN``):
 * ``libharp_async_op.so``        the PyTorch operator library for the QK RMSNorm
                                  and RoPE operators (namespace ``async_op``,
                                  async_rt/csrc/async_op_api.cc:54-57), on the GPU.
+* ``libharp_block_ops.so``       the PyTorch operator library for the residual
+                                 RMSNorm, 8-bit rows and their products
+                                 (namespace ``harp_block``).
 
 Run ``python -m harp_amd.build`` (or ``__graft_entry__.build()``).
 """
@@ -22,6 +25,8 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -31,13 +36,16 @@ OUT = ROOT / "kernels"
 ABI_LIB = OUT / "libharp_ra.so"
 OPS_LIB = OUT / "libring_attention_ops.so"
 ASYNC_OPS_LIB = OUT / "libharp_async_op.so"
+BLOCK_OPS_LIB = OUT / "libharp_block_ops.so"
 
-HIP_SOURCES = ["ra_kernels.hip", "fwd_asm.hip", "dq_asm.hip", "dkdv_asm.hip", "ra_abi.hip", "qk_kernels.hip", "qk_abi.hip", "proj_kernels.hip"]
-HIP_HEADERS = ["ra_common.h", "ra_kernels.h", "qk_kernels.h", "proj_kernels.h", "fwd_asm.inc", "fwd_asm_gen.py",
+HIP_SOURCES = ["ra_kernels.hip", "fwd_asm.hip", "dq_asm.hip", "dkdv_asm.hip", "ra_abi.hip", "qk_kernels.hip", "qk_abi.hip", "proj_kernels.hip",
+               "norm_kernels.hip", "prod8_kernels.hip", "blk_abi.hip"]
+HIP_HEADERS = ["ra_common.h", "ra_kernels.h", "qk_kernels.h", "proj_kernels.h", "blk_kernels.h", "fwd_asm.inc", "fwd_asm_gen.py",
                "dq_asm.inc", "dq_asm_gen.py", "dkdv_asm.inc",
                "dkdv_asm_gen.py", "asm_sched.py"]
 OPS_SOURCE = "torch_ring_attention_ops.cpp"
 ASYNC_OPS_SOURCE = "torch_async_op.cpp"
+BLOCK_OPS_SOURCE = "torch_block_ops.cpp"
 
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 OFFLOAD_ARCH = "gfx950"
@@ -87,10 +95,15 @@ def build_abi(verbose: bool = False) -> Path:
     generate_asm(verbose)
     OUT.mkdir(parents=True, exist_ok=True)
     tmp = ABI_LIB.with_suffix(".so.tmp")
-    cmd = [str(ROCM / "bin" / "hipcc"), *HIPCC_FLAGS, f"-I{INCLUDE}"]
-    cmd += [str(CSRC / s) for s in HIP_SOURCES]
-    cmd += ["-o", str(tmp)]
-    _run(cmd, verbose)
+    hipcc = [str(ROCM / "bin" / "hipcc"), *HIPCC_FLAGS]
+    with tempfile.TemporaryDirectory() as d:
+        objects = [os.path.join(d, f"{Path(src).stem}.o") for src in HIP_SOURCES]
+        with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+            jobs = [pool.submit(_run, [*hipcc, f"-I{INCLUDE}", "-c", str(CSRC / src), "-o", obj], verbose)
+                    for src, obj in zip(HIP_SOURCES, objects)]
+            for job in jobs:
+                job.result()
+        _run([*hipcc, *objects, "-o", str(tmp)], verbose)
     os.replace(tmp, ABI_LIB)
     return ABI_LIB
 
@@ -140,21 +153,27 @@ def build_async_ops(verbose: bool = False) -> Path:
     return build_ops(verbose, ASYNC_OPS_SOURCE, ASYNC_OPS_LIB, "harp_async_op")
 
 
+def build_block_ops(verbose: bool = False) -> Path:
+    """kernels/libharp_block_ops.so: the harp_block operators (residual RMSNorm, 8-bit rows and products)."""
+    return build_ops(verbose, BLOCK_OPS_SOURCE, BLOCK_OPS_LIB, "harp_block_ops")
+
+
 def build(verbose: bool = False) -> None:
     """Compile every library unconditionally (the build check)."""
     build_abi(verbose)
     build_ops(verbose)
     build_async_ops(verbose)
+    build_block_ops(verbose)
 
 
 def sources_newer_than_libs() -> bool:
     """True when a source file is newer than a built library (or one is missing)."""
-    libs = [ABI_LIB, OPS_LIB, ASYNC_OPS_LIB]
+    libs = [ABI_LIB, OPS_LIB, ASYNC_OPS_LIB, BLOCK_OPS_LIB]
     if not all(p.exists() for p in libs):
         return True
     newest_lib = min(p.stat().st_mtime for p in libs)
-    srcs = [CSRC / s for s in HIP_SOURCES + HIP_HEADERS + [OPS_SOURCE, ASYNC_OPS_SOURCE]]
-    srcs += [INCLUDE / "harp_ring_attn.h", INCLUDE / "harp_qk_norm_rope.h"]
+    srcs = [CSRC / s for s in HIP_SOURCES + HIP_HEADERS + [OPS_SOURCE, ASYNC_OPS_SOURCE, BLOCK_OPS_SOURCE]]
+    srcs += [INCLUDE / h for h in ("harp_ring_attn.h", "harp_qk_norm_rope.h", "harp_block_ops.h")]
     return any(s.stat().st_mtime > newest_lib for s in srcs)
 
 

@@ -1,0 +1,587 @@
+// gfx950 kernels of the residual addition with its RMSNorm, forward and
+// backward, and of 8-bit rows (quantise, norm + quantise, dequantise).
+//
+//   h = x + r                          (rounded once, to r's type)
+//   rho = 1 / sqrt(mean(h^2) + eps),   y = h * rho * w
+//   g = dy * w,  c = mean(g * h * rho)
+//   d = rho * (g - h * rho * c) + dh,  dx = d, dr = d,  dw = sum_rows dy * h * rho
+//   8-bit rows: a = max |v|, s = a / 127, q = v * 127 / a to nearest (ties to even)
+//
+// All arithmetic and sums are fp32 over the stored inputs; every output is
+// rounded once, to nearest.  y of the 8-bit rows is never rounded to bf16:
+// with v = h * w the common factor rho cancels from q = 127 v / max |v|, and
+// only the scale, rho * max |v| / 127, holds it, so the row's two reductions
+// (sum of squares, maximum) need one exchange.
+//
+// The kernels are bound by memory: each row is read once into registers (8
+// values per thread and vector) and finished there.  Rows need no alignment
+// beyond their element's: a 16-byte global access at any address is one
+// instruction on gfx950, and the vector at a row's end is taken apart.
+#include "blk_kernels.h"
+#include "ra_common.h"
+
+namespace harp_blk {
+
+using harp_ra::bf16;
+
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef u32x4 u32x4u __attribute__((aligned(2)));
+
+constexpr int kVec = 8;  // values per vector
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<kBf16> {
+  typedef uint16_t type;
+};
+template <>
+struct Elem<kF32> {
+  typedef float type;
+};
+template <>
+struct Elem<kNone> {
+  typedef float type;
+};
+
+__device__ __forceinline__ float from_bits(uint32_t b) { return __uint_as_float(b); }
+__device__ __forceinline__ uint16_t bf16_rne(float f) { return __builtin_bit_cast(uint16_t, (bf16)f); }
+
+// n (1 .. 8) values at p; the rest are zero
+template <int DT>
+__device__ __forceinline__ f32x8 load8(const typename Elem<DT>::type* p, int n) {
+  f32x8 v;
+  if (n == kVec) {
+    if constexpr (DT == kBf16) {
+      const u32x4 u = *(const u32x4u*)p;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = from_bits(u[i] << 16);
+        v[2 * i + 1] = from_bits(u[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const harp_ra::f32x4 u = *(const harp_ra::f32x4u*)(p + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * i + e] = u[e];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      v[e] = 0.f;
+      if (e < n) {
+        if constexpr (DT == kBf16)
+          v[e] = from_bits((uint32_t)p[e] << 16);
+        else
+          v[e] = p[e];
+      }
+    }
+  }
+  return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void store8(typename Elem<DT>::type* p, const f32x8& v, int n) {
+  if constexpr (DT == kBf16) {
+    uint16_t h[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) h[e] = bf16_rne(v[e]);
+    if (n == kVec) {
+      u32x4 u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = (uint32_t)h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+      *(u32x4u*)p = u;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (e < n) p[e] = h[e];
+    }
+  } else {
+    if (n == kVec) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        harp_ra::f32x4 u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = v[4 * i + e];
+        *(harp_ra::f32x4u*)(p + 4 * i) = u;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e)
+        if (e < n) p[e] = v[e];
+    }
+  }
+}
+
+// weight vector: a run-time type (its branch is the same in every thread)
+__device__ __forceinline__ f32x8 load_w(const void* w, int dtype, int c, int n) {
+  if (!w) {
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = 1.f;
+    return v;
+  }
+  return dtype == kF32 ? load8<kF32>((const float*)w + c, n) : load8<kBf16>((const uint16_t*)w + c, n);
+}
+
+// x + r as it is kept: in r's type
+template <int RD>
+__device__ __forceinline__ float round_to(float v) {
+  if constexpr (RD == kBf16) return (float)(bf16)v;
+  return v;
+}
+
+// Sum, and maximum of unsigned words, over the TPR threads of a row; every
+// thread gets the results.  Rows of one wave exchange within it; a row of
+// several waves goes through LDS (one row per block then).
+template <int TPR, bool SUM, bool MAX>
+__device__ __forceinline__ void row_reduce(float& s, uint32_t& m, float* lds_s, uint32_t* lds_m) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    if (SUM) s += __shfl_xor(s, d);
+    if (MAX) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+  }
+  if constexpr (TPR > 64) {
+    constexpr int kW = TPR / 64;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+      if (SUM) lds_s[wave] = s;
+      if (MAX) lds_m[wave] = m;
+    }
+    __syncthreads();
+    if (SUM) {
+      s = 0.f;
+#pragma unroll
+      for (int i = 0; i < kW; ++i) s += lds_s[i];
+    }
+    if (MAX) {
+      m = 0;
+#pragma unroll
+      for (int i = 0; i < kW; ++i) m = max(m, lds_m[i]);
+    }
+  }
+}
+
+// The scale of a row and what turns its values into steps.  The maximum comes
+// as the bits of |v|, which order as the values do with infinity and NaN on
+// top: a row that holds one has the scale NaN (and steps of zero), so that
+// whatever reads it is NaN too.  A row of zeros has scale and steps zero.
+// Maxima below 2^-100 are raised by 2^100 first, or 127 / a would overflow.
+struct Steps {
+  float pre, a, inv, scale;
+};
+__device__ __forceinline__ Steps row_steps(uint32_t max_bits, float factor) {
+  Steps t;
+  const float a = from_bits(max_bits);
+  t.pre = a < 0x1p-100f ? 0x1p100f : 1.f;
+  t.a = a * t.pre;
+  t.inv = __fdiv_rn(127.f, t.a);
+  t.scale = __fdiv_rn(a * factor, 127.f);
+  if (max_bits == 0) t.inv = t.scale = 0.f;
+  if (max_bits >= 0x7f800000u) {
+    t.inv = 0.f;
+    t.scale = __uint_as_float(0x7fc00000u);
+  }
+  return t;
+}
+
+// v * 127 / a to the nearest integer, ties to even, of one vector, packed.
+// v * inv is off by a few 2^-24 of its size, so only values that close to a
+// border between two steps can round to the wrong one: where a vector has
+// one, 127 v - q a is formed exactly and decides.
+__device__ __forceinline__ uint2 pack_steps(const f32x8& v, const Steps& t) {
+  f32x8 q;
+  float far = 0.f;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    const float f = v[e] * t.pre * t.inv;
+    q[e] = __builtin_rintf(f);
+    far = __builtin_fmaxf(far, __builtin_fabsf(f - q[e]));
+  }
+  if (__builtin_expect(far > 0.4999f, 0)) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      const float p = q[e] * t.a, err = __builtin_fmaf(q[e], t.a, -p);
+      const float d2 = 2.f * (__builtin_fmaf(127.f, v[e] * t.pre, -p) - err), ad = __builtin_fabsf(d2);
+      const bool odd = ((int)q[e] & 1) != 0;
+      if (ad > t.a || (ad == t.a && odd)) q[e] += __builtin_copysignf(1.f, d2);
+    }
+  }
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) w[e >> 2] |= ((uint32_t)(int)q[e] & 0xffu) << (8 * (e & 3));
+  return make_uint2(w[0], w[1]);
+}
+
+}  // namespace
+
+enum { kModeNorm = 0, kModeNorm8 = 1, kModeQuant = 2 };
+
+// TPR threads per row, NV vectors of 8 per thread; blocks of max(TPR, 256)
+// threads hold 256 / TPR rows, or one.
+template <int MODE, int XD, int RD, int TPR, int NV>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams p) {
+  constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
+  typedef typename Elem<XD>::type TX;
+  typedef typename Elem<RD>::type TR;
+  __shared__ float lds_s[16];
+  __shared__ uint32_t lds_m[16];
+  const int64_t row = (int64_t)blockIdx.x * kRows + (kRows > 1 ? threadIdx.x / TPR : 0);
+  if (row >= p.rows) return;  // whole waves: rows of several waves are alone in their block
+  const int t = threadIdx.x % TPR;
+  const TX* x = (const TX*)p.x + row * p.ldx;
+  const TR* r = (const TR*)p.res + row * p.ldr;
+
+  f32x8 v[NV];
+  float ss = 0.f;
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
+    if (n > 0) {
+      v[i] = load8<XD>(x + c, n);
+      if constexpr (RD != kNone) {
+        const f32x8 a = load8<RD>(r + c, n);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[i][e] = round_to<RD>(v[i][e] + a[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) v[i][e] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
+    if constexpr (RD != kNone)
+      if (p.h && n > 0) store8<RD>((TR*)p.h + row * p.ldh + c, v[i], n);
+    if constexpr (MODE != kModeQuant)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) ss = __builtin_fmaf(v[i][e], v[i][e], ss);
+    if constexpr (MODE == kModeNorm8)
+      if (n > 0) {
+        const f32x8 w = load_w(p.w, p.w_dtype, c, n);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[i][e] *= w[e];
+      }
+    if constexpr (MODE != kModeNorm)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) mx = max(mx, __float_as_uint(v[i][e]) & 0x7fffffffu);
+  }
+  row_reduce<TPR, MODE != kModeQuant, MODE != kModeNorm>(ss, mx, lds_s, lds_m);
+  float rho = 1.f;
+  if constexpr (MODE != kModeQuant) {
+    rho = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)p.cols) + p.eps));
+    if (p.rstd && t == 0) p.rstd[row] = rho;
+  }
+  if constexpr (MODE == kModeNorm) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
+      if (n > 0) {
+        const f32x8 w = load_w(p.w, p.w_dtype, c, n);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[i][e] = v[i][e] * rho * w[e];
+        store8<XD>((TX*)p.y + row * p.ldy + c, v[i], n);
+      }
+    }
+  } else {
+    const Steps st = row_steps(mx, rho);
+    const bool bad = mx >= 0x7f800000u;
+    if (t == 0) p.scale[row] = st.scale;
+    int8_t* q = p.q + row * p.ldq;
+    const int end = (p.cols + 15) & ~15;  // the last 16 bytes whole, zeros behind the row's values
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * kVec;
+      if (c < end) *(uint2*)(q + c) = bad ? make_uint2(0, 0) : pack_steps(v[i], st);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward.  A block of GROUPS groups of TPR threads walks its share of the
+// rows, one row per group at a time, and keeps the weight gradient's sums of
+// its columns in registers; the groups' sums are added in LDS at the end and
+// written as one partial row, so the order of every sum is fixed by the
+// launch alone.  KEEP: dy and h stay in registers between the row's two
+// passes; the longest rows have no room and read them again (out of L2).
+template <int XD, int HD, int TPR, int NV, int GROUPS, bool KEEP>
+__global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) {
+  typedef typename Elem<XD>::type TX;
+  typedef typename Elem<HD>::type TH;
+  constexpr int kW = TPR / 64;
+  __shared__ float lds_s[2][GROUPS][kW > 0 ? kW : 1];
+  const int grp = threadIdx.x / TPR;
+  int t = threadIdx.x % TPR;
+  f32x8 gw[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) gw[i][e] = 0.f;
+  const int64_t step = (int64_t)gridDim.x * GROUPS;
+  const int64_t n_iter = (p.rows + step - 1) / step;
+  for (int64_t it = 0; it < n_iter; ++it) {  // the same count in every group: the barrier below is in step
+    const int64_t row = it * step + (int64_t)blockIdx.x * GROUPS + grp;
+    const bool live = row < p.rows;
+    // (opaque, or every vector's bounds tests would be kept in SGPRs over the loop: 34 spilled)
+    asm volatile("" : "+v"(t));
+    constexpr int kKeep = KEEP ? NV : 1;
+    f32x8 gs[kKeep], hs[kKeep];
+    float c1 = 0.f;
+    const float rho = live ? p.rstd[row] : 0.f;
+    auto load = [&](int i, f32x8& g, f32x8& h) {
+      const int c = (i * TPR + t) * kVec, n = live ? min(kVec, p.cols - c) : 0;
+      if (n > 0) {
+        g = load8<XD>((const TX*)p.dy + row * p.ldy + c, n);
+        h = load8<HD>((const TH*)p.h + row * p.ldh + c, n);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) g[e] = h[e] = 0.f;
+      }
+    };
+    // g: dy -> dy w, h -> h rho
+    auto scale = [&](int i, f32x8& g, f32x8& h, bool sums) {
+      const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
+      if (n > 0) {
+        const f32x8 w = load_w(p.w, p.w_dtype, c, n);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          h[e] *= rho;
+          if (sums) gw[i][e] = __builtin_fmaf(g[e], h[e], gw[i][e]);
+          g[e] *= w[e];
+          if (sums) c1 = __builtin_fmaf(g[e], h[e], c1);
+        }
+      }
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load(i, gs[i], hs[i]);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) scale(i, gs[i], hs[i], true);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        load(i, gs[0], hs[0]);
+        scale(i, gs[0], hs[0], true);
+      }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) c1 += __shfl_xor(c1, d);
+    if constexpr (TPR > 64) {
+      // two buffers in turn: the next row's writes meet no reader of this one
+      float* s = lds_s[it & 1][grp];
+      if ((t & 63) == 0) s[t >> 6] = c1;
+      __syncthreads();
+      c1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < kW; ++i) c1 += s[i];
+    }
+    c1 = __fdiv_rn(c1, (float)p.cols);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * kVec, n = live ? min(kVec, p.cols - c) : 0;
+      f32x8 &g = gs[KEEP ? i : 0], &h = hs[KEEP ? i : 0];
+      if constexpr (!KEEP) {
+        load(i, g, h);
+        scale(i, g, h, false);
+      }
+      if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) g[e] = rho * __builtin_fmaf(-h[e], c1, g[e]);
+        if (p.dh) {
+          const f32x8 a = load8<HD>((const TH*)p.dh + row * p.lddh + c, n);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) g[e] += a[e];
+        }
+        store8<XD>((TX*)p.dx + row * p.lddx + c, g, n);
+        if (p.dres) store8<HD>((TH*)p.dres + row * p.lddr + c, g, n);
+      }
+    }
+  }
+  if (!p.wpart) return;
+  // the groups' sums, in group order, one vector column at a time
+  if constexpr (GROUPS > 1) {
+    __shared__ float part[GROUPS][TPR * kVec];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) part[grp][e * TPR + t] = gw[i][e];
+      __syncthreads();
+      if (grp == 0) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+#pragma unroll
+          for (int k = 1; k < GROUPS; ++k) gw[i][e] += part[k][e * TPR + t];
+      }
+    }
+    if (grp != 0) return;
+  }
+  float* out = p.wpart + (int64_t)blockIdx.x * p.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
+    if (n > 0) store8<kF32>(out + c, gw[i], n);
+  }
+}
+
+// grad_weight[c] = sum over the blocks' partial rows, in a fixed order: 32
+// columns per block, 8 row groups, then the groups in order.
+constexpr int kWgCols = 32, kWgGroups = 8;
+__global__ __launch_bounds__(kWgCols* kWgGroups) void wgrad_kernel(const float* part, int blocks, int cols, void* gw,
+                                                                   int gw_f32) {
+  __shared__ float sums[kWgGroups][kWgCols];
+  const int j = threadIdx.x % kWgCols, g = threadIdx.x / kWgCols;
+  const int c = blockIdx.x * kWgCols + j;
+  float s = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int b = g; b < blocks; b += kWgGroups) s += part[(int64_t)b * cols + c];
+  }
+  sums[g][j] = s;
+  __syncthreads();
+  if (g == 0 && c < cols) {
+#pragma unroll
+    for (int k = 1; k < kWgGroups; ++k) s += sums[k][j];
+    if (gw_f32)
+      ((float*)gw)[c] = s;
+    else
+      ((uint16_t*)gw)[c] = bf16_rne(s);
+  }
+}
+
+// out = q * scale, 16 values per thread
+template <int OD>
+__global__ __launch_bounds__(256) void dequant_kernel(const int8_t* q, int64_t ldq, const float* scale,
+                                                      typename Elem<OD>::type* out, int64_t ldo, int rows, int cols) {
+  const int per_row = (cols + 15) / 16;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / per_row;
+  if (row >= rows) return;
+  const int c = (int)(id - row * per_row) * 16;
+  const u32x4 u = *(const u32x4*)(q + row * ldq + c);
+  const float s = scale[row];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int n = min(kVec, cols - c - half * kVec);
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e)
+      v[e] = (float)((int)(u[half * 2 + (e >> 2)] << (24 - 8 * (e & 3))) >> 24) * s;
+    if (n > 0) store8<OD>(out + row * ldo + c + half * kVec, v, n);
+  }
+}
+
+// ---------------------------------------------------------------------------
+namespace {
+
+template <int MODE, int XD, int RD>
+hipError_t launch_fwd_t(const NormParams& p, hipStream_t stream) {
+  const int vecs = (p.cols + kVec - 1) / kVec;
+#define HARP_NORM_LAUNCH(TPR, NV)                                                                                  \
+  {                                                                                                                \
+    constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;                                                               \
+    hipLaunchKernelGGL((norm_kernel<MODE, XD, RD, TPR, NV>), dim3((unsigned)((p.rows + kRows - 1) / kRows)),       \
+                       dim3(TPR > 256 ? TPR : 256), 0, stream, p);                                                 \
+    return hipGetLastError();                                                                                      \
+  }
+  if (vecs <= 64) HARP_NORM_LAUNCH(64, 1)
+  if (vecs <= 128) HARP_NORM_LAUNCH(64, 2)
+  if (vecs <= 256) HARP_NORM_LAUNCH(256, 1)
+  if (vecs <= 512) HARP_NORM_LAUNCH(256, 2)
+  if (vecs <= 1024) HARP_NORM_LAUNCH(256, 4)
+  if (vecs <= 2048) HARP_NORM_LAUNCH(512, 4)
+  HARP_NORM_LAUNCH(512, 8)
+#undef HARP_NORM_LAUNCH
+}
+
+template <int MODE>
+hipError_t launch_fwd(const NormParams& p, hipStream_t stream) {
+  if (MODE == kModeQuant || !p.res) {
+    if (p.x_dtype == kBf16) return launch_fwd_t<MODE, kBf16, kNone>(p, stream);
+    return launch_fwd_t<MODE, kF32, kNone>(p, stream);
+  }
+  if constexpr (MODE != kModeQuant) {
+    if (p.x_dtype == kBf16)
+      return p.r_dtype == kBf16 ? launch_fwd_t<MODE, kBf16, kBf16>(p, stream)
+                                : launch_fwd_t<MODE, kBf16, kF32>(p, stream);
+    return p.r_dtype == kBf16 ? launch_fwd_t<MODE, kF32, kBf16>(p, stream)
+                              : launch_fwd_t<MODE, kF32, kF32>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+// threads per row and groups of the backward block, by the row's vectors
+struct BwdShape {
+  int groups;
+};
+BwdShape bwd_shape(int cols) {
+  const int vecs = (cols + kVec - 1) / kVec;
+  if (vecs <= 128) return {8};
+  if (vecs <= 1024) return {2};
+  return {1};
+}
+
+template <int XD, int HD>
+hipError_t launch_bwd_t(const NormBwdParams& p, hipStream_t stream) {
+  const int vecs = (p.cols + kVec - 1) / kVec;
+  const unsigned blocks = (unsigned)bwd_blocks(p.rows, p.cols);
+#define HARP_NORM_BWD(TPR, NV, GROUPS)                                                                               \
+  {                                                                                                                  \
+    hipLaunchKernelGGL((norm_bwd_kernel<XD, HD, TPR, NV, GROUPS, (NV * TPR <= 2048)>), dim3(blocks),                 \
+                       dim3(TPR * GROUPS), 0, stream, p);                                                            \
+    return hipGetLastError();                                                                                        \
+  }
+  if (vecs <= 64) HARP_NORM_BWD(64, 1, 8)
+  if (vecs <= 128) HARP_NORM_BWD(64, 2, 8)
+  if (vecs <= 256) HARP_NORM_BWD(256, 1, 2)
+  if (vecs <= 512) HARP_NORM_BWD(256, 2, 2)
+  if (vecs <= 1024) HARP_NORM_BWD(256, 4, 2)
+  if (vecs <= 2048) HARP_NORM_BWD(512, 4, 1)
+  HARP_NORM_BWD(1024, 4, 1)
+#undef HARP_NORM_BWD
+}
+
+}  // namespace
+
+int bwd_blocks(int rows, int cols) {
+  const int g = bwd_shape(cols).groups;
+  const int64_t need = ((int64_t)rows + g - 1) / g;
+  return (int)(need < 512 ? need : 512);
+}
+
+hipError_t launch_norm(const NormParams& p, hipStream_t stream) { return launch_fwd<kModeNorm>(p, stream); }
+hipError_t launch_norm_rows8(const NormParams& p, hipStream_t stream) { return launch_fwd<kModeNorm8>(p, stream); }
+hipError_t launch_quantize(const NormParams& p, hipStream_t stream) { return launch_fwd<kModeQuant>(p, stream); }
+
+hipError_t launch_norm_backward(const NormBwdParams& p, hipStream_t stream) {
+  if (p.x_dtype == kBf16)
+    return p.h_dtype == kBf16 ? launch_bwd_t<kBf16, kBf16>(p, stream) : launch_bwd_t<kBf16, kF32>(p, stream);
+  return p.h_dtype == kBf16 ? launch_bwd_t<kF32, kBf16>(p, stream) : launch_bwd_t<kF32, kF32>(p, stream);
+}
+
+hipError_t launch_wgrad(const float* wpart, int blocks, int cols, void* gw, int gw_f32, hipStream_t stream) {
+  hipLaunchKernelGGL(wgrad_kernel, dim3((unsigned)((cols + kWgCols - 1) / kWgCols)), dim3(kWgCols * kWgGroups), 0,
+                     stream, wpart, blocks, cols, gw, gw_f32);
+  return hipGetLastError();
+}
+
+hipError_t launch_dequantize(const int8_t* q, int64_t ldq, const float* scale, void* out, int64_t ldo, int o_dtype,
+                             int rows, int cols, hipStream_t stream) {
+  const int64_t threads = (int64_t)rows * ((cols + 15) / 16);
+  const dim3 grid((unsigned)((threads + 255) / 256));
+  if (o_dtype == kF32)
+    hipLaunchKernelGGL((dequant_kernel<kF32>), grid, dim3(256), 0, stream, q, ldq, scale, (float*)out, ldo, rows, cols);
+  else
+    hipLaunchKernelGGL((dequant_kernel<kBf16>), grid, dim3(256), 0, stream, q, ldq, scale, (uint16_t*)out, ldo, rows,
+                       cols);
+  return hipGetLastError();
+}
+
+}  // namespace harp_blk

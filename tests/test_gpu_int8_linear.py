@@ -1,0 +1,247 @@
+"""GPU tests of the products of 8-bit rows: harp_amd.int8_linear, Int8Linear
+and the q/k/v producer on 8-bit projections, against the formulas in 64 bits.
+
+Tolerances, with u = 2^-24 and half(t) half a step of the output's type: the
+integer sums are exact, so y = acc a t + b carries one rounding of the sum's
+conversion, two products and one addition:
+|y - y64| <= 4 u (|acc a t| + |b|) + half |y64|.  A normed and rotated value
+carries those, the norm's (64 squares a lane, a mean and a root: below 80 u),
+and four more: 100 u (|a| + |b|) of its pair's sizes, and half a step."""
+
+import pytest
+import torch
+from types import SimpleNamespace
+
+import harp_amd
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+U = 2.0 ** -24
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: U}
+B16, F32 = torch.bfloat16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _rows(g, rows, cols, pad=16, lead=0):
+    """Random 8-bit rows, -127 .. 127, in storage whose padding holds other values."""
+    ld = (lead + cols + pad - 1) // pad * pad
+    store = torch.randint(-127, 128, (rows, ld), generator=g, dtype=torch.int8).to(DEV)
+    scales = (torch.rand(rows, generator=g) * 0.02 + 1e-3).to(DEV)
+    return harp_amd.Int8Rows(store[:, lead:lead + cols], scales)
+
+
+def _exact(x, w):
+    """The integer sums, exactly, in 64 bits."""
+    return x.values.double() @ w.values.double().t()
+
+
+def _assert_linear(y, x, w, bias, what):
+    acc = _exact(x, w) * x.scales.double()[:, None] * w.scales.double()
+    b = torch.zeros(w.values.size(0), device=DEV, dtype=torch.float64) if bias is None else bias.double()
+    want = acc + b
+    bound = 4 * U * (acc.abs() + b.abs()) + HALF[y.dtype] * want.abs()
+    err = (y.double() - want).abs()
+    assert bool((err <= bound).all()), (what, int((err > bound).sum()), float(err.max()))
+
+
+MNK = [
+    (1, 1, 1), (1, 16, 16), (1, 100, 64), (2, 128, 128), (5, 130, 129), (16, 256, 640), (17, 129, 1000), (31, 4, 33),
+    (33, 300, 255), (64, 512, 512), (65, 513, 300), (127, 127, 127), (128, 128, 256), (129, 385, 384), (200, 1001, 70),
+    (256, 256, 128), (257, 257, 257), (300, 96, 4097), (1000, 264, 512), (520, 1024, 48), (1, 3840, 3840),
+    (3, 10240, 1000), (40, 17, 15360), (7, 33, 65536), (300, 2560, 640),
+]
+
+
+@pytest.mark.parametrize("M,N,K", MNK)
+def test_linear(M, N, K):
+    print(f"[int8_linear M={M} N={N} K={K}]", flush=True)
+    g = _gen(M + 3 * N + 5 * K)
+    x, w = _rows(g, M, K), _rows(g, N, K)
+    for bias in (None, torch.randn(N, generator=g).to(B16).to(DEV), torch.randn(N, generator=g).to(DEV)):
+        for dtype in (B16, F32):
+            y = harp_amd.int8_linear(x, w, bias, dtype)
+            assert y.shape == (M, N) and y.dtype == dtype and y.is_contiguous()
+            _assert_linear(y, x, w, bias, (M, N, K, dtype))
+
+
+def test_linear_layouts():
+    """Rows out of wider storage, repeated rows, batches and vectors."""
+    g = _gen(2)
+    w = _rows(g, 200, 100, pad=64)
+    x = _rows(g, 60, 100, pad=256, lead=48)
+    _assert_linear(harp_amd.int8_linear(x, w), x, w, None, "wide rows")
+    x1 = harp_amd.Int8Rows(x.values[:1].expand(40, 100), x.scales[:40].contiguous())
+    _assert_linear(harp_amd.int8_linear(x1, w), x1, w, None, "repeated rows")
+    xb = harp_amd.Int8Rows(x.values.unflatten(0, (3, 4, 5)), x.scales.view(3, 4, 5))
+    assert torch.equal(harp_amd.int8_linear(xb, w).view(60, 200), harp_amd.int8_linear(x, w))
+    xv = harp_amd.Int8Rows(x.values[7], x.scales[7])
+    assert torch.equal(harp_amd.int8_linear(xv, w), harp_amd.int8_linear(x, w)[7])
+    every = harp_amd.Int8Rows(x.values[::2], x.scales[::2])
+    assert torch.equal(harp_amd.int8_linear(every, w), harp_amd.int8_linear(x, w)[::2])
+    empty = harp_amd.Int8Rows(x.values[:0], x.scales[:0])
+    assert harp_amd.int8_linear(empty, w).shape == (0, 200)
+
+
+@pytest.mark.parametrize("M", [1, 20, 70, 300])
+def test_linear_extremes_and_nan(M):
+    """The largest sums (K = 65536 of -127 * 127 and 127 * 127) are exact; a
+    NaN scale makes its row NaN and no other."""
+    K, N = 65536, 130
+    x = torch.full((M, K), 127, dtype=torch.int8, device=DEV)
+    w = torch.full((N, K), -127, dtype=torch.int8, device=DEV)
+    w[1::2] = 127
+    s = torch.ones(M, device=DEV)
+    t = torch.ones(N, device=DEV)
+    y = harp_amd.int8_linear(harp_amd.Int8Rows(x, s), harp_amd.Int8Rows(w, t), None, F32)
+    top = float(127 * 127 * K)  # 16129 * 2^16: exact in fp32
+    assert bool((y[:, 1::2] == top).all()) and bool((y[:, 0::2] == -top).all())
+    s[M // 2] = float("nan")
+    y = harp_amd.int8_linear(harp_amd.Int8Rows(x, s), harp_amd.Int8Rows(w, t), None, F32)
+    nan = torch.isnan(y).all(1)
+    assert bool(nan[M // 2]) and int(nan.sum()) == 1 and int(torch.isnan(y).sum()) == N
+
+
+def test_lowest_value():
+    """-128, which no function here writes, multiplies as -128."""
+    x = torch.full((40, 64), -128, dtype=torch.int8, device=DEV)
+    one = torch.ones(40, device=DEV)
+    y = harp_amd.int8_linear(harp_amd.Int8Rows(x, one), harp_amd.Int8Rows(x, one), None, F32)
+    assert bool((y == 64 * 128 * 128).all())
+
+
+@pytest.mark.parametrize("M", [1, 19, 333])
+@pytest.mark.parametrize("dtype", [B16, F32], ids=str)
+def test_module_quantises_its_input(M, dtype):
+    g = _gen(M)
+    lin = torch.nn.Linear(250, 321, bias=True)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(321, 250, generator=g) / 16)
+        lin.bias.copy_(torch.randn(321, generator=g))
+    lin = lin.to(B16).to(DEV)
+    q = harp_amd.Int8Linear.from_linear(lin)
+    x = torch.randn(2, M, 250, generator=g).to(dtype).to(DEV)
+    rows = harp_amd.quantize_int8(x)
+    y = q(x)
+    assert y.shape == (2, M, 321) and torch.equal(y, q(rows))
+    flat = harp_amd.Int8Rows(rows.values.view(2 * M, 250), rows.scales.view(-1))
+    _assert_linear(y.view(2 * M, 321), flat, q.weight, lin.bias.detach(), "module")
+    # and it stands in for the Linear: both operands are off by half a step of
+    # max / 127 at most, a 250-term sum's error is within the sum of those
+    full = x.double() @ lin.weight.detach().double().t() + lin.bias.detach().double()
+    sx, sw = rows.scales.double(), q.weight.scales.double()
+    bound = 0.5 * (sx[..., None] * q.weight.dequantize(F32).double().abs().sum(-1) + x.double().abs().sum(-1)[..., None] * sw) \
+        + 250 * 0.25 * sx[..., None] * sw
+    err = (y.double() - full).abs()
+    assert bool((err <= 1.001 * bound + 2 ** -8 * full.abs()).all())
+
+
+def test_linear_refusals():
+    g = _gen(9)
+    x, w = _rows(g, 4, 64), _rows(g, 32, 64)
+    odd = torch.zeros(4, 70, dtype=torch.int8, device=DEV)[:, :64]
+    with pytest.raises(RuntimeError, match="multiples of 16 bytes"):
+        harp_amd.int8_linear(harp_amd.Int8Rows(odd, x.scales), w)
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        harp_amd.int8_linear(harp_amd.Int8Rows(torch.zeros(4, 80, dtype=torch.int8, device=DEV)[:, 8:72], x.scales), w)
+    with pytest.raises(RuntimeError, match="unit stride"):
+        harp_amd.int8_linear(harp_amd.Int8Rows(torch.zeros(64, 4, dtype=torch.int8, device=DEV).t(), x.scales), w)
+    with pytest.raises(RuntimeError, match="int8"):
+        harp_amd.int8_linear(harp_amd.Int8Rows(x.values.float(), x.scales), w)
+    with pytest.raises(RuntimeError, match="one scale for each row"):
+        harp_amd.int8_linear(harp_amd.Int8Rows(x.values, x.scales[:3]), w)
+    with pytest.raises(RuntimeError, match="float32"):
+        harp_amd.int8_linear(harp_amd.Int8Rows(x.values, x.scales.to(B16)), w)
+    with pytest.raises(RuntimeError, match=r"weight must be \[N, 64\]"):
+        harp_amd.int8_linear(x, _rows(g, 32, 48))
+    with pytest.raises(RuntimeError, match="bias"):
+        harp_amd.int8_linear(x, w, torch.zeros(31, device=DEV))
+    with pytest.raises(RuntimeError, match="bfloat16 or float32"):
+        harp_amd.int8_linear(x, w, None, torch.float16)
+
+
+# ---------------------------------------------------------------------------
+# q, k, v
+# ---------------------------------------------------------------------------
+
+def _freqs(S, batch=0):
+    ang = torch.arange(S, dtype=torch.float64)[:, None] * (256.0 ** (-torch.arange(0, 128, 2, dtype=torch.float64) / 128))
+    if batch:
+        ang = torch.stack([ang + 0.25 * b for b in range(batch)])
+    return torch.polar(torch.ones_like(ang), ang).to(torch.complex64).to(DEV)
+
+
+def _attn(g, H, K, norm_kind):
+    to = [harp_amd.Int8Linear(_rows(g, H * 128, K)) for _ in range(3)]
+    norms = [None, None]
+    if norm_kind is not None:
+        norms = [SimpleNamespace(weight=(1 + 0.2 * torch.randn(128, generator=g)).to(norm_kind).to(DEV), eps=1e-6)
+                 for _ in range(2)]
+    return SimpleNamespace(heads=H, to_q=to[0], to_k=to[1], to_v=to[2], norm_q=norms[0], norm_k=norms[1])
+
+
+def _assert_qkv(outs, attn, rows, freqs, what):
+    B, S = rows.scales.shape
+    H = attn.heads
+    flat = harp_amd.Int8Rows(rows.values.reshape(B * S, -1), rows.scales.reshape(-1))
+    for i, (y, lin) in enumerate(zip(outs, (attn.to_q, attn.to_k, attn.to_v))):
+        assert y.shape == (B, H, S, 128) and y.dtype == B16
+        assert y.stride() == (S * H * 128, 128, H * 128, 1)
+        want = (_exact(flat, lin.weight) * flat.scales.double()[:, None] * lin.weight.scales.double())
+        want = want.view(B, S, H, 128).transpose(1, 2)
+        norm = (attn.norm_q, attn.norm_k, None)[i]
+        size, steps = want.abs(), 4
+        if norm is not None:
+            want = want / torch.sqrt(want.square().mean(-1, keepdim=True) + norm.eps) * norm.weight.double()
+            size, steps = want.abs(), 100
+            if freqs is not None:
+                f = freqs.to(torch.complex128)
+                f = f[:, None] if f.dim() == 3 else f
+                pair = torch.view_as_complex(want.unflatten(-1, (64, 2)).contiguous())
+                size = size.unflatten(-1, (64, 2)).sum(-1, keepdim=True).expand(*want.shape[:-1], 64, 2).flatten(-2)
+                want = torch.view_as_real(pair * f).flatten(-2)
+        err = (y.double() - want).abs()
+        bound = steps * U * size + 2.0 ** -8 * want.abs()
+        assert bool((err <= bound).all()), (what, i, int((err > bound).sum()), float(err.max()))
+
+
+@pytest.mark.parametrize("B,S,H,K,norm,rope", [
+    (1, 1, 1, 128, B16, True), (1, 1, 5, 640, F32, True), (2, 3, 2, 100, B16, False), (1, 40, 3, 384, B16, True),
+    (2, 65, 2, 257, F32, True), (1, 128, 1, 128, None, False), (1, 300, 4, 512, B16, True), (3, 111, 3, 384, B16, True),
+    (1, 700, 2, 1000, None, False), (1, 1030, 5, 640, F32, True),
+])
+def test_qkv(B, S, H, K, norm, rope):
+    print(f"[qkv B={B} S={S} H={H} K={K} norm={norm} rope={rope}]", flush=True)
+    g = _gen(B + S + H + K)
+    attn = _attn(g, H, K, norm)
+    flat = _rows(g, B * S, K)
+    rows = harp_amd.Int8Rows(flat.values.unflatten(0, (B, S)), flat.scales.view(B, S))
+    freqs = _freqs(S, B if B > 2 else 0) if rope else None
+    outs = harp_amd.project_qkv(attn, rows, freqs)
+    _assert_qkv(outs, attn, rows, freqs, (B, S, H, K))
+
+
+def test_qkv_unfused_paths():
+    """What the one launch does not take runs as separate products and norms:
+    the results agree to the bf16 steps between the stages (a product rounded
+    to bf16, two values truncated to it: 2^-8 + 2 * 2^-7 of the pair, under
+    2^-5 with the pair's other value)."""
+    g = _gen(4)
+    attn = _attn(g, 2, 256, B16)
+    flat = _rows(g, 50, 256)
+    rows = harp_amd.Int8Rows(flat.values.unflatten(0, (1, 50)), flat.scales.view(1, 50))
+    f = _freqs(50)
+    fused = harp_amd.project_qkv(attn, rows, f)
+    apart = harp_amd.project_qkv(attn, rows, f, fused=False)
+    for a, b in zip(fused, apart):
+        assert a.shape == b.shape
+        size = a.double().abs().unflatten(-1, (64, 2)).sum(-1, keepdim=True).expand(*a.shape[:-1], 64, 2).flatten(-2)
+        assert bool(((a.double() - b.double()).abs() <= 2 ** -5 * size + 1e-6).all())
+    assert torch.equal(fused[2], apart[2])
+    # a bias keeps the products apart
+    attn.to_v = harp_amd.Int8Linear(attn.to_v.weight, torch.ones(256, device=DEV))
+    v = harp_amd.project_qkv(attn, rows, f)[2]
+    assert torch.equal(v, attn.to_v(rows).unflatten(-1, (2, 128)).transpose(1, 2))
