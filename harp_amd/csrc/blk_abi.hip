@@ -35,6 +35,7 @@ int ok() {
 constexpr int64_t kMaxLd8 = (int64_t)1 << 22;  // a 256-row tile of 8-bit rows spans < 2^32 bytes
 constexpr int kMaxK = 1 << 16;                 // 2^16 products of at most 2^14: below 2^31
 constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr int kMaxTokens = 1 << 30;            // of a product: token indexes stay in 32 bits past the last tile
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 int elem_size(int dt) { return dt == HARP_BLK_F32 ? 4 : 2; }
@@ -262,6 +263,7 @@ int harp_blk_linear_int8(const int8_t* x, int64_t ld_x, const float* x_scales, c
   int rc;
   if (M < 0 || N < 1 || K < 1) return fail(HARP_BLK_EINVAL, "M=%d, N=%d, K=%d: N and K must be positive", M, N, K);
   if (K > kMaxK) return fail(HARP_BLK_EUNSUPPORTED, "K=%d > %d is not supported", K, kMaxK);
+  if (M > kMaxTokens || N > kMaxTokens) return fail(HARP_BLK_EUNSUPPORTED, "M=%d, N=%d: more than 2^30", M, N);
   if (M == 0) return ok();
   if ((rc = check_rows8(x, ld_x, K, kMaxLd8, false, "x"))) return rc;
   if ((rc = check_floats(x_scales, "x_scales"))) return rc;
@@ -295,11 +297,12 @@ int harp_blk_qkv_int8(const int8_t* x, int64_t ld_x, const float* x_scales, int 
                       int n_outs, void* stream) {
   int rc;
   if (batch < 0 || seq < 0) return fail(HARP_BLK_EINVAL, "batch=%d and seq=%d must not be negative", batch, seq);
-  if ((int64_t)batch * seq >= ((int64_t)1 << 31)) return fail(HARP_BLK_EUNSUPPORTED, "batch * seq >= 2^31");
+  if ((int64_t)batch * seq > kMaxTokens) return fail(HARP_BLK_EUNSUPPORTED, "batch * seq > 2^30");
   if (k_dim < 1) return fail(HARP_BLK_EINVAL, "k_dim=%d must be positive", k_dim);
   if (k_dim > kMaxK) return fail(HARP_BLK_EUNSUPPORTED, "k_dim=%d > %d is not supported", k_dim, kMaxK);
   if (n_out < 128 || n_out % 128)
     return fail(HARP_BLK_EUNSUPPORTED, "n_out=%d must be a positive multiple of 128 (heads of 128)", n_out);
+  if (n_out > kMaxTokens) return fail(HARP_BLK_EUNSUPPORTED, "n_out=%d > 2^30", n_out);
   if (!outs || n_outs < 1 || n_outs > kMaxOuts8)
     return fail(HARP_BLK_EINVAL, "outs must hold 1 to %d outputs (got %d)", kMaxOuts8, n_outs);
   if ((int64_t)batch * seq == 0) return ok();

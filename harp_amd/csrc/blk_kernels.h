@@ -70,7 +70,7 @@ hipError_t launch_dequantize(const int8_t* q, int64_t ldq, const float* scale, v
 
 // ---------------------------------------------------------------------------
 constexpr int kMaxOuts8 = 3;
-constexpr int kKTile8 = 128;  // contraction elements (= bytes) per LDS tile
+constexpr int kKTile8 = 128;  // bytes of K per unit of the kinds' measured times
 
 // One product y = (x w^T) * x_scale * w_scale + bias of 8-bit rows.
 struct Prod8Out {
@@ -93,6 +93,7 @@ struct Prod8Params {
   const float* x_scale;  // [M]
   int M, N, K;
   int S;               // tokens of one batch entry (rows of the RoPE table)
+  int m_base;          // x's first row among the call's tokens (0, or set by launch_prod8)
   const float* freqs;  // RoPE table of the normed outputs, fp32 (cos, sin) pairs; NULL = none
   int64_t f_stride_b, f_stride_s;
   int n_outs;

@@ -17,6 +17,7 @@ namespace harp_blk {
 
 using harp_ra::bf16;
 using harp_ra::f32x4;
+using harp_ra::kOOB;
 using harp_ra::f32x4u;
 using harp_ra::lds_dma_b128;
 using harp_ra::lds_void;
@@ -32,18 +33,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4u __attribute__((aligned(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2u __attribute__((aligned(2)));
 
-constexpr int kTokenGroups = 4;       // waves per feature group of a block, along the tokens
-constexpr int kFeat = 128;            // features of one wave (one head)
-constexpr int kRowBytes = kKTile8;    // 128: one row of a tile
-constexpr int kGroupOrder = 4;        // feature tiles per group of the block order
+constexpr int kFeat = 128;       // features of one head
+constexpr int kGroupOrder = 4;   // feature tiles per group of the block order
 constexpr int kLds8Bytes = 144 * 1024;
-
-template <int I>
-struct Int {
-  static constexpr int value = I;
-  constexpr operator int() const { return I; }
-};
 
 // 32 x 32 x 32: lane L holds row L % 32 of A and of B with the same 16 values
 // of k, picked by L / 32; C as every 32 x 32 product (ra_common.h)
@@ -51,16 +46,21 @@ __device__ __forceinline__ i32x16 mfma32x32x32(i32x4 a, i32x4 b, i32x16 c) {
   return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
 }
 
-// Tile layout: rows of 128 bytes = 8 chunks of 16; chunk c of row r sits at
-// position c ^ ((r >> 1) & 7), so that the 16 lanes of a fragment read that
-// are served together (rows r0 .. r0 + 15 at one chunk) touch every 16-byte
-// bank group of the 256-byte bank line once.
-__device__ __forceinline__ int tile_pos(int r, int c) { return c ^ ((r >> 1) & 7); }
+// Tile layout: rows of KT bytes in chunks of 16; chunk c of row r sits at a
+// position that differs from c by a few of r's bits, so that the 16 lanes of a
+// fragment read that are served together (rows r0 .. r0 + 15 at one chunk)
+// touch every 16-byte bank group of the 256-byte bank line once.
+template <int KT>
+__device__ __forceinline__ int tile_pos(int r, int c) {
+  static_assert(KT == 256 || KT == 128 || KT == 64, "row bytes");
+  return KT == 256 ? c ^ (r & 15) : KT == 128 ? c ^ ((r >> 1) & 7) : c ^ ((r >> 2) & 3);
+}
 
 // Source byte offset (within the tile's rows) of 16-byte LDS slot `slot`.
+template <int KT>
 __device__ __forceinline__ uint32_t slot_src(int slot, int64_t ld) {
-  const int r = slot >> 3;
-  return (uint32_t)(r * ld + tile_pos(r, slot & 7) * 16);
+  const int r = slot / (KT / 16);
+  return (uint32_t)(r * ld + tile_pos<KT>(r, slot % (KT / 16)) * 16);
 }
 
 __device__ __forceinline__ float bits_f32(uint32_t b) { return __uint_as_float(b); }
@@ -69,55 +69,80 @@ __device__ __forceinline__ float vec_at(const void* v, int f32, int64_t i) {
   return f32 ? ((const float*)v)[i] : bits_f32((uint32_t)((const uint16_t*)v)[i] << 16);
 }
 
+// 16 bytes at byte offset off of a buffer (zeros past its end)
+__device__ __forceinline__ i32x4 buffer_load16(rsrc_t r, uint32_t off) {
+  const uint64_t a = (uint64_t)r.x | ((uint64_t)r.y << 32);
+  const auto b = __builtin_amdgcn_make_buffer_rsrc((void*)a, 0, r.z, r.w);
+  return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0));
+}
+
 // byte mask of dword i of a 16-byte chunk whose first n (0 .. 16) bytes count
 __device__ __forceinline__ uint32_t dword_mask(int n, int i) {
   const int b = n - 4 * i;
   return b >= 4 ? 0xffffffffu : (b <= 0 ? 0u : (1u << (8 * b)) - 1u);
 }
 
-template <int NJ>
+template <int FB, int NJ>
 struct Frags {
-  i32x4 a[4];   // w rows: 32 features each
+  i32x4 a[FB];  // w rows: 32 features each
   i32x4 b[NJ];  // x rows: 32 tokens each
 };
+
+// v_permlane32_swap on two dwords: afterwards x holds (x of lanes 0 .. 31, y
+// of lanes 0 .. 31) and y (x of lanes 32 .. 63, y of lanes 32 .. 63)
+__device__ __forceinline__ void swap_halves(uint32_t& x, uint32_t& y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = r[0];
+  y = r[1];
+}
 
 }  // namespace
 
 // Tile kernel.  C^T = W x^T, so a lane holds one token and 16 features per
-// accumulator.  A block is 4 x GROUPS waves and covers GROUPS x 128 features
-// by 4 x TPW tokens; a wave 128 features by TPW tokens (4 x TPW / 32
-// accumulators of 32 x 32).  K-tiles of 128 bytes a row are copied global ->
+// accumulator.  A wave covers FB x NJ blocks of 32 features by 32 tokens; a
+// block is GROUPS x FB x 32 features by TG x NJ x 32 tokens, each part covered
+// by KG waves that share the k-steps of a tile and add their sums at the end.  K-tiles of KT bytes a row are copied global ->
 // LDS by buffer_load ... lds, STAGES of them in flight, one barrier per tile
 // in its last k-step; fragment reads run on across tile boundaries.
 // Rows past the last token or feature and bytes past the descriptors' ends
 // load zeros; the last tile's bytes past K are cleared in the w tile, which
 // makes whatever x holds there count for nothing.
-template <int TPW, int GROUPS, int STAGES, bool NORM>
-__global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Prod8Params p) {
-  constexpr int kWaves = kTokenGroups * GROUPS;
+template <int FB, int NJ, int TG, int GROUPS, int KG, int KT, int STAGES, bool NORM>
+__global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Params p) {
+  constexpr int kWaves = TG * GROUPS * KG;
   constexpr int kThreads = 64 * kWaves;
-  constexpr int kFeatures = GROUPS * kFeat;
-  constexpr int kWBytes = kFeatures * kRowBytes;
+  constexpr int kWaveFeat = 32 * FB, TPW = 32 * NJ;
+  constexpr int kFeatures = GROUPS * kWaveFeat;
+  constexpr int kWBytes = kFeatures * KT;
   constexpr int kWPerWave = kWBytes / 1024 / kWaves;
-  constexpr int NJ = TPW / 32;
-  constexpr int kTok = kTokenGroups * TPW;
-  constexpr int kXBytes = kTok * kRowBytes;
+  constexpr int kTok = TG * TPW;
+  constexpr int kXBytes = kTok * KT;
   constexpr int kXPerWave = kXBytes / 1024 / kWaves;
   constexpr int kDmaPerWave = kXPerWave + kWPerWave;
-  constexpr int kMfma = 4 * NJ;
+  constexpr int kMfma = FB * NJ;
+  constexpr int kOwn = KT / 32 / KG;  // k-steps of a wave in a tile
   constexpr int kRing = STAGES * (kXBytes + kWBytes);
   static_assert(kXBytes % (1024 * kWaves) == 0 && kWBytes % (1024 * kWaves) == 0, "copies split evenly");
   static_assert(kRing <= kLds8Bytes, "LDS budget");
-  static_assert(kWaves * 32 * kFeat * 4 <= kRing, "a wave's staging of 32 fp32 rows fits the stages");
+  static_assert(kOwn * KG * 32 == KT && (kOwn % 2 == 0 || STAGES % 2 == 0), "whole k-steps; fragments in turn");
+  // what a wave finishes of the sums it shares: whole token blocks where there
+  // is one for each (a head stays in one wave), else feature blocks of one
+  // (with fewer blocks than waves, the last waves have none)
+  constexpr int kOwnJ = NJ % KG == 0 ? NJ / KG : 1, kOwnF = FB * NJ >= KG ? FB * NJ / KG / kOwnJ : 1;
+  constexpr int kParts = FB / kOwnF;  // waves that finish a token block between them
+  static_assert((kOwnJ * kOwnF * KG == FB * NJ || FB * NJ < KG) && FB % kOwnF == 0, "equal shares");
+  static_assert(!NORM || (FB == 4 && (kParts == 1 || GROUPS == 1)), "a head in one wave, or in the waves of one sum");
+  static_assert(KG == 1 || kWaves * FB * NJ * 4096 <= kRing, "the sums fit the stages");
   __shared__ __attribute__((aligned(16))) char lds[kRing];
   __shared__ float wsc[kFeatures], wbias[kFeatures];  // feature scales; bias, or the norm's weight
+  __shared__ float part_ss[NORM && kParts > 1 ? KG : 1][32];
   auto Xs = [&](int s) { return lds + s * kXBytes; };
   auto Ws = [&](int s) { return lds + STAGES * kXBytes + s * kWBytes; };
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, g = lane >> 5;
-  const int hh = wave % GROUPS, tg = wave / GROUPS;
+  const int kg = wave % KG, hh = wave / KG % GROUPS, tg = wave / KG / GROUPS;
 
   // block -> (token tile, feature tile): each XCD (workgroups are dealt to
   // them round-robin) gets a contiguous range of an order that walks groups
@@ -142,19 +167,19 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
 
   uint32_t xsrc[kXPerWave], wsrc[kWPerWave];
 #pragma unroll
-  for (int k = 0; k < kXPerWave; ++k) xsrc[k] = slot_src((wave + kWaves * k) * 64 + lane, p.ldx);
+  for (int k = 0; k < kXPerWave; ++k) xsrc[k] = slot_src<KT>((wave + kWaves * k) * 64 + lane, p.ldx);
 #pragma unroll
-  for (int k = 0; k < kWPerWave; ++k) wsrc[k] = slot_src((wave + kWaves * k) * 64 + lane, o.ldw);
-  const int nt = (p.K + kKTile8 - 1) / kKTile8;
-  const int k_last = p.K - (nt - 1) * kKTile8;  // bytes of the last tile, 1 .. 128
+  for (int k = 0; k < kWPerWave; ++k) wsrc[k] = slot_src<KT>((wave + kWaves * k) * 64 + lane, o.ldw);
+  const int nt = (p.K + KT - 1) / KT;
+  const int k_last = p.K - (nt - 1) * KT;  // bytes of the last tile, 1 .. KT
   // descriptors of tile t's rows; past the last tile they are empty (the
   // copies then write zeros and read nothing)
   auto x_rsrc = [&](int t) {
-    const int k0 = t * kKTile8;
+    const int k0 = t * KT;
     return make_rsrc(xb + (t < nt ? k0 : 0), t < nt ? x_bytes - (uint32_t)k0 : 0u);
   };
   auto w_rsrc = [&](int t) {
-    const int k0 = t * kKTile8;
+    const int k0 = t * KT;
     return make_rsrc(wb + (t < nt ? k0 : 0), t < nt ? w_bytes - (uint32_t)k0 : 0u);
   };
   const uint32_t lds_wave = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(lds + wave * 1024));
@@ -165,15 +190,14 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
       lds_dma_b128(wr, base + STAGES * kXBytes + s * kWBytes + kWaves * (j - kXPerWave) * 1024,
                    wsrc[j - kXPerWave]);
   };
-  // clear the bytes past K of the last w tile, in stage s (two threads a row)
+  // clear the bytes past K of the last w tile, in stage s
   auto clear_tail = [&](int s) {
-    static_assert(kThreads == 2 * kFeatures, "two threads per row of the w tile");
-    const int r = tid >> 1;
-#pragma unroll
-    for (int c4 = 0; c4 < 4; ++c4) {
-      const int c = 4 * (tid & 1) + c4, n = k_last - 16 * c;
+    constexpr int kChunks = KT / 16;
+#pragma unroll 1
+    for (int id = tid; id < kFeatures * kChunks; id += kThreads) {
+      const int r = id / kChunks, c = id % kChunks, n = k_last - 16 * c;
       if (n < 16) {
-        u32x4* q = (u32x4*)(Ws(s) + r * kRowBytes + (tile_pos(r, c) << 4));
+        u32x4* q = (u32x4*)(Ws(s) + r * KT + (tile_pos<KT>(r, c) << 4));
         u32x4 v = *q;
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] &= dword_mask(n, i);
@@ -182,28 +206,29 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
     }
   };
 
-  int foff[4];
+  // lane part of the fragments' LDS offsets: the wave's k-steps kg kOwn ..
+  int foff[kOwn];
 #pragma unroll
-  for (int ks = 0; ks < 4; ++ks) foff[ks] = l32 * kRowBytes + (tile_pos(l32, 2 * ks + g) << 4);
+  for (int ks = 0; ks < kOwn; ++ks) foff[ks] = l32 * KT + (tile_pos<KT>(l32, 2 * (kg * kOwn + ks) + g) << 4);
   auto load = [&](int s, int ks) {
-    Frags<NJ> f;
-    const char* xs = Xs(s) + tg * TPW * kRowBytes + foff[ks];
-    const char* ws = Ws(s) + hh * kFeat * kRowBytes + foff[ks];
+    Frags<FB, NJ> f;
+    const char* xs = Xs(s) + tg * TPW * KT + foff[ks];
+    const char* ws = Ws(s) + hh * kWaveFeat * KT + foff[ks];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) f.b[j] = *(const i32x4*)(xs + 32 * j * kRowBytes);
+    for (int j = 0; j < NJ; ++j) f.b[j] = *(const i32x4*)(xs + 32 * j * KT);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f.a[i] = *(const i32x4*)(ws + 32 * i * kRowBytes);
+    for (int i = 0; i < FB; ++i) f.a[i] = *(const i32x4*)(ws + 32 * i * KT);
     return f;
   };
 
-  i32x16 acc[4][NJ];
+  i32x16 acc[FB][NJ];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < FB; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-  auto mma = [&](const Frags<NJ>& f, bool copy, const rsrc_t& xr, const rsrc_t& wr, int s) {
+  auto mma = [&](const Frags<FB, NJ>& f, bool copy, const rsrc_t& xr, const rsrc_t& wr, int s) {
     // (opaque, or every stage's addresses would be kept in SGPRs over the loop)
     uint32_t base = lds_wave;
     asm volatile("" : "+s"(base));
@@ -228,6 +253,7 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
       r_b = vec_at(o.bias, o.bias_f32, n0 + tid);
     }
   }
+  static_assert(kThreads >= kFeatures, "a thread per feature");
 
 #pragma unroll
   for (int t = 0; t < STAGES; ++t) {
@@ -237,53 +263,45 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
   }
   wait_lds_loads_but<(STAGES - 1) * kDmaPerWave>();
   __syncthreads();
-  if (nt == 1 && k_last < kKTile8) {
+  if (nt == 1 && k_last < KT) {
     clear_tail(0);
     __syncthreads();
   }
-  Frags<NJ> f0 = load(0, 0), f1;
+  Frags<FB, NJ> f[2];
+  f[0] = load(0, 0);
 
   // After the last tile the fragment reads of "tile t + 1" read a stale
   // stage and the copies of "tile t + STAGES" are empty: both stay in bounds
   // and their results are never used.
-  auto tile = [&](auto SC, int t) {
-    constexpr int S = decltype(SC)::value, S1 = (S + 1) % STAGES;
-    f1 = load(S, 1);
-    sched_fence();
-    mma(f0, false, {}, {}, S);
-    sched_fence();
-    f0 = load(S, 2);
-    sched_fence();
-    mma(f1, false, {}, {}, S);
-    sched_fence();
-    f1 = load(S, 3);
-    sched_fence();
-    mma(f0, false, {}, {}, S);
-    sched_fence();
+  auto tile = [&](int S, int t) {  // stage S, a constant of the unrolled loop below
+    const int S1 = (S + 1) % STAGES;
+    const int P = kOwn % 2 ? S & 1 : 0;  // the fragments of the tile's first k-step
+#pragma unroll
+    for (int ks = 0; ks + 1 < kOwn; ++ks) {
+      f[(P + ks + 1) & 1] = load(S, ks + 1);
+      sched_fence();
+      mma(f[(P + ks) & 1], false, {}, {}, S);
+      sched_fence();
+    }
     // every wave has its last fragments of tile t, and tile t + 1 is
     // complete: only the copies of tiles t + 2 .. t + STAGES - 1 are younger
     wait_lds_loads_but<(STAGES - 2) * kDmaPerWave>();
     __syncthreads();
-    if (t + 2 == nt && k_last < kKTile8) {
+    if (t + 2 == nt && k_last < KT) {
       clear_tail(S1);
       __syncthreads();
     }
     const rsrc_t xr = x_rsrc(t + STAGES), wr = w_rsrc(t + STAGES);
-    f0 = load(S1, 0);
+    f[(P + kOwn) & 1] = load(S1, 0);
     sched_fence();
-    mma(f1, true, xr, wr, S);
+    mma(f[(P + kOwn - 1) & 1], true, xr, wr, S);
     sched_fence();
   };
 #pragma unroll 1
   for (int t = 0; t < nt; t += STAGES) {
-    tile(Int<0>{}, t);
-    if (t + 1 < nt) tile(Int<1>{}, t + 1);
-    if constexpr (STAGES > 2) {
-      if (t + 2 < nt) tile(Int<2>{}, t + 2);
-    }
-    if constexpr (STAGES > 3) {
-      if (t + 3 < nt) tile(Int<3>{}, t + 3);
-    }
+#pragma unroll
+    for (int S = 0; S < STAGES; ++S)
+      if (t + S < nt) tile(S, t + S);
   }
   // no copy may still write the LDS when the stages become staging rows
   wait_lds_loads();
@@ -293,49 +311,94 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
   }
   __syncthreads();
 
-  // ---- epilogue: this lane holds tokens m0 + TPW tg + 32 j + l32 and
-  // features 32 i + 8 q + 4 g + e of its wave's 128, e < 4
-  const int fw = n0 + hh * kFeat;  // the wave's first feature
-  if (fw >= p.N) return;
+  // the KG waves of a sum put theirs into LDS, and each adds up its share
+  i32x16 own[kOwnF][kOwnJ];
+  const int i_own = kOwnF == FB ? 0 : kg / NJ * kOwnF, j_own = kOwnF == FB ? kg * kOwnJ : kg % NJ;
+  if constexpr (KG > 1) {
+    i32x4* const sums = (i32x4*)lds + lane;  // [wave][FB][NJ][4] x 64 lanes
+#pragma unroll
+    for (int i = 0; i < FB; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          sums[((((wave * FB) + i) * NJ + j) * 4 + q) * 64] =
+              i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOwnF; ++i)
+#pragma unroll
+      for (int j = 0; j < kOwnJ; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const i32x4* s0 = sums + (((((wave - kg) * FB) + i_own + i) * NJ + j_own + j) * 4 + q) * 64;
+          i32x4 v = s0[0];
+#pragma unroll
+          for (int k = 1; k < KG; ++k) v += s0[k * FB * NJ * 4 * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) own[i][j][4 * q + e] = v[e];
+        }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kOwnF; ++i)
+#pragma unroll
+      for (int j = 0; j < kOwnJ; ++j) own[i][j] = acc[i][j];
+  }
+
+  // ---- epilogue: this lane holds tokens m_own + 32 j + l32 and features
+  // f_own + 32 i + 8 q + 4 g + e of the block's, e < 4
+  const int f_own = hh * kWaveFeat + 32 * i_own, m_own = m0 + TPW * tg + 32 * j_own;
+  const int fw = n0 + f_own;
+  if (fw >= p.N || (FB * NJ < KG && kg >= FB * NJ)) return;  // (a norm's N has whole heads: no wave of one leaves)
   const int lane_e = harp_ra::lane_id_fresh(), l32e = lane_e & 31, ge = lane_e >> 5;
-  char* const stg = lds + wave * (32 * kFeat * 4);  // 32 rows of 256 or 512 bytes, one token block at a time
   const bool norm = NORM && o.norm_w != nullptr;
   const bool rope = norm && p.freqs != nullptr;
 
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int mj = m0 + TPW * tg + 32 * j;  // the token block's first token
-    const int m = min(mj + l32e, p.M - 1);
+  for (int j = 0; j < kOwnJ; ++j) {
+    const int mj = m_own + 32 * j + l32e;  // the lane's token
+    const int m = min(mj, p.M - 1);
     const float sx = p.x_scale[m];
-    f32x4 v[4][4];
+    f32x4 v[kOwnF][4];
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < kOwnF; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int d0 = 32 * i + 8 * q + 4 * ge;
-        const f32x4 ws = *(const f32x4*)(wsc + hh * kFeat + d0);
+        const int d0 = f_own + 32 * i + 8 * q + 4 * ge;
+        const f32x4 ws = *(const f32x4*)(wsc + d0);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[i][q][e] = (float)acc[i][j][4 * q + e] * sx * ws[e];
+          v[i][q][e] = (float)own[i][j][4 * q + e] * sx * ws[e];
           if (NORM) ss = __builtin_fmaf(v[i][q][e], v[i][q][e], ss);
         }
         if (!NORM) {
-          const f32x4 b = *(const f32x4*)(wbias + hh * kFeat + d0);
+          const f32x4 b = *(const f32x4*)(wbias + d0);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[i][q][e] += b[e];
         }
       }
     if (NORM && norm) {
-      ss = harp_ra::wave_half_sum(ss);  // this lane's 64 features and its partner lane's
-      const float rho = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)kFeat) + o.eps));
-      const float* fr = rope ? p.freqs + (int64_t)(m / p.S) * p.f_stride_b + (int64_t)(m % p.S) * p.f_stride_s : nullptr;
+      ss = harp_ra::wave_half_sum(ss);  // this lane's features of the token and its partner lane's
+      if constexpr (kParts > 1) {
+        static_assert(kOwnJ == 1, "one exchange");
+        // the waves of the token block: kg = part * NJ + token block
+        part_ss[kg][l32e] = ss;
+        __syncthreads();
+        ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < kParts; ++k) ss += part_ss[k * NJ + kg % NJ][l32e];
+      }
+      const float rho = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)kFeat) + o.eps));
+      const int mt_all = m + p.m_base;  // the token among the call's
+      const float* fr =
+          rope ? p.freqs + (int64_t)(mt_all / p.S) * p.f_stride_b + (int64_t)(mt_all % p.S) * p.f_stride_s : nullptr;
+#pragma unroll
+      for (int i = 0; i < kOwnF; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int d0 = 32 * i + 8 * q + 4 * ge;
-          const f32x4 w = *(const f32x4*)(wbias + hh * kFeat + d0);
+          const int d0 = 32 * (i_own + i) + 8 * q + 4 * ge;
+          const f32x4 w = *(const f32x4*)(wbias + hh * kWaveFeat + d0);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[i][q][e] = v[i][q][e] * rho * w[e];
           if (rope) {
@@ -349,80 +412,272 @@ __global__ __launch_bounds__(64 * kTokenGroups * GROUPS, 1) void prod8_kernel(Pr
           }
         }
     }
-    // out through LDS: the wave's own rows (16-byte chunk c of row r at
-    // position c ^ (r & 15)), then 16 bytes per lane along the rows; LDS
-    // operations of one wave stay in order, so there is no barrier
+    // stores: 16 bytes per lane, 32 in a row of y.  bf16: the halves of the
+    // wave hold 4 of a chunk's 8 features each; they exchange two chunks so
+    // that each half has one whole.
     if (NORM || !o.y_f32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kOwnF; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          *(uint2*)(stg + l32e * 256 + (((4 * i + q) ^ (l32e & 15)) << 4) + ge * 8) =
-              make_uint2(bf16_rne(v[i][q][0]) | (bf16_rne(v[i][q][1]) << 16),
-                         bf16_rne(v[i][q][2]) | (bf16_rne(v[i][q][3]) << 16));
+        for (int q = 0; q < 4; q += 2) {
+          u32x4 u;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = 4 * k + (lane_e >> 4), c = lane_e & 15, n = fw + c * 8;
-        const u32x4 u = *(const u32x4*)(stg + r * 256 + ((c ^ (r & 15)) << 4));
-        uint16_t* dst = (uint16_t*)o.y + (int64_t)(mj + r) * o.ldy + n;
-        if (mj + r < p.M) {
-          if (n + 8 <= p.N) {
-            *(u32x4u*)dst = u;
-          } else {
+          for (int h = 0; h < 2; ++h) {
+            u[h] = bf16_rne(v[i][q][2 * h]) | (bf16_rne(v[i][q][2 * h + 1]) << 16);
+            u[2 + h] = bf16_rne(v[i][q + 1][2 * h]) | (bf16_rne(v[i][q + 1][2 * h + 1]) << 16);
+          }
+          uint32_t x0 = u[0], x1 = u[1], y0 = u[2], y1 = u[3];
+          swap_halves(x0, y0);
+          swap_halves(x1, y1);
+          u = u32x4{x0, x1, y0, y1};
+          const int n = fw + 32 * i + 8 * (q + ge);
+          uint16_t* dst = (uint16_t*)o.y + (int64_t)mj * o.ldy + n;
+          if (mj < p.M) {
+            if (n + 8 <= p.N) {
+              *(u32x4u*)dst = u;
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < p.N) dst[e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+              for (int e = 0; e < 8; ++e)
+                if (n + e < p.N) dst[e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+            }
           }
         }
-      }
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kOwnF; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int c = 8 * i + 2 * q + ge;
-          *(f32x4*)(stg + l32e * 512 + ((c ^ (l32e & 15)) << 4)) = v[i][q];
-        }
+          const int n = fw + 32 * i + 8 * q + 4 * ge;
+          float* dst = (float*)o.y + (int64_t)mj * o.ldy + n;
+          if (mj < p.M) {
+            if (n + 4 <= p.N) {
+              *(f32x4u*)dst = v[i][q];
+            } else {
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const int r = 2 * k + (lane_e >> 5), c = lane_e & 31, n = fw + c * 4;
-        const f32x4 u = *(const f32x4*)(stg + r * 512 + ((c ^ (r & 15)) << 4));
-        float* dst = (float*)o.y + (int64_t)(mj + r) * o.ldy + n;
-        if (mj + r < p.M) {
-          if (n + 4 <= p.N) {
-            *(f32x4u*)dst = u;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < p.N) dst[e] = u[e];
+              for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) dst[e] = v[i][q][e];
+            }
           }
         }
+    }
+  }
+}
+
+// Few-token kernel, up to 16 tokens.  A block is 16 features and splits the
+// contraction over 4 waves, which read their operands from global memory
+// straight into the fragments of v_mfma_i32_16x16x64_i8 (each byte of w is
+// used once, so LDS would only add a stop), 4 chunks of 128 bytes a row in
+// flight.  The waves' sums are added in LDS.
+constexpr int kFewWaves = 4, kFewChunks = 4;
+__global__ __launch_bounds__(64 * kFewWaves) void few8_kernel(Prod8Params p) {
+  __shared__ i32x4 red[kFewWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l16 = lane & 15, g = lane >> 4;
+  const Prod8Out o = blockIdx.y == 0 ? p.out[0] : (blockIdx.y == 1 ? p.out[1] : p.out[2]);
+  const int n0 = (int)blockIdx.x * 16;
+  const int rows_w = min(16, p.N - n0);
+  const int k16 = (p.K + 15) & ~15;
+  // rows past the last feature or token, and chunks past K, read as zeros
+  const rsrc_t wr = make_rsrc(o.w + (int64_t)n0 * o.ldw, (uint32_t)((rows_w - 1) * o.ldw + k16));
+  const rsrc_t xr = make_rsrc(p.x, (uint32_t)((p.M - 1) * p.ldx + k16));
+  const uint32_t woff = l16 < rows_w ? (uint32_t)(l16 * o.ldw) : kOOB;
+  const uint32_t xoff = l16 < p.M ? (uint32_t)(l16 * p.ldx) : kOOB;
+
+  // the scales and bias of the result that this thread may finish come in
+  // with the first operands: token l16, features n0 + 4 g + e
+  float ws[4], bs[4], sx = 0.f;
+  if (wave == 0) {
+    sx = p.x_scale[min(l16, p.M - 1)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = min(n0 + 4 * g + e, p.N - 1);
+      ws[e] = o.w_scale[n];
+      bs[e] = o.bias ? vec_at(o.bias, o.bias_f32, n) : 0.f;
+    }
+  }
+
+  i32x4 acc = {0, 0, 0, 0};
+  const int chunks = (p.K + 127) / 128, part = p.K & 15;
+#pragma unroll 1
+  for (int c0 = wave; c0 < chunks; c0 += kFewWaves * kFewChunks) {
+    i32x4 a[kFewChunks][2], b[kFewChunks][2];
+#pragma unroll
+    for (int u = 0; u < kFewChunks; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int kk = (c0 + kFewWaves * u) * 128 + 64 * h + 16 * g;
+        a[u][h] = buffer_load16(wr, kk < p.K ? woff + kk : kOOB);
+        b[u][h] = buffer_load16(xr, kk < p.K ? xoff + kk : kOOB);
       }
+#pragma unroll
+    for (int u = 0; u < kFewChunks; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (part) {  // the chunk that ends inside 16 bytes: w's bytes past K count for nothing
+          const int left = p.K - ((c0 + kFewWaves * u) * 128 + 64 * h + 16 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[u][h][i] &= dword_mask(left, i);
+        }
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u][h], b[u][h], acc, 0, 0, 0);
+      }
+  }
+  red[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || l16 >= p.M) return;
+#pragma unroll
+  for (int w = 1; w < kFewWaves; ++w) acc += red[w][lane];
+  const int n = n0 + 4 * g;
+  f32x4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (float)acc[e] * sx * ws[e] + bs[e];
+  if (o.y_f32) {
+    float* dst = (float*)o.y + (int64_t)l16 * o.ldy + n;
+    if (n + 4 <= p.N) {
+      *(f32x4u*)dst = y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) dst[e] = y[e];
+    }
+  } else {
+    uint16_t* dst = (uint16_t*)o.y + (int64_t)l16 * o.ldy + n;
+    if (n + 4 <= p.N) {
+      *(u32x2u*)dst = u32x2{bf16_rne(y[0]) | (bf16_rne(y[1]) << 16), bf16_rne(y[2]) | (bf16_rne(y[3]) << 16)};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.N) dst[e] = (uint16_t)bf16_rne(y[e]);
     }
   }
 }
 
 namespace {
 
-template <int TPW, int GROUPS, int STAGES>
+// Compute units of the current device (cached per device).
+int device_cus() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (!cached[dev]) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess) cached[dev] = n;
+  }
+  return cached[dev] > 0 ? cached[dev] : 256;
+}
+
+template <int FB, int NJ, int TG, int GROUPS, int KG, int KT, int STAGES>
 hipError_t launch_tiles(const Prod8Params& p, bool norm, hipStream_t stream) {
-  constexpr int kTok = kTokenGroups * TPW, kFeatures = GROUPS * kFeat;
+  constexpr int kTok = TG * NJ * 32, kFeatures = GROUPS * FB * 32;
   const int64_t blocks = (int64_t)((p.M + kTok - 1) / kTok) * ((p.N + kFeatures - 1) / kFeatures);
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)blocks, (unsigned)p.n_outs), block(64 * kTokenGroups * GROUPS);
-  if (norm)
-    hipLaunchKernelGGL((prod8_kernel<TPW, GROUPS, STAGES, true>), grid, block, 0, stream, p);
-  else
-    hipLaunchKernelGGL((prod8_kernel<TPW, GROUPS, STAGES, false>), grid, block, 0, stream, p);
+  const dim3 grid((unsigned)blocks, (unsigned)p.n_outs), block(64 * TG * GROUPS * KG);
+  if constexpr (FB == 4)
+    if (norm) {
+      hipLaunchKernelGGL((prod8_kernel<FB, NJ, TG, GROUPS, KG, KT, STAGES, true>), grid, block, 0, stream, p);
+      return hipGetLastError();
+    }
+  if (norm) return hipErrorInvalidValue;  // a head needs four feature blocks
+  hipLaunchKernelGGL((prod8_kernel<FB, NJ, TG, GROUPS, KG, KT, STAGES, false>), grid, block, 0, stream, p);
   return hipGetLastError();
+}
+
+hipError_t launch_few(const Prod8Params& p, bool, hipStream_t stream) {
+  hipLaunchKernelGGL(few8_kernel, dim3((unsigned)((p.N + 15) / 16), (unsigned)p.n_outs), dim3(64 * kFewWaves), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+
+// The kinds of blocks and what they were measured to take (weights out of
+// HBM): one round of the CUs takes base + per_tile microseconds for each 128
+// bytes of K, a further round `more` and the tiles again.  At K = 3840: 32
+// features x 32 tokens 8 us, 64 x 64 13, 128 x 128 23, 256 x 256 50 a round,
+// and 8192 tokens x 10240 features (5 rounds of the largest) 290 us, where
+// the same in 128 x 128 takes 417 and in 64 x 64 634.
+struct Kind {
+  int tokens, features;
+  bool heads;        // takes a norm: whole heads
+  int max_tokens;    // of the call
+  double base, per_tile, more;
+  int per_cu;
+  hipError_t (*launch)(const Prod8Params&, bool, hipStream_t);
+};
+constexpr int kAny = 0x7fffffff;
+const Kind kKinds[] = {
+    {16, 16, false, 16, 3.4, 0.11, 0.0, 2, launch_few},
+    {32, 32, false, kAny, 3.6, 0.13, 0.0, 1, launch_tiles<1, 1, 1, 1, 4, 256, 4>},
+    {32, 64, false, kAny, 4.0, 0.21, 0.0, 1, launch_tiles<2, 1, 1, 1, 2, 256, 4>},
+    {64, 64, false, kAny, 4.0, 0.28, 0.0, 1, launch_tiles<2, 2, 1, 1, 4, 256, 3>},
+    {32, 128, true, kAny, 5.0, 0.34, 0.0, 1, launch_tiles<4, 1, 1, 1, 4, 256, 3>},
+    {64, 128, true, kAny, 5.5, 0.40, 1.0, 1, launch_tiles<4, 2, 1, 1, 4, 256, 3>},
+    {128, 128, true, kAny, 6.0, 0.56, 4.0, 1, launch_tiles<4, 1, 4, 1, 1, 128, 4>},
+    {128, 256, true, kAny, 7.5, 0.83, 9.0, 1, launch_tiles<4, 1, 4, 2, 1, 128, 3>},
+    {256, 256, true, kAny, 11.0, 1.35, 15.0, 1, launch_tiles<4, 2, 4, 2, 1, 128, 2>},
+};
+
+double kind_us(const Kind& k, const Prod8Params& p, int64_t rows, int cus) {
+  const int64_t blocks = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features) * ((rows + k.tokens - 1) / k.tokens);
+  const int64_t slots = (int64_t)cus * k.per_cu;
+  const double rounds = (double)((blocks + slots - 1) / slots), tiles = (double)((p.K + kKTile8 - 1) / kKTile8);
+  return k.base + rounds * k.per_tile * tiles + (rounds - 1) * k.more;
+}
+
+const Kind* best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, double* us) {
+  const Kind* best = nullptr;
+  for (const Kind& k : kKinds) {
+    if ((norm && !k.heads) || rows > k.max_tokens) continue;
+    const double t = kind_us(k, p, rows, cus);
+    if (!best || t < *us) {
+      best = &k;
+      *us = t;
+    }
+  }
+  return best;
 }
 
 }  // namespace
 
-hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
+// The kind with the smallest time for the call; where a kind's last round
+// would be part full, its whole rounds may run as one launch and the rows left
+// as another of a smaller kind (2 us between the two).
+hipError_t launch_prod8(const Prod8Params& p_in, hipStream_t stream) {
+  Prod8Params p = p_in;
   bool norm = false;
   for (int i = 0; i < p.n_outs; ++i) norm |= p.out[i].norm_w != nullptr;
-  return launch_tiles<64, 2, 2>(p, norm, stream);
+  const int cus = device_cus();
+  double us = 0;
+  const Kind* kind = best_kind(p, norm, p.M, cus, &us);
+  const Kind *first = nullptr, *rest = nullptr;
+  int rows1 = 0;
+  for (const Kind& k : kKinds) {
+    if ((norm && !k.heads) || k.max_tokens != kAny) continue;
+    const int64_t per_row_tile = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features);
+    const int64_t slots = (int64_t)cus * k.per_cu;
+    const int64_t blocks = per_row_tile * ((p.M + k.tokens - 1) / k.tokens);
+    const int64_t rows = blocks / slots * slots / per_row_tile * k.tokens;
+    if (rows < 1 || rows >= p.M) continue;
+    double t2 = 0;
+    const Kind* r = best_kind(p, norm, p.M - rows, cus, &t2);
+    const double t = kind_us(k, p, rows, cus) + 2.0 + t2;
+    if (t < us) {
+      us = t;
+      first = &k;
+      rest = r;
+      rows1 = (int)rows;
+    }
+  }
+  if (!first) return kind->launch(p, norm, stream);
+  Prod8Params a = p;
+  a.M = rows1;
+  const hipError_t e = first->launch(a, norm, stream);
+  if (e != hipSuccess) return e;
+  p.M -= rows1;
+  p.m_base += rows1;
+  p.x += (int64_t)rows1 * p.ldx;
+  p.x_scale += rows1;
+  for (int i = 0; i < p.n_outs; ++i)
+    p.out[i].y = (char*)p.out[i].y + (int64_t)rows1 * p.out[i].ldy * (p.out[i].y_f32 ? 4 : 2);
+  return rest->launch(p, norm, stream);
 }
 
 }  // namespace harp_blk
