@@ -35,7 +35,7 @@ from .ops import (  # noqa: F401
     ring_attention,
 )
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn  # noqa: F401
-from .residual_norm import AddRMSNormFn, add_rms_norm, add_rms_norm_int8  # noqa: F401
+from .residual_norm import add_rms_norm, add_rms_norm_int8  # noqa: F401
 from .int8 import Int8Linear, Int8Rows, int8_linear, quantize_attention, quantize_int8  # noqa: F401
 from .attention import RingZAttention, project_qkv  # noqa: F401
 from .wait_engine import CommWork, WaitEngine  # noqa: F401

@@ -1,13 +1,14 @@
 // kernels/libharp_block_ops.so — PyTorch-ROCm operators of the kernels around
 // the attention block (include/harp_block_ops.h), namespace harp_block:
-//   add_rms_norm_forward, add_rms_norm_backward     residual addition + RMSNorm
+//   add_rms_norm                                    residual addition + RMSNorm
+//   add_rms_norm_forward, add_rms_norm_backward     its two directions
 //   add_rms_norm_int8, quantize_int8, dequantize_int8
 //   linear_int8, qkv_int8                           products of 8-bit rows
 // The operators allocate their results from PyTorch's allocator and run on
 // the current HIP stream of the input's device.  Implementations are
 // registered for the CUDA dispatch key (HIP tensors carry it); the CPU key
-// raises.  None records a gradient: harp_amd.AddRMSNormFn is the
-// differentiable form of the norm, the 8-bit operators are forward only.
+// raises.  add_rms_norm is differentiable (once); the others record no
+// gradient.
 //
 // Matrices are [.., C] tensors read as rows of C elements.  A tensor whose
 // leading dimensions are no single row stride, or whose last stride is not 1,
@@ -16,6 +17,8 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -168,6 +171,84 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_backward(const at::T
                                      want_weight ? ws.data_ptr() : nullptr, wsb, stream_of(dy)),
       "add_rms_norm_backward");
   return {dx, dres, gw};
+}
+
+// (y, h) without a gradient; h is x without a residual
+std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const OptTensor& residual,
+                                                const OptTensor& weight, double eps) {
+  auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, false);
+  return {y, given(residual) ? h : x.alias()};
+}
+
+// The differentiable form: y, and h where there is a residual.
+class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                const OptTensor& residual, const OptTensor& weight, double eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, true);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["x_dtype"] = x.scalar_type();
+    ctx->saved_data["need"] = std::vector<bool>{x.requires_grad(), given(residual) && residual->requires_grad(),
+                                                given(weight) && weight->requires_grad()};
+    const at::Tensor w = given(weight) ? *weight : at::Tensor();
+    if (!given(residual)) {
+      ctx->save_for_backward({x, w, rstd});
+      return {y};
+    }
+    ctx->save_for_backward({h, w, rstd});
+    return {y, h};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto x_dtype = ctx->saved_data["x_dtype"].toScalarType();
+    const auto need = ctx->saved_data["need"].toBoolList();
+    const at::Tensor &h = saved[0], &w = saved[1], &rstd = saved[2], &dy = grads[0];
+    const at::Tensor dh = grads.size() > 1 ? grads[1] : at::Tensor();
+    torch::autograd::variable_list out(4);
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      if (dy.defined()) {
+        auto [dx, dres, gw] = add_rms_norm_backward(dy, dh, h, w, rstd, need[1], need[2]);
+        if (need[0]) out[0] = dx;
+        if (need[1]) out[1] = dres.numel() || dx.numel() == 0 ? dres.reshape(dx.sizes()) : dx;  // equal where the types are
+        if (need[2]) out[2] = gw;
+      } else if (dh.defined()) {  // y took no part: the addition alone
+        if (need[0]) out[0] = dh.to(x_dtype);
+        if (need[1]) out[1] = dh;
+      }
+    }
+    if (at::GradMode::is_enabled()) {  // create_graph: a gradient of these gradients raises
+      torch::autograd::variable_list given_out;
+      for (auto& t : out)
+        if (t.defined()) given_out.push_back(t.detach().requires_grad_());
+      if (!given_out.empty()) {
+        auto error = std::make_shared<torch::autograd::DelayedError>("add_rms_norm is differentiable once only",
+                                                                    given_out.size());
+        given_out = (*error)(std::move(given_out));
+        size_t i = 0;
+        for (auto& t : out)
+          if (t.defined()) t = given_out[i++];
+      }
+    }
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, const OptTensor& residual,
+                                                         const OptTensor& weight, double eps) {
+  const bool record = at::GradMode::is_enabled() &&
+                      (x.requires_grad() || (given(residual) && residual->requires_grad()) ||
+                       (given(weight) && weight->requires_grad()));
+  if (!record) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, false);
+    return {y, given(residual) ? h : x};
+  }
+  auto out = AddRMSNorm::apply(x, residual, weight, eps);
+  return {out[0], given(residual) ? out[1] : x};
 }
 
 // int8 values of shape `sizes` whose rows are padded to 16 bytes
@@ -359,6 +440,9 @@ std::vector<at::Tensor> qkv_int8(const at::Tensor& x, const at::Tensor& x_scales
 [[noreturn]] void no_cpu(const char* op) {
   TORCH_CHECK(false, "harp_block.", op, ": this library runs on a HIP device only (CPU tensors given)");
 }
+std::tuple<at::Tensor, at::Tensor> add_rms_norm_cpu(const at::Tensor&, const OptTensor&, const OptTensor&, double) {
+  no_cpu("add_rms_norm");
+}
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_forward_cpu(const at::Tensor&, const OptTensor&,
                                                                         const OptTensor&, double, bool) {
   no_cpu("add_rms_norm_forward");
@@ -387,6 +471,7 @@ std::vector<at::Tensor> qkv_int8_cpu(const at::Tensor&, const at::Tensor&, const
 }  // namespace
 
 TORCH_LIBRARY(harp_block, m) {
+  m.def("add_rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps) -> (Tensor, Tensor)");
   m.def(
       "add_rms_norm_forward(Tensor x, Tensor? residual, Tensor? weight, float eps, bool keep) -> (Tensor, Tensor, "
       "Tensor)");
@@ -404,7 +489,10 @@ TORCH_LIBRARY(harp_block, m) {
       "eps, Tensor? freqs_cis) -> Tensor[]");
 }
 
+TORCH_LIBRARY_IMPL(harp_block, AutogradCUDA, m) { m.impl("add_rms_norm", &add_rms_norm_autograd); }
+
 TORCH_LIBRARY_IMPL(harp_block, CUDA, m) {
+  m.impl("add_rms_norm", &add_rms_norm);
   m.impl("add_rms_norm_forward", &add_rms_norm_forward);
   m.impl("add_rms_norm_backward", &add_rms_norm_backward);
   m.impl("add_rms_norm_int8", &add_rms_norm_int8);
@@ -415,6 +503,7 @@ TORCH_LIBRARY_IMPL(harp_block, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(harp_block, CPU, m) {
+  m.impl("add_rms_norm", &add_rms_norm_cpu);
   m.impl("add_rms_norm_forward", &add_rms_norm_forward_cpu);
   m.impl("add_rms_norm_backward", &add_rms_norm_backward_cpu);
   m.impl("add_rms_norm_int8", &add_rms_norm_int8_cpu);

@@ -35,9 +35,16 @@ from . import _lib
 HEAD_DIM = 128
 
 
+_harp_block = None
+
+
 def _ops():
-    _lib.load_block_ops()
-    return torch.ops.harp_block
+    """torch.ops.harp_block, its library loaded at the first call."""
+    global _harp_block
+    if _harp_block is None:
+        _lib.load_block_ops()
+        _harp_block = torch.ops.harp_block
+    return _harp_block
 
 
 def _refuse_grad(what: str, *tensors: Optional[torch.Tensor]) -> None:

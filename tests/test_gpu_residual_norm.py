@@ -319,3 +319,21 @@ def test_outputs_next_to_others_are_left_alone():
     assert rc == 0
     assert torch.equal(q[:rows, :cols], harp_amd.quantize_int8(x).values)
     assert bool((q[:rows, cols:80] == 0).all()) and bool((q[:rows, 80:] == 9).all()) and bool((q[rows:] == 9).all())
+
+
+def test_differentiable_once():
+    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+    y, _ = harp_amd.add_rms_norm(x)
+    (gx,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        gx.sum().backward()
+
+
+def test_saved_tensors_are_guarded():
+    """h is kept for the backward: changing it in place raises there."""
+    x = torch.randn(3, 64, device=DEV, requires_grad=True)
+    y, h = harp_amd.add_rms_norm(x, torch.zeros(3, 64, device=DEV))
+    with torch.no_grad():
+        h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
