@@ -3,7 +3,7 @@
 //   add_rms_norm                                    residual addition + RMSNorm
 //   add_rms_norm_forward, add_rms_norm_backward     its two directions
 //   add_rms_norm_int8, quantize_int8, dequantize_int8
-//   linear_int8, qkv_int8                           products of 8-bit rows
+//   linear_int8, linear_int8_dynamic, qkv_int8      products of 8-bit rows
 // The operators allocate their results from PyTorch's allocator and run on
 // the current HIP stream of the input's device.  Implementations are
 // registered for the CUDA dispatch key (HIP tensors carry it); the CPU key
@@ -16,9 +16,11 @@
 // here, whose storage pads each row to 16 bytes.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <tuple>
@@ -237,6 +239,20 @@ class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
   }
 };
 
+// While a graph of an earlier call is alive, a leaf keeps the accumulator node
+// of that graph, with the stream it was made on.  A backward captured on
+// another stream would have the engine wait across the two streams inside the
+// capture, which ends the process: such a call is refused while it can be.
+void check_capture(const OptTensor& t, const c10::Stream& current, const char* name) {
+  if (!given(t) || !t->requires_grad() || t->grad_fn()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+  if (!node) return;
+  const auto made_on = node->stream();
+  TORCH_CHECK(!made_on || *made_on == current, "add_rms_norm: ", name,
+              " belongs to a live autograd graph of another stream, so its gradient cannot be captured: delete that "
+              "graph's tensors (an earlier step's outputs or loss) before the capture");
+}
+
 std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, const OptTensor& residual,
                                                          const OptTensor& weight, double eps) {
   const bool record = at::GradMode::is_enabled() &&
@@ -246,6 +262,12 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, co
     at::AutoDispatchBelowADInplaceOrView guard;
     auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, false);
     return {y, given(residual) ? h : x};
+  }
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+    const c10::Stream current = c10::hip::getCurrentHIPStream(x.get_device()).unwrap();
+    check_capture(x, current, "x");
+    check_capture(residual, current, "residual");
+    check_capture(weight, current, "weight");
   }
   auto out = AddRMSNorm::apply(x, residual, weight, eps);
   return {out[0], given(residual) ? out[1] : x};
@@ -350,11 +372,13 @@ at::Tensor dequantize_int8(const at::Tensor& values, const at::Tensor& scales, a
   return out;
 }
 
+// 8-bit rows x times the first x.size(-1) columns of weight (a module's
+// padded storage, or rows of exactly that many)
 at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
                        const at::Tensor& weight_scales, const OptTensor& bias, at::ScalarType dtype) {
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "linear_int8: bfloat16 or float32, got ", dtype);
   const Rows8 xr = rows8_of(x, x_scales, "x");
-  TORCH_CHECK(weight.dim() == 2 && weight.size(1) == xr.cols && weight.device() == x.device(),
+  TORCH_CHECK(weight.dim() == 2 && weight.size(1) >= xr.cols && weight.device() == x.device(),
               "weight must be [N, ", xr.cols, "] on ", x.device(), ", got ", weight.sizes(), " on ", weight.device());
   const Rows8 wr = rows8_of(weight, weight_scales, "weight");
   const c10::DeviceGuard guard(x.device());
@@ -367,6 +391,13 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at
                                       wr.rows, code(dtype), (int)xr.rows, (int)wr.rows, (int)xr.cols, stream_of(x)),
                  "linear_int8");
   return y;
+}
+
+// the same of a bf16 or fp32 tensor, quantised first
+at::Tensor linear_int8_dynamic(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scales,
+                               const OptTensor& bias, at::ScalarType dtype) {
+  const auto [q, scales] = quantize_int8(x);
+  return linear_int8(q, scales, weight, weight_scales, bias, dtype);
 }
 
 // fp32 (cos, sin) rows of the complex [S, 64] or [B or 1, S, 64] table
@@ -462,6 +493,10 @@ at::Tensor linear_int8_cpu(const at::Tensor&, const at::Tensor&, const at::Tenso
                            const OptTensor&, at::ScalarType) {
   no_cpu("linear_int8");
 }
+at::Tensor linear_int8_dynamic_cpu(const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
+                                   at::ScalarType) {
+  no_cpu("linear_int8_dynamic");
+}
 std::vector<at::Tensor> qkv_int8_cpu(const at::Tensor&, const at::Tensor&, const std::vector<at::Tensor>&,
                                      const std::vector<at::Tensor>&, const c10::List<OptTensor>&,
                                      const std::vector<double>&, const OptTensor&) {
@@ -485,6 +520,8 @@ TORCH_LIBRARY(harp_block, m) {
       "linear_int8(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype) -> "
       "Tensor");
   m.def(
+      "linear_int8_dynamic(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype) -> Tensor");
+  m.def(
       "qkv_int8(Tensor x, Tensor x_scales, Tensor[] weights, Tensor[] weight_scales, Tensor?[] norm_weights, float[] "
       "eps, Tensor? freqs_cis) -> Tensor[]");
 }
@@ -499,6 +536,7 @@ TORCH_LIBRARY_IMPL(harp_block, CUDA, m) {
   m.impl("quantize_int8", &quantize_int8);
   m.impl("dequantize_int8", &dequantize_int8);
   m.impl("linear_int8", &linear_int8);
+  m.impl("linear_int8_dynamic", &linear_int8_dynamic);
   m.impl("qkv_int8", &qkv_int8);
 }
 
@@ -510,5 +548,6 @@ TORCH_LIBRARY_IMPL(harp_block, CPU, m) {
   m.impl("quantize_int8", &quantize_int8_cpu);
   m.impl("dequantize_int8", &dequantize_int8_cpu);
   m.impl("linear_int8", &linear_int8_cpu);
+  m.impl("linear_int8_dynamic", &linear_int8_dynamic_cpu);
   m.impl("qkv_int8", &qkv_int8_cpu);
 }

@@ -78,6 +78,8 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
     """x [.., K] times the transpose of weight [N, K], plus bias [N]: a
     bfloat16 or float32 tensor [.., N].  K up to 65536."""
     _refuse_grad("int8_linear", bias)
+    if weight.values.size(-1) != x.values.size(-1):
+        raise RuntimeError(f"weight must be [N, {x.values.size(-1)}], got {tuple(weight.values.shape)}")
     return _ops().linear_int8(x.values, x.scales, weight.values, weight.scales, bias, out_dtype)
 
 
@@ -126,8 +128,16 @@ class Int8Linear(nn.Module):
         return Int8Rows(self.weight_values[:, :self.in_features], self.weight_scales)
 
     def forward(self, x: Union[torch.Tensor, Int8Rows]) -> torch.Tensor:
-        rows = x if isinstance(x, Int8Rows) else quantize_int8(x)
-        return int8_linear(rows, self.weight, self.bias, self.out_dtype)
+        rows = isinstance(x, Int8Rows)
+        features = (x.values if rows else x).size(-1)
+        if features != self.in_features:
+            raise RuntimeError(f"Int8Linear of {self.in_features} features got rows of {features}")
+        # the operators read the weight's first in_features columns
+        if rows:
+            return _ops().linear_int8(x.values, x.scales, self.weight_values, self.weight_scales, self.bias,
+                                      self.out_dtype)
+        _refuse_grad("Int8Linear", x)
+        return _ops().linear_int8_dynamic(x, self.weight_values, self.weight_scales, self.bias, self.out_dtype)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
