@@ -96,6 +96,135 @@ __device__ __forceinline__ void swap_halves(uint32_t& x, uint32_t& y) {
   y = r[1];
 }
 
+// Chunks q and q + 1 (features 8 q .. 8 q + 15) of a lane's token: each half
+// of the wave holds 4 of a chunk's 8 features; they exchange, and lane half 0
+// has chunk q, half 1 chunk q + 1, as bf16.
+__device__ __forceinline__ u32x4 pack_chunks(const f32x4& a, const f32x4& b) {
+  uint32_t u[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u[h] = bf16_rne(a[2 * h]) | (bf16_rne(a[2 * h + 1]) << 16);
+    u[2 + h] = bf16_rne(b[2 * h]) | (bf16_rne(b[2 * h + 1]) << 16);
+  }
+  swap_halves(u[0], u[2]);
+  swap_halves(u[1], u[3]);
+  return u32x4{u[0], u[1], u[2], u[3]};
+}
+
+// The end of a token block: sums of OF feature blocks for this lane's token mj
+// (features fw + 32 i + 8 q + 4 ge + e, e < 4) become results and are stored.
+// wsc, wb: the scales, and bias or norm weight, from feature fw on; a norm's
+// results are bf16.
+template <int OF, bool NORM, class Combine>
+__device__ __forceinline__ void finish_tokens(const Prod8Params& p, const Prod8Out& o, const i32x16 (&own)[OF],
+                                              float sx, const float* wsc, const float* wb, int d_own, int fw, int mj,
+                                              int ge, Combine combine) {
+  const bool norm = NORM && o.norm_w != nullptr, rope = norm && p.freqs != nullptr;
+  f32x4 v[OF][4];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < OF; ++i) {
+    sched_fence();  // (one feature block's scales at a time: all would not fit beside the sums)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 ws = *(const f32x4*)(wsc + 32 * i + 8 * q + 4 * ge);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[i][q][e] = (float)own[i][4 * q + e] * sx * ws[e];
+        if (NORM) ss = __builtin_fmaf(v[i][q][e], v[i][q][e], ss);
+      }
+      if (!NORM) {
+        const f32x4 b = *(const f32x4*)(wb + 32 * i + 8 * q + 4 * ge);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[i][q][e] += b[e];
+      }
+      // (opaque, or the arithmetic would sink to the stores, behind their bounds tests, and its operands stay)
+      if (!NORM) asm volatile("" : "+v"(v[i][q]));
+    }
+  }
+  sched_fence();
+  if (NORM && norm) {
+    ss = combine(harp_ra::wave_half_sum(ss));  // this lane's features of the token and its partner lane's; all the head's
+    const float rho = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)kFeat) + o.eps));
+    const int mt = min(mj, p.M - 1) + p.m_base;  // the token among the call's
+    const float* fr = p.freqs + (int64_t)(mt / p.S) * p.f_stride_b + (int64_t)(mt % p.S) * p.f_stride_s + d_own + 4 * ge;
+    constexpr int kPart = OF > 1 ? 2 : 1;  // feature blocks whose row of the table is loaded at once
+#pragma unroll
+    for (int i0 = 0; i0 < OF; i0 += kPart) {
+      f32x4 fq[kPart][4];
+      if (rope) {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) fq[i][q] = *(const f32x4*)(fr + 32 * (i0 + i) + 8 * q);
+      }
+#pragma unroll
+      for (int i = i0; i < i0 + kPart; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 w = *(const f32x4*)(wb + 32 * i + 8 * q + 4 * ge);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i][q][e] = v[i][q][e] * rho * w[e];
+        }
+      if (rope) {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const f32x4 f = fq[i][q];
+              const float a = v[i0 + i][q][e], b = v[i0 + i][q][e + 1];
+              v[i0 + i][q][e] = __builtin_fmaf(-b, f[e + 1], a * f[e]);
+              v[i0 + i][q][e + 1] = __builtin_fmaf(a, f[e + 1], b * f[e]);
+            }
+      }
+    }
+  }
+  // stores: 16 bytes per lane, 32 in a row of y.  (The lane's half is opaque
+  // at each guarded store, or every store's bounds tests would be formed ahead
+  // and kept in SGPRs.)
+  int gs = ge;
+  if (NORM || !o.y_f32) {
+#pragma unroll
+    for (int i = 0; i < OF; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        const u32x4 w = pack_chunks(v[i][q], v[i][q + 1]);
+        asm volatile("" : "+v"(gs));
+        const int n = fw + 32 * i + 8 * (q + gs);
+        uint16_t* dst = (uint16_t*)o.y + (int64_t)mj * o.ldy + n;
+        if (mj < p.M) {
+          if (n + 8 <= p.N) {
+            *(u32x4u*)dst = w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < p.N) dst[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+  } else {
+#pragma unroll
+    for (int i = 0; i < OF; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        asm volatile("" : "+v"(gs));
+        const int n = fw + 32 * i + 8 * q + 4 * gs;
+        float* dst = (float*)o.y + (int64_t)mj * o.ldy + n;
+        if (mj < p.M) {
+          if (n + 4 <= p.N) {
+            *(f32x4u*)dst = v[i][q];
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < p.N) dst[e] = v[i][q][e];
+          }
+        }
+      }
+  }
+}
+
 }  // namespace
 
 // Tile kernel.  C^T = W x^T, so a lane holds one token and 16 features per
@@ -129,13 +258,13 @@ __global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Pa
   // is one for each (a head stays in one wave), else feature blocks of one
   // (with fewer blocks than waves, the last waves have none)
   constexpr int kOwnJ = NJ % KG == 0 ? NJ / KG : 1, kOwnF = FB * NJ >= KG ? FB * NJ / KG / kOwnJ : 1;
-  constexpr int kParts = FB / kOwnF;  // waves that finish a token block between them
   static_assert((kOwnJ * kOwnF * KG == FB * NJ || FB * NJ < KG) && FB % kOwnF == 0, "equal shares");
-  static_assert(!NORM || (FB == 4 && (kParts == 1 || GROUPS == 1)), "a head in one wave, or in the waves of one sum");
+  constexpr int kParts = kFeat / 32 / kOwnF;  // waves that finish a head's token block between them (norm)
+  static_assert(!NORM || kFeatures % kFeat == 0, "whole heads");
   static_assert(KG == 1 || kWaves * FB * NJ * 4096 <= kRing, "the sums fit the stages");
   __shared__ __attribute__((aligned(16))) char lds[kRing];
   __shared__ float wsc[kFeatures], wbias[kFeatures];  // feature scales; bias, or the norm's weight
-  __shared__ float part_ss[NORM && kParts > 1 ? KG : 1][32];
+  __shared__ float part_ss[NORM ? kParts : 1][NORM ? kFeatures / kFeat : 1][NORM ? kTok : 1];
   auto Xs = [&](int s) { return lds + s * kXBytes; };
   auto Ws = [&](int s) { return lds + STAGES * kXBytes + s * kWBytes; };
 
@@ -254,6 +383,12 @@ __global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Pa
     }
   }
   static_assert(kThreads >= kFeatures, "a thread per feature");
+  // what the wave finishes (see the epilogue), and its tokens' scales
+  const int i_own = kOwnF == FB ? 0 : kg / NJ * kOwnF, j_own = kOwnF == FB ? kg * kOwnJ : kg % NJ;
+  const int f_own = hh * kWaveFeat + 32 * i_own, m_own = m0 + TPW * tg + 32 * j_own;
+  float sx[kOwnJ];
+#pragma unroll
+  for (int j = 0; j < kOwnJ; ++j) sx[j] = p.x_scale[min(m_own + 32 * j + l32, p.M - 1)];
 
 #pragma unroll
   for (int t = 0; t < STAGES; ++t) {
@@ -313,7 +448,6 @@ __global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Pa
 
   // the KG waves of a sum put theirs into LDS, and each adds up its share
   i32x16 own[kOwnF][kOwnJ];
-  const int i_own = kOwnF == FB ? 0 : kg / NJ * kOwnF, j_own = kOwnF == FB ? kg * kOwnJ : kg % NJ;
   if constexpr (KG > 1) {
     i32x4* const sums = (i32x4*)lds + lane;  // [wave][FB][NJ][4] x 64 lanes
 #pragma unroll
@@ -347,119 +481,27 @@ __global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Pa
 
   // ---- epilogue: this lane holds tokens m_own + 32 j + l32 and features
   // f_own + 32 i + 8 q + 4 g + e of the block's, e < 4
-  const int f_own = hh * kWaveFeat + 32 * i_own, m_own = m0 + TPW * tg + 32 * j_own;
   const int fw = n0 + f_own;
-  if (fw >= p.N || (FB * NJ < KG && kg >= FB * NJ)) return;  // (a norm's N has whole heads: no wave of one leaves)
+  // (with a norm every wave stays for the exchange; those past the last head store nothing)
+  if ((!NORM && fw >= p.N) || (FB * NJ < KG && kg >= FB * NJ)) return;
   const int lane_e = harp_ra::lane_id_fresh(), l32e = lane_e & 31, ge = lane_e >> 5;
-  const bool norm = NORM && o.norm_w != nullptr;
-  const bool rope = norm && p.freqs != nullptr;
-
 #pragma unroll
   for (int j = 0; j < kOwnJ; ++j) {
-    const int mj = m_own + 32 * j + l32e;  // the lane's token
-    const int m = min(mj, p.M - 1);
-    const float sx = p.x_scale[m];
-    f32x4 v[kOwnF][4];
-    float ss = 0.f;
+    i32x16 col[kOwnF];
 #pragma unroll
-    for (int i = 0; i < kOwnF; ++i)
+    for (int i = 0; i < kOwnF; ++i) col[i] = own[i][j];
+    finish_tokens<kOwnF, NORM>(p, o, col, sx[j], wsc + f_own, wbias + f_own, f_own % kFeat, fw, m_own + 32 * j + l32e,
+                               ge, [&](float ss) {
+                                 if constexpr (NORM && kParts > 1) {
+                                   const int t = m_own - m0 + 32 * j + l32e, h = f_own / kFeat;
+                                   part_ss[f_own % kFeat / (32 * kOwnF)][h][t] = ss;
+                                   __syncthreads();
+                                   ss = 0.f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int d0 = f_own + 32 * i + 8 * q + 4 * ge;
-        const f32x4 ws = *(const f32x4*)(wsc + d0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[i][q][e] = (float)own[i][j][4 * q + e] * sx * ws[e];
-          if (NORM) ss = __builtin_fmaf(v[i][q][e], v[i][q][e], ss);
-        }
-        if (!NORM) {
-          const f32x4 b = *(const f32x4*)(wbias + d0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[i][q][e] += b[e];
-        }
-      }
-    if (NORM && norm) {
-      ss = harp_ra::wave_half_sum(ss);  // this lane's features of the token and its partner lane's
-      if constexpr (kParts > 1) {
-        static_assert(kOwnJ == 1, "one exchange");
-        // the waves of the token block: kg = part * NJ + token block
-        part_ss[kg][l32e] = ss;
-        __syncthreads();
-        ss = 0.f;
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) ss += part_ss[k * NJ + kg % NJ][l32e];
-      }
-      const float rho = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)kFeat) + o.eps));
-      const int mt_all = m + p.m_base;  // the token among the call's
-      const float* fr =
-          rope ? p.freqs + (int64_t)(mt_all / p.S) * p.f_stride_b + (int64_t)(mt_all % p.S) * p.f_stride_s : nullptr;
-#pragma unroll
-      for (int i = 0; i < kOwnF; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int d0 = 32 * (i_own + i) + 8 * q + 4 * ge;
-          const f32x4 w = *(const f32x4*)(wbias + hh * kWaveFeat + d0);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[i][q][e] = v[i][q][e] * rho * w[e];
-          if (rope) {
-            const f32x4 f = *(const f32x4*)(fr + d0);
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const float a = v[i][q][e], b = v[i][q][e + 1];
-              v[i][q][e] = __builtin_fmaf(-b, f[e + 1], a * f[e]);
-              v[i][q][e + 1] = __builtin_fmaf(a, f[e + 1], b * f[e]);
-            }
-          }
-        }
-    }
-    // stores: 16 bytes per lane, 32 in a row of y.  bf16: the halves of the
-    // wave hold 4 of a chunk's 8 features each; they exchange two chunks so
-    // that each half has one whole.
-    if (NORM || !o.y_f32) {
-#pragma unroll
-      for (int i = 0; i < kOwnF; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          u32x4 u;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            u[h] = bf16_rne(v[i][q][2 * h]) | (bf16_rne(v[i][q][2 * h + 1]) << 16);
-            u[2 + h] = bf16_rne(v[i][q + 1][2 * h]) | (bf16_rne(v[i][q + 1][2 * h + 1]) << 16);
-          }
-          uint32_t x0 = u[0], x1 = u[1], y0 = u[2], y1 = u[3];
-          swap_halves(x0, y0);
-          swap_halves(x1, y1);
-          u = u32x4{x0, x1, y0, y1};
-          const int n = fw + 32 * i + 8 * (q + ge);
-          uint16_t* dst = (uint16_t*)o.y + (int64_t)mj * o.ldy + n;
-          if (mj < p.M) {
-            if (n + 8 <= p.N) {
-              *(u32x4u*)dst = u;
-            } else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (n + e < p.N) dst[e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
-            }
-          }
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kOwnF; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = fw + 32 * i + 8 * q + 4 * ge;
-          float* dst = (float*)o.y + (int64_t)mj * o.ldy + n;
-          if (mj < p.M) {
-            if (n + 4 <= p.N) {
-              *(f32x4u*)dst = v[i][q];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (n + e < p.N) dst[e] = v[i][q][e];
-            }
-          }
-        }
-    }
+                                   for (int k = 0; k < kParts; ++k) ss += part_ss[k][h][t];
+                                 }
+                                 return ss;
+                               });
   }
 }
 
@@ -572,14 +614,25 @@ hipError_t launch_tiles(const Prod8Params& p, bool norm, hipStream_t stream) {
   const int64_t blocks = (int64_t)((p.M + kTok - 1) / kTok) * ((p.N + kFeatures - 1) / kFeatures);
   if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks, (unsigned)p.n_outs), block(64 * TG * GROUPS * KG);
-  if constexpr (FB == 4)
+  if constexpr (kFeatures % kFeat == 0)
     if (norm) {
       hipLaunchKernelGGL((prod8_kernel<FB, NJ, TG, GROUPS, KG, KT, STAGES, true>), grid, block, 0, stream, p);
       return hipGetLastError();
     }
-  if (norm) return hipErrorInvalidValue;  // a head needs four feature blocks
+  if (norm) return hipErrorInvalidValue;  // blocks without whole heads
   hipLaunchKernelGGL((prod8_kernel<FB, NJ, TG, GROUPS, KG, KT, STAGES, false>), grid, block, 0, stream, p);
   return hipGetLastError();
+}
+
+// p without its first `rows` tokens
+Prod8Params rows_from(Prod8Params p, int rows) {
+  p.M -= rows;
+  p.m_base += rows;
+  p.x += (int64_t)rows * p.ldx;
+  p.x_scale += rows;
+  for (int i = 0; i < p.n_outs; ++i)
+    p.out[i].y = (char*)p.out[i].y + (int64_t)rows * p.out[i].ldy * (p.out[i].y_f32 ? 4 : 2);
+  return p;
 }
 
 hipError_t launch_few(const Prod8Params& p, bool, hipStream_t stream) {
@@ -591,9 +644,14 @@ hipError_t launch_few(const Prod8Params& p, bool, hipStream_t stream) {
 // The kinds of blocks and what they were measured to take (weights out of
 // HBM): one round of the CUs takes base + per_tile microseconds for each 128
 // bytes of K, a further round `more` and the tiles again.  At K = 3840: 32
-// features x 32 tokens 8 us, 64 x 64 13, 128 x 128 23, 256 x 256 50 a round,
-// and 8192 tokens x 10240 features (5 rounds of the largest) 290 us, where
-// the same in 128 x 128 takes 417 and in 64 x 64 634.
+// tokens x 32 features 8 us, 64 x 64 13, 128 x 128 22, 256 x 256 50 a round;
+// 8192 tokens x 10240 features (5 rounds of the largest) take 290 us, in 128 x
+// 128 blocks 384 and in 64 x 64 519.  What bounds them: the small ones the
+// latency of a block's start, first bytes and end (their `base`), then 64
+// bytes per clock and CU into the LDS; the large ones the board's power (the
+// 256 x 256 blocks keep the matrix pipes 57% busy at 1.85 of 2.4 GHz; the
+// copies into LDS cost a fifth of the rate, LDS reads 6%, the stores of the
+// results, whether or not anything runs beside them, a tenth).
 struct Kind {
   int tokens, features;
   bool heads;        // takes a norm: whole heads
@@ -605,20 +663,21 @@ struct Kind {
 constexpr int kAny = 0x7fffffff;
 const Kind kKinds[] = {
     {16, 16, false, 16, 3.4, 0.11, 0.0, 2, launch_few},
-    {32, 32, false, kAny, 3.6, 0.13, 0.0, 1, launch_tiles<1, 1, 1, 1, 4, 256, 4>},
+    {32, 32, false, kAny, 3.6, 0.15, 0.0, 2, launch_tiles<1, 1, 1, 1, 4, 256, 4>},
     {32, 64, false, kAny, 4.0, 0.21, 0.0, 1, launch_tiles<2, 1, 1, 1, 2, 256, 4>},
-    {64, 64, false, kAny, 4.0, 0.28, 0.0, 1, launch_tiles<2, 2, 1, 1, 4, 256, 3>},
+    {64, 64, false, kAny, 4.0, 0.30, 0.0, 2, launch_tiles<2, 2, 1, 1, 4, 128, 4>},
     {32, 128, true, kAny, 5.0, 0.34, 0.0, 1, launch_tiles<4, 1, 1, 1, 4, 256, 3>},
     {64, 128, true, kAny, 5.5, 0.40, 1.0, 1, launch_tiles<4, 2, 1, 1, 4, 256, 3>},
-    {128, 128, true, kAny, 6.0, 0.56, 4.0, 1, launch_tiles<4, 1, 4, 1, 1, 128, 4>},
-    {128, 256, true, kAny, 7.5, 0.83, 9.0, 1, launch_tiles<4, 1, 4, 2, 1, 128, 3>},
-    {256, 256, true, kAny, 11.0, 1.35, 15.0, 1, launch_tiles<4, 2, 4, 2, 1, 128, 2>},
+    {128, 128, true, kAny, 6.0, 0.54, 4.0, 1, launch_tiles<2, 2, 2, 2, 2, 128, 4>},
+    {128, 256, true, kAny, 7.5, 0.80, 8.0, 1, launch_tiles<2, 2, 2, 4, 1, 128, 3>},
+    {256, 256, true, kAny, 11.0, 1.33, 15.0, 1, launch_tiles<2, 4, 2, 4, 1, 128, 2>},
 };
 
 double kind_us(const Kind& k, const Prod8Params& p, int64_t rows, int cus) {
   const int64_t blocks = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features) * ((rows + k.tokens - 1) / k.tokens);
-  const int64_t slots = (int64_t)cus * k.per_cu;
-  const double rounds = (double)((blocks + slots - 1) / slots), tiles = (double)((p.K + kKTile8 - 1) / kKTile8);
+  const double tiles = (double)((p.K + kKTile8 - 1) / kKTile8);
+  // blocks that share a CU run out one by one, larger ones round by round
+  const double rounds = k.per_cu > 1 ? (blocks > cus ? (double)blocks / cus + 0.25 : 1.0) : (double)((blocks + cus - 1) / cus);
   return k.base + rounds * k.per_tile * tiles + (rounds - 1) * k.more;
 }
 
@@ -640,8 +699,7 @@ const Kind* best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, do
 // The kind with the smallest time for the call; where a kind's last round
 // would be part full, its whole rounds may run as one launch and the rows left
 // as another of a smaller kind (2 us between the two).
-hipError_t launch_prod8(const Prod8Params& p_in, hipStream_t stream) {
-  Prod8Params p = p_in;
+hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
   bool norm = false;
   for (int i = 0; i < p.n_outs; ++i) norm |= p.out[i].norm_w != nullptr;
   const int cus = device_cus();
@@ -650,11 +708,10 @@ hipError_t launch_prod8(const Prod8Params& p_in, hipStream_t stream) {
   const Kind *first = nullptr, *rest = nullptr;
   int rows1 = 0;
   for (const Kind& k : kKinds) {
-    if ((norm && !k.heads) || k.max_tokens != kAny) continue;
+    if ((norm && !k.heads) || k.per_cu > 1) continue;
     const int64_t per_row_tile = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features);
-    const int64_t slots = (int64_t)cus * k.per_cu;
     const int64_t blocks = per_row_tile * ((p.M + k.tokens - 1) / k.tokens);
-    const int64_t rows = blocks / slots * slots / per_row_tile * k.tokens;
+    const int64_t rows = blocks / cus * cus / per_row_tile * k.tokens;
     if (rows < 1 || rows >= p.M) continue;
     double t2 = 0;
     const Kind* r = best_kind(p, norm, p.M - rows, cus, &t2);
@@ -671,13 +728,7 @@ hipError_t launch_prod8(const Prod8Params& p_in, hipStream_t stream) {
   a.M = rows1;
   const hipError_t e = first->launch(a, norm, stream);
   if (e != hipSuccess) return e;
-  p.M -= rows1;
-  p.m_base += rows1;
-  p.x += (int64_t)rows1 * p.ldx;
-  p.x_scale += rows1;
-  for (int i = 0; i < p.n_outs; ++i)
-    p.out[i].y = (char*)p.out[i].y + (int64_t)rows1 * p.out[i].ldy * (p.out[i].y_f32 ? 4 : 2);
-  return rest->launch(p, norm, stream);
+  return rest->launch(rows_from(p, rows1), norm, stream);
 }
 
 }  // namespace harp_blk

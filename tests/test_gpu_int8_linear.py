@@ -212,7 +212,7 @@ def _assert_qkv(outs, attn, rows, freqs, what):
     (1, 1, 1, 128, B16, True), (1, 1, 5, 640, F32, True), (2, 3, 2, 100, B16, False), (1, 40, 3, 384, B16, True),
     (2, 65, 2, 257, F32, True), (1, 128, 1, 128, None, False), (1, 300, 4, 512, B16, True), (3, 111, 3, 384, B16, True),
     (1, 700, 2, 1000, None, False), (1, 1030, 5, 640, F32, True),
-    (1, 200, 30, 200, B16, True), (2, 350, 30, 130, F32, True), (2, 2100, 30, 100, B16, True), (5, 1333, 13, 64, B16, True),
+    (1, 200, 30, 200, B16, True), (2, 350, 30, 130, F32, True), (2, 2100, 30, 100, B16, True), (5, 1333, 13, 64, B16, True), (1, 8100, 27, 1000, B16, True), (3, 2731, 28, 900, F32, True),
 ])
 def test_qkv(B, S, H, K, norm, rope):
     print(f"[qkv B={B} S={S} H={H} K={K} norm={norm} rope={rope}]", flush=True)

@@ -337,3 +337,41 @@ def test_saved_tensors_are_guarded():
         h.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_one_tensor_as_both_inputs():
+    """x added to itself: its gradient is the sum of both inputs'."""
+    g = _gen(21)
+    x, dy, dh = (_rand(g, 9, 200, dtype=F32) for _ in range(3))
+    a = x.clone().requires_grad_(True)
+    y, h = harp_amd.add_rms_norm(a, a)
+    (got,) = torch.autograd.grad((y, h), a, (dy, dh))
+    b, c = x.clone().requires_grad_(True), x.clone().requires_grad_(True)
+    y2, h2 = harp_amd.add_rms_norm(b, c)
+    gb, gc = torch.autograd.grad((y2, h2), (b, c), (dy, dh))
+    assert torch.equal(y, y2) and torch.equal(got, gb + gc)
+    a = x.clone().requires_grad_(True)
+    y, h = harp_amd.add_rms_norm(a, a)
+    (y * dy).sum().backward(inputs=[a], retain_graph=True)
+    first = a.grad.clone()
+    (y * dy).sum().backward(inputs=[a])
+    assert torch.equal(a.grad, 2 * first)
+
+
+@pytest.mark.parametrize("need", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1)], ids=str)
+@pytest.mark.parametrize("rd", [B16, F32], ids=str)
+def test_gradients_of_some_inputs(need, rd):
+    """Any subset of the inputs' gradients equals the one taken with all."""
+    g, x, r, w = _case(6, 136, (B16, rd, F32), 4)
+    dy, dh = _rand(g, 6, 136), _rand(g, 6, 136, dtype=rd)
+    full = [t.clone().requires_grad_(True) for t in (x, r, w)]
+    want = torch.autograd.grad(harp_amd.add_rms_norm(*full), full, (dy, dh))
+    some = [t.clone().requires_grad_(bool(n)) for t, n in zip((x, r, w), need)]
+    leaves = [t for t in some if t.requires_grad]
+    got = torch.autograd.grad(harp_amd.add_rms_norm(*some), leaves, (dy, dh))
+    assert all(torch.equal(a, b) for a, b in zip(got, [v for v, n in zip(want, need) if n]))
+    with torch.inference_mode():
+        y, h = harp_amd.add_rms_norm(x, r, w)
+    with torch.no_grad():
+        y2, h2 = harp_amd.add_rms_norm(*some)
+    assert torch.equal(y, y2) and torch.equal(h, h2) and not y2.requires_grad
