@@ -1,7 +1,6 @@
 // kernels/libharp_block_ops.so — PyTorch-ROCm operators of the kernels around
 // the attention block (include/harp_block_ops.h), namespace harp_block:
 //   add_rms_norm                                    residual addition + RMSNorm
-//   add_rms_norm_forward, add_rms_norm_backward     its two directions
 //   add_rms_norm_int8, quantize_int8, dequantize_int8
 //   linear_int8, linear_int8_dynamic, qkv_int8      products of 8-bit rows
 // The operators allocate their results from PyTorch's allocator and run on
@@ -102,76 +101,64 @@ void check_residual(const at::Tensor& residual, const at::Tensor& x) {
 }
 
 // ---------------------------------------------------------------------------
-// (y, h, rstd); h is empty without a residual, rstd without keep
+// (y, h, rstd); h is undefined without a residual, rstd without keep
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_forward(const at::Tensor& x, const OptTensor& residual,
                                                                     const OptTensor& weight, double eps, bool keep) {
-  check_input(x, "add_rms_norm_forward");
+  check_input(x, "add_rms_norm");
   if (given(residual)) check_residual(*residual, x);
   const c10::DeviceGuard guard(x.device());
   const Rows xr = rows_of(x, "x");
   const Vec w = vec_of(weight, x, xr.cols, "weight");
   at::Tensor y = at::empty(x.sizes(), x.options());
-  at::Tensor h, rstd = at::empty({keep ? xr.rows : 0}, x.options().dtype(at::kFloat));
+  at::Tensor h, rstd;
+  if (keep) rstd = at::empty({xr.rows}, x.options().dtype(at::kFloat));
   Rows rr;
   if (given(residual)) {
     rr = rows_of(*residual, "residual");
     h = at::empty(x.sizes(), residual->options());
   }
-  check_status(harp_blk_add_rms_norm_forward(xr.p, xr.ld, code(x.scalar_type()), rr.p, rr.ld,
-                                             rr.p ? code(rr.t.scalar_type()) : HARP_BLK_BF16, w.p, w.dtype, (float)eps,
-                                             y.data_ptr(), xr.cols, h.defined() && xr.rows ? h.data_ptr() : nullptr,
-                                             xr.cols, keep && xr.rows ? rstd.data_ptr<float>() : nullptr,
-                                             (int)xr.rows, checked_int(xr.cols, "cols"), stream_of(x)),
-               "add_rms_norm_forward");
-  if (!h.defined()) h = at::empty({0}, x.options());
+  if (xr.rows)
+    check_status(harp_blk_add_rms_norm_forward(xr.p, xr.ld, code(x.scalar_type()), rr.p, rr.ld,
+                                               rr.p ? code(rr.t.scalar_type()) : HARP_BLK_BF16, w.p, w.dtype,
+                                               (float)eps, y.data_ptr(), xr.cols, h.defined() ? h.data_ptr() : nullptr,
+                                               xr.cols, keep ? rstd.data_ptr<float>() : nullptr, (int)xr.rows,
+                                               checked_int(xr.cols, "cols"), stream_of(x)),
+                 "add_rms_norm");
   return {y, h, rstd};
 }
 
-// (dx, dresidual, grad_weight): dresidual is empty where it equals dx (same
-// type) or is not wanted, grad_weight without want_weight
-std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_backward(const at::Tensor& dy, const OptTensor& dh,
-                                                                     const at::Tensor& h, const OptTensor& weight,
+// (dx, dresidual, grad_weight): dresidual is undefined where it equals dx
+// (same type) or is not wanted, grad_weight without want_weight
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_backward(const at::Tensor& dy, const at::Tensor& dh,
+                                                                     const at::Tensor& h, const at::Tensor& weight,
                                                                      const at::Tensor& rstd, bool want_residual,
                                                                      bool want_weight) {
-  check_input(dy, "add_rms_norm_backward");
-  check_float(h, dy, "h");
-  TORCH_CHECK(h.sizes() == dy.sizes(), "h must have dy's shape ", dy.sizes(), ", got ", h.sizes());
   const c10::DeviceGuard guard(dy.device());
   const Rows dyr = rows_of(dy, "dy"), hr = rows_of(h, "h");
   Rows dhr;
-  if (given(dh)) {
-    check_float(*dh, dy, "dh");
-    TORCH_CHECK(dh->sizes() == dy.sizes() && dh->scalar_type() == h.scalar_type(), "dh must be like h");
-    dhr = rows_of(*dh, "dh");
-  }
-  TORCH_CHECK(rstd.is_cuda() && rstd.device() == dy.device() && rstd.scalar_type() == at::kFloat &&
-                  rstd.is_contiguous() && rstd.numel() == dyr.rows,
-              "rstd must be a contiguous float32 vector of ", dyr.rows, " elements");
+  if (dh.defined()) dhr = rows_of(dh, "dh");
   const Vec w = vec_of(weight, dy, dyr.cols, "weight");
-  TORCH_CHECK(!want_weight || w.p, "there is no weight to take a gradient of");
-  at::Tensor dx = at::empty(dy.sizes(), dy.options());
-  at::Tensor dres = want_residual && h.scalar_type() != dy.scalar_type() ? at::empty(dy.sizes(), h.options())
-                                                                         : at::empty({0}, h.options());
-  at::Tensor gw = at::empty({want_weight ? dyr.cols : 0}, want_weight ? w.t.options() : dy.options());
+  at::Tensor dx = at::empty(dy.sizes(), dy.options()), dres, gw, ws;
+  if (want_residual && h.scalar_type() != dy.scalar_type()) dres = at::empty(dy.sizes(), h.options());
+  if (want_weight) gw = at::empty({dyr.cols}, w.t.options());
   const int rows = (int)dyr.rows, cols = checked_int(dyr.cols, "cols");
   if (rows == 0) {
-    gw.zero_();
+    if (want_weight) gw.zero_();
     return {dx, dres, gw};
   }
   size_t wsb = 0;
-  at::Tensor ws;
   if (want_weight) {
     wsb = harp_blk_backward_workspace_bytes(rows, cols);
-    TORCH_CHECK(wsb != (size_t)-1, "harp_block.add_rms_norm_backward: ", harp_blk_last_error());
+    TORCH_CHECK(wsb != (size_t)-1, "harp_block.add_rms_norm: ", harp_blk_last_error());
     ws = at::empty({(int64_t)(wsb / 4)}, dy.options().dtype(at::kFloat));
   }
   check_status(
       harp_blk_add_rms_norm_backward(dyr.p, dyr.ld, code(dy.scalar_type()), dhr.p, dhr.ld, hr.p, hr.ld,
                                      code(h.scalar_type()), w.p, w.dtype, rstd.const_data_ptr<float>(), dx.data_ptr(),
-                                     cols, dres.numel() ? dres.data_ptr() : nullptr, cols,
+                                     cols, dres.defined() ? dres.data_ptr() : nullptr, cols,
                                      want_weight ? gw.data_ptr() : nullptr, w.dtype, rows, cols,
                                      want_weight ? ws.data_ptr() : nullptr, wsb, stream_of(dy)),
-      "add_rms_norm_backward");
+      "add_rms_norm (backward)");
   return {dx, dres, gw};
 }
 
@@ -190,9 +177,10 @@ class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
     at::AutoDispatchBelowADInplaceOrView guard;
     auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, true);
     ctx->set_materialize_grads(false);
-    ctx->saved_data["x_dtype"] = x.scalar_type();
-    ctx->saved_data["need"] = std::vector<bool>{x.requires_grad(), given(residual) && residual->requires_grad(),
-                                                given(weight) && weight->requires_grad()};
+    // x's type, and which of the three gradients are wanted
+    ctx->saved_data["wanted"] = (int64_t)x.scalar_type() * 8 + x.requires_grad() +
+                                2 * (given(residual) && residual->requires_grad()) +
+                                4 * (given(weight) && weight->requires_grad());
     const at::Tensor w = given(weight) ? *weight : at::Tensor();
     if (!given(residual)) {
       ctx->save_for_backward({x, w, rstd});
@@ -205,21 +193,21 @@ class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const auto x_dtype = ctx->saved_data["x_dtype"].toScalarType();
-    const auto need = ctx->saved_data["need"].toBoolList();
+    const int64_t wanted = ctx->saved_data["wanted"].toInt();
+    const bool need_x = wanted & 1, need_residual = wanted & 2, need_weight = wanted & 4;
     const at::Tensor &h = saved[0], &w = saved[1], &rstd = saved[2], &dy = grads[0];
     const at::Tensor dh = grads.size() > 1 ? grads[1] : at::Tensor();
     torch::autograd::variable_list out(4);
     {
       at::AutoDispatchBelowADInplaceOrView guard;
       if (dy.defined()) {
-        auto [dx, dres, gw] = add_rms_norm_backward(dy, dh, h, w, rstd, need[1], need[2]);
-        if (need[0]) out[0] = dx;
-        if (need[1]) out[1] = dres.numel() || dx.numel() == 0 ? dres.reshape(dx.sizes()) : dx;  // equal where the types are
-        if (need[2]) out[2] = gw;
+        auto [dx, dres, gw] = add_rms_norm_backward(dy, dh, h, w, rstd, need_residual, need_weight);
+        if (need_x) out[0] = dx;
+        if (need_residual) out[1] = dres.defined() ? dres : dx;
+        if (need_weight) out[2] = gw;
       } else if (dh.defined()) {  // y took no part: the addition alone
-        if (need[0]) out[0] = dh.to(x_dtype);
-        if (need[1]) out[1] = dh;
+        if (need_x) out[0] = dh.to((at::ScalarType)(wanted / 8));
+        if (need_residual) out[1] = dh;
       }
     }
     if (at::GradMode::is_enabled()) {  // create_graph: a gradient of these gradients raises
@@ -474,15 +462,6 @@ std::vector<at::Tensor> qkv_int8(const at::Tensor& x, const at::Tensor& x_scales
 std::tuple<at::Tensor, at::Tensor> add_rms_norm_cpu(const at::Tensor&, const OptTensor&, const OptTensor&, double) {
   no_cpu("add_rms_norm");
 }
-std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_forward_cpu(const at::Tensor&, const OptTensor&,
-                                                                        const OptTensor&, double, bool) {
-  no_cpu("add_rms_norm_forward");
-}
-std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_backward_cpu(const at::Tensor&, const OptTensor&,
-                                                                         const at::Tensor&, const OptTensor&,
-                                                                         const at::Tensor&, bool, bool) {
-  no_cpu("add_rms_norm_backward");
-}
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8_cpu(const at::Tensor&, const OptTensor&,
                                                                      const OptTensor&, double) {
   no_cpu("add_rms_norm_int8");
@@ -507,12 +486,6 @@ std::vector<at::Tensor> qkv_int8_cpu(const at::Tensor&, const at::Tensor&, const
 
 TORCH_LIBRARY(harp_block, m) {
   m.def("add_rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps) -> (Tensor, Tensor)");
-  m.def(
-      "add_rms_norm_forward(Tensor x, Tensor? residual, Tensor? weight, float eps, bool keep) -> (Tensor, Tensor, "
-      "Tensor)");
-  m.def(
-      "add_rms_norm_backward(Tensor dy, Tensor? dh, Tensor h, Tensor? weight, Tensor rstd, bool want_residual, bool "
-      "want_weight) -> (Tensor, Tensor, Tensor)");
   m.def("add_rms_norm_int8(Tensor x, Tensor? residual, Tensor? weight, float eps) -> (Tensor, Tensor, Tensor)");
   m.def("quantize_int8(Tensor x) -> (Tensor, Tensor)");
   m.def("dequantize_int8(Tensor values, Tensor scales, ScalarType dtype) -> Tensor");
@@ -530,8 +503,6 @@ TORCH_LIBRARY_IMPL(harp_block, AutogradCUDA, m) { m.impl("add_rms_norm", &add_rm
 
 TORCH_LIBRARY_IMPL(harp_block, CUDA, m) {
   m.impl("add_rms_norm", &add_rms_norm);
-  m.impl("add_rms_norm_forward", &add_rms_norm_forward);
-  m.impl("add_rms_norm_backward", &add_rms_norm_backward);
   m.impl("add_rms_norm_int8", &add_rms_norm_int8);
   m.impl("quantize_int8", &quantize_int8);
   m.impl("dequantize_int8", &dequantize_int8);
@@ -542,8 +513,6 @@ TORCH_LIBRARY_IMPL(harp_block, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(harp_block, CPU, m) {
   m.impl("add_rms_norm", &add_rms_norm_cpu);
-  m.impl("add_rms_norm_forward", &add_rms_norm_forward_cpu);
-  m.impl("add_rms_norm_backward", &add_rms_norm_backward_cpu);
   m.impl("add_rms_norm_int8", &add_rms_norm_int8_cpu);
   m.impl("quantize_int8", &quantize_int8_cpu);
   m.impl("dequantize_int8", &dequantize_int8_cpu);
