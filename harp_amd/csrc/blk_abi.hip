@@ -34,7 +34,6 @@ int ok() {
 
 constexpr int64_t kMaxLd8 = (int64_t)1 << 22;  // a 256-row tile of 8-bit rows spans < 2^32 bytes
 constexpr int kMaxK = 1 << 16;                 // 2^16 products of at most 2^14: below 2^31
-constexpr int64_t kMaxGrid = 0x7fffffff;
 constexpr int kMaxTokens = 1 << 30;            // of a product: token indexes stay in 32 bits past the last tile
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -251,8 +250,6 @@ int harp_blk_dequantize_int8(const int8_t* q, int64_t ld_q, const float* scales,
   if ((rc = check_rows8(q, ld_q, cols, INT64_MAX, false, "q"))) return rc;
   if ((rc = check_floats(scales, "scales"))) return rc;
   if ((rc = check_matrix(out, ld_out, out_dtype, cols, true, "out"))) return rc;
-  if (((int64_t)rows * (((int64_t)cols + 15) / 16) + 255) / 256 > kMaxGrid)
-    return fail(HARP_BLK_EUNSUPPORTED, "%d rows of %d values: too many", rows, cols);
   return launched(launch_dequantize(q, ld_q, scales, out, ld_out, out_dtype, rows, cols, (hipStream_t)stream),
                   "dequantise");
 }

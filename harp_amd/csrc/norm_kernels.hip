@@ -170,7 +170,9 @@ __device__ __forceinline__ void row_reduce(float& s, uint32_t& m, float* lds_s, 
 // The scale of a row and what turns its values into steps.  The maximum comes
 // as the bits of |v|, which order as the values do with infinity and NaN on
 // top: a row that holds one has the scale NaN (and steps of zero), so that
-// whatever reads it is NaN too.  A row of zeros has scale and steps zero.
+// whatever reads it is NaN too; so has a row whose normed values are not finite
+// (factor infinite: eps 0 and squares that sum to 0).  A row of zeros has scale
+// and steps zero.
 // Maxima below 2^-100 are raised by 2^100 first, or 127 / a would overflow.
 struct Steps {
   float pre, a, inv, scale;
@@ -182,8 +184,8 @@ __device__ __forceinline__ Steps row_steps(uint32_t max_bits, float factor) {
   t.a = a * t.pre;
   t.inv = __fdiv_rn(127.f, t.a);
   t.scale = __fdiv_rn(a * factor, 127.f);
-  if (max_bits == 0) t.inv = t.scale = 0.f;
-  if (max_bits >= 0x7f800000u) {
+  if (max_bits == 0) t.inv = 0.f;
+  if (!(t.scale < __builtin_inff())) {
     t.inv = 0.f;
     t.scale = __uint_as_float(0x7fc00000u);
   }
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams 
     }
   } else {
     const Steps st = row_steps(mx, rho);
-    const bool bad = mx >= 0x7f800000u;
+    const bool bad = !(st.scale < __builtin_inff());
     if (t == 0) p.scale[row] = st.scale;
     int8_t* q = p.q + row * p.ldq;
     const int end = (p.cols + 15) & ~15;  // the last 16 bytes whole, zeros behind the row's values
@@ -481,16 +483,43 @@ __global__ __launch_bounds__(256) void dequant_kernel(const int8_t* q, int64_t l
 // ---------------------------------------------------------------------------
 namespace {
 
+constexpr int kMaxBlocks = 1 << 22;  // of one launch: a grid holds fewer than 2^32 threads
+
+// p without its first `rows` rows
+template <int XD, int RD>
+NormParams rows_from(NormParams p, int rows) {
+  typedef typename Elem<XD>::type TX;
+  typedef typename Elem<RD>::type TR;
+  p.rows -= rows;
+  p.x = (const TX*)p.x + rows * p.ldx;
+  if (p.res) p.res = (const TR*)p.res + rows * p.ldr;
+  if (p.h) p.h = (TR*)p.h + rows * p.ldh;
+  if (p.y) p.y = (TX*)p.y + rows * p.ldy;
+  if (p.rstd) p.rstd += rows;
+  if (p.q) p.q += rows * p.ldq;
+  if (p.scale) p.scale += rows;
+  return p;
+}
+
+template <int MODE, int XD, int RD, int TPR, int NV>
+hipError_t launch_fwd_rows(NormParams p, hipStream_t stream) {
+  constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
+  for (;;) {
+    const int left = p.rows - kMaxBlocks * kRows;
+    if (left > 0) p.rows = kMaxBlocks * kRows;
+    hipLaunchKernelGGL((norm_kernel<MODE, XD, RD, TPR, NV>), dim3((unsigned)((p.rows + kRows - 1) / kRows)),
+                       dim3(TPR > 256 ? TPR : 256), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || left <= 0) return e;
+    p = rows_from<XD, RD>(p, p.rows);
+    p.rows = left;
+  }
+}
+
 template <int MODE, int XD, int RD>
 hipError_t launch_fwd_t(const NormParams& p, hipStream_t stream) {
   const int vecs = (p.cols + kVec - 1) / kVec;
-#define HARP_NORM_LAUNCH(TPR, NV)                                                                                  \
-  {                                                                                                                \
-    constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;                                                               \
-    hipLaunchKernelGGL((norm_kernel<MODE, XD, RD, TPR, NV>), dim3((unsigned)((p.rows + kRows - 1) / kRows)),       \
-                       dim3(TPR > 256 ? TPR : 256), 0, stream, p);                                                 \
-    return hipGetLastError();                                                                                      \
-  }
+#define HARP_NORM_LAUNCH(TPR, NV) return launch_fwd_rows<MODE, XD, RD, TPR, NV>(p, stream);
   if (vecs <= 64) HARP_NORM_LAUNCH(64, 1)
   if (vecs <= 128) HARP_NORM_LAUNCH(64, 2)
   if (vecs <= 256) HARP_NORM_LAUNCH(256, 1)
@@ -574,14 +603,21 @@ hipError_t launch_wgrad(const float* wpart, int blocks, int cols, void* gw, int 
 
 hipError_t launch_dequantize(const int8_t* q, int64_t ldq, const float* scale, void* out, int64_t ldo, int o_dtype,
                              int rows, int cols, hipStream_t stream) {
-  const int64_t threads = (int64_t)rows * ((cols + 15) / 16);
-  const dim3 grid((unsigned)((threads + 255) / 256));
-  if (o_dtype == kF32)
-    hipLaunchKernelGGL((dequant_kernel<kF32>), grid, dim3(256), 0, stream, q, ldq, scale, (float*)out, ldo, rows, cols);
-  else
-    hipLaunchKernelGGL((dequant_kernel<kBf16>), grid, dim3(256), 0, stream, q, ldq, scale, (uint16_t*)out, ldo, rows,
-                       cols);
-  return hipGetLastError();
+  const int64_t per_row = (cols + 15) / 16;
+  const int64_t most = (int64_t)kMaxBlocks * 256 / per_row;  // rows of one launch (cols < 2^31: at least 7)
+  for (int64_t r0 = 0; r0 < rows; r0 += most) {
+    const int n = (int)(rows - r0 < most ? rows - r0 : most);
+    const dim3 grid((unsigned)((n * per_row + 255) / 256));
+    if (o_dtype == kF32)
+      hipLaunchKernelGGL((dequant_kernel<kF32>), grid, dim3(256), 0, stream, q + r0 * ldq, ldq, scale + r0,
+                         (float*)out + r0 * ldo, ldo, n, cols);
+    else
+      hipLaunchKernelGGL((dequant_kernel<kBf16>), grid, dim3(256), 0, stream, q + r0 * ldq, ldq, scale + r0,
+                         (uint16_t*)out + r0 * ldo, ldo, n, cols);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace harp_blk

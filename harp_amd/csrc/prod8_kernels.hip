@@ -612,7 +612,6 @@ template <int FB, int NJ, int TG, int GROUPS, int KG, int KT, int STAGES>
 hipError_t launch_tiles(const Prod8Params& p, bool norm, hipStream_t stream) {
   constexpr int kTok = TG * NJ * 32, kFeatures = GROUPS * FB * 32;
   const int64_t blocks = (int64_t)((p.M + kTok - 1) / kTok) * ((p.N + kFeatures - 1) / kFeatures);
-  if (blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)blocks, (unsigned)p.n_outs), block(64 * TG * GROUPS * KG);
   if constexpr (kFeatures % kFeat == 0)
     if (norm) {
@@ -661,6 +660,7 @@ struct Kind {
   hipError_t (*launch)(const Prod8Params&, bool, hipStream_t);
 };
 constexpr int kAny = 0x7fffffff;
+constexpr int64_t kMaxBlocks = 1 << 22;  // of one launch: a grid holds fewer than 2^32 threads
 const Kind kKinds[] = {
     {16, 16, false, 16, 3.4, 0.11, 0.0, 2, launch_few},
     {32, 32, false, kAny, 3.6, 0.15, 0.0, 2, launch_tiles<1, 1, 1, 1, 4, 256, 4>},
@@ -681,10 +681,15 @@ double kind_us(const Kind& k, const Prod8Params& p, int64_t rows, int cus) {
   return k.base + rounds * k.per_tile * tiles + (rounds - 1) * k.more;
 }
 
+bool takes(const Kind& k, const Prod8Params& p, bool norm, int64_t rows) {
+  const int64_t tiles = (int64_t)((p.N + k.features - 1) / k.features) * ((rows + k.tokens - 1) / k.tokens);
+  return (!norm || k.heads) && rows <= k.max_tokens && tiles <= kMaxBlocks;
+}
+
 const Kind* best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, double* us) {
   const Kind* best = nullptr;
   for (const Kind& k : kKinds) {
-    if ((norm && !k.heads) || rows > k.max_tokens) continue;
+    if (!takes(k, p, norm, rows)) continue;
     const double t = kind_us(k, p, rows, cus);
     if (!best || t < *us) {
       best = &k;
@@ -708,22 +713,23 @@ hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
   const Kind *first = nullptr, *rest = nullptr;
   int rows1 = 0;
   for (const Kind& k : kKinds) {
-    if ((norm && !k.heads) || k.per_cu > 1) continue;
+    if (!takes(k, p, norm, 1) || k.per_cu > 1) continue;
     const int64_t per_row_tile = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features);
     const int64_t blocks = per_row_tile * ((p.M + k.tokens - 1) / k.tokens);
     const int64_t rows = blocks / cus * cus / per_row_tile * k.tokens;
-    if (rows < 1 || rows >= p.M) continue;
+    if (rows < 1 || rows >= p.M || !takes(k, p, norm, rows)) continue;
     double t2 = 0;
     const Kind* r = best_kind(p, norm, p.M - rows, cus, &t2);
+    if (!r) continue;
     const double t = kind_us(k, p, rows, cus) + 2.0 + t2;
-    if (t < us) {
+    if (!kind || t < us) {
       us = t;
       first = &k;
       rest = r;
       rows1 = (int)rows;
     }
   }
-  if (!first) return kind->launch(p, norm, stream);
+  if (!first) return kind ? kind->launch(p, norm, stream) : hipErrorInvalidConfiguration;
   Prod8Params a = p;
   a.M = rows1;
   const hipError_t e = first->launch(a, norm, stream);

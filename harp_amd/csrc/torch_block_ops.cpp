@@ -366,7 +366,8 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at
                        const at::Tensor& weight_scales, const OptTensor& bias, at::ScalarType dtype) {
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "linear_int8: bfloat16 or float32, got ", dtype);
   const Rows8 xr = rows8_of(x, x_scales, "x");
-  TORCH_CHECK(weight.dim() == 2 && weight.size(1) >= xr.cols && weight.device() == x.device(),
+  TORCH_CHECK(weight.dim() == 2 && (weight.size(1) == xr.cols || weight.size(1) == ld8(xr.cols)) &&
+                  weight.device() == x.device(),
               "weight must be [N, ", xr.cols, "] on ", x.device(), ", got ", weight.sizes(), " on ", weight.device());
   const Rows8 wr = rows8_of(weight, weight_scales, "weight");
   const c10::DeviceGuard guard(x.device());

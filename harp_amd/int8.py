@@ -64,6 +64,7 @@ class Int8Rows(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """values * scales as a bfloat16 or float32 tensor."""
+        _refuse_grad("Int8Rows.dequantize", self.scales)
         return _ops().dequantize_int8(self.values, self.scales, dtype)
 
 
@@ -77,7 +78,7 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """x [.., K] times the transpose of weight [N, K], plus bias [N]: a
     bfloat16 or float32 tensor [.., N].  K up to 65536."""
-    _refuse_grad("int8_linear", bias)
+    _refuse_grad("int8_linear", x.scales, weight.scales, bias)
     if weight.values.size(-1) != x.values.size(-1):
         raise RuntimeError(f"weight must be [N, {x.values.size(-1)}], got {tuple(weight.values.shape)}")
     return _ops().linear_int8(x.values, x.scales, weight.values, weight.scales, bias, out_dtype)
@@ -134,6 +135,7 @@ class Int8Linear(nn.Module):
             raise RuntimeError(f"Int8Linear of {self.in_features} features got rows of {features}")
         # the operators read the weight's first in_features columns
         if rows:
+            _refuse_grad("Int8Linear", x.scales)
             return _ops().linear_int8(x.values, x.scales, self.weight_values, self.weight_scales, self.bias,
                                       self.out_dtype)
         _refuse_grad("Int8Linear", x)
@@ -190,7 +192,7 @@ def project_qkv_int8(attn, rows: Int8Rows, freqs_cis: Optional[torch.Tensor]
     float32 with one rounding at the end."""
     norms = [getattr(attn, "norm_q", None), getattr(attn, "norm_k", None), None]
     weights = [None if nm is None else nm.weight for nm in norms]
-    _refuse_grad("project_qkv with 8-bit projections", *weights)
+    _refuse_grad("project_qkv with 8-bit projections", rows.scales, *weights)
     w = [m.weight for m in (attn.to_q, attn.to_k, attn.to_v)]
     q, k, v = _ops().qkv_int8(rows.values, rows.scales, [r.values for r in w], [r.scales for r in w], weights,
                               [0.0 if nm is None else float(nm.eps) for nm in norms], freqs_cis)

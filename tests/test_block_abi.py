@@ -232,3 +232,14 @@ def test_rows_need_8_bit_projections():
     rows = harp_amd.Int8Rows(torch.zeros(1, 3, 64, dtype=torch.int8), torch.zeros(1, 3))
     with pytest.raises(ValueError, match="8-bit projections"):
         harp_amd.project_qkv(attn, rows, None)
+
+
+def test_gradients_of_scales_are_refused():
+    values, scales = torch.zeros(3, 64, dtype=torch.int8), torch.zeros(3, requires_grad=True)
+    rows, plain = harp_amd.Int8Rows(values, scales), harp_amd.Int8Rows(values, scales.detach())
+    for call in (lambda: rows.dequantize(), lambda: harp_amd.int8_linear(rows, plain),
+                 lambda: harp_amd.int8_linear(plain, rows), lambda: harp_amd.Int8Linear(plain)(rows)):
+        with pytest.raises(RuntimeError, match="forward only"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="HIP device only"):
+            call()

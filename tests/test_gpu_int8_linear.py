@@ -246,3 +246,27 @@ def test_qkv_unfused_paths():
     attn.to_v = harp_amd.Int8Linear(attn.to_v.weight, torch.ones(256, device=DEV))
     v = harp_amd.project_qkv(attn, rows, f)[2]
     assert torch.equal(v, attn.to_v(rows).unflatten(-1, (2, 128)).transpose(1, 2))
+
+
+@pytest.mark.parametrize("M,N", [(1, 2 ** 28 + 40), (2 ** 27 + 9, 3)])
+def test_more_blocks_than_one_launch_holds(M, N):
+    """A grid holds fewer than 2^32 threads: the smallest blocks make way."""
+    K = 16
+    g = torch.Generator(DEV).manual_seed(M % 97)
+    x, w = (harp_amd.Int8Rows(torch.empty(n, K, dtype=torch.int8, device=DEV).random_(-127, 128, generator=g),
+                              torch.rand(n, generator=g, device=DEV)) for n in (M, N))
+    y = harp_amd.int8_linear(x, w)
+    for lo in (0, max(M, N) // 2, max(M, N) - 512):
+        s = slice(lo, lo + 512)
+        if M == 1:
+            _assert_linear(y[:, s], x, harp_amd.Int8Rows(w.values[s], w.scales[s]), None, lo)
+        else:
+            _assert_linear(y[s], harp_amd.Int8Rows(x.values[s], x.scales[s]), w, None, lo)
+
+
+def test_weight_of_other_width_is_refused():
+    x = harp_amd.quantize_int8(torch.ones(3, 40, device=DEV))
+    for cols in (64, 47, 32):
+        w = harp_amd.quantize_int8(torch.ones(8, cols, device=DEV))
+        with pytest.raises(RuntimeError, match="weight must be"):
+            torch.ops.harp_block.linear_int8(x.values, x.scales, w.values, w.scales, None, B16)

@@ -375,3 +375,50 @@ def test_gradients_of_some_inputs(need, rd):
     with torch.no_grad():
         y2, h2 = harp_amd.add_rms_norm(*some)
     assert torch.equal(y, y2) and torch.equal(h, h2) and not y2.requires_grad
+
+
+def _slices(rows, *at):
+    """512 rows at both ends and around each of `at`."""
+    return [slice(max(0, c - 256), min(rows, c + 256)) for c in (256, *at, rows - 256)]
+
+
+def test_more_rows_than_one_launch_holds():
+    """A grid holds fewer than 2^32 threads: more rows run as several launches."""
+    rows, cols = 2 ** 26 + 5, 8  # 4 rows in a block of 256 threads
+    g = torch.Generator(DEV).manual_seed(5)
+    x = torch.empty(rows, cols, dtype=B16, device=DEV).normal_(generator=g)
+    r = torch.empty(rows, cols, dtype=F32, device=DEV).normal_(generator=g)
+    q = harp_amd.quantize_int8(x)
+    y, h = harp_amd.add_rms_norm(x, r, None, 1e-6)
+    for s in _slices(rows, 2 ** 24, 2 ** 26):
+        small = harp_amd.quantize_int8(x[s])
+        assert torch.equal(q.values[s], small.values) and torch.equal(q.scales[s], small.scales), s
+        ys, hs = harp_amd.add_rms_norm(x[s], r[s], None, 1e-6)
+        assert torch.equal(y[s], ys) and torch.equal(h[s], hs), s
+
+
+def test_more_values_than_one_dequantise_launch_holds():
+    rows, cols = 2 ** 25 + 3, 520  # 33 vectors of 16 values a row, 2^30 to a launch
+    g = torch.Generator(DEV).manual_seed(6)
+    store = torch.empty(rows, 528, dtype=torch.int8, device=DEV).random_(-127, 128, generator=g)
+    scales = torch.rand(rows, generator=g, device=DEV)
+    out = harp_amd.Int8Rows(store[:, :cols], scales).dequantize(B16)
+    for s in _slices(rows, 2 ** 30 // 33):
+        assert torch.equal(out[s], (store[s, :cols].float() * scales[s, None]).to(B16)), s
+
+
+def test_rows_whose_norm_is_not_finite():
+    """eps 0 and squares that sum to 0: the normed values are infinite or NaN,
+    so the scale is NaN, as every row's that holds one."""
+    x = torch.zeros(4, 72, dtype=F32, device=DEV)
+    x[1, 3] = 1e-30  # its square is 0 in fp32
+    x[2] = 1.0
+    x[3, 0] = 3e38  # its square is infinite: the normed values are 0
+    y, _ = harp_amd.add_rms_norm(x, None, None, 0.0)
+    rows, _ = harp_amd.add_rms_norm_int8(x, None, None, 0.0)
+    assert not bool(torch.isfinite(y[:2]).all(-1).any())
+    assert bool(torch.isnan(rows.scales[:2]).all()) and bool((rows.values[:2] == 0).all())
+    assert bool((y[2] == 1).all()) and bool((rows.values[2] == 127).all())
+    assert bool((y[3] == 0).all()) and bool((rows.dequantize(F32)[3] == 0).all())
+    rows, _ = harp_amd.add_rms_norm_int8(x, None, None, 1e-6)
+    assert float(rows.scales[0]) == 0.0 and bool((rows.values[0] == 0).all())
