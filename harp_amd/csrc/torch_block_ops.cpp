@@ -360,13 +360,21 @@ at::Tensor dequantize_int8(const at::Tensor& values, const at::Tensor& scales, a
   return out;
 }
 
+// Bytes of a row of a module's weight (int8.py): whole cache lines for long
+// rows, so that a tile's 128 bytes of a row are one line (1333 tokens x 1001
+// features of 2570 columns: 12.6 us instead of 14.6).
+int64_t weight_ld8(int64_t cols) {
+  const int64_t unit = cols < 1024 ? 16 : 128;
+  return (cols + unit - 1) / unit * unit;
+}
+
 // 8-bit rows x times the first x.size(-1) columns of weight (a module's
 // padded storage, or rows of exactly that many)
 at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
                        const at::Tensor& weight_scales, const OptTensor& bias, at::ScalarType dtype) {
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "linear_int8: bfloat16 or float32, got ", dtype);
   const Rows8 xr = rows8_of(x, x_scales, "x");
-  TORCH_CHECK(weight.dim() == 2 && (weight.size(1) == xr.cols || weight.size(1) == ld8(xr.cols)) &&
+  TORCH_CHECK(weight.dim() == 2 && (weight.size(1) == xr.cols || weight.size(1) == weight_ld8(xr.cols)) &&
                   weight.device() == x.device(),
               "weight must be [N, ", xr.cols, "] on ", x.device(), ", got ", weight.sizes(), " on ", weight.device());
   const Rows8 wr = rows8_of(weight, weight_scales, "weight");

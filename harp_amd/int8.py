@@ -84,12 +84,18 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
     return _ops().linear_int8(x.values, x.scales, weight.values, weight.scales, bias, out_dtype)
 
 
+def _weight_row_bytes(cols: int) -> int:
+    """Bytes of a row of a module's weight: whole 128-byte cache lines for long rows."""
+    unit = 16 if cols < 1024 else 128
+    return -(-cols // unit) * unit
+
+
 class Int8Linear(nn.Module):
     """An ``nn.Linear`` with its weight in 8-bit rows, forward only.
 
-    ``weight_values`` holds the rows padded to multiples of 16 bytes,
-    ``weight_scales`` their scales (float32, also where the module's other
-    tensors are converted to 16 bits: convert before quantising)."""
+    ``weight_values`` holds the rows padded to multiples of 16 bytes (128 from
+    1024 columns on), ``weight_scales`` their scales (float32, also where the
+    module's other tensors are converted to 16 bits: convert before quantising)."""
 
     def __init__(self, weight: Int8Rows, bias: Optional[torch.Tensor] = None,
                  out_dtype: torch.dtype = torch.bfloat16):
@@ -106,7 +112,7 @@ class Int8Linear(nn.Module):
             raise ValueError(f"out_dtype must be bfloat16 or float32, got {out_dtype}")
         self.out_features, self.in_features = values.shape
         self.out_dtype = out_dtype
-        store = torch.zeros((values.size(0), -(-values.size(1) // 16) * 16), dtype=torch.int8, device=values.device)
+        store = torch.zeros((values.size(0), _weight_row_bytes(values.size(1))), dtype=torch.int8, device=values.device)
         store[:, :self.in_features] = values
         self.register_buffer("weight_values", store)
         self.register_buffer("weight_scales", scales.detach().clone())

@@ -270,3 +270,20 @@ def test_weight_of_other_width_is_refused():
         w = harp_amd.quantize_int8(torch.ones(8, cols, device=DEV))
         with pytest.raises(RuntimeError, match="weight must be"):
             torch.ops.harp_block.linear_int8(x.values, x.scales, w.values, w.scales, None, B16)
+
+
+@pytest.mark.parametrize("K", [1008, 1024, 1030, 2570])
+def test_module_with_padded_rows(K):
+    """Long weight rows are padded to whole cache lines: same results as unpadded ones."""
+    g = _gen(K)
+    w = _rows(g, 200, K, pad=16)
+    lin = harp_amd.Int8Linear(w)
+    assert lin.weight_values.size(1) == (1008 if K == 1008 else -(-K // 128) * 128)
+    assert torch.equal(lin.weight.values, w.values) and bool((lin.weight_values[:, K:] == 0).all())
+    for M in (1, 20, 150):
+        x = _rows(g, M, K)
+        y = lin(x)
+        assert torch.equal(y, harp_amd.int8_linear(x, w))
+        _assert_linear(y, x, w, None, M)
+        xf = torch.randn(M, K, generator=g).to(DEV)
+        assert torch.equal(lin(xf), lin(harp_amd.quantize_int8(xf)))
