@@ -17,6 +17,13 @@
 // values per thread and vector) and finished there.  Rows need no alignment
 // beyond their element's: a 16-byte global access at any address is one
 // instruction on gfx950, and the vector at a row's end is taken apart.
+//
+// Measured, 8192 rows of 3840 (a copy of 1 GiB reaches 5.23 TB/s here): norm
+// of a bf16 x with its fp32 residual 70 us (378 MB, 5.4 TB/s), backward 101 us
+// (503 MB, 5.0 TB/s) and 5 us for the weight's gradient; norm to 8 bits of
+// bf16 rows and residual 45 us (220 MB, 4.9 TB/s), dequantise 17.6 us (94 MB,
+// 5.4 TB/s).  256 rows: 5.5, 7.3 + 2 .. 3 us, which is a launch, one trip to
+// HBM and one exchange; one row to 8 bits 3.6 us.
 #include "blk_kernels.h"
 #include "ra_common.h"
 
@@ -225,7 +232,10 @@ __device__ __forceinline__ uint2 pack_steps(const f32x8& v, const Steps& t) {
 enum { kModeNorm = 0, kModeNorm8 = 1, kModeQuant = 2 };
 
 // TPR threads per row, NV vectors of 8 per thread; blocks of max(TPR, 256)
-// threads hold 256 / TPR rows, or one.
+// threads hold 256 / TPR rows, or one.  TPR is a wave up to 1024 columns (no
+// LDS, no barrier), then 256, and 512 where 256 would need more than 4 vectors
+// each: the row's registers (16 of fp32 at 3840 columns) leave 8 blocks on a
+// CU, whose loads hide each other's exchanges.
 template <int MODE, int XD, int RD, int TPR, int NV>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams p) {
   constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
@@ -311,7 +321,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams 
 // rows, one row per group at a time, and keeps the weight gradient's sums of
 // its columns in registers; the groups' sums are added in LDS at the end and
 // written as one partial row, so the order of every sum is fixed by the
-// launch alone.  KEEP: dy and h stay in registers between the row's two
+// launch alone.  At most 512 blocks, two to a CU: more would only lengthen the
+// partial rows that wgrad_kernel reads (512 x 3840 fp32 are 8 MB, which stay in
+// the caches: 5 us).  KEEP: dy and h stay in registers between the row's two
 // passes; the longest rows have no room and read them again (out of L2).
 template <int XD, int HD, int TPR, int NV, int GROUPS, bool KEEP>
 __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) {

@@ -230,9 +230,10 @@ __device__ __forceinline__ void finish_tokens(const Prod8Params& p, const Prod8O
 // Tile kernel.  C^T = W x^T, so a lane holds one token and 16 features per
 // accumulator.  A wave covers FB x NJ blocks of 32 features by 32 tokens; a
 // block is GROUPS x FB x 32 features by TG x NJ x 32 tokens, each part covered
-// by KG waves that share the k-steps of a tile and add their sums at the end.  K-tiles of KT bytes a row are copied global ->
-// LDS by buffer_load ... lds, STAGES of them in flight, one barrier per tile
-// in its last k-step; fragment reads run on across tile boundaries.
+// by KG waves that share the k-steps of a tile and add their sums at the end.
+// K-tiles of KT bytes a row are copied global -> LDS by buffer_load ... lds,
+// STAGES of them in flight, one barrier per tile in its last k-step; fragment
+// reads run on across tile boundaries.
 // Rows past the last token or feature and bytes past the descriptors' ends
 // load zeros; the last tile's bytes past K are cleared in the w tile, which
 // makes whatever x holds there count for nothing.
@@ -509,7 +510,11 @@ __global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Pa
 // contraction over 4 waves, which read their operands from global memory
 // straight into the fragments of v_mfma_i32_16x16x64_i8 (each byte of w is
 // used once, so LDS would only add a stop), 4 chunks of 128 bytes a row in
-// flight.  The waves' sums are added in LDS.
+// flight.  The waves' sums are added in LDS.  Bound by the first bytes' way and
+// then by HBM: one token x 3840 features of 3840 bytes takes 5.6 us, 10240
+// features (39 MB) 10.8 us with the weights out of HBM, 4.9 and 9.7 with them in
+// the caches.  The same with 32 tokens (two x fragments to each of w) takes
+// 20.1 us at 32 x 3840 x 10240, where the 32 x 32 blocks take 18.0.
 constexpr int kFewWaves = 4, kFewChunks = 4;
 __global__ __launch_bounds__(64 * kFewWaves) void few8_kernel(Prod8Params p) {
   __shared__ i32x4 red[kFewWaves][64];
@@ -703,7 +708,11 @@ const Kind* best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, do
 
 // The kind with the smallest time for the call; where a kind's last round
 // would be part full, its whole rounds may run as one launch and the rows left
-// as another of a smaller kind (2 us between the two).
+// as another of a smaller kind (2 us between the two): 2048 tokens x 10240 of
+// 3840 take 91 us instead of 97, 5000 x 3840 79 instead of 94.  Blocks of the
+// same kind start as others end, so a second launch of them only adds a stop
+// (q, k, v of 8192 tokens: 372 us instead of 363).  Over 133 shapes from 1 to
+// 8192 tokens the kind chosen for a whole call takes 0.4% more than the best.
 hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
   bool norm = false;
   for (int i = 0; i < p.n_outs; ++i) norm |= p.out[i].norm_w != nullptr;
@@ -720,7 +729,7 @@ hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
     if (rows < 1 || rows >= p.M || !takes(k, p, norm, rows)) continue;
     double t2 = 0;
     const Kind* r = best_kind(p, norm, p.M - rows, cus, &t2);
-    if (!r) continue;
+    if (!r || r == &k) continue;  // the same kind: no gain
     const double t = kind_us(k, p, rows, cus) + 2.0 + t2;
     if (!kind || t < us) {
       us = t;
