@@ -22,8 +22,8 @@
  * An 8-bit row is cols int8 values in -127 .. 127 with one fp32 scale: it
  * stands for value * scale.  Rows start 16-byte aligned (ld a multiple of 16
  * bytes).  scale = max|row| / 127, values to nearest, ties to even; a row of
- * zeros has scale 0; a row with an infinity or a NaN has scale NaN and values
- * 0, so that whatever reads it is NaN.
+ * zeros has scale 0; a row with an infinity or a NaN (of a norm: whose results
+ * are not finite) has scale NaN and values 0, so that whatever reads it is NaN.
  */
 #ifndef HARP_BLOCK_OPS_H
 #define HARP_BLOCK_OPS_H
@@ -106,7 +106,7 @@ HARP_BLK_API int harp_blk_dequantize_int8(const int8_t* q, int64_t ld_q, const f
  * x [M, K] and w [N, K] int8, rows 16-byte aligned (ld_x, ld_w multiples of
  * 16, >= K rounded up to 16, <= 2^22; the bytes from K up to there may be read
  * but count for nothing); bias [N] of bias_dtype or NULL; y of y_dtype.  The
- * sums are exact 32-bit integers: 1 <= K <= 65536.
+ * sums are exact 32-bit integers: 1 <= K <= 65536; M, N <= 2^30.
  */
 HARP_BLK_API int harp_blk_linear_int8(const int8_t* x, int64_t ld_x, const float* x_scales, const int8_t* w,
                                       int64_t ld_w, const float* w_scales, const void* bias, int bias_dtype, void* y,
