@@ -19,11 +19,11 @@
 // instruction on gfx950, and the vector at a row's end is taken apart.
 //
 // Measured, 8192 rows of 3840 (a copy of 1 GiB reaches 5.23 TB/s here): norm
-// of a bf16 x with its fp32 residual 70 us (378 MB, 5.4 TB/s), backward 101 us
-// (503 MB, 5.0 TB/s) and 5 us for the weight's gradient; norm to 8 bits of
-// bf16 rows and residual 45 us (220 MB, 4.9 TB/s), dequantise 17.6 us (94 MB,
-// 5.4 TB/s).  256 rows: 5.5, 7.3 + 2 .. 3 us, which is a launch, one trip to
-// HBM and one exchange; one row to 8 bits 3.6 us.
+// of a bf16 x with its fp32 residual 67 us (378 MB, 5.6 TB/s), backward 103 us
+// (503 MB, 4.9 TB/s) and 5 us for the weight's gradient; norm to 8 bits of
+// bf16 rows and residual 37 us (220 MB, 5.9 TB/s, part of it out of the last
+// caches), dequantise 17.4 us (94 MB, 5.4 TB/s).  256 rows: 4.5, 6.2 + 2 .. 3
+// us, which is a launch, a trip to HBM and an exchange; one row to 8 bits 3 us.
 #include "blk_kernels.h"
 #include "ra_common.h"
 
@@ -92,6 +92,64 @@ __device__ __forceinline__ f32x8 load8(const typename Elem<DT>::type* p, int n) 
   return v;
 }
 
+// A vector as it is in memory; zeros where it lies behind the row.  load_raw
+// only loads: a vector that would reach past the row's end is read at the row's
+// last 8 values instead, and unpack moves the n that count to the front, zeros
+// behind them.  So a kernel's loads are all on their way before the first is
+// waited for; converted where they are loaded, they went one by one (norm to 8
+// bits of 8192 rows of 3840: 45 us, this way 37).  Rows of 8 values or more.
+template <int DT>
+struct Raw {
+  u32x4 u;
+};
+template <>
+struct Raw<kF32> {
+  harp_ra::f32x4 lo, hi;
+};
+template <>
+struct Raw<kNone> {};
+
+template <int DT>
+__device__ __forceinline__ Raw<DT> load_raw(const typename Elem<DT>::type* row, int c, int cols) {
+  Raw<DT> r{};
+  const auto* p = row + min(c, cols - kVec);
+  if constexpr (DT == kBf16) {
+    if (c < cols) r.u = *(const u32x4u*)p;
+  } else if constexpr (DT == kF32) {
+    if (c < cols) {
+      r.lo = *(const harp_ra::f32x4u*)p;
+      r.hi = *(const harp_ra::f32x4u*)(p + 4);
+    }
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ f32x8 unpack(const Raw<DT>& r, int n) {
+  f32x8 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == kBf16) {
+      v[2 * i] = from_bits(r.u[i] << 16);
+      v[2 * i + 1] = from_bits(r.u[i] & 0xffff0000u);
+    } else {
+      v[i] = r.lo[i];
+      v[4 + i] = r.hi[i];
+    }
+  }
+  if (n > 0 && n < kVec) {
+    const int by = kVec - n;
+#pragma unroll
+    for (int step = 1; step < kVec; step *= 2)
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const float next = e + step < kVec ? v[e + step] : 0.f;
+        if (by & step) v[e] = next;
+      }
+  }
+  return v;
+}
+
 template <int DT>
 __device__ __forceinline__ void store8(typename Elem<DT>::type* p, const f32x8& v, int n) {
   if constexpr (DT == kBf16) {
@@ -136,6 +194,31 @@ __device__ __forceinline__ f32x8 load_w(const void* w, int dtype, int c, int n) 
   return dtype == kF32 ? load8<kF32>((const float*)w + c, n) : load8<kBf16>((const uint16_t*)w + c, n);
 }
 
+// the same in two steps, for rows of 8 values or more
+struct RawW {
+  u32x4 lo, hi;  // bf16: lo alone
+};
+__device__ __forceinline__ void load_raw_w(RawW& r, const void* w, int dtype, int c, int cols) {
+  if (dtype == kF32) {
+    const Raw<kF32> f = load_raw<kF32>((const float*)w, c, cols);
+    r.lo = __builtin_bit_cast(u32x4, f.lo);
+    r.hi = __builtin_bit_cast(u32x4, f.hi);
+  } else {
+    r.lo = load_raw<kBf16>((const uint16_t*)w, c, cols).u;
+  }
+}
+__device__ __forceinline__ f32x8 unpack_w(const RawW& r, const void* w, int dtype, int n) {
+  if (!w) {
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = 1.f;
+    return v;
+  }
+  if (dtype == kF32)
+    return unpack<kF32>({__builtin_bit_cast(harp_ra::f32x4, r.lo), __builtin_bit_cast(harp_ra::f32x4, r.hi)}, n);
+  return unpack<kBf16>({r.lo}, n);
+}
+
 // x + r as it is kept: in r's type
 template <int RD>
 __device__ __forceinline__ float round_to(float v) {
@@ -149,7 +232,7 @@ __device__ __forceinline__ float round_to(float v) {
 template <int TPR, bool SUM, bool MAX>
 __device__ __forceinline__ void row_reduce(float& s, uint32_t& m, float* lds_s, uint32_t* lds_m) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
+  for (int d = (TPR < 64 ? TPR : 64) / 2; d > 0; d >>= 1) {
     if (SUM) s += __shfl_xor(s, d);
     if (MAX) m = max(m, (uint32_t)__shfl_xor((int)m, d));
   }
@@ -232,41 +315,69 @@ __device__ __forceinline__ uint2 pack_steps(const f32x8& v, const Steps& t) {
 enum { kModeNorm = 0, kModeNorm8 = 1, kModeQuant = 2 };
 
 // TPR threads per row, NV vectors of 8 per thread; blocks of max(TPR, 256)
-// threads hold 256 / TPR rows, or one.  TPR is a wave up to 1024 columns (no
-// LDS, no barrier), then 256, and 512 where 256 would need more than 4 vectors
-// each: the row's registers (16 of fp32 at 3840 columns) leave 8 blocks on a
-// CU, whose loads hide each other's exchanges.
+// threads hold 256 / TPR rows, or one.  TPR is a quarter of a wave up to 128
+// columns (20000 rows of 64 take 5 us, with a wave for each 9 to 12), a wave up
+// to 1024 (no LDS, no barrier), then 256, and 512 where 256 would need more than
+// 4 vectors each: the row's registers (16 of fp32 at 3840 columns) leave 7 or 8
+// blocks on a CU, whose loads hide each other's exchanges.
 template <int MODE, int XD, int RD, int TPR, int NV>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams p) {
   constexpr int kRows = TPR > 256 ? 1 : 256 / TPR;
+  constexpr bool kEarlyW = MODE != kModeQuant && NV <= 2;  // the weight is loaded with the row (more have no room)
   typedef typename Elem<XD>::type TX;
   typedef typename Elem<RD>::type TR;
   __shared__ float lds_s[16];
   __shared__ uint32_t lds_m[16];
   const int64_t row = (int64_t)blockIdx.x * kRows + (kRows > 1 ? threadIdx.x / TPR : 0);
-  if (row >= p.rows) return;  // whole waves: rows of several waves are alone in their block
+  if (row >= p.rows) return;  // whole rows: rows of several waves are alone in their block
   const int t = threadIdx.x % TPR;
   const TX* x = (const TX*)p.x + row * p.ldx;
   const TR* r = (const TR*)p.res + row * p.ldr;
 
   f32x8 v[NV];
+  RawW wr[NV];
   float ss = 0.f;
   uint32_t mx = 0;
+  if (TPR > 64 || NV > 1 || p.cols >= kVec) {
+    Raw<XD> xr[NV];
+    Raw<RD> rr[NV];
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
-    if (n > 0) {
-      v[i] = load8<XD>(x + c, n);
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * TPR + t) * kVec;
+      xr[i] = load_raw<XD>(x, c, p.cols);
+      if constexpr (RD != kNone) rr[i] = load_raw<RD>(r, c, p.cols);
+    }
+    if (kEarlyW && p.w) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) load_raw_w(wr[i], p.w, p.w_dtype, (i * TPR + t) * kVec, p.cols);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int n = p.cols - (i * TPR + t) * kVec;
+      v[i] = unpack<XD>(xr[i], n);
       if constexpr (RD != kNone) {
-        const f32x8 a = load8<RD>(r + c, n);
+        const f32x8 a = unpack<RD>(rr[i], n);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) v[i][e] = round_to<RD>(v[i][e] + a[e]);
       }
-    } else {
+    }
+  } else {  // a row of fewer values than a vector (NV is 1)
+    const int n = p.cols - t * kVec;
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) v[i][e] = 0.f;
+    for (int e = 0; e < kVec; ++e) v[0][e] = 0.f;
+    if (n > 0) {
+      v[0] = load8<XD>(x, n);
+      if constexpr (RD != kNone) {
+        const f32x8 a = load8<RD>(r, n);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[0][e] = round_to<RD>(v[0][e] + a[e]);
+      }
     }
   }
+  auto weight = [&](int i, int c, int n) {
+    return kEarlyW && (TPR > 64 || NV > 1 || p.cols >= kVec) ? unpack_w(wr[i], p.w, p.w_dtype, n)
+                                                             : load_w(p.w, p.w_dtype, c, n);
+  };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
@@ -277,7 +388,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams 
       for (int e = 0; e < kVec; ++e) ss = __builtin_fmaf(v[i][e], v[i][e], ss);
     if constexpr (MODE == kModeNorm8)
       if (n > 0) {
-        const f32x8 w = load_w(p.w, p.w_dtype, c, n);
+        const f32x8 w = weight(i, c, n);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) v[i][e] *= w[e];
       }
@@ -296,7 +407,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(NormParams 
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * kVec, n = min(kVec, p.cols - c);
       if (n > 0) {
-        const f32x8 w = load_w(p.w, p.w_dtype, c, n);
+        const f32x8 w = weight(i, c, n);
 #pragma unroll
         for (int e = 0; e < kVec; ++e) v[i][e] = v[i][e] * rho * w[e];
         store8<XD>((TX*)p.y + row * p.ldy + c, v[i], n);
@@ -338,6 +449,8 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < kVec; ++e) gw[i][e] = 0.f;
+  constexpr bool kEarlyDh = KEEP && NV <= 2;  // a row's dh is loaded with its dy and h (more have no room)
+  const bool raw = KEEP && (TPR > 64 || NV > 1 || p.cols >= kVec);  // rows of a vector or more
   const int64_t step = (int64_t)gridDim.x * GROUPS;
   const int64_t n_iter = (p.rows + step - 1) / step;
   for (int64_t it = 0; it < n_iter; ++it) {  // the same count in every group: the barrier below is in step
@@ -347,13 +460,17 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
     asm volatile("" : "+v"(t));
     constexpr int kKeep = KEEP ? NV : 1;
     f32x8 gs[kKeep], hs[kKeep];
+    Raw<HD> dhr[kEarlyDh ? NV : 1];
     float c1 = 0.f;
     const float rho = live ? p.rstd[row] : 0.f;
+    const TX* dy = (const TX*)p.dy + row * p.ldy;
+    const TH* hp = (const TH*)p.h + row * p.ldh;
+    const TH* dhp = (const TH*)p.dh + row * p.lddh;
     auto load = [&](int i, f32x8& g, f32x8& h) {
       const int c = (i * TPR + t) * kVec, n = live ? min(kVec, p.cols - c) : 0;
       if (n > 0) {
-        g = load8<XD>((const TX*)p.dy + row * p.ldy + c, n);
-        h = load8<HD>((const TH*)p.h + row * p.ldh + c, n);
+        g = load8<XD>(dy + c, n);
+        h = load8<HD>(hp + c, n);
       } else {
 #pragma unroll
         for (int e = 0; e < kVec; ++e) g[e] = h[e] = 0.f;
@@ -374,8 +491,36 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
       }
     };
     if constexpr (KEEP) {
+      if (raw) {
+        if (live) {
+          Raw<XD> gr[NV];
+          Raw<HD> hr[NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) load(i, gs[i], hs[i]);
+          for (int i = 0; i < NV; ++i) {
+            const int c = (i * TPR + t) * kVec;
+            gr[i] = load_raw<XD>(dy, c, p.cols);
+            hr[i] = load_raw<HD>(hp, c, p.cols);
+          }
+          if (kEarlyDh && p.dh) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) dhr[i] = load_raw<HD>(dhp, (i * TPR + t) * kVec, p.cols);
+          }
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int n = p.cols - (i * TPR + t) * kVec;
+            gs[i] = unpack<XD>(gr[i], n);
+            hs[i] = unpack<HD>(hr[i], n);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) gs[i][e] = hs[i][e] = 0.f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) load(i, gs[i], hs[i]);
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) scale(i, gs[i], hs[i], true);
     } else {
@@ -386,7 +531,7 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
       }
     }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) c1 += __shfl_xor(c1, d);
+    for (int d = (TPR < 64 ? TPR : 64) / 2; d > 0; d >>= 1) c1 += __shfl_xor(c1, d);
     if constexpr (TPR > 64) {
       // two buffers in turn: the next row's writes meet no reader of this one
       float* s = lds_s[it & 1][grp];
@@ -409,7 +554,7 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
 #pragma unroll
         for (int e = 0; e < kVec; ++e) g[e] = rho * __builtin_fmaf(-h[e], c1, g[e]);
         if (p.dh) {
-          const f32x8 a = load8<HD>((const TH*)p.dh + row * p.lddh + c, n);
+          const f32x8 a = kEarlyDh && raw ? unpack<HD>(dhr[kEarlyDh ? i : 0], n) : load8<HD>(dhp + c, n);
 #pragma unroll
           for (int e = 0; e < kVec; ++e) g[e] += a[e];
         }
@@ -532,6 +677,7 @@ template <int MODE, int XD, int RD>
 hipError_t launch_fwd_t(const NormParams& p, hipStream_t stream) {
   const int vecs = (p.cols + kVec - 1) / kVec;
 #define HARP_NORM_LAUNCH(TPR, NV) return launch_fwd_rows<MODE, XD, RD, TPR, NV>(p, stream);
+  if (vecs <= 16) HARP_NORM_LAUNCH(16, 1)
   if (vecs <= 64) HARP_NORM_LAUNCH(64, 1)
   if (vecs <= 128) HARP_NORM_LAUNCH(64, 2)
   if (vecs <= 256) HARP_NORM_LAUNCH(256, 1)
@@ -564,6 +710,7 @@ struct BwdShape {
 };
 BwdShape bwd_shape(int cols) {
   const int vecs = (cols + kVec - 1) / kVec;
+  if (vecs <= 16) return {32};
   if (vecs <= 128) return {8};
   if (vecs <= 1024) return {2};
   return {1};
@@ -579,6 +726,7 @@ hipError_t launch_bwd_t(const NormBwdParams& p, hipStream_t stream) {
                        dim3(TPR * GROUPS), 0, stream, p);                                                            \
     return hipGetLastError();                                                                                        \
   }
+  if (vecs <= 16) HARP_NORM_BWD(16, 1, 32)
   if (vecs <= 64) HARP_NORM_BWD(64, 1, 8)
   if (vecs <= 128) HARP_NORM_BWD(64, 2, 8)
   if (vecs <= 256) HARP_NORM_BWD(256, 1, 2)

@@ -422,3 +422,12 @@ def test_rows_whose_norm_is_not_finite():
     assert bool((y[3] == 0).all()) and bool((rows.dequantize(F32)[3] == 0).all())
     rows, _ = harp_amd.add_rms_norm_int8(x, None, None, 1e-6)
     assert float(rows.scales[0]) == 0.0 and bool((rows.values[0] == 0).all())
+
+
+@pytest.mark.parametrize("types", TYPES[:4], ids=str)
+@pytest.mark.parametrize("rows,cols", [(33, 15), (530, 33), (1000, 100), (77, 128), (2049, 8), (600, 520)])
+def test_many_narrow_rows(rows, cols, types):
+    """Rows that share a wave, the last ones of a block missing, in both directions and to 8 bits."""
+    test_forward_backward(rows, cols, types)
+    test_norm_int8(rows, cols, types[0], types[1])
+    test_quantize_is_exact(rows, cols, types[0])
