@@ -251,6 +251,7 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, co
     auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, false);
     return {y, given(residual) ? h : x};
   }
+  const c10::DeviceGuard guard(x.device());  // the capture of x's device
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
     const c10::Stream current = c10::hip::getCurrentHIPStream(x.get_device()).unwrap();
     check_capture(x, current, "x");

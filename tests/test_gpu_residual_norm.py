@@ -431,3 +431,14 @@ def test_many_narrow_rows(rows, cols, types):
     test_forward_backward(rows, cols, types)
     test_norm_int8(rows, cols, types[0], types[1])
     test_quantize_is_exact(rows, cols, types[0])
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_tensors_of_two_devices_are_refused(which):
+    for grad in (False, True):
+        ts = [torch.ones(3, 64, device=DEV), torch.ones(3, 64, device=DEV), torch.ones(64, device=DEV)]
+        ts[which] = ts[which].cpu()
+        for t in ts:
+            t.requires_grad_(grad)
+        with pytest.raises(RuntimeError, match="HIP device"):
+            harp_amd.add_rms_norm(*ts)
