@@ -567,6 +567,7 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
   // the groups' sums, in group order, one vector column at a time
   if constexpr (GROUPS > 1) {
     __shared__ float part[GROUPS][TPR * kVec];
+    constexpr int kAtOnce = GROUPS > 8 ? 2 : GROUPS;  // (32 groups at once would take 229 registers)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       __syncthreads();
@@ -574,10 +575,10 @@ __global__ __launch_bounds__(TPR* GROUPS) void norm_bwd_kernel(NormBwdParams p) 
       for (int e = 0; e < kVec; ++e) part[grp][e * TPR + t] = gw[i][e];
       __syncthreads();
       if (grp == 0) {
+#pragma unroll kAtOnce
+        for (int k = 1; k < GROUPS; ++k)
 #pragma unroll
-        for (int e = 0; e < kVec; ++e)
-#pragma unroll
-          for (int k = 1; k < GROUPS; ++k) gw[i][e] += part[k][e * TPR + t];
+          for (int e = 0; e < kVec; ++e) gw[i][e] += part[k][e * TPR + t];
       }
     }
     if (grp != 0) return;

@@ -42,7 +42,7 @@ extern "C" {
 enum {
   HARP_BLK_OK = 0,
   HARP_BLK_EINVAL = 1,       /* bad pointer, size, stride, alignment or dtype */
-  HARP_BLK_EUNSUPPORTED = 2, /* valid request this build does not handle (e.g. cols > 32768) */
+  HARP_BLK_EUNSUPPORTED = 2, /* valid request that the library does not handle (e.g. cols > 32768) */
   HARP_BLK_ENOMEM = 3,       /* workspace too small */
   HARP_BLK_ELAUNCH = 4       /* HIP launch or runtime error */
 };
