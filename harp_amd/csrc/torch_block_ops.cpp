@@ -6,14 +6,16 @@
 // The operators allocate their results from PyTorch's allocator and run on
 // the current HIP stream of the input's device.  Implementations are
 // registered for the CUDA dispatch key (HIP tensors carry it); the CPU key
-// raises.  add_rms_norm is differentiable (once); the others record no
-// gradient.
+// raises.  add_rms_norm is differentiable (once, in reverse mode); the others
+// have no derivative, and where a gradient would be recorded, or an argument
+// carries a forward-mode tangent, a call raises.
 //
 // Matrices are [.., C] tensors read as rows of C elements.  A tensor whose
 // leading dimensions are no single row stride, or whose last stride is not 1,
 // is copied first.  8-bit rows are never copied: they come from the operators
 // here, whose storage pads each row to 16 bytes.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -22,6 +24,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
+#include <string>
 #include <tuple>
 
 #include "harp_block_ops.h"
@@ -89,6 +92,12 @@ Vec vec_of(const OptTensor& v, const at::Tensor& ref, int64_t n, const char* nam
 }
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// A forward-mode tangent would be lost below the autograd keys.
+void refuse_tangent(const at::Tensor& t, const char* op) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "harp_block.", op,
+              " has no forward-mode derivative: an argument carries a tangent");
+}
 
 void check_input(const at::Tensor& x, const char* op) {
   TORCH_CHECK(x.is_cuda(), "harp_block.", op, ": tensors must be on a HIP device");
@@ -197,6 +206,7 @@ class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
     const bool need_x = wanted & 1, need_residual = wanted & 2, need_weight = wanted & 4;
     const at::Tensor &h = saved[0], &w = saved[1], &rstd = saved[2], &dy = grads[0];
     const at::Tensor dh = grads.size() > 1 ? grads[1] : at::Tensor();
+    for (const auto& t : grads) refuse_tangent(t, "add_rms_norm (backward)");
     torch::autograd::variable_list out(4);
     {
       at::AutoDispatchBelowADInplaceOrView guard;
@@ -241,8 +251,15 @@ void check_capture(const OptTensor& t, const c10::Stream& current, const char* n
               "graph's tensors (an earlier step's outputs or loss) before the capture");
 }
 
+void refuse_tangents(const at::Tensor& x, const OptTensor& residual, const OptTensor& weight) {
+  refuse_tangent(x, "add_rms_norm");
+  if (given(residual)) refuse_tangent(*residual, "add_rms_norm");
+  if (given(weight)) refuse_tangent(*weight, "add_rms_norm");
+}
+
 std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, const OptTensor& residual,
                                                          const OptTensor& weight, double eps) {
+  refuse_tangents(x, residual, weight);
   const bool record = at::GradMode::is_enabled() &&
                       (x.requires_grad() || (given(residual) && residual->requires_grad()) ||
                        (given(weight) && weight->requires_grad()));
@@ -472,6 +489,11 @@ std::vector<at::Tensor> qkv_int8(const at::Tensor& x, const at::Tensor& x_scales
 std::tuple<at::Tensor, at::Tensor> add_rms_norm_cpu(const at::Tensor&, const OptTensor&, const OptTensor&, double) {
   no_cpu("add_rms_norm");
 }
+std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd_cpu(const at::Tensor& x, const OptTensor& residual,
+                                                             const OptTensor& weight, double) {
+  refuse_tangents(x, residual, weight);
+  no_cpu("add_rms_norm");
+}
 std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8_cpu(const at::Tensor&, const OptTensor&,
                                                                      const OptTensor&, double) {
   no_cpu("add_rms_norm_int8");
@@ -492,6 +514,53 @@ std::vector<at::Tensor> qkv_int8_cpu(const at::Tensor&, const at::Tensor&, const
   no_cpu("qkv_int8");
 }
 
+// ---------------------------------------------------------------------------
+// The autograd kernels of the operators without a derivative: the checks, then
+// the operator below the autograd keys.
+void refuse_derivative(const char* op, const at::Tensor& t) {
+  refuse_tangent(t, op);
+  TORCH_CHECK(!t.defined() || !t.requires_grad() || !at::GradMode::is_enabled(), "harp_block.", op,
+              " is forward only: call it under torch.no_grad(), or on tensors that need no gradient");
+}
+void refuse_derivative(const char* op, const OptTensor& t) {
+  if (t.has_value()) refuse_derivative(op, *t);
+}
+void refuse_derivative(const char* op, const std::vector<at::Tensor>& ts) {
+  for (const auto& t : ts) refuse_derivative(op, t);
+}
+void refuse_derivative(const char* op, const c10::List<OptTensor>& ts) {
+  for (size_t i = 0; i < ts.size(); ++i) refuse_derivative(op, ts.get(i));
+}
+template <class T>
+void refuse_derivative(const char*, const T&) {}  // no tensor
+
+constexpr char kAddRmsNormInt8[] = "add_rms_norm_int8", kQuantizeInt8[] = "quantize_int8",
+               kDequantizeInt8[] = "dequantize_int8", kLinearInt8[] = "linear_int8",
+               kLinearInt8Dynamic[] = "linear_int8_dynamic", kQkvInt8[] = "qkv_int8";
+
+template <const char* OP, class F>
+struct ForwardOnly;
+template <const char* OP, class R, class... Args>
+struct ForwardOnly<OP, R(Args...)> {
+  static R call(Args... args) {
+    (refuse_derivative(OP, args), ...);
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow((std::string("harp_block::") + OP).c_str(), "")
+                               .template typed<R(Args...)>();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(args...);
+  }
+};
+
+void forward_only_kernels(torch::Library& m) {
+  m.impl(kAddRmsNormInt8, &ForwardOnly<kAddRmsNormInt8, decltype(add_rms_norm_int8)>::call);
+  m.impl(kQuantizeInt8, &ForwardOnly<kQuantizeInt8, decltype(quantize_int8)>::call);
+  m.impl(kDequantizeInt8, &ForwardOnly<kDequantizeInt8, decltype(dequantize_int8)>::call);
+  m.impl(kLinearInt8, &ForwardOnly<kLinearInt8, decltype(linear_int8)>::call);
+  m.impl(kLinearInt8Dynamic, &ForwardOnly<kLinearInt8Dynamic, decltype(linear_int8_dynamic)>::call);
+  m.impl(kQkvInt8, &ForwardOnly<kQkvInt8, decltype(qkv_int8)>::call);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(harp_block, m) {
@@ -509,7 +578,15 @@ TORCH_LIBRARY(harp_block, m) {
       "eps, Tensor? freqs_cis) -> Tensor[]");
 }
 
-TORCH_LIBRARY_IMPL(harp_block, AutogradCUDA, m) { m.impl("add_rms_norm", &add_rms_norm_autograd); }
+TORCH_LIBRARY_IMPL(harp_block, AutogradCUDA, m) {
+  m.impl("add_rms_norm", &add_rms_norm_autograd);
+  forward_only_kernels(m);
+}
+
+TORCH_LIBRARY_IMPL(harp_block, AutogradCPU, m) {
+  m.impl("add_rms_norm", &add_rms_norm_autograd_cpu);
+  forward_only_kernels(m);
+}
 
 TORCH_LIBRARY_IMPL(harp_block, CUDA, m) {
   m.impl("add_rms_norm", &add_rms_norm);

@@ -243,3 +243,66 @@ def test_gradients_of_scales_are_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="HIP device only"):
             call()
+
+
+def _dual_calls(dual, plain):
+    """Every operator with one argument made dual; plain gives an int8 [3, 64] and floats."""
+    f, q, s, w, ops = plain["f"], plain["q"], plain["s"], plain["w"], torch.ops.harp_block
+    rows = harp_amd.Int8Rows(q, s)
+    lin = harp_amd.Int8Linear(rows, w[:3])
+    biased = harp_amd.Int8Linear(rows)
+    biased.bias = dual(w[:3])
+    qkv = (q.view(1, 3, 64), s.view(1, 3), [q.repeat(43, 1)[:128]], [s.repeat(43)[:128]])
+    return [
+        lambda: harp_amd.add_rms_norm(dual(f)), lambda: harp_amd.add_rms_norm(f, dual(f)),
+        lambda: harp_amd.add_rms_norm(f, f, dual(w)),
+        lambda: harp_amd.add_rms_norm(dual(f.clone().requires_grad_(True))),
+        lambda: harp_amd.add_rms_norm_int8(dual(f)), lambda: harp_amd.add_rms_norm_int8(f, dual(f)),
+        lambda: harp_amd.add_rms_norm_int8(f, None, dual(w)),
+        lambda: harp_amd.quantize_int8(dual(f)), lambda: harp_amd.Int8Rows(q, dual(s)).dequantize(),
+        lambda: harp_amd.int8_linear(harp_amd.Int8Rows(q, dual(s)), rows),
+        lambda: harp_amd.int8_linear(rows, harp_amd.Int8Rows(q, dual(s))),
+        lambda: harp_amd.int8_linear(rows, rows, dual(w[:3])),
+        lambda: lin(dual(f)), lambda: lin(harp_amd.Int8Rows(q, dual(s))), lambda: biased(f), lambda: biased(rows),
+        lambda: ops.qkv_int8(qkv[0], dual(qkv[1]), *qkv[2:], [None], [0.0], None),
+        lambda: ops.qkv_int8(*qkv[:3], [dual(qkv[3][0])], [None], [0.0], None),
+        lambda: ops.qkv_int8(*qkv, [dual(torch.ones_like(qkv[3][0]))], [1e-6], None),
+    ]
+
+
+def assert_tangents_are_refused(device):
+    import torch.autograd.forward_ad as fwAD
+
+    g = torch.Generator().manual_seed(1)
+    plain = {"f": torch.randn(3, 64, generator=g), "s": torch.rand(3, generator=g), "w": torch.rand(64, generator=g),
+             "q": torch.randint(-127, 128, (3, 64), generator=g, dtype=torch.int8)}
+    plain = {k: v.to(device) for k, v in plain.items()}
+    for grad in (True, False):
+        with fwAD.dual_level(), torch.set_grad_enabled(grad):
+            for i, call in enumerate(_dual_calls(lambda t: fwAD.make_dual(t, torch.ones_like(t)), plain)):
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call()
+                    pytest.fail(f"call {i} dropped its tangent")
+    with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        torch.func.jvp(lambda t: harp_amd.quantize_int8(t)[1], (plain["f"],), (plain["f"],))
+
+
+def test_forward_mode_derivatives_are_refused():
+    assert_tangents_are_refused("cpu")
+
+
+def test_operators_refuse_gradients():
+    """The operators themselves, as the Python functions do."""
+    ops = torch.ops.harp_block
+    x, w = torch.zeros(3, 64, requires_grad=True), torch.zeros(64, requires_grad=True)
+    q, s = torch.zeros(3, 64, dtype=torch.int8), torch.zeros(3)
+    ws = torch.zeros(3, requires_grad=True)
+    for call in (lambda: ops.quantize_int8(x), lambda: ops.add_rms_norm_int8(x.detach(), None, w, 1e-5),
+                 lambda: ops.linear_int8(q, s, q, ws, None, torch.float32),
+                 lambda: ops.linear_int8_dynamic(x, q, s, None, torch.float32),
+                 lambda: ops.dequantize_int8(q, ws, torch.float32),
+                 lambda: ops.qkv_int8(q.view(1, 3, 64), s.view(1, 3), [q], [ws], [None], [0.0], None)):
+        with pytest.raises(RuntimeError, match="forward only"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="HIP device only"):
+            call()

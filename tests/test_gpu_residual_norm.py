@@ -442,3 +442,22 @@ def test_tensors_of_two_devices_are_refused(which):
             t.requires_grad_(grad)
         with pytest.raises(RuntimeError, match="HIP device"):
             harp_amd.add_rms_norm(*ts)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent on any argument, or on a gradient given to the backward, raises and is not dropped."""
+    import torch.autograd.forward_ad as fwAD
+
+    from tests.test_block_abi import assert_tangents_are_refused
+
+    assert_tangents_are_refused(DEV)
+    g, x, r, w = _case(4, 72, (F32, F32, F32), 2)
+    x.requires_grad_(True)
+    y, h = harp_amd.add_rms_norm(x, r, w)
+    with fwAD.dual_level():
+        one = fwAD.make_dual(torch.ones_like(y), torch.ones_like(y))
+        for out in (y, h):
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                torch.autograd.grad(out, x, one, retain_graph=True)
+    (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert bool(torch.isfinite(gx).all())
