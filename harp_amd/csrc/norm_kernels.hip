@@ -263,14 +263,16 @@ __device__ __forceinline__ void row_reduce(float& s, uint32_t& m, float* lds_s, 
 // whatever reads it is NaN too; so has a row whose normed values are not finite
 // (factor infinite: eps 0 and squares that sum to 0).  A row of zeros has scale
 // and steps zero.
-// Maxima below 2^-100 are raised by 2^100 first, or 127 / a would overflow.
+// Maxima below 2^-100 are raised by 2^100 first, or 127 / a would overflow;
+// those above 2^100 are lowered by it, or 127 v would.  (Values that become
+// denormal or zero by that are far below a step.)
 struct Steps {
   float pre, a, inv, scale;
 };
 __device__ __forceinline__ Steps row_steps(uint32_t max_bits, float factor) {
   Steps t;
   const float a = from_bits(max_bits);
-  t.pre = a < 0x1p-100f ? 0x1p100f : 1.f;
+  t.pre = a < 0x1p-100f ? 0x1p100f : a > 0x1p100f ? 0x1p-100f : 1.f;
   t.a = a * t.pre;
   t.inv = __fdiv_rn(127.f, t.a);
   t.scale = __fdiv_rn(a * factor, 127.f);
@@ -283,9 +285,15 @@ __device__ __forceinline__ Steps row_steps(uint32_t max_bits, float factor) {
 }
 
 // v * 127 / a to the nearest integer, ties to even, of one vector, packed.
-// v * inv is off by a few 2^-24 of its size, so only values that close to a
-// border between two steps can round to the wrong one: where a vector has
-// one, 127 v - q a is formed exactly and decides.
+// f = v * inv is off by 2^-23 of its size (two roundings; 127 steps: 1.52e-5),
+// so only values that close to a border between two steps can round to the wrong
+// one: where a vector has one, the sign of 254 v - m a decides, with m / 2 the
+// border on f's side of q.  It is exact: m a is its rounding p and the rounding's
+// error; 254 v - p is less than 2^-13 a beside a border and, v being at least
+// a / 254, a multiple of 2^-31 a, so one fma forms it without a rounding.  (Taken
+// from 127 v - q a in one fp32, 51 of 12000 values within one fp32 step of a
+// border came out a step off; in 64 bits 8192 bf16 rows of 3840, many of whose
+// values lie on a border, take 22.5 us instead of 20.5.)
 __device__ __forceinline__ uint2 pack_steps(const f32x8& v, const Steps& t) {
   f32x8 q;
   float far = 0.f;
@@ -295,13 +303,14 @@ __device__ __forceinline__ uint2 pack_steps(const f32x8& v, const Steps& t) {
     q[e] = __builtin_rintf(f);
     far = __builtin_fmaxf(far, __builtin_fabsf(f - q[e]));
   }
-  if (__builtin_expect(far > 0.4999f, 0)) {
+  if (__builtin_expect(far > 0.49998f, 0)) {
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
-      const float p = q[e] * t.a, err = __builtin_fmaf(q[e], t.a, -p);
-      const float d2 = 2.f * (__builtin_fmaf(127.f, v[e] * t.pre, -p) - err), ad = __builtin_fabsf(d2);
+      const float x = v[e] * t.pre, one = __builtin_copysignf(1.f, x * t.inv - q[e]), m = 2.f * q[e] + one;
+      const float p = m * t.a, err = __builtin_fmaf(m, t.a, -p);
+      const float over = one * (__builtin_fmaf(254.f, x, -p) - err);
       const bool odd = ((int)q[e] & 1) != 0;
-      if (ad > t.a || (ad == t.a && odd)) q[e] += __builtin_copysignf(1.f, d2);
+      if (over > 0.f || (over == 0.f && odd)) q[e] += one;
     }
   }
   uint32_t w[2] = {0, 0};

@@ -461,3 +461,38 @@ def test_forward_mode_derivatives_are_refused():
                 torch.autograd.grad(out, x, one, retain_graph=True)
     (gx,) = torch.autograd.grad(y, x, torch.ones_like(y))
     assert bool(torch.isfinite(gx).all())
+
+
+def _border_rows(g, rows, scale):
+    """fp32 rows with a maximum of up to `scale` and, for every border between two steps, the value nearest to it
+    and that value's neighbours, either sign."""
+    most = ((torch.rand(rows, 1, generator=g) + 1) * (scale / 2)).float()
+    at = ((torch.arange(127, dtype=torch.float64) + 0.5) / 127 * most.double()).float()
+    up, down = torch.nextafter(at, most * 2 if scale < 1e38 else most), torch.nextafter(at, torch.zeros(()))
+    sign = torch.randint(0, 2, (rows, 381), generator=g) * 2.0 - 1.0
+    return torch.cat([most, torch.cat([at, up, down], -1) * sign, most / 2], -1)
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -140, 1e-30, 2.0 ** -100, 1.0, 197.0, 1e30, 2.0 ** 121, 2.0 ** 122, 3.4e38], ids=str)
+def test_quantize_beside_borders(scale):
+    """fp32 values next to a border between two steps go to the nearer one, and halves to the even one.  In 64 bits
+    127 x is exact and its quotient with the maximum nowhere nearer than 2^-33 to a border that it is not on."""
+    x = _border_rows(_gen(7), 400, scale).to(DEV)
+    if scale == 197.0:
+        x[0, 0], x[0, 1:] = 196.8303680419922, 0.7749227285385132  # 0.5 + 1.3e-8 steps: 1
+    q, s = harp_amd.quantize_int8(x)
+    most = x.double().abs().amax(-1, keepdim=True)
+    want = torch.round(127 * x.double() / most)
+    assert torch.equal(q.double(), want), int((q.double() != want).sum())
+    assert scale != 197.0 or bool((q[0, 1:] == 1).all())
+
+
+@pytest.mark.parametrize("types", [(B16, B16, B16), (B16, None, B16), (B16, B16, None), (F32, F32, None), (B16, F32, None)],
+                         ids=str)
+def test_norm_int8_steps_are_exact(types):
+    """The factor 1 / rms cancels from the steps: where h w is exact in fp32 (16-bit h and weight, or no weight),
+    they equal those of 127 h w / max |h w| in 64 bits."""
+    _, x, r, w = _case(700, 3840, types, 31)
+    (q, _), h = harp_amd.add_rms_norm_int8(x, r, w, 1e-5)
+    v = h.double() if w is None else h.double() * w.double()
+    assert torch.equal(q.double(), torch.round(127 * v / v.abs().amax(-1, keepdim=True)))
