@@ -66,7 +66,9 @@ Rows rows_of(const at::Tensor& t, const char* name) {
   TORCH_CHECK(r.cols >= 1, name, " must have a last dimension of at least 1");
   r.rows = t.numel() / r.cols;
   checked_int(r.rows, "rows");
-  r.t = t.stride(-1) == 1 || r.cols == 1 ? t : t.contiguous();
+  // (the dispatcher resolves a negated view only for what is called through it)
+  r.t = t.is_neg() ? t.resolve_neg() : t;
+  if (r.t.stride(-1) != 1 && r.cols != 1) r.t = r.t.contiguous();
   if (r.t.dim() != 2) r.t = r.t.reshape({r.rows, r.cols});
   r.p = r.t.const_data_ptr();
   r.ld = r.rows > 1 ? r.t.stride(0) : r.cols;
@@ -85,7 +87,7 @@ Vec vec_of(const OptTensor& v, const at::Tensor& ref, int64_t n, const char* nam
   if (!v.has_value() || !v->defined()) return r;
   check_float(*v, ref, name);
   TORCH_CHECK(v->dim() == 1 && v->numel() == n, name, " must be a vector of ", n, " elements, got ", v->sizes());
-  r.t = v->contiguous();
+  r.t = (v->is_neg() ? v->resolve_neg() : *v).contiguous();
   r.p = r.t.const_data_ptr();
   r.dtype = code(r.t.scalar_type());
   return r;

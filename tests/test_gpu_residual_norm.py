@@ -496,3 +496,34 @@ def test_norm_int8_steps_are_exact(types):
     (q, _), h = harp_amd.add_rms_norm_int8(x, r, w, 1e-5)
     v = h.double() if w is None else h.double() * w.double()
     assert torch.equal(q.double(), torch.round(127 * v / v.abs().amax(-1, keepdim=True)))
+
+
+@pytest.mark.parametrize("cols", [1, 72])
+@pytest.mark.parametrize("grad", [False, True])
+def test_negated_views(grad, cols):
+    """The imaginary part of a conjugate is a view whose sign is turned lazily (with a stride of 2: rows of one
+    value are read in place)."""
+    def turned(t):
+        v = torch.complex(torch.zeros_like(t), -t).conj().imag
+        assert v.is_neg() and torch.equal(v, t)
+        return v
+
+    g, x, r, w = _case(6, cols, (F32, F32, F32), 17)
+    dy, dh = _rand(g, 6, cols, dtype=F32), _rand(g, 6, cols, dtype=F32)
+    plain = [t.requires_grad_(grad) for t in (x, r, w)]
+    views = [turned(t.detach()).requires_grad_(grad) for t in plain]
+    want, got = harp_amd.add_rms_norm(*plain), harp_amd.add_rms_norm(*views)
+    alone, alone2 = harp_amd.add_rms_norm(x, None, w), harp_amd.add_rms_norm(views[0], None, views[2])
+    assert all(torch.equal(a, b) for a, b in zip((*want, *alone), (*got, *alone2)))
+    if grad:
+        a = torch.autograd.grad(want, plain, (dy, dh)) + torch.autograd.grad(alone[0], (x, w), dy)
+        b = torch.autograd.grad(got, views, (turned(dy), turned(dh))) \
+            + torch.autograd.grad(alone2[0], (views[0], views[2]), turned(dy))
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    x, w = x.detach(), w.detach()
+    for a, b in ((harp_amd.quantize_int8(x), harp_amd.quantize_int8(turned(x))),
+                 (harp_amd.add_rms_norm_int8(x, x, w)[0], harp_amd.add_rms_norm_int8(turned(x), turned(x), turned(w))[0])):
+        assert torch.equal(a.values, b.values) and torch.equal(a.scales, b.scales)
+    lin = harp_amd.Int8Linear.from_linear(torch.nn.Linear(cols, 9, device=DEV))
+    with torch.no_grad():
+        assert torch.equal(lin(x), lin(turned(x)))
