@@ -380,21 +380,15 @@ at::Tensor dequantize_int8(const at::Tensor& values, const at::Tensor& scales, a
   return out;
 }
 
-// Bytes of a row of a module's weight (int8.py): whole cache lines for long
-// rows, so that a tile's 128 bytes of a row are one line (1333 tokens x 1001
-// features of 2570 columns: 12.6 us instead of 14.6).
-int64_t weight_ld8(int64_t cols) {
-  const int64_t unit = cols < 1024 ? 16 : 128;
-  return (cols + unit - 1) / unit * unit;
-}
-
-// 8-bit rows x times the first x.size(-1) columns of weight (a module's
-// padded storage, or rows of exactly that many)
+// 8-bit rows x times those of weight; in_features: times weight's first
+// in_features columns (a module's padded storage, without a view of it)
 at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at::Tensor& weight,
-                       const at::Tensor& weight_scales, const OptTensor& bias, at::ScalarType dtype) {
+                       const at::Tensor& weight_scales, const OptTensor& bias, at::ScalarType dtype,
+                       std::optional<int64_t> in_features) {
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "linear_int8: bfloat16 or float32, got ", dtype);
   const Rows8 xr = rows8_of(x, x_scales, "x");
-  TORCH_CHECK(weight.dim() == 2 && (weight.size(1) == xr.cols || weight.size(1) == weight_ld8(xr.cols)) &&
+  TORCH_CHECK(!in_features || *in_features == xr.cols, "x must have ", *in_features, " columns, got ", xr.cols);
+  TORCH_CHECK(weight.dim() == 2 && (in_features ? weight.size(1) >= xr.cols : weight.size(1) == xr.cols) &&
                   weight.device() == x.device(),
               "weight must be [N, ", xr.cols, "] on ", x.device(), ", got ", weight.sizes(), " on ", weight.device());
   const Rows8 wr = rows8_of(weight, weight_scales, "weight");
@@ -412,9 +406,9 @@ at::Tensor linear_int8(const at::Tensor& x, const at::Tensor& x_scales, const at
 
 // the same of a bf16 or fp32 tensor, quantised first
 at::Tensor linear_int8_dynamic(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& weight_scales,
-                               const OptTensor& bias, at::ScalarType dtype) {
+                               const OptTensor& bias, at::ScalarType dtype, std::optional<int64_t> in_features) {
   const auto [q, scales] = quantize_int8(x);
-  return linear_int8(q, scales, weight, weight_scales, bias, dtype);
+  return linear_int8(q, scales, weight, weight_scales, bias, dtype, in_features);
 }
 
 // fp32 (cos, sin) rows of the complex [S, 64] or [B or 1, S, 64] table
@@ -503,11 +497,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_int8_cpu(const at::T
 std::tuple<at::Tensor, at::Tensor> quantize_int8_cpu(const at::Tensor&) { no_cpu("quantize_int8"); }
 at::Tensor dequantize_int8_cpu(const at::Tensor&, const at::Tensor&, at::ScalarType) { no_cpu("dequantize_int8"); }
 at::Tensor linear_int8_cpu(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                           const OptTensor&, at::ScalarType) {
+                           const OptTensor&, at::ScalarType, std::optional<int64_t>) {
   no_cpu("linear_int8");
 }
 at::Tensor linear_int8_dynamic_cpu(const at::Tensor&, const at::Tensor&, const at::Tensor&, const OptTensor&,
-                                   at::ScalarType) {
+                                   at::ScalarType, std::optional<int64_t>) {
   no_cpu("linear_int8_dynamic");
 }
 std::vector<at::Tensor> qkv_int8_cpu(const at::Tensor&, const at::Tensor&, const std::vector<at::Tensor>&,
@@ -571,10 +565,11 @@ TORCH_LIBRARY(harp_block, m) {
   m.def("quantize_int8(Tensor x) -> (Tensor, Tensor)");
   m.def("dequantize_int8(Tensor values, Tensor scales, ScalarType dtype) -> Tensor");
   m.def(
-      "linear_int8(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype) -> "
-      "Tensor");
+      "linear_int8(Tensor x, Tensor x_scales, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype, "
+      "int? in_features=None) -> Tensor");
   m.def(
-      "linear_int8_dynamic(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype) -> Tensor");
+      "linear_int8_dynamic(Tensor x, Tensor weight, Tensor weight_scales, Tensor? bias, ScalarType dtype, int? "
+      "in_features=None) -> Tensor");
   m.def(
       "qkv_int8(Tensor x, Tensor x_scales, Tensor[] weights, Tensor[] weight_scales, Tensor?[] norm_weights, float[] "
       "eps, Tensor? freqs_cis) -> Tensor[]");

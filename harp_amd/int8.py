@@ -85,7 +85,9 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
 
 
 def _weight_row_bytes(cols: int) -> int:
-    """Bytes of a row of a module's weight: whole 128-byte cache lines for long rows."""
+    """Bytes of a row of a module's weight: whole 128-byte cache lines for long rows, so that a
+    tile's 128 bytes of a row are one line (1333 tokens x 1001 features of 2570 columns: 12.6 us
+    instead of 14.6)."""
     unit = 16 if cols < 1024 else 128
     return -(-cols // unit) * unit
 
@@ -143,9 +145,10 @@ class Int8Linear(nn.Module):
         if rows:
             _refuse_grad("Int8Linear", x.scales)
             return _ops().linear_int8(x.values, x.scales, self.weight_values, self.weight_scales, self.bias,
-                                      self.out_dtype)
+                                      self.out_dtype, self.in_features)
         _refuse_grad("Int8Linear", x)
-        return _ops().linear_int8_dynamic(x, self.weight_values, self.weight_scales, self.bias, self.out_dtype)
+        return _ops().linear_int8_dynamic(x, self.weight_values, self.weight_scales, self.bias, self.out_dtype,
+                                          self.in_features)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

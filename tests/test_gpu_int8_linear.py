@@ -287,3 +287,23 @@ def test_module_with_padded_rows(K):
         _assert_linear(y, x, w, None, M)
         xf = torch.randn(M, K, generator=g).to(DEV)
         assert torch.equal(lin(xf), lin(harp_amd.quantize_int8(xf)))
+
+
+@pytest.mark.parametrize("K,wide", [(40, 48), (40, 56), (1001, 1024), (2570, 2576), (2570, 2688)])
+def test_wider_weight_is_refused(K, wide):
+    """Columns are dropped only where in_features says how many count."""
+    ops = torch.ops.harp_block
+    g = _gen(K)
+    x, w = _rows(g, 3, K), _rows(g, 8, wide)
+    xf = torch.randn(3, K, generator=g).to(DEV)
+    for call in (lambda: ops.linear_int8(x.values, x.scales, w.values, w.scales, None, F32),
+                 lambda: ops.linear_int8_dynamic(xf, w.values, w.scales, None, F32),
+                 lambda: ops.linear_int8(x.values, x.scales, w.values, w.scales, None, F32, K - 1),
+                 lambda: ops.linear_int8(x.values, x.scales, w.values, w.scales, None, F32, wide),
+                 lambda: ops.linear_int8(x.values, x.scales, w.values[:, :K - 1], w.scales, None, F32, K)):
+        with pytest.raises(RuntimeError, match="must (be|have)"):
+            call()
+    first = harp_amd.Int8Rows(w.values[:, :K], w.scales)
+    y = ops.linear_int8(x.values, x.scales, w.values, w.scales, None, F32, K)
+    assert torch.equal(y, harp_amd.int8_linear(x, first, None, F32))
+    _assert_linear(y, x, first, None, (K, wide))
