@@ -246,6 +246,7 @@ int harp_blk_dequantize_int8(const int8_t* q, int64_t ld_q, const float* scales,
                              int out_dtype, int rows, int cols, void* stream) {
   int rc;
   if (rows < 0 || cols < 1) return fail(HARP_BLK_EINVAL, "rows=%d, cols=%d: rows of at least one value", rows, cols);
+  if (cols > kMaxTokens) return fail(HARP_BLK_EUNSUPPORTED, "cols=%d > 2^30", cols);  // indexes of a row stay in 32 bits
   if (rows == 0) return ok();
   if ((rc = check_rows8(q, ld_q, cols, INT64_MAX, false, "q"))) return rc;
   if ((rc = check_floats(scales, "scales"))) return rc;

@@ -96,7 +96,7 @@ HARP_BLK_API int harp_blk_add_rms_norm_int8(const void* x, int64_t ld_x, int x_d
 HARP_BLK_API int harp_blk_quantize_int8(const void* x, int64_t ld_x, int x_dtype, int8_t* q, int64_t ld_q,
                                         float* scales, int rows, int cols, void* stream);
 
-/* out = values * scales, in out_dtype. */
+/* out = values * scales, in out_dtype.  1 <= cols <= 2^30. */
 HARP_BLK_API int harp_blk_dequantize_int8(const int8_t* q, int64_t ld_q, const float* scales, void* out,
                                           int64_t ld_out, int out_dtype, int rows, int cols, void* stream);
 

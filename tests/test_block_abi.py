@@ -306,3 +306,23 @@ def test_operators_refuse_gradients():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="HIP device only"):
             call()
+
+
+@pytest.mark.parametrize("over,code,msg", [
+    (dict(cols=2 ** 31 - 1, ldq=2 ** 31, ldo=2 ** 31), EUNSUPPORTED, "2^30"),  # 15 more would pass 31 bits
+    (dict(cols=2 ** 30 + 1, ldq=2 ** 31, ldo=2 ** 31), EUNSUPPORTED, "2^30"),
+    (dict(cols=0), EINVAL, "at least one value"),
+    (dict(rows=-1), EINVAL, "at least one value"),
+    (dict(q=FAKE + 8), EINVAL, "16-byte aligned"),
+    (dict(ldq=48), EINVAL, "multiple of 16 in [64"),
+    (dict(s=None), EINVAL, "scales is NULL"),
+    (dict(o=None), EINVAL, "out is NULL"),
+    (dict(ldo=63), EINVAL, "may not overlap"),
+    (dict(od=2), EINVAL, "dtype"),
+    (dict(rows=0, q=None), 0, ""),
+])
+def test_dequantize_refuses(over, code, msg):
+    a = {**dict(q=FAKE, ldq=64, s=FAKE, o=FAKE, ldo=64, od=BF16, rows=4, cols=64), **over}
+    rc = harp_amd.load_abi().harp_blk_dequantize_int8(a["q"], a["ldq"], a["s"], a["o"], a["ldo"], a["od"], a["rows"],
+                                                      a["cols"], None)
+    assert rc == code and msg in _err(), (rc, _err())
