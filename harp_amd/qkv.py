@@ -72,7 +72,8 @@ def fused_supported(attn, hidden_states: torch.Tensor, freqs_cis: Optional[torch
     if x.is_contiguous() and not _aligned16(x):  # qkv_project passes x itself (a copy only when strided)
         return False
     lins = [getattr(attn, n, None) for n in ("to_q", "to_k", "to_v")]
-    if any(m is None or getattr(m, "bias", None) is not None or not hasattr(m, "weight") for m in lins):
+    if any(m is None or getattr(m, "bias", None) is not None or not isinstance(getattr(m, "weight", None), torch.Tensor)
+           for m in lins):  # (an Int8Linear's weight is no tensor)
         return False
     n_out = lins[0].weight.size(0)
     if n_out % HEAD_DIM or n_out != attn.heads * HEAD_DIM:

@@ -296,3 +296,19 @@ def test_modules_round_trip():
         q8.to_q(x.detach()[..., :128])
     with pytest.raises(ValueError, match="multiple of sp_size"):
         harp_amd.RingZAttention(q8, 3)(x.detach(), f)
+
+
+@pytest.mark.parametrize("which", [("to_q",), ("to_v",), ("to_q", "to_k")], ids=str)
+def test_some_projections_in_8_bits(which):
+    """An Int8Linear stands in for any of the projections: they then run one by one."""
+    attn = _attention(_gen(14), 256, 2)
+    for name in which:
+        setattr(attn, name, harp_amd.Int8Linear.from_linear(getattr(attn, name)))
+    x, f = _rand(_gen(15), 1, 64, 256), _freqs(64)
+    with torch.no_grad():
+        for a, b in zip(harp_amd.project_qkv(attn, x, f), harp_amd.project_qkv(attn, x, f, fused=False)):
+            assert a.shape == (1, 2, 64, 128) and torch.equal(a, b)
+        assert torch.equal(harp_amd.project_qkv(attn, x, f)[2], attn.to_v(x).unflatten(-1, (2, 128)).transpose(1, 2))
+        assert bool(torch.isfinite(harp_amd.RingZAttention(attn, 2)(x, f)).all())
+        with pytest.raises(ValueError, match="8-bit projections"):
+            harp_amd.project_qkv(attn, harp_amd.quantize_int8(x), f)
