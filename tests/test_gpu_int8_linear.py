@@ -292,6 +292,7 @@ def test_module_with_padded_rows(K):
 @pytest.mark.parametrize("K,wide", [(40, 48), (40, 56), (1001, 1024), (2570, 2576), (2570, 2688)])
 def test_wider_weight_is_refused(K, wide):
     """Columns are dropped only where in_features says how many count."""
+    harp_amd.load_block_ops()
     ops = torch.ops.harp_block
     g = _gen(K)
     x, w = _rows(g, 3, K), _rows(g, 8, wide)
