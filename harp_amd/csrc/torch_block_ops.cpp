@@ -173,11 +173,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rms_norm_backward(const at::T
   return {dx, dres, gw};
 }
 
-// (y, h) without a gradient; h is x without a residual
+// (y, h) without a gradient; h is undefined (None) without a residual: no result shares memory with x
 std::tuple<at::Tensor, at::Tensor> add_rms_norm(const at::Tensor& x, const OptTensor& residual,
                                                 const OptTensor& weight, double eps) {
   auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, false);
-  return {y, given(residual) ? h : x.alias()};
+  return {y, h};
 }
 
 // The differentiable form: y, and h where there is a residual.
@@ -267,8 +267,7 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, co
                        (given(weight) && weight->requires_grad()));
   if (!record) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [y, h, rstd] = add_rms_norm_forward(x, residual, weight, eps, false);
-    return {y, given(residual) ? h : x};
+    return add_rms_norm(x, residual, weight, eps);
   }
   const c10::DeviceGuard guard(x.device());  // the capture of x's device
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
@@ -278,7 +277,7 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, co
     check_capture(weight, current, "weight");
   }
   auto out = AddRMSNorm::apply(x, residual, weight, eps);
-  return {out[0], given(residual) ? out[1] : x};
+  return {out[0], given(residual) ? out[1] : at::Tensor()};
 }
 
 // int8 values of shape `sizes` whose rows are padded to 16 bytes

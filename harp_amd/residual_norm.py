@@ -32,7 +32,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
                  eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
     """(y, h): h = x + residual in the residual's type (x itself without a
     residual), y = h / sqrt(mean(h^2) + eps) * weight in x's type."""
-    return _ops().add_rms_norm(x, residual, weight, eps)
+    y, h = _ops().add_rms_norm(x, residual, weight, eps)
+    return y, (x if residual is None else h)
 
 
 def add_rms_norm_int8(x: torch.Tensor, residual: Optional[torch.Tensor] = None,

@@ -527,3 +527,17 @@ def test_negated_views(grad, cols):
     lin = harp_amd.Int8Linear.from_linear(torch.nn.Linear(cols, 9, device=DEV))
     with torch.no_grad():
         assert torch.equal(lin(x), lin(turned(x)))
+
+
+@pytest.mark.parametrize("mode", ["grad", "no_grad", "inference"])
+def test_operator_results_share_no_memory_with_x(mode):
+    """The schema declares new tensors: without a residual the second is None, and the function gives x itself."""
+    harp_amd.load_block_ops()
+    x, w = torch.randn(4, 72, device=DEV).requires_grad_(mode == "grad"), torch.ones(72, device=DEV)
+    with torch.inference_mode(mode == "inference"), torch.set_grad_enabled(mode == "grad"):
+        y, h = torch.ops.harp_block.add_rms_norm(x, None, w, 1e-5)
+        assert h is None
+        y2, h2 = harp_amd.add_rms_norm(x, None, w, 1e-5)
+        assert h2 is x and torch.equal(y, y2) and y.requires_grad == (mode == "grad")
+        _, h = torch.ops.harp_block.add_rms_norm(x, x, w, 1e-5)
+        assert torch.equal(h, x + x) and h.data_ptr() != x.data_ptr()
