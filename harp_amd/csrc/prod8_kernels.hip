@@ -677,6 +677,7 @@ const Kind kKinds[] = {
     {128, 256, true, kAny, 7.5, 0.80, 8.0, 1, launch_tiles<2, 2, 2, 4, 1, 128, 3>},
     {256, 256, true, kAny, 11.0, 1.33, 15.0, 1, launch_tiles<2, 4, 2, 4, 1, 128, 2>},
 };
+constexpr int kNumKinds = sizeof(kKinds) / sizeof(kKinds[0]);
 
 double kind_us(const Kind& k, const Prod8Params& p, int64_t rows, int cus) {
   const int64_t blocks = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features) * ((rows + k.tokens - 1) / k.tokens);
@@ -691,20 +692,24 @@ bool takes(const Kind& k, const Prod8Params& p, bool norm, int64_t rows) {
   return (!norm || k.heads) && rows <= k.max_tokens && tiles <= kMaxBlocks;
 }
 
-const Kind* best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, double* us) {
-  const Kind* best = nullptr;
-  for (const Kind& k : kKinds) {
-    if (!takes(k, p, norm, rows)) continue;
-    const double t = kind_us(k, p, rows, cus);
-    if (!best || t < *us) {
-      best = &k;
+// index of the kind with the smallest time, or -1
+int best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, double* us) {
+  int best = -1;
+  for (int i = 0; i < kNumKinds; ++i) {
+    if (!takes(kKinds[i], p, norm, rows)) continue;
+    const double t = kind_us(kKinds[i], p, rows, cus);
+    if (best < 0 || t < *us) {
+      best = i;
       *us = t;
     }
   }
   return best;
 }
 
-}  // namespace
+// The launches of a call: kind of the first rows, and of the rest (-1: none).
+struct Plan {
+  int first = -1, rest = -1, rows = 0;
+};
 
 // The kind with the smallest time for the call; where a kind's last round
 // would be part full, its whole rounds may run as one launch and the rows left
@@ -713,37 +718,73 @@ const Kind* best_kind(const Prod8Params& p, bool norm, int64_t rows, int cus, do
 // same kind start as others end, so a second launch of them only adds a stop
 // (q, k, v of 8192 tokens: 372 us instead of 363).  Over 133 shapes from 1 to
 // 8192 tokens the kind chosen for a whole call takes 0.4% more than the best.
-hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
-  bool norm = false;
-  for (int i = 0; i < p.n_outs; ++i) norm |= p.out[i].norm_w != nullptr;
-  const int cus = device_cus();
+Plan plan_of(const Prod8Params& p, bool norm, int cus) {
   double us = 0;
-  const Kind* kind = best_kind(p, norm, p.M, cus, &us);
-  const Kind *first = nullptr, *rest = nullptr;
-  int rows1 = 0;
-  for (const Kind& k : kKinds) {
+  Plan plan;
+  plan.first = best_kind(p, norm, p.M, cus, &us);
+  plan.rows = p.M;
+  for (int i = 0; i < kNumKinds; ++i) {
+    const Kind& k = kKinds[i];
     if (!takes(k, p, norm, 1) || k.per_cu > 1) continue;
     const int64_t per_row_tile = (int64_t)p.n_outs * ((p.N + k.features - 1) / k.features);
     const int64_t blocks = per_row_tile * ((p.M + k.tokens - 1) / k.tokens);
     const int64_t rows = blocks / cus * cus / per_row_tile * k.tokens;
     if (rows < 1 || rows >= p.M || !takes(k, p, norm, rows)) continue;
     double t2 = 0;
-    const Kind* r = best_kind(p, norm, p.M - rows, cus, &t2);
-    if (!r || r == &k) continue;  // the same kind: no gain
+    const int r = best_kind(p, norm, p.M - rows, cus, &t2);
+    if (r < 0 || r == i) continue;  // the same kind: no gain
     const double t = kind_us(k, p, rows, cus) + 2.0 + t2;
-    if (!kind || t < us) {
+    if (plan.first < 0 || t < us) {
       us = t;
-      first = &k;
-      rest = r;
-      rows1 = (int)rows;
+      plan = {i, r, (int)rows};
     }
   }
-  if (!first) return kind ? kind->launch(p, norm, stream) : hipErrorInvalidConfiguration;
+  return plan;
+}
+
+bool has_norm(const Prod8Params& p) {
+  bool norm = false;
+  for (int i = 0; i < p.n_outs; ++i) norm |= p.out[i].norm_w != nullptr;
+  return norm;
+}
+
+}  // namespace
+
+hipError_t launch_prod8(const Prod8Params& p, hipStream_t stream) {
+  const bool norm = has_norm(p);
+  const Plan plan = plan_of(p, norm, device_cus());
+  if (plan.first < 0) return hipErrorInvalidConfiguration;
   Prod8Params a = p;
-  a.M = rows1;
-  const hipError_t e = first->launch(a, norm, stream);
-  if (e != hipSuccess) return e;
-  return rest->launch(rows_from(p, rows1), norm, stream);
+  a.M = plan.rows;
+  const hipError_t e = kKinds[plan.first].launch(a, norm, stream);
+  if (e != hipSuccess || plan.rest < 0) return e;
+  return kKinds[plan.rest].launch(rows_from(p, plan.rows), norm, stream);
 }
 
 }  // namespace harp_blk
+
+// Used by the tests, which have to reach every kind: what a product of M x N x
+// K (n_outs of them) runs as.  out: tokens and features of the first launch's
+// blocks, its rows, tokens and features of the second's (0: none); kinds: the
+// table's (tokens, features, whole heads), `room` entries at most.  cus 0: the
+// current device's.  Returns the number of kinds, or -1 for a call that none takes.
+extern "C" __attribute__((visibility("default"))) int harp_prod8_plan(int M, int N, int K, int n_outs, int norm,
+                                                                      int cus, int* out, int* kinds, int room) {
+  using namespace harp_blk;
+  Prod8Params p{};
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.n_outs = n_outs;
+  const Plan plan = plan_of(p, norm != 0, cus > 0 ? cus : device_cus());
+  if (plan.first < 0) return -1;
+  const Kind &a = kKinds[plan.first], *b = plan.rest < 0 ? nullptr : &kKinds[plan.rest];
+  const int v[5] = {a.tokens, a.features, plan.rows, b ? b->tokens : 0, b ? b->features : 0};
+  for (int i = 0; i < 5; ++i) out[i] = v[i];
+  for (int i = 0; i < kNumKinds && i < room; ++i) {
+    kinds[3 * i] = kKinds[i].tokens;
+    kinds[3 * i + 1] = kKinds[i].features;
+    kinds[3 * i + 2] = kKinds[i].heads;
+  }
+  return kNumKinds;
+}

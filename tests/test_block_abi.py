@@ -326,3 +326,27 @@ def test_dequantize_refuses(over, code, msg):
     rc = harp_amd.load_abi().harp_blk_dequantize_int8(a["q"], a["ldq"], a["s"], a["o"], a["ldo"], a["od"], a["rows"],
                                                       a["cols"], None)
     assert rc == code and msg in _err(), (rc, _err())
+
+
+def test_every_kind_of_block_has_its_tests():
+    """The shapes of the products' GPU tests run, on 256 CUs, in the kinds that the tests name, and reach every kind
+    the library has, with a norm where the kind takes one, as the first launch of a call and as the second."""
+    from tests.test_gpu_int8_linear import NORMED, PLAIN, product_plan
+
+    _, _, kinds = product_plan(1, 1, 1, cus=256)
+    plain, normed = {}, {}
+    for M, N, K, want in PLAIN:
+        launches, rows, _ = product_plan(M, N, K, cus=256)
+        assert launches == want and (rows < M) == (len(want) == 2), (M, N, K, launches)
+        for i, k in enumerate(launches):
+            plain.setdefault(k, set()).add(i)
+    for B, S, H, K, want in NORMED:
+        launches, rows, _ = product_plan(B * S, 128 * H, K, 3, True, 256)
+        assert launches == want and (rows < B * S) == (len(want) == 2), (B, S, H, K, launches)
+        for i, k in enumerate(launches):
+            normed.setdefault(k, set()).add(i)
+    assert set(plain) == {k[:2] for k in kinds} and set(normed) == {k[:2] for k in kinds if k[2]}
+    # every kind but the largest can be the second launch of a call
+    largest = max(k[:2] for k in kinds)
+    assert all(1 in plain[k[:2]] for k in kinds if k[:2] != largest)
+    assert all(1 in normed[k[:2]] for k in kinds if k[2] and k[:2] != largest)

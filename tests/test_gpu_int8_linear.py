@@ -308,3 +308,104 @@ def test_wider_weight_is_refused(K, wide):
     y = ops.linear_int8(x.values, x.scales, w.values, w.scales, None, F32, K)
     assert torch.equal(y, harp_amd.int8_linear(x, first, None, F32))
     _assert_linear(y, x, first, None, (K, wide))
+
+
+# ---------------------------------------------------------------------------
+# every kind of block
+# ---------------------------------------------------------------------------
+
+def product_plan(M, N, K, n_outs=1, norm=False, cus=0):
+    """((tokens, features) of the blocks of a product's one or two launches, the first one's rows, all kinds)."""
+    import ctypes
+
+    out, kinds = (ctypes.c_int * 5)(), (ctypes.c_int * 96)()
+    n = harp_amd.load_abi().harp_prod8_plan(M, N, K, n_outs, int(norm), cus, out, kinds, 32)
+    assert 0 < n <= 32
+    launches = [(out[0], out[1])] + ([(out[3], out[4])] if out[3] else [])
+    return launches, out[2], [tuple(kinds[3 * i:3 * i + 3]) for i in range(n)]
+
+
+# tokens, features, K (none a multiple of 16) and the launches that such a product runs as on 256 CUs
+PLAIN = [
+    (9, 41, 5483, [(16, 16)]),
+    (540, 37, 3123, [(32, 32)]),
+    (269, 1533, 1971, [(32, 64)]),
+    (91, 8771, 3571, [(32, 128)]),
+    (422, 5643, 571, [(64, 64)]),
+    (265, 5251, 3215, [(64, 128)]),
+    (558, 5545, 1817, [(128, 128)]),
+    (2834, 2365, 1515, [(128, 256)]),
+    (2184, 4413, 2195, [(256, 256)]),
+    (905, 4207, 5363, [(128, 128), (16, 16)]),
+    (1415, 5405, 2331, [(128, 256), (32, 32)]),
+    (1195, 6985, 2561, [(128, 256), (32, 64)]),
+    (2718, 3279, 5603, [(128, 256), (32, 128)]),
+    (1236, 7079, 2721, [(128, 256), (64, 64)]),
+    (1179, 8089, 4707, [(128, 256), (64, 128)]),
+    (3378, 5727, 1541, [(256, 256), (128, 128)]),
+    (2367, 8847, 1485, [(256, 256), (128, 256)]),
+]
+# batch, tokens, heads, K of a q/k/v product with norms
+NORMED = [
+    (1, 271, 2, 555, [(32, 128)]),
+    (1, 361, 8, 2265, [(64, 128)]),
+    (2, 258, 14, 1845, [(128, 128)]),
+    (1, 900, 15, 2055, [(128, 256)]),
+    (1, 1372, 27, 2121, [(256, 256)]),
+    (2, 326, 29, 4209, [(128, 256), (32, 128)]),
+    (1, 932, 28, 4281, [(128, 256), (64, 128)]),
+    (1, 2390, 17, 3215, [(256, 256), (32, 128)]),
+    (2, 1262, 17, 2531, [(256, 256), (64, 128)]),
+    (3, 1015, 16, 2509, [(256, 256), (128, 128)]),
+    (1, 3337, 29, 1463, [(256, 256), (128, 256)]),
+]
+
+
+@pytest.mark.parametrize("M,N,K,kinds", PLAIN)
+def test_linear_in_every_kind_of_block(M, N, K, kinds):
+    """Tails in all three sizes over several K-tiles, both result types and all biases; every result within bounds
+    and the same as in a call of some of the rows."""
+    print(f"[int8_linear M={M} N={N} K={K} {kinds}]", flush=True)
+    launches, rows, _ = product_plan(M, N, K)
+    assert launches == kinds
+    g = _gen(M + N)
+    x, w = _rows(g, M, K), _rows(g, N, K)
+    acc = _exact(x, w) * x.scales.double()[:, None] * w.scales.double()
+    some = harp_amd.Int8Rows(x.values[max(0, rows - 9):rows + 7], x.scales[max(0, rows - 9):rows + 7])
+    for bias in (None, torch.randn(N, generator=g).to(B16).to(DEV), torch.randn(N, generator=g).to(DEV)):
+        b = torch.zeros(N, device=DEV, dtype=torch.float64) if bias is None else bias.double()
+        for dtype in (B16, F32):
+            y = harp_amd.int8_linear(x, w, bias, dtype)
+            want = acc + b
+            err = (y.double() - want).abs()
+            bad = err > 4 * U * (acc.abs() + b.abs()) + HALF[dtype] * want.abs()
+            assert not bool(bad.any()), (dtype, int(bad.sum()), bad.nonzero()[0].tolist(), float(err.max()))
+            assert torch.equal(harp_amd.int8_linear(some, w, bias, dtype), y[max(0, rows - 9):rows + 7])
+
+
+@pytest.mark.parametrize("M,N,K", [(8000, 5001, 100), (8000, 3841, 1), (1000, 5000, 100), (600, 8000, 100), (2049, 2049, 127),
+                                   (4100, 4100, 127), (8000, 3000, 257)])
+def test_linear_of_few_k_tiles(M, N, K):
+    print(f"[int8_linear M={M} N={N} K={K} {product_plan(M, N, K)[0]}]", flush=True)
+    g = _gen(M + K)
+    x, w = _rows(g, M, K), _rows(g, N, K)
+    bias = torch.randn(N, generator=g).to(DEV)
+    for dtype in (B16, F32):
+        _assert_linear(harp_amd.int8_linear(x, w, bias, dtype), x, w, bias, (M, N, K, dtype))
+
+
+@pytest.mark.parametrize("B,S,H,K,kinds", NORMED)
+@pytest.mark.parametrize("norm", [B16, F32], ids=str)
+def test_qkv_in_every_kind_of_block(B, S, H, K, kinds, norm):
+    print(f"[qkv B={B} S={S} H={H} K={K} norm={norm} {kinds}]", flush=True)
+    assert product_plan(B * S, 128 * H, K, 3, True)[0] == kinds
+    g = _gen(B + S + H + K)
+    attn = _attn(g, H, K, norm)
+    flat = _rows(g, B * S, K)
+    rows = harp_amd.Int8Rows(flat.values.unflatten(0, (B, S)), flat.scales.view(B, S))
+    freqs = _freqs(S, B if B > 1 else 0) if norm == B16 else None
+    _assert_qkv(harp_amd.project_qkv(attn, rows, freqs), attn, rows, freqs, (B, S, H, K))
+    if norm == F32:
+        return
+    attn.norm_q = attn.norm_k = None  # the same sizes without a norm run in other kinds
+    _assert_qkv(harp_amd.project_qkv(attn, rows, None), attn, rows, None, (B, S, H, K))
