@@ -121,17 +121,18 @@ __device__ __forceinline__ void finish_tokens(const Prod8Params& p, const Prod8O
                                               int ge, Combine combine) {
   const bool norm = NORM && o.norm_w != nullptr, rope = norm && p.freqs != nullptr;
   f32x4 v[OF][4];
-  float ss = 0.f;
+  float sq[OF];  // sums of the squares of each feature block
 #pragma unroll
   for (int i = 0; i < OF; ++i) {
     sched_fence();  // (one feature block's scales at a time: all would not fit beside the sums)
+    sq[i] = 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const f32x4 ws = *(const f32x4*)(wsc + 32 * i + 8 * q + 4 * ge);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         v[i][q][e] = (float)own[i][4 * q + e] * sx * ws[e];
-        if (NORM) ss = __builtin_fmaf(v[i][q][e], v[i][q][e], ss);
+        if (NORM) sq[i] = __builtin_fmaf(v[i][q][e], v[i][q][e], sq[i]);
       }
       if (!NORM) {
         const f32x4 b = *(const f32x4*)(wb + 32 * i + 8 * q + 4 * ge);
@@ -144,7 +145,15 @@ __device__ __forceinline__ void finish_tokens(const Prod8Params& p, const Prod8O
   }
   sched_fence();
   if (NORM && norm) {
-    ss = combine(harp_ra::wave_half_sum(ss));  // this lane's features of the token and its partner lane's; all the head's
+    // the head's sum, of its four feature blocks' sums (this lane's features and its partner lane's) taken in pairs:
+    // the same order in every kind, so that a token's result does not depend on the kind its call runs in
+#pragma unroll
+    for (int i = 0; i < OF; ++i) sq[i] = harp_ra::wave_half_sum(sq[i]);
+    static_assert(OF == 1 || OF == 2 || OF == 4, "pairs of feature blocks");
+    float ss = sq[0];
+    if constexpr (OF > 1) ss += sq[1];
+    if constexpr (OF > 2) ss += sq[2] + sq[3];
+    ss = combine(ss);
     const float rho = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)kFeat) + o.eps));
     const int mt = min(mj, p.M - 1) + p.m_base;  // the token among the call's
     const float* fr = p.freqs + (int64_t)(mt / p.S) * p.f_stride_b + (int64_t)(mt % p.S) * p.f_stride_s + d_own + 4 * ge;
@@ -497,9 +506,9 @@ __global__ __launch_bounds__(64 * TG * GROUPS * KG, 1) void prod8_kernel(Prod8Pa
                                    const int t = m_own - m0 + 32 * j + l32e, h = f_own / kFeat;
                                    part_ss[f_own % kFeat / (32 * kOwnF)][h][t] = ss;
                                    __syncthreads();
-                                   ss = 0.f;
-#pragma unroll
-                                   for (int k = 0; k < kParts; ++k) ss += part_ss[k][h][t];
+                                   static_assert(kParts == 2 || kParts == 4, "pairs of parts");
+                                   ss = part_ss[0][h][t] + part_ss[1][h][t];
+                                   if constexpr (kParts > 2) ss += part_ss[2][h][t] + part_ss[3][h][t];
                                  }
                                  return ss;
                                });

@@ -409,3 +409,20 @@ def test_qkv_in_every_kind_of_block(B, S, H, K, kinds, norm):
         return
     attn.norm_q = attn.norm_k = None  # the same sizes without a norm run in other kinds
     _assert_qkv(harp_amd.project_qkv(attn, rows, None), attn, rows, None, (B, S, H, K))
+
+
+@pytest.mark.parametrize("B,S,H,K,kinds", [c for c in NORMED if c[0] == 1])
+def test_qkv_does_not_depend_on_the_batch(B, S, H, K, kinds):
+    """A token's q, k and v are the same alone, among a few and among all, whatever kinds of blocks the calls run in."""
+    g = _gen(S)
+    attn, flat, freqs = _attn(g, H, K, B16), _rows(g, S, K), _freqs(S)
+    full = harp_amd.project_qkv(attn, harp_amd.Int8Rows(flat.values[None], flat.scales[None]), freqs)
+    seen = {tuple(kinds)}
+    for n in (1, 40, 70, 200, 300, 520):
+        n = min(n, S)
+        seen.add(tuple(product_plan(n, 128 * H, K, 3, True)[0]))
+        for s in (slice(0, n), slice(S - n, S)):
+            some = harp_amd.project_qkv(attn, harp_amd.Int8Rows(flat.values[None, s], flat.scales[None, s]), freqs[s])
+            for name, a, b in zip("qkv", full, some):
+                assert torch.equal(a[:, :, s], b), (name, n, int((a[:, :, s] != b).sum()))
+    assert len(seen) > 1 or H * K < 5000, seen
