@@ -541,3 +541,33 @@ def test_operator_results_share_no_memory_with_x(mode):
         assert h2 is x and torch.equal(y, y2) and y.requires_grad == (mode == "grad")
         _, h = torch.ops.harp_block.add_rms_norm(x, x, w, 1e-5)
         assert torch.equal(h, x + x) and h.data_ptr() != x.data_ptr()
+
+
+def test_more_wide_rows_than_one_launch_holds():
+    """Rows with a wave each run 4 to a block, so that 2^24 fill a launch, and longer ones fill it with 2^22: what
+    follows in the next launch (a row's y, h, rstd, 8-bit values and scale) is as in a call of a few rows."""
+    rows, cols = 2 ** 24 + 5, 136
+    g = torch.Generator(DEV).manual_seed(8)
+    x = torch.empty(rows, cols, dtype=B16, device=DEV).normal_(generator=g)
+    r = torch.empty(rows, cols, dtype=B16, device=DEV).normal_(generator=g)
+    w = torch.rand(cols, generator=g, device=DEV) + 0.5
+    q, n8 = harp_amd.quantize_int8(x), harp_amd.add_rms_norm_int8(x, r, w, 1e-6)
+    x.requires_grad_(True)
+    y, h = harp_amd.add_rms_norm(x, r, w, 1e-6)
+    (dx,) = torch.autograd.grad((y, h), x, (r, r))
+    for s in _slices(rows, 2 ** 24):
+        small = harp_amd.quantize_int8(x.detach()[s])
+        assert torch.equal(q.values[s], small.values) and torch.equal(q.scales[s], small.scales), s
+        small, hs = harp_amd.add_rms_norm_int8(x.detach()[s], r[s], w, 1e-6)
+        assert torch.equal(n8[0].values[s], small.values) and torch.equal(n8[0].scales[s], small.scales), s
+        assert torch.equal(n8[1][s], hs) and torch.equal(h[s], hs), s
+        xs = x.detach()[s].requires_grad_(True)
+        ys, hs = harp_amd.add_rms_norm(xs, r[s], w, 1e-6)
+        assert torch.equal(y[s], ys) and torch.equal(dx[s], torch.autograd.grad((ys, hs), xs, (r[s], r[s]))[0]), s
+    del x, r, y, h, dx, q, n8
+    rows, cols = 2 ** 22 + 3, 1040
+    x = torch.empty(rows, cols, dtype=B16, device=DEV).normal_(generator=g)
+    q = harp_amd.quantize_int8(x)
+    for s in _slices(rows, 2 ** 22):
+        small = harp_amd.quantize_int8(x[s])
+        assert torch.equal(q.values[s], small.values) and torch.equal(q.scales[s], small.scales), s
