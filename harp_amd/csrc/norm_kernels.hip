@@ -714,43 +714,41 @@ hipError_t launch_fwd(const NormParams& p, hipStream_t stream) {
   return hipErrorInvalidValue;
 }
 
-// threads per row and groups of the backward block, by the row's vectors
+// The backward's block by the row's vectors: TPR threads with NV vectors each for
+// one row, GROUPS rows at a time.  The grid, the partial rows of the workspace and
+// the kernel's instance all come from here.
+template <int TPR_, int NV_, int GROUPS_>
 struct BwdShape {
-  int groups;
+  static constexpr int TPR = TPR_, NV = NV_, GROUPS = GROUPS_;
 };
-BwdShape bwd_shape(int cols) {
+template <class F>
+auto with_bwd_shape(int cols, F f) {
   const int vecs = (cols + kVec - 1) / kVec;
-  if (vecs <= 16) return {32};
-  if (vecs <= 128) return {8};
-  if (vecs <= 1024) return {2};
-  return {1};
+  if (vecs <= 16) return f(BwdShape<16, 1, 32>());
+  if (vecs <= 64) return f(BwdShape<64, 1, 8>());
+  if (vecs <= 128) return f(BwdShape<64, 2, 8>());
+  if (vecs <= 256) return f(BwdShape<256, 1, 2>());
+  if (vecs <= 512) return f(BwdShape<256, 2, 2>());
+  if (vecs <= 1024) return f(BwdShape<256, 4, 2>());
+  if (vecs <= 2048) return f(BwdShape<512, 4, 1>());
+  return f(BwdShape<1024, 4, 1>());
 }
 
 template <int XD, int HD>
 hipError_t launch_bwd_t(const NormBwdParams& p, hipStream_t stream) {
-  const int vecs = (p.cols + kVec - 1) / kVec;
   const unsigned blocks = (unsigned)bwd_blocks(p.rows, p.cols);
-#define HARP_NORM_BWD(TPR, NV, GROUPS)                                                                               \
-  {                                                                                                                  \
-    hipLaunchKernelGGL((norm_bwd_kernel<XD, HD, TPR, NV, GROUPS, (NV * TPR <= 2048)>), dim3(blocks),                 \
-                       dim3(TPR * GROUPS), 0, stream, p);                                                            \
-    return hipGetLastError();                                                                                        \
-  }
-  if (vecs <= 16) HARP_NORM_BWD(16, 1, 32)
-  if (vecs <= 64) HARP_NORM_BWD(64, 1, 8)
-  if (vecs <= 128) HARP_NORM_BWD(64, 2, 8)
-  if (vecs <= 256) HARP_NORM_BWD(256, 1, 2)
-  if (vecs <= 512) HARP_NORM_BWD(256, 2, 2)
-  if (vecs <= 1024) HARP_NORM_BWD(256, 4, 2)
-  if (vecs <= 2048) HARP_NORM_BWD(512, 4, 1)
-  HARP_NORM_BWD(1024, 4, 1)
-#undef HARP_NORM_BWD
+  return with_bwd_shape(p.cols, [&](auto s) {
+    typedef decltype(s) S;
+    hipLaunchKernelGGL((norm_bwd_kernel<XD, HD, S::TPR, S::NV, S::GROUPS, (S::NV * S::TPR <= 2048)>), dim3(blocks),
+                       dim3(S::TPR * S::GROUPS), 0, stream, p);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace
 
 int bwd_blocks(int rows, int cols) {
-  const int g = bwd_shape(cols).groups;
+  const int g = with_bwd_shape(cols, [](auto s) { return decltype(s)::GROUPS; });
   const int64_t need = ((int64_t)rows + g - 1) / g;
   return (int)(need < 512 ? need : 512);
 }
