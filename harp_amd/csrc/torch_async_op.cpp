@@ -90,7 +90,7 @@ struct Freqs {
 Freqs freqs_of(const at::Tensor& f, const at::Tensor& x4) {
   TORCH_CHECK(f.is_cuda() && f.device() == x4.device(), "freqs_cis must be on the input's device");
   at::Tensor r = f.is_complex() ? at::view_as_real(f).flatten(-2) : f;
-  TORCH_CHECK(r.scalar_type() == at::kFloat, "freqs_cis must be complex64 (or its float32 view_as_real)");
+  TORCH_CHECK(r.scalar_type() == at::kFloat, "freqs_cis must be complex64 [.., S, D/2], or float32 (cos, sin) rows [.., S, D]");
   r = r.contiguous();
   TORCH_CHECK(r.dim() == 2 || r.dim() == 3, "freqs_cis must be [S, D/2] or [B, S, D/2] complex, got ", f.sizes());
   const int64_t B = x4.size(0), S = x4.size(2), D = x4.size(3);

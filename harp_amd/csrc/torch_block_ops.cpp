@@ -418,10 +418,11 @@ struct Freqs {
 Freqs freqs_of(const at::Tensor& f, const at::Tensor& x, int64_t B, int64_t S) {
   TORCH_CHECK(f.is_cuda() && f.device() == x.device(), "freqs_cis must be on the input's device");
   at::Tensor r = f.is_complex() ? at::view_as_real(f).flatten(-2) : f;
-  TORCH_CHECK(r.scalar_type() == at::kFloat, "freqs_cis must be complex64 (or its float32 view_as_real)");
+  TORCH_CHECK(r.scalar_type() == at::kFloat, "freqs_cis must be complex64 [.., S, 64], or float32 (cos, sin) rows [.., S, 128]");
   r = r.contiguous();
   TORCH_CHECK((r.dim() == 2 || r.dim() == 3) && r.size(-1) == 128 && r.size(-2) == S,
-              "freqs_cis must be [S, 64] or [B, S, 64] complex with S=", S, ", got ", f.sizes());
+              "freqs_cis must be complex [S, 64] or [B, S, 64], or float32 (cos, sin) rows [.., S, 128], with S=", S,
+              ", got ", f.sizes());
   TORCH_CHECK(r.dim() == 2 || r.size(0) == B || r.size(0) == 1, "freqs_cis batch must be 1 or ", B);
   Freqs q;
   q.t = r;

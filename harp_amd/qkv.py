@@ -40,10 +40,11 @@ def _freqs_table(freqs_cis: torch.Tensor, B: int, S: int) -> Tuple[torch.Tensor,
     the async_op operators read it."""
     r = torch.view_as_real(freqs_cis).flatten(-2) if freqs_cis.is_complex() else freqs_cis
     if r.dtype != torch.float32:
-        raise ValueError("freqs_cis must be complex64 (or its float32 view_as_real)")
+        raise ValueError("freqs_cis must be complex64 [.., S, 64], or float32 (cos, sin) rows [.., S, 128]")
     r = r.contiguous()
     if r.dim() not in (2, 3) or r.size(-1) != HEAD_DIM or r.size(-2) != S:
-        raise ValueError(f"freqs_cis must be [S, 64] or [B, S, 64] complex with S={S}, got {tuple(freqs_cis.shape)}")
+        raise ValueError(f"freqs_cis must be complex [S, 64] or [B, S, 64], or float32 (cos, sin) rows [.., S, 128], "
+                         f"with S={S}, got {tuple(freqs_cis.shape)}")
     if r.dim() == 3 and r.size(0) not in (1, B):
         raise ValueError(f"freqs_cis batch must be 1 or {B}")
     sb = r.stride(0) if (r.dim() == 3 and r.size(0) > 1) else 0

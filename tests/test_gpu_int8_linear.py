@@ -426,3 +426,16 @@ def test_qkv_does_not_depend_on_the_batch(B, S, H, K, kinds):
             for name, a, b in zip("qkv", full, some):
                 assert torch.equal(a[:, :, s], b), (name, n, int((a[:, :, s] != b).sum()))
     assert len(seen) > 1 or H * K < 5000, seen
+
+
+def test_rope_table_forms():
+    """The complex table and its (cos, sin) rows give the same; view_as_real's own shape is refused with what is taken."""
+    g = _gen(3)
+    attn, flat, f = _attn(g, 2, 256, B16), _rows(g, 30, 256), _freqs(30)
+    rows = harp_amd.Int8Rows(flat.values[None], flat.scales[None])
+    want = harp_amd.project_qkv(attn, rows, f)
+    got = harp_amd.project_qkv(attn, rows, torch.view_as_real(f).flatten(-2))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    for bad in (torch.view_as_real(f), f[:29], f.to(torch.complex128)):
+        with pytest.raises(RuntimeError, match=r"float32 \(cos, sin\) rows \[\.\., S, 128\]"):
+            harp_amd.project_qkv(attn, rows, bad)
