@@ -19,8 +19,8 @@ replaces the projections of the model's attention module, which
 q, k and v in one launch, with the QK RMSNorm and RoPE in its epilogue where
 the heads have 128 features.
 
-No gradient is recorded: where one would be, the functions raise.  There is no
-CPU path.
+No gradient is recorded: where one would be, or an argument carries a
+forward-mode tangent, the functions raise.  There is no CPU path.
 """
 
 from __future__ import annotations

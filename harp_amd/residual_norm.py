@@ -1,15 +1,17 @@
 """The residual addition with its RMSNorm, on the GPU.
 
-Every block of the model adds the attention's and the feed-forward's results
-to the residual stream and normalises it before the next layer
+The model's blocks add the attention's and the feed-forward's results to the
+residual stream and normalise it before the next layer
 (src/models/z_image/module/block.py).  :func:`add_rms_norm` is that pair in
 one pass over the rows::
 
     h = x + residual                                # rounded to the residual's type
     y = h / sqrt(mean(h^2) + eps) * weight          # in x's type
 
-and differentiable, once (one kernel for the gradients of x and the residual,
-one small reduction for the weight's).
+and differentiable, once and in reverse mode (one kernel for the gradients of x
+and the residual, one small reduction for the weight's).  There is no factor per
+sample on the norm's result and no gate on the addition: a block with such a
+modulation multiplies x before the call, and y after it.
 :func:`add_rms_norm_int8` gives y as 8-bit rows instead
 (:class:`harp_amd.Int8Rows`), for a Linear layer in 8-bit integers; it is
 forward only.

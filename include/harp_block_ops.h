@@ -5,8 +5,9 @@
  * (Linear layers, and the q/k/v producer with QK RMSNorm and RoPE).
  *
  * HARP's model normalises the hidden states with an RMSNorm in front of the
- * attention and the feed-forward of every block and adds their results to the
- * residual stream (src/models/z_image/module/block.py), and runs its Linear
+ * attention and the feed-forward of its blocks and adds their results to the
+ * residual stream (src/models/z_image/module/block.py; factors per sample and
+ * gates, where a block has them, are the caller's), and runs its Linear
  * layers through xhblas_gemm (gemm/bgemm/bgemm.h:20-26) in bf16; the 8-bit
  * forms have no reference counterpart.  libharp_ra.so exports the functions
  * declared here next to those of harp_ring_attn.h and harp_qk_norm_rope.h.
