@@ -29,6 +29,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
+from .int8 import Int8Linear
 
 HEAD_DIM = 128
 K_TILE = 64
@@ -73,8 +74,9 @@ def fused_supported(attn, hidden_states: torch.Tensor, freqs_cis: Optional[torch
     if x.is_contiguous() and not _aligned16(x):  # qkv_project passes x itself (a copy only when strided)
         return False
     lins = [getattr(attn, n, None) for n in ("to_q", "to_k", "to_v")]
-    if any(m is None or getattr(m, "bias", None) is not None or not isinstance(getattr(m, "weight", None), torch.Tensor)
-           for m in lins):  # (an Int8Linear's weight is no tensor)
+    if any(m is None or getattr(m, "bias", None) is not None or not hasattr(m, "weight") for m in lins):
+        return False
+    if any(isinstance(m, Int8Linear) for m in lins):  # their weights are 8-bit rows
         return False
     n_out = lins[0].weight.size(0)
     if n_out % HEAD_DIM or n_out != attn.heads * HEAD_DIM:

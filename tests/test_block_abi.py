@@ -350,3 +350,15 @@ def test_every_kind_of_block_has_its_tests():
     largest = max(k[:2] for k in kinds)
     assert all(1 in plain[k[:2]] for k in kinds if k[:2] != largest)
     assert all(1 in normed[k[:2]] for k in kinds if k[2] and k[:2] != largest)
+
+
+@pytest.mark.parametrize("name", ["to_q", "to_k", "to_v"])
+def test_some_projections_in_8_bits_are_not_fused(name):
+    """The fused bf16 kernel takes no module with an Int8Linear among its projections."""
+    from harp_amd import qkv
+    from tests.test_qk_abi import _DevView, _module
+
+    attn, x = _module(), _DevView(torch.zeros(1, 16, 128, dtype=torch.bfloat16))
+    assert qkv.fused_supported(attn, x, None)
+    setattr(attn, name, harp_amd.Int8Linear(harp_amd.Int8Rows(torch.zeros(256, 128, dtype=torch.int8), torch.zeros(256))))
+    assert not qkv.fused_supported(attn, x, None)
