@@ -11,7 +11,11 @@ the output projection as the model's attention block does.  Around it
 (``include/harp_block_ops.h``, ``kernels/libharp_block_ops.so``):
 :func:`add_rms_norm`, the residual addition with its RMSNorm, and the Linear
 layers in 8-bit integers for forward-only use (:class:`Int8Linear`,
-:func:`quantize_attention`).  Build with ``python -m harp_amd.build``.
+:func:`quantize_attention`).  For a batch of requests
+(``include/harp_request_ops.h``, ``kernels/libharp_request_ops.so``):
+:func:`qk_norm_axial_rope`, the QK RMSNorm and rotation by each token's
+positions along several axes, and low-rank adapters beside the projections
+(:func:`add_adapters`, :class:`AdaptedLinear`, :func:`adapt_attention`).  Build with ``python -m harp_amd.build``.
 """
 
 from ._lib import (  # noqa: F401
@@ -19,10 +23,12 @@ from ._lib import (  # noqa: F401
     ASYNC_OPS_LIB,
     BLOCK_OPS_LIB,
     OPS_LIB,
+    REQUEST_OPS_LIB,
     load_abi,
     load_async_ops,
     load_block_ops,
     load_ops,
+    load_request_ops,
 )
 from .ops import (  # noqa: F401
     RingAttention,
@@ -37,6 +43,8 @@ from .ops import (  # noqa: F401
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn  # noqa: F401
 from .residual_norm import add_rms_norm, add_rms_norm_int8  # noqa: F401
 from .int8 import Int8Linear, Int8Rows, int8_linear, quantize_attention, quantize_int8  # noqa: F401
+from .rope import AxialPositions, AxialRope, qk_norm_axial_rope  # noqa: F401
+from .adapters import AdaptedLinear, AdapterRequests, Adapters, adapt_attention, add_adapters  # noqa: F401
 from .attention import RingZAttention, project_qkv  # noqa: F401
 from .wait_engine import CommWork, WaitEngine  # noqa: F401
 from .gemm import xhblas_gemm  # noqa: F401

@@ -22,6 +22,7 @@ ABI_LIB = KERNELS / "libharp_ra.so"
 OPS_LIB = KERNELS / "libring_attention_ops.so"
 ASYNC_OPS_LIB = KERNELS / "libharp_async_op.so"
 BLOCK_OPS_LIB = KERNELS / "libharp_block_ops.so"
+REQUEST_OPS_LIB = KERNELS / "libharp_request_ops.so"
 
 HARP_RA_OK = 0
 HARP_RA_EINVAL = 1
@@ -38,6 +39,7 @@ _abi: ctypes.CDLL | None = None
 _ops_loaded = False
 _async_ops_loaded = False
 _block_ops_loaded = False
+_request_ops_loaded = False
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -156,6 +158,80 @@ BLK_PROTOTYPES = {
 }
 
 
+HARP_REQ_OK = 0
+HARP_REQ_F32 = 0
+HARP_REQ_BF16 = 1
+HARP_REQ_I32 = 2
+HARP_REQ_I64 = 3
+HARP_REQ_MAX_AXES = 4
+
+
+class ReqAxes(ctypes.Structure):
+    """harp_req_axes_t of include/harp_request_ops.h (the axes of a rotary embedding)."""
+
+    _fields_ = [
+        ("n", _i),
+        ("width", _i * HARP_REQ_MAX_AXES),
+        ("theta", ctypes.c_double * HARP_REQ_MAX_AXES),
+        ("half", _i),
+    ]
+
+
+class ReqPositions(ctypes.Structure):
+    """harp_req_positions_t of include/harp_request_ops.h."""
+
+    _fields_ = [("p", _p), ("dtype", _i), ("stride_b", _i64), ("stride_s", _i64), ("stride_a", _i64)]
+
+
+class ReqHeads(ctypes.Structure):
+    """harp_req_heads_t of include/harp_request_ops.h (q or k)."""
+
+    _fields_ = [
+        ("x", _p),
+        ("x_stride", _i64 * 3),
+        ("y", _p),
+        ("y_stride", _i64 * 3),
+        ("heads", _i),
+        ("norm", _i),
+        ("weight", _p),
+        ("weight_dtype", _i),
+        ("eps", _f),
+        ("dy", _p),
+        ("dy_stride", _i64 * 3),
+        ("grad_weight", _p),
+    ]
+
+
+class ReqRequests(ctypes.Structure):
+    """harp_req_requests_t of include/harp_request_ops.h."""
+
+    _fields_ = [("index", _p), ("index_dtype", _i), ("offsets", _p), ("offsets_dtype", _i), ("count", _i)]
+
+
+class ReqAdapters(ctypes.Structure):
+    """harp_req_adapters_t of include/harp_request_ops.h."""
+
+    _fields_ = [("a", _p), ("b", _p), ("scales", _p), ("n", _i), ("rank", _i)]
+
+
+_axes_p, _pos_p, _heads_p = (ctypes.POINTER(t) for t in (ReqAxes, ReqPositions, ReqHeads))
+_req_p, _adapters_p = ctypes.POINTER(ReqRequests), ctypes.POINTER(ReqAdapters)
+
+# (restype, argtypes) of every symbol include/harp_request_ops.h declares
+REQ_PROTOTYPES = {
+    "harp_req_qk_norm_rope_forward": (_i, [_axes_p, _pos_p, _heads_p, _i, _i, _i, _p]),
+    "harp_req_qk_norm_rope_backward": (_i, [_axes_p, _pos_p, _heads_p, _i, _i, _i, _p, _sz, _p]),
+    "harp_req_qk_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "harp_req_rope_table": (_i, [_axes_p, _pos_p, _i, _i, _p, _p]),
+    "harp_req_adapter_columns": (_i, [_i]),
+    "harp_req_add_adapters_forward": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _adapters_p, _req_p, _p, _i, _i, _i, _p]),
+    "harp_req_add_adapters_backward": (_i, [_p, _i64, _p, _i64, _p, _adapters_p, _req_p, _p, _i64, _i, _p, _p, _i, _i,
+                                            _i, _p, _sz, _p]),
+    "harp_req_adapter_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "harp_req_last_error": (ctypes.c_char_p, []),
+}
+
+
 def _missing(path: Path) -> RuntimeError:
     return RuntimeError(
         f"{path} is not built; run `python -m harp_amd.build` (or __graft_entry__.build()). "
@@ -171,7 +247,7 @@ def load_abi() -> ctypes.CDLL:
             if not ABI_LIB.exists():
                 raise _missing(ABI_LIB)
             lib = ctypes.CDLL(str(ABI_LIB))
-            for name, (res, args) in {**ABI_PROTOTYPES, **QK_PROTOTYPES, **BLK_PROTOTYPES}.items():
+            for name, (res, args) in {**ABI_PROTOTYPES, **QK_PROTOTYPES, **BLK_PROTOTYPES, **REQ_PROTOTYPES}.items():
                 fn = getattr(lib, name)
                 fn.restype = res
                 fn.argtypes = args
@@ -213,6 +289,18 @@ def load_block_ops() -> None:
             raise _missing(BLOCK_OPS_LIB)
         torch.ops.load_library(str(BLOCK_OPS_LIB))
         _block_ops_loaded = True
+
+
+def load_request_ops() -> None:
+    """Register torch.ops.harp_request (rotary positions, low-rank adapters) from kernels/libharp_request_ops.so."""
+    global _request_ops_loaded
+    with _lock:
+        if _request_ops_loaded:
+            return
+        if not REQUEST_OPS_LIB.exists():
+            raise _missing(REQUEST_OPS_LIB)
+        torch.ops.load_library(str(REQUEST_OPS_LIB))
+        _request_ops_loaded = True
 
 
 def qk_check(rc: int, what: str) -> None:

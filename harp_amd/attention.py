@@ -22,6 +22,11 @@ A module whose projections are :class:`harp_amd.Int8Linear`
 only; ``hidden_states`` may then be 8-bit rows (:class:`harp_amd.Int8Rows`),
 as :func:`harp_amd.add_rms_norm_int8` writes them.
 
+The rotation may be given as positions along several axes
+(:class:`harp_amd.AxialPositions`) instead of a complex table, and a module with
+low-rank adapters beside its projections (:func:`harp_amd.adapt_attention`) takes
+``requests``, which say whose tokens take which adapter.
+
 ``attn_mask`` is accepted and ignored, as in the reference (attn.py:91-97).
 :func:`project_qkv` is steps 1-2 on their own (the producer of q, k, v).
 """
@@ -33,10 +38,12 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import nn
 
-from .int8 import Int8Rows, fused_int8_supported, is_int8, project_qkv_int8, quantize_int8
+from .adapters import AdapterRequests, add_adapters, is_adapted
+from .int8 import Int8Linear, Int8Rows, fused_int8_supported, is_int8, project_qkv_int8, quantize_int8
 from .ops import RingAttention
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn
-from .qkv import ProjectQKVFn, fused_supported, qkv_project
+from .qkv import HEAD_DIM, ProjectQKVFn, fused_supported, qkv_project
+from .rope import AxialPositions, qk_norm_axial_rope
 
 
 def _norm_rope(x: torch.Tensor, norm: Optional[nn.Module], freqs_cis: Optional[torch.Tensor]) -> torch.Tensor:
@@ -53,15 +60,74 @@ def _norm_rope(x: torch.Tensor, norm: Optional[nn.Module], freqs_cis: Optional[t
     return x
 
 
-def project_qkv(attn: nn.Module, hidden_states: Union[torch.Tensor, Int8Rows], freqs_cis: Optional[torch.Tensor],
-                fused: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+Freqs = Union[None, torch.Tensor, AxialPositions]
+
+
+def _norms(attn) -> Tuple[Optional[nn.Module], Optional[nn.Module]]:
+    return getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)
+
+
+def _norm_axial_rope(attn, query: torch.Tensor, key: torch.Tensor, freqs: AxialPositions):
+    """The QK RMSNorms where the module has them, and the rotation, q and k in one launch."""
+    nq, nk = _norms(attn)
+    return qk_norm_axial_rope(query, key, freqs.positions, freqs.rope, getattr(nq, "weight", None),
+                              getattr(nk, "weight", None),
+                              tuple(None if n is None else float(n.eps) for n in (nq, nk)))
+
+
+def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: Freqs,
+                     requests: Optional[AdapterRequests]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """project_qkv of a module with adapters."""
+    x, heads, rows = hidden_states, attn.heads, None
+    bases = [m.base if is_adapted(m) else m for m in (attn.to_q, attn.to_k, attn.to_v)]
+    int8 = [isinstance(m, Int8Linear) for m in bases]
+    if isinstance(x, Int8Rows):
+        if not all(int8):
+            raise ValueError("8-bit hidden states need 8-bit projections (harp_amd.quantize_attention)")
+        rows, x = x, x.dequantize() if requests is not None else x
+    elif any(int8):
+        rows = quantize_int8(x)  # once for all three
+
+    def project(module, quantised):
+        y = module(rows if quantised else x)
+        if requests is not None and is_adapted(module):
+            y = add_adapters(y, x, module.adapters, requests)
+        return y.unflatten(-1, (heads, -1)).transpose(1, 2)
+
+    query, key, value = (project(m, i) for m, i in zip((attn.to_q, attn.to_k, attn.to_v), int8))
+    if isinstance(freqs, AxialPositions):
+        query, key = _norm_axial_rope(attn, query, key, freqs)
+    else:
+        nq, nk = _norms(attn)
+        query, key = _norm_rope(query, nq, freqs), _norm_rope(key, nk, freqs)
+    return query, key, value
+
+
+def project_qkv(attn: nn.Module, hidden_states: Union[torch.Tensor, Int8Rows], freqs_cis: Freqs, fused: bool = True,
+                requests: Optional[AdapterRequests] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """q, k, v as token-major [B, H, S, D] views: projections, then QK RMSNorm
     and RoPE (attn.py:69-89).  With ``fused`` (default) and a module and input
     the fused kernel takes (:func:`harp_amd.qkv.fused_supported`: head dim
     128, no bias), all of it is one launch (:class:`ProjectQKVFn`); otherwise
     three library GEMMs and the separate norm + RoPE kernels.  With 8-bit
     projections the one launch is :func:`harp_amd.int8.project_qkv_int8` where
-    it applies, else three 8-bit products and the separate kernels."""
+    it applies, else three 8-bit products and the separate kernels.
+
+    ``freqs_cis`` may be positions along several axes
+    (:class:`harp_amd.AxialPositions`): the one-launch forms read their table,
+    otherwise :func:`harp_amd.qk_norm_axial_rope` norms and rotates q and k.
+    ``requests``: which tokens take which of the module's adapters
+    (:func:`harp_amd.adapt_attention`); without it none is added."""
+    adapted = any(is_adapted(getattr(attn, n, None)) for n in ("to_q", "to_k", "to_v"))
+    if requests is not None and not adapted and not _adapted_out(attn):
+        raise ValueError("requests need an attention module with adapters (harp_amd.adapt_attention)")
+    if adapted:
+        return _project_adapted(attn, hidden_states, freqs_cis, requests)
+    axial = freqs_cis if isinstance(freqs_cis, AxialPositions) else None
+    if axial is not None:
+        # the one-launch forms: neighbouring pairs of heads of 128 features
+        fused = fused and axial.rope.layout == "interleaved" and axial.rope.dim == HEAD_DIM
+        freqs_cis = axial.table() if fused else None
     if is_int8(attn):
         if not isinstance(hidden_states, Int8Rows):
             hidden_states = quantize_int8(hidden_states)  # once for all three
@@ -85,9 +151,17 @@ def project_qkv(attn: nn.Module, hidden_states: Union[torch.Tensor, Int8Rows], f
     query = attn.to_q(hidden_states).unflatten(-1, (heads, -1)).transpose(1, 2)
     key = attn.to_k(hidden_states).unflatten(-1, (heads, -1)).transpose(1, 2)
     value = attn.to_v(hidden_states).unflatten(-1, (heads, -1)).transpose(1, 2)
+    if axial is not None:
+        query, key = _norm_axial_rope(attn, query, key, axial)
+        return query, key, value
     query = _norm_rope(query, getattr(attn, "norm_q", None), freqs_cis)
     key = _norm_rope(key, getattr(attn, "norm_k", None), freqs_cis)
     return query, key, value
+
+
+def _adapted_out(attn) -> bool:
+    to_out = getattr(attn, "to_out", None)
+    return to_out is not None and len(to_out) > 0 and is_adapted(to_out[0])
 
 
 class RingZAttention(nn.Module):
@@ -104,15 +178,15 @@ class RingZAttention(nn.Module):
         self.attn = pretrained_attn
         self.sp_size = sp_size
 
-    def forward(self, hidden_states: Union[torch.Tensor, Int8Rows], RoPE_embeds: Optional[torch.Tensor],
-                attn_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward(self, hidden_states: Union[torch.Tensor, Int8Rows], RoPE_embeds: Freqs,
+                attn_mask: Optional[torch.Tensor] = None, requests: Optional[AdapterRequests] = None) -> torch.Tensor:
         attn = self.attn
         tokens = (hidden_states.values if isinstance(hidden_states, Int8Rows) else hidden_states).size(1)
         if tokens % self.sp_size:
             raise ValueError(f"sequence length {tokens} is not a multiple of sp_size {self.sp_size}")
-        query, key, value = project_qkv(attn, hidden_states, RoPE_embeds)
+        query, key, value = project_qkv(attn, hidden_states, RoPE_embeds, requests=requests)
         out = RingAttention.apply(query, key, value, self.sp_size).transpose(1, 2).flatten(2, 3)
-        out = attn.to_out[0](out)
+        out = attn.to_out[0](out, requests) if _adapted_out(attn) else attn.to_out[0](out)
         if len(attn.to_out) > 1:  # dropout / identity
             out = attn.to_out[1](out)
         return out

@@ -4,7 +4,8 @@ Outputs (all under ``kernels/`` at the repository root, next to each other
 so the operator libraries find the C-ABI library through ``$ORIGIN``):
 
 * ``libharp_ra.so``              HIP kernels + the C ABIs of include/harp_ring_attn.h,
-                                 include/harp_qk_norm_rope.h and include/harp_block_ops.h
+                                 include/harp_qk_norm_rope.h, include/harp_block_ops.h
+                                 and include/harp_request_ops.h
                                  (hipcc, --offload-arch=gfx950).
 * ``libring_attention_ops.so``   the PyTorch operator library (namespace
                                  ``ring_attention_ops``), the drop-in for the
@@ -16,6 +17,9 @@ so the operator libraries find the C-ABI library through ``$ORIGIN``):
 * ``libharp_block_ops.so``       the PyTorch operator library for the residual
                                  RMSNorm, 8-bit rows and their products
                                  (namespace ``harp_block``).
+* ``libharp_request_ops.so``     the PyTorch operator library for rotary positions
+                                 with several axes and low-rank adapters of many
+                                 requests (namespace ``harp_request``).
 
 Run ``python -m harp_amd.build`` (or ``__graft_entry__.build()``).
 """
@@ -37,15 +41,18 @@ ABI_LIB = OUT / "libharp_ra.so"
 OPS_LIB = OUT / "libring_attention_ops.so"
 ASYNC_OPS_LIB = OUT / "libharp_async_op.so"
 BLOCK_OPS_LIB = OUT / "libharp_block_ops.so"
+REQUEST_OPS_LIB = OUT / "libharp_request_ops.so"
 
 HIP_SOURCES = ["ra_kernels.hip", "fwd_asm.hip", "dq_asm.hip", "dkdv_asm.hip", "ra_abi.hip", "qk_kernels.hip", "qk_abi.hip", "proj_kernels.hip",
-               "norm_kernels.hip", "prod8_kernels.hip", "blk_abi.hip"]
-HIP_HEADERS = ["ra_common.h", "ra_kernels.h", "qk_kernels.h", "proj_kernels.h", "blk_kernels.h", "fwd_asm.inc", "fwd_asm_gen.py",
+               "norm_kernels.hip", "prod8_kernels.hip", "blk_abi.hip", "rope_kernels.hip", "adapter_kernels.hip",
+               "req_abi.hip"]
+HIP_HEADERS = ["ra_common.h", "ra_kernels.h", "qk_kernels.h", "proj_kernels.h", "blk_kernels.h", "req_kernels.h", "fwd_asm.inc", "fwd_asm_gen.py",
                "dq_asm.inc", "dq_asm_gen.py", "dkdv_asm.inc",
-               "dkdv_asm_gen.py", "asm_sched.py"]
+               "dkdv_asm_gen.py", "asm_sched.py", "torch_autograd_util.h"]
 OPS_SOURCE = "torch_ring_attention_ops.cpp"
 ASYNC_OPS_SOURCE = "torch_async_op.cpp"
 BLOCK_OPS_SOURCE = "torch_block_ops.cpp"
+REQUEST_OPS_SOURCE = "torch_request_ops.cpp"
 
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 OFFLOAD_ARCH = "gfx950"
@@ -158,22 +165,29 @@ def build_block_ops(verbose: bool = False) -> Path:
     return build_ops(verbose, BLOCK_OPS_SOURCE, BLOCK_OPS_LIB, "harp_block_ops")
 
 
+def build_request_ops(verbose: bool = False) -> Path:
+    """kernels/libharp_request_ops.so: the harp_request operators (rotary positions, low-rank adapters)."""
+    return build_ops(verbose, REQUEST_OPS_SOURCE, REQUEST_OPS_LIB, "harp_request_ops")
+
+
 def build(verbose: bool = False) -> None:
     """Compile every library unconditionally (the build check)."""
     build_abi(verbose)
     build_ops(verbose)
     build_async_ops(verbose)
     build_block_ops(verbose)
+    build_request_ops(verbose)
 
 
 def sources_newer_than_libs() -> bool:
     """True when a source file is newer than a built library (or one is missing)."""
-    libs = [ABI_LIB, OPS_LIB, ASYNC_OPS_LIB, BLOCK_OPS_LIB]
+    libs = [ABI_LIB, OPS_LIB, ASYNC_OPS_LIB, BLOCK_OPS_LIB, REQUEST_OPS_LIB]
     if not all(p.exists() for p in libs):
         return True
     newest_lib = min(p.stat().st_mtime for p in libs)
-    srcs = [CSRC / s for s in HIP_SOURCES + HIP_HEADERS + [OPS_SOURCE, ASYNC_OPS_SOURCE, BLOCK_OPS_SOURCE]]
-    srcs += [INCLUDE / h for h in ("harp_ring_attn.h", "harp_qk_norm_rope.h", "harp_block_ops.h")]
+    srcs = [CSRC / s for s in HIP_SOURCES + HIP_HEADERS
+            + [OPS_SOURCE, ASYNC_OPS_SOURCE, BLOCK_OPS_SOURCE, REQUEST_OPS_SOURCE]]
+    srcs += [INCLUDE / h for h in ("harp_ring_attn.h", "harp_qk_norm_rope.h", "harp_block_ops.h", "harp_request_ops.h")]
     return any(s.stat().st_mtime > newest_lib for s in srcs)
 
 

@@ -1,0 +1,478 @@
+// C ABI of the kernels for requests of one batch (rotary positions, low-rank
+// adapters): argument validation and kernel sequencing.  See
+// include/harp_request_ops.h.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <string>
+#include <utility>
+
+#include "../../include/harp_request_ops.h"
+#include "req_kernels.h"
+
+using namespace harp_req;
+
+static_assert(HARP_REQ_F32 == kF32 && HARP_REQ_BF16 == kBf16 && HARP_REQ_I32 == kI32 && HARP_REQ_I64 == kI64,
+              "the kernels' element types");
+static_assert(HARP_REQ_MAX_AXES == kMaxAxes && HARP_REQ_MAX_RANK == kMaxRank, "the kernels' limits");
+
+namespace {
+
+thread_local std::string g_last_error;
+
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return code;
+}
+int ok() {
+  g_last_error.clear();
+  return HARP_REQ_OK;
+}
+int launched(hipError_t e, const char* what) {
+  if (e != hipSuccess) return fail(HARP_REQ_ELAUNCH, "%s launch failed: %s", what, hipGetErrorString(e));
+  return ok();
+}
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+constexpr int64_t kMaxRows = (int64_t)1 << 31;
+constexpr int kMaxTokens = 1 << 28, kMaxDim = 1 << 22, kMaxCount = 1 << 20, kMaxAdapters = 1 << 14;
+
+// ---------------------------------------------------------------------------
+// Rope
+// ---------------------------------------------------------------------------
+int check_axes(const harp_req_axes_t* in, RopeAxes& ax, int& D) {
+  if (!in) return fail(HARP_REQ_EINVAL, "axes is NULL");
+  if (in->n < 1 || in->n > kMaxAxes) return fail(HARP_REQ_EINVAL, "%d axes: 1 to %d", in->n, kMaxAxes);
+  ax = RopeAxes{};
+  ax.n = in->n;
+  int64_t pairs = 0;
+  for (int a = 0; a < in->n; ++a) {
+    const int w = in->width[a];
+    if (w < 2 || w % 2 || w > kMaxRopeDim)
+      return fail(HARP_REQ_EINVAL, "width[%d]=%d must be even, 2 to %d", a, w, kMaxRopeDim);
+    if (!(in->theta[a] > 0.0) || !std::isfinite(in->theta[a]))
+      return fail(HARP_REQ_EINVAL, "theta[%d] must be positive and finite", a);
+    // turns: theta^(-2 j / w) / (2 pi) = 2^(c0 + c1 p), j = p - pairs
+    ax.c1[a] = -2.0 / w * std::log2(in->theta[a]);
+    ax.c0[a] = -2.6514961294723187980 - ax.c1[a] * (double)pairs;  // log2(1 / (2 pi))
+    pairs += w / 2;
+    ax.end[a] = (int)pairs;
+  }
+  D = (int)(2 * pairs);
+  if (D % 8 || D > kMaxRopeDim)
+    return fail(HARP_REQ_EUNSUPPORTED, "heads of %d features: the axes' widths must add up to a multiple of 8, at most %d",
+                D, kMaxRopeDim);
+  return HARP_REQ_OK;
+}
+int check_positions(const harp_req_positions_t* in, RopePos& pos) {
+  if (!in || !in->p) return fail(HARP_REQ_EINVAL, "positions is NULL");
+  if (in->dtype != kI32 && in->dtype != kI64 && in->dtype != kF32)
+    return fail(HARP_REQ_EINVAL, "positions dtype must be I32, I64 or F32");
+  if (!aligned(in->p, in->dtype == kI64 ? 8 : 4)) return fail(HARP_REQ_EINVAL, "positions must be aligned to its elements");
+  pos = RopePos{in->p, in->dtype, in->stride_b, in->stride_s, in->stride_a};
+  return HARP_REQ_OK;
+}
+int check_batch(int batch, int seq) {
+  if (batch < 0 || seq < 0) return fail(HARP_REQ_EINVAL, "batch=%d and seq=%d must not be negative", batch, seq);
+  if ((int64_t)batch * seq > kMaxRows) return fail(HARP_REQ_EUNSUPPORTED, "batch * seq > 2^31");
+  return HARP_REQ_OK;
+}
+int check_view(const void* p, const int64_t (&st)[3], const char* t, const char* name, RopeStrides& out) {
+  if (!p || !aligned(p, 16)) return fail(HARP_REQ_EINVAL, "%s.%s must be a 16-byte aligned device pointer", t, name);
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] % 8 || (i && st[i] > INT32_MAX))
+      return fail(HARP_REQ_EINVAL, "%s.%s strides (%lld, %lld, %lld) must be multiples of 8, not negative, the last two below 2^31",
+                  t, name, (long long)st[0], (long long)st[1], (long long)st[2]);
+  out = RopeStrides{st[0], (int)st[1], (int)st[2]};
+  return HARP_REQ_OK;
+}
+// no two elements at one address: sorted by stride, each covers what lies inside it
+bool overlaps(const int64_t (&st)[3], int B, int H, int S, int D) {
+  int64_t stride[3] = {st[0], st[1], st[2]}, size[3] = {B, H, S};
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 3; ++j)
+      if (stride[j] < stride[i]) {
+        std::swap(stride[i], stride[j]);
+        std::swap(size[i], size[j]);
+      }
+  __int128 extent = D;
+  for (int i = 0; i < 3; ++i) {
+    if (size[i] == 1) continue;
+    if (stride[i] < extent) return true;
+    extent += (__int128)stride[i] * (size[i] - 1);
+  }
+  return false;
+}
+int check_heads(const harp_req_heads_t* in, RopeParams& p, bool backward) {
+  if (!in) return fail(HARP_REQ_EINVAL, "heads is NULL");
+  static const char* const names[2] = {"q", "k"};
+  int64_t all = 0;
+  for (int i = 0; i < 2; ++i) {
+    const harp_req_heads_t& h = in[i];
+    RopeHeads& t = p.t[i];
+    int rc;
+    if (h.heads < 0) return fail(HARP_REQ_EINVAL, "%s.heads=%d must not be negative", names[i], h.heads);
+    all += h.heads;
+    if (!h.heads) continue;
+    t.H = h.heads;
+    t.norm = h.norm != 0;
+    if (!backward || h.norm) {
+      if ((rc = check_view(h.x, h.x_stride, names[i], "x", t.sx))) return rc;
+      t.x = h.x;
+    }
+    if ((rc = check_view(h.y, h.y_stride, names[i], "y", t.sy))) return rc;
+    t.y = h.y;
+    if (overlaps(h.y_stride, p.B, h.heads, p.S, p.D))
+      return fail(HARP_REQ_EINVAL, "%s.y has two elements at one address", names[i]);
+    if (backward) {
+      if ((rc = check_view(h.dy, h.dy_stride, names[i], "dy", t.sdy))) return rc;
+      t.dy = h.dy;
+    }
+    if (h.norm) {
+      if (!(h.eps >= 0.f)) return fail(HARP_REQ_EINVAL, "%s.eps must be a non-negative number", names[i]);
+      t.eps = h.eps;
+      if (h.weight) {
+        if (h.weight_dtype != kF32 && h.weight_dtype != kBf16)
+          return fail(HARP_REQ_EINVAL, "%s.weight dtype must be F32 or BF16", names[i]);
+        if (!aligned(h.weight, h.weight_dtype == kF32 ? 4 : 2))
+          return fail(HARP_REQ_EINVAL, "%s.weight must be aligned to its elements", names[i]);
+        t.w = h.weight;
+        t.w_f32 = h.weight_dtype == kF32;
+      }
+    } else if (h.weight || h.grad_weight) {
+      return fail(HARP_REQ_EINVAL, "%s has a weight without a norm", names[i]);
+    }
+    if (backward && h.grad_weight && (!h.weight || !aligned(h.grad_weight, h.weight_dtype == kF32 ? 4 : 2)))
+      return fail(HARP_REQ_EINVAL, "%s.grad_weight needs a weight and its alignment", names[i]);
+  }
+  if ((int64_t)p.B * p.S * all > kMaxRows) return fail(HARP_REQ_EUNSUPPORTED, "batch * seq * heads > 2^31");
+  return HARP_REQ_OK;
+}
+int rope_inputs(RopeParams& p, const harp_req_axes_t* axes, const harp_req_positions_t* positions,
+                const harp_req_heads_t* heads, int batch, int seq, int dtype, bool backward) {
+  int rc;
+  if ((rc = check_axes(axes, p.axes, p.D))) return rc;
+  if ((rc = check_batch(batch, seq))) return rc;
+  if (dtype != kF32 && dtype != kBf16) return fail(HARP_REQ_EINVAL, "dtype must be F32 or BF16");
+  p.B = batch;
+  p.S = seq;
+  p.half = axes->half != 0;
+  p.f32 = dtype == kF32;
+  p.sign = backward ? -1.f : 1.f;
+  if (!((int64_t)batch * seq)) return HARP_REQ_OK;
+  if ((rc = check_positions(positions, p.pos))) return rc;
+  return check_heads(heads, p, backward);
+}
+
+// ---------------------------------------------------------------------------
+// Adapters
+// ---------------------------------------------------------------------------
+int check_adapters(const harp_req_adapters_t* a, int K, int N, bool pointers) {
+  if (!a) return fail(HARP_REQ_EINVAL, "adapters is NULL");
+  if (a->n < 1 || a->rank < 1) return fail(HARP_REQ_EINVAL, "n=%d and rank=%d must be positive", a->n, a->rank);
+  if (a->n > kMaxAdapters) return fail(HARP_REQ_EUNSUPPORTED, "n=%d adapters > %d", a->n, kMaxAdapters);
+  if (a->rank > kMaxRank) return fail(HARP_REQ_EUNSUPPORTED, "rank=%d > %d", a->rank, kMaxRank);
+  if (K < 1 || N < 1) return fail(HARP_REQ_EINVAL, "k_dim=%d and n_dim=%d must be positive", K, N);
+  if (K > kMaxDim || N > kMaxDim) return fail(HARP_REQ_EUNSUPPORTED, "k_dim=%d, n_dim=%d: more than 2^22", K, N);
+  if (!pointers) return HARP_REQ_OK;
+  if (!a->a || !aligned(a->a, 2) || !a->b || !aligned(a->b, 2))
+    return fail(HARP_REQ_EINVAL, "a and b must be device pointers aligned to their elements");
+  if (!aligned(a->scales, 4)) return fail(HARP_REQ_EINVAL, "scales must be 4-byte aligned");
+  return HARP_REQ_OK;
+}
+int check_tokens(int tokens) {
+  if (tokens < 0) return fail(HARP_REQ_EINVAL, "tokens=%d must not be negative", tokens);
+  if (tokens > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "tokens=%d > 2^28", tokens);
+  return HARP_REQ_OK;
+}
+int check_requests(const harp_req_requests_t* r, int tokens, int n, Requests& q) {
+  if (!r) return fail(HARP_REQ_EINVAL, "requests is NULL");
+  if (r->count < 1) return fail(HARP_REQ_EINVAL, "count=%d must be positive", r->count);
+  if (r->count > kMaxCount) return fail(HARP_REQ_EUNSUPPORTED, "count=%d > 2^20", r->count);
+  auto ints = [](const void* p, int dtype, const char* name) {
+    if (dtype != kI32 && dtype != kI64) return fail(HARP_REQ_EINVAL, "%s dtype must be I32 or I64", name);
+    if (!aligned(p, dtype == kI64 ? 8 : 4)) return fail(HARP_REQ_EINVAL, "%s must be aligned to its elements", name);
+    return (int)HARP_REQ_OK;
+  };
+  int rc;
+  if (!r->index) return fail(HARP_REQ_EINVAL, "index is NULL");
+  if ((rc = ints(r->index, r->index_dtype, "index"))) return rc;
+  if (r->offsets) {
+    if ((rc = ints(r->offsets, r->offsets_dtype, "offsets"))) return rc;
+  } else if (tokens % r->count) {
+    return fail(HARP_REQ_EINVAL, "%d tokens are not %d requests of one length: offsets are needed", tokens, r->count);
+  }
+  q = Requests{r->index,         r->offsets, r->index_dtype == kI64, r->offsets && r->offsets_dtype == kI64, r->count,
+               tokens / r->count, tokens,     n};
+  return HARP_REQ_OK;
+}
+int check_matrix(const void* p, int64_t ld, int dtype, int cols, bool output, const char* name) {
+  if (!p) return fail(HARP_REQ_EINVAL, "%s is NULL", name);
+  if (!aligned(p, dtype == kF32 ? 4 : 2)) return fail(HARP_REQ_EINVAL, "%s must be aligned to its elements", name);
+  if (output ? ld < cols : ld < 0)
+    return fail(HARP_REQ_EINVAL, "%s row stride %lld must be %s", name, (long long)ld,
+                output ? "at least its columns (rows may not overlap)" : "non-negative");
+  return HARP_REQ_OK;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// the backward's workspace: u, B and A transposed, partial gradients
+struct BackwardPlan {
+  GradParams grad;
+  size_t u, bt, at, part, total;  // offsets
+};
+BackwardPlan backward_plan(int tokens, int K, int N, int n, int rank, int count, bool dx, bool da, bool db) {
+  BackwardPlan w{};
+  const size_t rp = rank_pad(rank);
+  w.grad.req.count = count;
+  w.grad.req.tokens = tokens;
+  w.grad.req.n = n;
+  w.grad.r = rank;
+  w.grad.rp = (int)rp;
+  // (the pointers tell which sums run; only whether they are NULL counts here)
+  w.grad.part[0].C = K;
+  w.grad.part[0].out = da ? (void*)1 : nullptr;
+  w.grad.part[1].C = N;
+  w.grad.part[1].out = db ? (void*)1 : nullptr;
+  w.grad.splits = grad_splits(w.grad);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t r = at;
+    at += align256(bytes);
+    return r;
+  };
+  w.u = take(dx || da ? (size_t)tokens * rp * 4 : 0);
+  w.bt = take(dx || da ? (size_t)n * rank * N * 2 : 0);
+  w.at = take(dx ? (size_t)n * rank * K * 2 : 0);
+  w.part = take(w.grad.splits > 1 ? (size_t)w.grad.splits * n * rank * ((da ? K : 0) + (size_t)(db ? N : 0)) * 4 : 0);
+  w.total = at;
+  return w;
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* harp_req_last_error(void) { return g_last_error.c_str(); }
+
+int harp_req_qk_norm_rope_forward(const harp_req_axes_t* axes, const harp_req_positions_t* positions,
+                                  const harp_req_heads_t* heads, int batch, int seq, int dtype, void* stream) {
+  RopeParams p{};
+  const int rc = rope_inputs(p, axes, positions, heads, batch, seq, dtype, false);
+  if (rc) return rc;
+  if (!(p.t[0].H + p.t[1].H) || !((int64_t)batch * seq)) return ok();
+  return launched(launch_rope_forward(p, (hipStream_t)stream), "QK norm and rotation");
+}
+
+size_t harp_req_qk_backward_workspace_bytes(int batch, int seq, int d, int q_heads, int k_heads) {
+  if (check_batch(batch, seq)) return (size_t)-1;
+  if (d < 8 || d % 8 || d > kMaxRopeDim || q_heads < 0 || k_heads < 0 ||
+      (int64_t)batch * seq * ((int64_t)q_heads + k_heads) > kMaxRows) {
+    fail(HARP_REQ_EINVAL, "d=%d, q_heads=%d, k_heads=%d: no such call", d, q_heads, k_heads);
+    return (size_t)-1;
+  }
+  RopeParams p{};
+  p.B = batch;
+  p.S = seq;
+  p.D = d;
+  p.t[0].H = q_heads;
+  p.t[1].H = k_heads;
+  int n[2];
+  rope_bwd_blocks(p, n);
+  return ((size_t)n[0] + n[1]) * d * sizeof(float);
+}
+
+int harp_req_qk_norm_rope_backward(const harp_req_axes_t* axes, const harp_req_positions_t* positions,
+                                   const harp_req_heads_t* heads, int batch, int seq, int dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  RopeParams p{};
+  int rc = rope_inputs(p, axes, positions, heads, batch, seq, dtype, true);
+  if (rc) return rc;
+  if (!(p.t[0].H + p.t[1].H) || !((int64_t)batch * seq)) return ok();
+  // a tensor without a norm is turned back by the forward kernel, the others by the backward kernel
+  RopeParams turn = p, back = p;
+  void* gw[2] = {nullptr, nullptr};
+  int gw_f32[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    if (p.t[i].norm) {
+      turn.t[i].H = 0;
+      gw[i] = p.t[i].H ? heads[i].grad_weight : nullptr;
+      gw_f32[i] = p.t[i].w_f32;
+    } else {
+      back.t[i].H = 0;
+      turn.t[i].x = p.t[i].dy;
+      turn.t[i].sx = p.t[i].sdy;
+    }
+  }
+  int blocks[2];
+  rope_bwd_blocks(back, blocks);
+  if (gw[0] || gw[1]) {
+    const size_t need = ((size_t)blocks[0] + blocks[1]) * p.D * sizeof(float);
+    if (!workspace || workspace_bytes < need)
+      return fail(HARP_REQ_ENOMEM, "workspace of %zu bytes is smaller than the %zu bytes needed",
+                  workspace ? workspace_bytes : (size_t)0, need);
+    if (!aligned(workspace, 16)) return fail(HARP_REQ_EINVAL, "workspace must be 16-byte aligned");
+    back.wpart = (float*)workspace;
+  }
+  if (turn.t[0].H + turn.t[1].H &&
+      (rc = launched(launch_rope_forward(turn, (hipStream_t)stream), "rotation backward")))
+    return rc;
+  if (back.t[0].H + back.t[1].H &&
+      (rc = launched(launch_rope_backward(back, (hipStream_t)stream), "QK norm and rotation backward")))
+    return rc;
+  if (!back.wpart) return ok();
+  return launched(launch_rope_wgrad(back.wpart, blocks, p.D, gw, gw_f32, (hipStream_t)stream),
+                  "weight-gradient reduction");
+}
+
+int harp_req_rope_table(const harp_req_axes_t* axes, const harp_req_positions_t* positions, int batch, int seq,
+                        float* table, void* stream) {
+  RopeAxes ax;
+  RopePos pos;
+  int rc, D;
+  if ((rc = check_axes(axes, ax, D))) return rc;
+  if ((rc = check_batch(batch, seq))) return rc;
+  if (!((int64_t)batch * seq)) return ok();
+  if ((rc = check_positions(positions, pos))) return rc;
+  if (!table || !aligned(table, 8)) return fail(HARP_REQ_EINVAL, "table must be an 8-byte aligned device pointer");
+  return launched(launch_rope_table(ax, pos, batch, seq, D, table, (hipStream_t)stream), "rotary table");
+}
+
+int harp_req_adapter_columns(int rank) {
+  if (rank < 1 || rank > kMaxRank) {
+    fail(HARP_REQ_EINVAL, "rank=%d: 1 to %d", rank, kMaxRank);
+    return -1;
+  }
+  return rank_pad(rank);
+}
+
+int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base, int64_t ld_base, void* out,
+                                  int64_t ld_out, int dtype, const harp_req_adapters_t* adapters,
+                                  const harp_req_requests_t* requests, float* t, int tokens, int k_dim, int n_dim,
+                                  void* stream) {
+  int rc;
+  Requests q;
+  if (dtype != kF32 && dtype != kBf16) return fail(HARP_REQ_EINVAL, "dtype must be F32 or BF16");
+  if ((rc = check_tokens(tokens))) return rc;
+  if ((rc = check_adapters(adapters, k_dim, n_dim, tokens > 0))) return rc;
+  if (tokens == 0) return ok();
+  if ((rc = check_requests(requests, tokens, adapters->n, q))) return rc;
+  if ((rc = check_matrix(x, ld_x, kBf16, k_dim, false, "x"))) return rc;
+  if ((rc = check_matrix(base, ld_base, dtype, n_dim, base == out, "base"))) return rc;
+  if ((rc = check_matrix(out, ld_out, dtype, n_dim, true, "out"))) return rc;
+  if (base == out && ld_base != ld_out) return fail(HARP_REQ_EINVAL, "out in base's place needs base's row stride");
+  if (!t || !aligned(t, 16)) return fail(HARP_REQ_EINVAL, "t must be a 16-byte aligned device pointer");
+  ShrinkParams s{};
+  s.req = q;
+  s.x = x;
+  s.ldx = ld_x;
+  s.K = k_dim;
+  s.r = adapters->rank;
+  s.rp = rank_pad(adapters->rank);
+  s.ldt = s.rp;
+  s.sets = 1;
+  s.set[0] = ShrinkSet{adapters->a, adapters->scales, t};
+  if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
+  ExpandParams e{};
+  e.req = q;
+  e.t = t;
+  e.ldt = s.rp;
+  e.b = adapters->b;
+  e.base = base;
+  e.ld_base = ld_base;
+  e.out = out;
+  e.ld_out = ld_out;
+  e.f32 = dtype == kF32;
+  e.N = n_dim;
+  e.r = s.r;
+  e.rp = s.rp;
+  return launched(launch_expand(e, (hipStream_t)stream), "adapters (t B^T)");
+}
+
+size_t harp_req_adapter_backward_workspace_bytes(int tokens, int k_dim, int n_dim, int n, int rank, int count,
+                                                 int want_da, int want_db) {
+  const harp_req_adapters_t a{nullptr, nullptr, nullptr, n, rank};
+  if (check_tokens(tokens) || check_adapters(&a, k_dim, n_dim, false)) return (size_t)-1;
+  if (count < 1 || count > kMaxCount) {
+    fail(HARP_REQ_EINVAL, "count=%d: 1 to 2^20", count);
+    return (size_t)-1;
+  }
+  return backward_plan(tokens, k_dim, n_dim, n, rank, count, true, want_da, want_db).total;
+}
+
+int harp_req_add_adapters_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const float* t,
+                                   const harp_req_adapters_t* adapters, const harp_req_requests_t* requests, void* dx,
+                                   int64_t ld_dx, int add_to_dx, void* da, void* db, int tokens, int k_dim, int n_dim,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  Requests q;
+  if ((rc = check_tokens(tokens))) return rc;
+  if ((rc = check_adapters(adapters, k_dim, n_dim, tokens > 0))) return rc;
+  if (tokens == 0 || (!dx && !da && !db)) return ok();  // (no token: the gradients of a and b are the caller's zeros)
+  if ((rc = check_requests(requests, tokens, adapters->n, q))) return rc;
+  if ((rc = check_matrix(dy, ld_dy, kBf16, n_dim, false, "dy"))) return rc;
+  if (da && (rc = check_matrix(x, ld_x, kBf16, k_dim, false, "x"))) return rc;
+  if (dx && (rc = check_matrix(dx, ld_dx, kBf16, k_dim, true, "dx"))) return rc;
+  if (!aligned(da, 2) || !aligned(db, 2)) return fail(HARP_REQ_EINVAL, "da and db must be aligned to their elements");
+  if (db && (!t || !aligned(t, 16))) return fail(HARP_REQ_EINVAL, "t must be a 16-byte aligned device pointer");
+  const int n = adapters->n, r = adapters->rank, rp = rank_pad(r);
+  BackwardPlan w = backward_plan(tokens, k_dim, n_dim, n, r, q.count, dx, da, db);
+  if (w.total && (!workspace || workspace_bytes < w.total))
+    return fail(HARP_REQ_ENOMEM, "workspace of %zu bytes is smaller than the %zu bytes needed",
+                workspace ? workspace_bytes : (size_t)0, w.total);
+  if (!aligned(workspace, 16)) return fail(HARP_REQ_EINVAL, "workspace must be 16-byte aligned");
+  char* const ws = (char*)workspace;
+  float* const u = (float*)(ws + w.u);
+  hipStream_t st = (hipStream_t)stream;
+  if (dx || da) {
+    TransposeParams tp{};
+    tp.n = n;
+    tp.part[0] = TransposePart{adapters->b, ws + w.bt, n_dim, r};
+    if (dx) tp.part[1] = TransposePart{adapters->a, ws + w.at, r, k_dim};
+    if ((rc = launched(launch_transpose(tp, st), "adapters' transpose"))) return rc;
+    ShrinkParams s{};
+    s.req = q;
+    s.x = dy;
+    s.ldx = ld_dy;
+    s.K = n_dim;
+    s.r = r;
+    s.rp = rp;
+    s.ldt = rp;
+    s.sets = 1;
+    s.set[0] = ShrinkSet{ws + w.bt, adapters->scales, u};
+    if ((rc = launched(launch_shrink(s, st), "adapters (dy B)"))) return rc;
+  }
+  if (dx) {
+    ExpandParams e{};
+    e.req = q;
+    e.t = u;
+    e.ldt = rp;
+    e.b = ws + w.at;
+    e.base = add_to_dx ? dx : nullptr;
+    e.ld_base = ld_dx;
+    e.out = dx;
+    e.ld_out = ld_dx;
+    e.N = k_dim;
+    e.r = r;
+    e.rp = rp;
+    if ((rc = launched(launch_expand(e, st), "adapters (u A)"))) return rc;
+  }
+  if (!da && !db) return ok();
+  GradParams& g = w.grad;
+  g.req = q;
+  g.part[0] = GradPart{x, ld_x, u, rp, k_dim, 0, da};
+  g.part[1] = GradPart{dy, ld_dy, t, rp, n_dim, 1, db};
+  g.work = (float*)(ws + w.part);
+  return launched(launch_adapter_grad(g, st), "adapters' gradients");
+}
+
+}  // extern "C"

@@ -1,0 +1,566 @@
+// gfx950 kernels of the QK RMSNorm with a rotary embedding of several axes
+// (time, height, width of a token), forward and backward, and of its table.
+//
+//   rho = 1 / sqrt(mean(x^2) + eps),  n = x rho w            (or n = x without a norm)
+//   phi_p = position[axis of p] * theta^(-2 j / width)       (j: the pair's place in its axis)
+//   (y0, y1) = (n0 cos - n1 sin, n0 sin + n1 cos)            pairs (2p, 2p + 1) or (p, p + D / 2)
+//   d = dy turned back by phi,  g = d w,  dx = rho (g - x rho mean(g x rho)),  dw = sum_rows d x rho
+//
+// All arithmetic is fp32 over the stored inputs, every output rounded once, to
+// nearest.  The angle is formed in 64 bits as a share of a turn (position *
+// rate, less its whole turns and then its whole quarters), so that a far
+// position loses nothing; what is left, within an eighth of a turn, takes the
+// Taylor series of sine and cosine in 32 bits (remainders (pi/4)^11 / 11! =
+// 1.8e-9 and (pi/4)^10 / 10! = 2.5e-8).
+//
+// Layout: LPR lanes (8, 16 or 32 for D <= 64, 128, 256) hold a row, 8 values
+// (four pairs) each, so a lane's pairs are the same in every row: their four
+// rates are formed once per thread and their angles once per token, for R heads
+// of that token.  The kernels are bound by memory; the angles' arithmetic runs
+// while the rows' loads are on their way, and no table is read.
+#include <algorithm>
+#include <type_traits>
+
+#include "ra_common.h"
+#include "req_kernels.h"
+
+namespace harp_req {
+
+namespace {
+
+using harp_ra::bf16;
+using harp_ra::f32x4;
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over the LPR lanes of a row's group, the same value in all of them
+template <int LPR>
+__device__ __forceinline__ float group_sum(float v) {
+  if constexpr (LPR == 32)
+    v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401f));  // lane ^ 16
+  if constexpr (LPR >= 16) {
+    v += dpp<0x128>(v);  // row_ror:8
+    v += dpp<0x124>(v);  // row_ror:4
+  } else {
+    v += dpp<0x1b>(dpp<0x141>(v));  // row_half_mirror, then quad_perm:[3,2,1,0]: lane ^ 4
+  }
+  v += dpp<0x4e>(v);  // quad_perm:[2,3,0,1]
+  v += dpp<0xb1>(v);  // quad_perm:[1,0,3,2]
+  return v;
+}
+
+// A lane's 8 values as they are in memory: two runs of four, next to each
+// other (pairs 2p, 2p + 1) or D / 2 apart (HALF).
+template <bool F32>
+struct Raw {
+  typedef u32x2 Run;
+  Run v[2];
+};
+template <>
+struct Raw<true> {
+  typedef f32x4 Run;
+  Run v[2];
+};
+
+template <bool F32, bool HALF>
+__device__ __forceinline__ Raw<F32> load_raw(const char* row, int sub, int D) {
+  Raw<F32> r;
+  constexpr int es = F32 ? 4 : 2;
+  if constexpr (!HALF && !F32) {
+    const u32x4 u = *(const u32x4*)(row + sub * 16);
+    r.v[0] = u32x2{u[0], u[1]};
+    r.v[1] = u32x2{u[2], u[3]};
+  } else {
+    const char* p = row + (HALF ? 4 * sub : 8 * sub) * es;
+    r.v[0] = *(const typename Raw<F32>::Run*)p;
+    r.v[1] = *(const typename Raw<F32>::Run*)(p + (HALF ? D / 2 : 4) * es);
+  }
+  return r;
+}
+// to fp32, in the order of the pairs: (v[0], v[1]) is pair 4 sub, and so on
+template <bool F32, bool HALF>
+__device__ __forceinline__ void unpack(const Raw<F32>& r, float (&v)[8]) {
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[4 * i + k] = r.v[i][k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        t[4 * i + 2 * k] = __uint_as_float(r.v[i][k] << 16);
+        t[4 * i + 2 * k + 1] = __uint_as_float(r.v[i][k] & 0xffff0000u);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    v[2 * k] = HALF ? t[k] : t[2 * k];
+    v[2 * k + 1] = HALF ? t[4 + k] : t[2 * k + 1];
+  }
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {(bf16)lo, (bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+template <bool F32, bool HALF>
+__device__ __forceinline__ void store_row(char* row, int sub, int D, const float (&v)[8]) {
+  float t[8];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    t[HALF ? k : 2 * k] = v[2 * k];
+    t[HALF ? 4 + k : 2 * k + 1] = v[2 * k + 1];
+  }
+  constexpr int es = F32 ? 4 : 2;
+  char* p = row + (HALF ? 4 * sub : 8 * sub) * es;
+  char* q = p + (HALF ? D / 2 : 4) * es;
+  if constexpr (F32) {
+    *(f32x4*)p = f32x4{t[0], t[1], t[2], t[3]};
+    *(f32x4*)q = f32x4{t[4], t[5], t[6], t[7]};
+  } else {
+    const u32x4 u = {pack_bf16(t[0], t[1]), pack_bf16(t[2], t[3]), pack_bf16(t[4], t[5]), pack_bf16(t[6], t[7])};
+    if constexpr (HALF) {
+      *(u32x2*)p = u32x2{u[0], u[1]};
+      *(u32x2*)q = u32x2{u[2], u[3]};
+    } else {
+      *(u32x4*)p = u;
+    }
+  }
+}
+// a lane's weights, in the order of the pairs (any alignment of the vector)
+template <bool HALF>
+__device__ __forceinline__ void load_weight(const void* w, int w_f32, int sub, int D, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 1.f;
+  if (!w) return;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int e0 = HALF ? 4 * sub + k : 8 * sub + 2 * k, e1 = HALF ? e0 + D / 2 : e0 + 1;
+    v[2 * k] = w_f32 ? ((const float*)w)[e0] : __uint_as_float((uint32_t)((const uint16_t*)w)[e0] << 16);
+    v[2 * k + 1] = w_f32 ? ((const float*)w)[e1] : __uint_as_float((uint32_t)((const uint16_t*)w)[e1] << 16);
+  }
+}
+
+// turns per unit of position of pair p, and its axis
+__device__ __forceinline__ double rate_of(const RopeAxes& ax, int p, int& axis) {
+  double c0 = ax.c0[0], c1 = ax.c1[0];
+  axis = 0;
+#pragma unroll
+  for (int a = 1; a < kMaxAxes; ++a)
+    if (a < ax.n && p >= ax.end[a - 1]) {
+      axis = a;
+      c0 = ax.c0[a];
+      c1 = ax.c1[a];
+    }
+  return exp2(__builtin_fma(c1, (double)p, c0));
+}
+// the elements at base + off[k]
+template <int N>
+__device__ __forceinline__ void load_pos(const RopePos& q, int64_t base, const int64_t (&off)[N], double (&v)[N]) {
+  if (q.dtype == kI32) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = (double)((const int32_t*)q.p + base)[off[k]];
+  } else if (q.dtype == kI64) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = (double)((const int64_t*)q.p + base)[off[k]];
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = (double)((const float*)q.p + base)[off[k]];
+  }
+}
+// cos and sin of `turns` turns
+__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
+  turns -= __builtin_rint(turns);                // within half a turn, exact
+  const double q = __builtin_rint(4.0 * turns);  // quarters: -2 .. 2
+  const float x = (float)__builtin_fma(4.0, turns, -q) * 1.57079632679489662f;  // within pi / 4
+  const int n = (int)q;
+  const float x2 = x * x;
+  // x - x^3/3! + x^5/5! - x^7/7! + x^9/9!, and 1 - x^2/2! + x^4/4! - x^6/6! + x^8/8!
+  const float sp = __builtin_fmaf(
+      x * x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f),
+      x);
+  const float cp = __builtin_fmaf(
+      x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 1.f / 40320.f, -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
+  const bool odd = n & 1;
+  s = odd ? cp : sp;
+  c = odd ? sp : cp;
+  if (n == 2 || n == -2 || n == -1) s = -s;
+  if (n == 2 || n == -2 || n == 1) c = -c;
+}
+
+// Workgroups are dealt to the 8 XCDs round-robin: each XCD takes one contiguous
+// range of the work, so that what its L2 holds is one window of memory.
+__device__ __forceinline__ int64_t xcd_block(uint32_t bid, uint32_t blocks) {
+  const uint32_t q = blocks / 8, r = blocks % 8, x = bid % 8, local = bid / 8;
+  return x < r ? x * (q + 1) + local : r * (q + 1) + (x - r) * q + local;
+}
+
+// A launch's blocks: those of q, then those of k (so a block's tensor is
+// uniform).  The heads of a token are dealt to J groups of lanes, R to each.
+struct Range {
+  int64_t first;  // of the tensor's blocks
+  int n;
+};
+struct Ranges {
+  Range q, k;
+};
+struct Unit {
+  uint32_t b, s;
+  int j;
+};
+__device__ __forceinline__ Unit unit_at(int S, int J, int64_t unit) {
+  Unit u;
+  const int64_t tok = unit / J;
+  u.j = (int)(unit - tok * J);
+  u.b = (uint32_t)(tok / S);
+  u.s = (uint32_t)(tok - (int64_t)u.b * S);
+  return u;
+}
+// n units on, in 32 bits (n is a block's groups)
+__device__ __forceinline__ Unit unit_after(uint32_t S, uint32_t J, const Unit& u, uint32_t n) {
+  const uint32_t v = u.j + n, dt = v / J, s = u.s + dt, db = s / S;
+  return Unit{u.b + db, s - db * S, (int)(v - dt * J)};
+}
+__device__ __forceinline__ int64_t offset_of(const RopeStrides& st, const Unit& u, int h) {
+  return u.b * st.b + (int64_t)h * st.h + (int64_t)u.s * st.s;
+}
+
+struct Angles {
+  double rate[4];
+  int64_t axis[4];  // offsets of the pairs' axes in a token's position
+  __device__ __forceinline__ void init(const RopeParams& p, int sub) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      int a;
+      rate[k] = rate_of(p.axes, min(4 * sub + k, p.D / 2 - 1), a);
+      axis[k] = a * p.pos.sa;
+    }
+  }
+  __device__ __forceinline__ void at(const RopeParams& p, const Unit& u, float sign, float (&c)[4], float (&s)[4]) const {
+    const int64_t base = (int64_t)u.b * p.pos.sb + (int64_t)u.s * p.pos.ss;
+    double pos[4];
+    load_pos(p.pos, base, axis, pos);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      cos_sin(pos[k] * rate[k], c[k], s[k]);
+      s[k] *= sign;
+    }
+  }
+};
+
+__device__ __forceinline__ void rotate(float (&v)[8], const float (&c)[4], const float (&s)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float a = v[2 * k], b = v[2 * k + 1];
+    v[2 * k] = __builtin_fmaf(-b, s[k], a * c[k]);
+    v[2 * k + 1] = __builtin_fmaf(b, c[k], a * s[k]);
+  }
+}
+__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
+  float d = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) d = __builtin_fmaf(a[k], b[k], d);
+  return d;
+}
+__device__ __forceinline__ float inv_rms(float ss, int D, float eps) {
+  return __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + eps));
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// Forward, and (sign -1, no norm) the rotation's own backward
+// ---------------------------------------------------------------------------
+template <bool F32, bool HALF, int LPR, int R>
+__global__ __launch_bounds__(kThreads) void rope_forward_kernel(RopeParams p, Ranges ranges) {
+  constexpr int es = F32 ? 4 : 2;
+  const int grp = threadIdx.x / LPR, sub = threadIdx.x % LPR;
+  const bool is_k = (int)blockIdx.x >= ranges.q.n;
+  const RopeHeads t = is_k ? p.t[1] : p.t[0];
+  const Range rg = is_k ? ranges.k : ranges.q;
+  const int64_t blk = rg.first + xcd_block(blockIdx.x - (is_k ? ranges.q.n : 0), rg.n);
+  const int J = (t.H + R - 1) / R;
+  const int64_t unit = blk * (kThreads / LPR) + grp;
+  if (unit >= (int64_t)p.B * p.S * J) return;  // whole groups
+  const Unit u = unit_at(p.S, J, unit);
+  const bool live = 8 * sub < p.D;
+  const int lane = live ? sub : 0;  // lanes behind D repeat the first values and store nothing
+  Raw<F32> raw[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    raw[i] = load_raw<F32, HALF>((const char*)t.x + offset_of(t.sx, u, min(u.j + J * i, t.H - 1)) * es, lane, p.D);
+  Angles ang;
+  ang.init(p, lane);
+  float c[4], s[4], w[8];
+  ang.at(p, u, p.sign, c, s);
+  load_weight<HALF>(t.w, t.w_f32, lane, p.D, w);
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int h = u.j + J * i;
+    float v[8];
+    unpack<F32, HALF>(raw[i], v);
+    if (t.norm) {
+      const float inv = inv_rms(group_sum<LPR>(live ? dot8(v, v) : 0.f), p.D, t.eps);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = v[k] * inv * w[k];
+    }
+    rotate(v, c, s);
+    if (live && h < t.H) store_row<F32, HALF>((char*)t.y + offset_of(t.sy, u, h) * es, lane, p.D, v);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward: a block walks its share of the units with the sums of both weights'
+// gradients in registers and writes one partial row of each; a second kernel
+// adds those in a fixed order.
+// ---------------------------------------------------------------------------
+namespace {
+// The block's share blk of `blocks` of one tensor, t
+template <bool F32, bool HALF, int LPR, int R>
+__device__ __forceinline__ void backward_share(const RopeParams& p, const RopeHeads& t, const Angles& ang, uint32_t bid,
+                                               int blocks, float (&part)[kThreads / LPR][LPR * 8 + 4]) {
+  constexpr int es = F32 ? 4 : 2, kGroups = kThreads / LPR;
+  const int grp = threadIdx.x / LPR, sub = threadIdx.x % LPR;
+  const int64_t blk = xcd_block(bid, blocks);
+  const int J = (t.H + R - 1) / R;
+  const int64_t units = (int64_t)p.B * p.S * J, steps = (units + kGroups - 1) / kGroups;
+  const int64_t begin = steps * blk / blocks, end = steps * (blk + 1) / blocks;
+  const bool live = 8 * sub < p.D;
+  const int lane = live ? sub : 0;
+  float wg[8], w[8];
+  load_weight<HALF>(t.w, t.w_f32, lane, p.D, w);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) wg[k] = 0.f;
+  Unit u = unit_at(p.S, J, begin * kGroups + grp);
+  // (only the last step of all is short, by whole groups)
+  int left = (int)(end - begin) - (begin < end && (end - 1) * kGroups + grp >= units);
+  for (; left > 0; --left, u = unit_after(p.S, J, u, kGroups)) {
+    Raw<F32> rx[R], rd[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int h = min(u.j + J * i, t.H - 1);
+      rd[i] = load_raw<F32, HALF>((const char*)t.dy + offset_of(t.sdy, u, h) * es, lane, p.D);
+      rx[i] = load_raw<F32, HALF>((const char*)t.x + offset_of(t.sx, u, h) * es, lane, p.D);
+    }
+    float c[4], s[4];
+    ang.at(p, u, -1.f, c, s);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int h = u.j + J * i;
+      const bool mine = live && h < t.H;
+      float x[8], g[8];
+      unpack<F32, HALF>(rd[i], g);
+      unpack<F32, HALF>(rx[i], x);
+      rotate(g, c, s);
+      const float inv = inv_rms(group_sum<LPR>(live ? dot8(x, x) : 0.f), p.D, t.eps);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        x[k] = mine ? x[k] * inv : 0.f;  // a row past H repeats the last one and counts for nothing
+        wg[k] = __builtin_fmaf(g[k], x[k], wg[k]);
+        g[k] *= w[k];
+      }
+      const float mean = __fdiv_rn(group_sum<LPR>(dot8(g, x)), (float)p.D);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) g[k] = inv * __builtin_fmaf(-x[k], mean, g[k]);
+      if (mine) store_row<F32, HALF>((char*)t.y + offset_of(t.sy, u, h) * es, lane, p.D, g);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) part[grp][8 * sub + k] = wg[k];
+}
+}  // namespace
+
+template <bool F32, bool HALF, int LPR, int R>
+__global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p, Ranges ranges) {
+  constexpr int kGroups = kThreads / LPR;
+  __shared__ float part[kGroups][LPR * 8 + 4];
+  Angles ang;
+  ang.init(p, 8 * (threadIdx.x % LPR) < p.D ? threadIdx.x % LPR : 0);
+  harp_ra::sched_fence();
+  // (two copies of the walk: both tensors' strides side by side do not fit the scalar registers)
+  if ((int)blockIdx.x < ranges.q.n)
+    backward_share<F32, HALF, LPR, R>(p, p.t[0], ang, blockIdx.x, ranges.q.n, part);
+  else
+    backward_share<F32, HALF, LPR, R>(p, p.t[1], ang, blockIdx.x - ranges.q.n, ranges.k.n, part);
+  if (!p.wpart) return;
+  __syncthreads();
+  // value 2 k + e of the partial row is element e of pair k
+  if ((int)threadIdx.x < p.D) {
+    const int at = threadIdx.x, pair = at / 2;
+    float sum = 0.f;
+#pragma unroll
+    for (int gi = 0; gi < kGroups; ++gi) sum += part[gi][at];
+    p.wpart[(int64_t)blockIdx.x * p.D + (HALF ? pair + (at & 1) * (p.D / 2) : at)] = sum;
+  }
+}
+
+// gw[e] = sum of wpart[block][e] over a tensor's blocks: 8 columns a block, 128
+// lanes of rows, added in a fixed order
+constexpr int kWgCols = 8, kWgLanes = 128;
+__global__ __launch_bounds__(kWgCols* kWgLanes) void rope_wgrad_kernel(const float* src, int q_blocks, int k_blocks,
+                                                                       int D, void* gq, int gq_f32, void* gk,
+                                                                       int gk_f32) {
+  __shared__ float part[kWgLanes][kWgCols + 1];
+  const int tx = threadIdx.x % kWgCols, ty = threadIdx.x / kWgCols;
+  const int t = blockIdx.y, e = blockIdx.x * kWgCols + tx;  // D is a multiple of 8
+  void* const dst = t ? gk : gq;
+  const int f32 = t ? gk_f32 : gq_f32;
+  if (!dst) return;
+  const int blocks = t ? k_blocks : q_blocks;
+  if (t) src += (int64_t)q_blocks * D;
+  float acc = 0.f;
+#pragma unroll 4
+  for (int i = ty; i < blocks; i += kWgLanes) acc += src[(int64_t)i * D + e];
+  part[ty][tx] = acc;
+  __syncthreads();
+  if (ty < 8) {
+    acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < kWgLanes / 8; ++k) acc += part[ty * (kWgLanes / 8) + k][tx];
+  }
+  __syncthreads();
+  if (ty < 8) part[ty][tx] = acc;
+  __syncthreads();
+  if (ty != 0) return;
+  acc = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc += part[k][tx];
+  if (f32) ((float*)dst)[e] = acc;
+  else ((bf16*)dst)[e] = (bf16)acc;
+}
+
+// ---------------------------------------------------------------------------
+// The table: a thread keeps one pair and walks the tokens
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(kThreads) void rope_table_kernel(RopeAxes axes, RopePos pos, int S, int64_t tokens,
+                                                              int pairs, float2* out) {
+  const int per = kThreads / pairs;  // tokens of a block's step
+  const int p = threadIdx.x % pairs, at = threadIdx.x / pairs;
+  if (at >= per) return;
+  int axis;
+  const double rate = rate_of(axes, p, axis);
+  for (int64_t tok = (int64_t)blockIdx.x * per + at; tok < tokens; tok += (int64_t)gridDim.x * per) {
+    const int64_t b = tok / S, s = tok - b * S;
+    const int64_t off[1] = {axis * pos.sa};
+    double v[1];
+    load_pos(pos, b * pos.sb + s * pos.ss, off, v);
+    float2 cs;
+    cos_sin(v[0] * rate, cs.x, cs.y);
+    out[tok * pairs + p] = cs;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Launchers
+// ---------------------------------------------------------------------------
+namespace {
+
+int lanes_per_row(int D) { return D > 128 ? 32 : D > 64 ? 16 : 8; }
+
+constexpr int kFillBlocks = 1024;    // four blocks for each of 256 CUs
+constexpr int kBwdMaxBlocks = 1024;
+constexpr int64_t kLaunchBlocks = 1 << 22;  // of q and of k, 256 threads each: below 2^32 threads a launch
+
+int64_t blocks_of(const RopeParams& p, const RopeHeads& t, int R) {
+  const int per = kThreads / lanes_per_row(p.D);
+  return ((int64_t)p.B * p.S * ((t.H + R - 1) / R) + per - 1) / per;
+}
+int64_t blocks_of(const RopeParams& p, int R) { return blocks_of(p, p.t[0], R) + blocks_of(p, p.t[1], R); }
+// heads of a token for one group of lanes: as many as leave kFillBlocks blocks
+int heads_per_group(const RopeParams& p, int most) {
+  for (int R = most; R > 1; R /= 2)
+    if (blocks_of(p, R) >= kFillBlocks) return R;
+  return 1;
+}
+template <template <bool, bool, int, int> class K>
+hipError_t dispatch(const RopeParams& p, int R, const Ranges& r, hipStream_t st) {
+  auto heads = [&](auto f32, auto half, auto l) {
+    constexpr bool F = decltype(f32)::value, H = decltype(half)::value;
+    constexpr int L = decltype(l)::value;
+    if (R == 4) K<F, H, L, 4>::launch(p, r, st);
+    else if (R == 2) K<F, H, L, 2>::launch(p, r, st);
+    else K<F, H, L, 1>::launch(p, r, st);
+  };
+  auto lanes = [&](auto f32, auto half) {
+    const int l = lanes_per_row(p.D);
+    if (l == 32) heads(f32, half, std::integral_constant<int, 32>{});
+    else if (l == 16) heads(f32, half, std::integral_constant<int, 16>{});
+    else heads(f32, half, std::integral_constant<int, 8>{});
+  };
+  auto layout = [&](auto f32) { p.half ? lanes(f32, std::true_type{}) : lanes(f32, std::false_type{}); };
+  p.f32 ? layout(std::true_type{}) : layout(std::false_type{});
+  return hipGetLastError();
+}
+template <bool F, bool H, int L, int R>
+struct Forward {
+  static void launch(const RopeParams& p, const Ranges& r, hipStream_t st) {
+    hipLaunchKernelGGL((rope_forward_kernel<F, H, L, R>), dim3((unsigned)(r.q.n + r.k.n)), dim3(kThreads), 0, st, p, r);
+  }
+};
+constexpr int kBwdHeads = 2;  // rows of x and dy of four heads would leave a CU half the waves
+template <bool F, bool H, int L, int R>
+struct Backward {
+  static void launch(const RopeParams& p, const Ranges& r, hipStream_t st) {
+    constexpr int B = R > kBwdHeads ? kBwdHeads : R;
+    hipLaunchKernelGGL((rope_backward_kernel<F, H, L, B>), dim3((unsigned)(r.q.n + r.k.n)), dim3(kThreads), 0, st, p, r);
+  }
+};
+
+// at most kBwdMaxBlocks, as few as leave the busiest one no more steps
+int bwd_blocks(const RopeParams& p, const RopeHeads& t, int most) {
+  const int64_t steps = blocks_of(p, t, heads_per_group(p, kBwdHeads));
+  const int64_t each = (steps + most - 1) / most;
+  return each ? (int)((steps + each - 1) / each) : 0;
+}
+
+}  // namespace
+
+hipError_t launch_rope_forward(const RopeParams& p, hipStream_t stream) {
+  const int R = heads_per_group(p, 4);
+  const int64_t total[2] = {blocks_of(p, p.t[0], R), blocks_of(p, p.t[1], R)};
+  for (int64_t first = 0; first < std::max(total[0], total[1]); first += kLaunchBlocks) {
+    auto part = [&](int64_t n) { return Range{first, (int)std::max((int64_t)0, std::min(n - first, kLaunchBlocks))}; };
+    const hipError_t e = dispatch<Forward>(p, R, Ranges{part(total[0]), part(total[1])}, stream);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+void rope_bwd_blocks(const RopeParams& p, int blocks[2]) {
+  const int rows = p.t[0].H + p.t[1].H;
+  for (int i = 0; i < 2; ++i)  // each tensor's share of the blocks
+    blocks[i] = p.t[i].H ? bwd_blocks(p, p.t[i], std::max(1, (int)((int64_t)kBwdMaxBlocks * p.t[i].H / rows))) : 0;
+}
+hipError_t launch_rope_backward(const RopeParams& p, hipStream_t stream) {
+  int n[2];
+  rope_bwd_blocks(p, n);
+  return dispatch<Backward>(p, heads_per_group(p, kBwdHeads), Ranges{Range{0, n[0]}, Range{0, n[1]}}, stream);
+}
+
+hipError_t launch_rope_wgrad(const float* wpart, const int blocks[2], int D, void* const gw[2], const int gw_f32[2],
+                             hipStream_t stream) {
+  hipLaunchKernelGGL(rope_wgrad_kernel, dim3((unsigned)(D / kWgCols), 2), dim3(kWgCols * kWgLanes), 0, stream, wpart,
+                     blocks[0], blocks[1], D, gw[0], gw_f32[0], gw[1], gw_f32[1]);
+  return hipGetLastError();
+}
+
+hipError_t launch_rope_table(const RopeAxes& axes, const RopePos& pos, int B, int S, int D, float* out,
+                             hipStream_t stream) {
+  const int pairs = D / 2, per = kThreads / pairs;
+  const int64_t tokens = (int64_t)B * S, need = (tokens + per - 1) / per;
+  const int64_t blocks = need < 2048 ? need : 2048;
+  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, axes, pos, S, tokens, pairs,
+                     (float2*)out);
+  return hipGetLastError();
+}
+
+}  // namespace harp_req

@@ -20,18 +20,18 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <string>
 #include <tuple>
 
 #include "harp_block_ops.h"
+#include "torch_autograd_util.h"
 
 namespace {
 
-using OptTensor = std::optional<at::Tensor>;
+using harp_torch::given;
+using harp_torch::OptTensor;
 
 void check_status(int rc, const char* op) {
   TORCH_CHECK(rc == HARP_BLK_OK, "harp_block.", op, ": ", harp_blk_last_error(), " (status ", rc, ")");
@@ -93,12 +93,8 @@ Vec vec_of(const OptTensor& v, const at::Tensor& ref, int64_t n, const char* nam
   return r;
 }
 
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-// A forward-mode tangent would be lost below the autograd keys.
 void refuse_tangent(const at::Tensor& t, const char* op) {
-  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), "harp_block.", op,
-              " has no forward-mode derivative: an argument carries a tangent");
+  harp_torch::refuse_tangent(t, "harp_block", op);
 }
 
 void check_input(const at::Tensor& x, const char* op) {
@@ -222,35 +218,13 @@ class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
         if (need_residual) out[1] = dh;
       }
     }
-    if (at::GradMode::is_enabled()) {  // create_graph: a gradient of these gradients raises
-      torch::autograd::variable_list given_out;
-      for (auto& t : out)
-        if (t.defined()) given_out.push_back(t.detach().requires_grad_());
-      if (!given_out.empty()) {
-        auto error = std::make_shared<torch::autograd::DelayedError>("add_rms_norm is differentiable once only",
-                                                                    given_out.size());
-        given_out = (*error)(std::move(given_out));
-        size_t i = 0;
-        for (auto& t : out)
-          if (t.defined()) t = given_out[i++];
-      }
-    }
+    harp_torch::once_only(out, "add_rms_norm");
     return out;
   }
 };
 
-// While a graph of an earlier call is alive, a leaf keeps the accumulator node
-// of that graph, with the stream it was made on.  A backward captured on
-// another stream would have the engine wait across the two streams inside the
-// capture, which ends the process: such a call is refused while it can be.
 void check_capture(const OptTensor& t, const c10::Stream& current, const char* name) {
-  if (!given(t) || !t->requires_grad() || t->grad_fn()) return;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-  if (!node) return;
-  const auto made_on = node->stream();
-  TORCH_CHECK(!made_on || *made_on == current, "add_rms_norm: ", name,
-              " belongs to a live autograd graph of another stream, so its gradient cannot be captured: delete that "
-              "graph's tensors (an earlier step's outputs or loss) before the capture");
+  harp_torch::check_capture(t, current, "add_rms_norm", name);
 }
 
 void refuse_tangents(const at::Tensor& x, const OptTensor& residual, const OptTensor& weight) {

@@ -1,0 +1,632 @@
+// kernels/libharp_request_ops.so — PyTorch-ROCm operators of the kernels that
+// give every request of a batch its own positions and its own adapter
+// (include/harp_request_ops.h), namespace harp_request:
+//   qk_norm_rope    RMSNorm and rotation of queries and keys by their positions
+//   rope_table      the rotation's table
+//   add_adapters    low-rank adapters beside a projection's result
+//   check_capture   refuses leaves whose gradients cannot be captured
+// The operators allocate their results and workspaces from PyTorch's allocator
+// and run on the current HIP stream of the input's device.  Implementations are
+// registered for the CUDA dispatch key (HIP tensors carry it); the CPU key
+// raises.  qk_norm_rope and add_adapters are differentiable (once, in reverse
+// mode); an argument with a forward-mode tangent raises.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/library.h>
+
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "harp_request_ops.h"
+#include "torch_autograd_util.h"
+
+namespace {
+
+using harp_torch::given;
+using harp_torch::OptTensor;
+
+void check_status(int rc, const char* op) {
+  TORCH_CHECK(rc == HARP_REQ_OK, "harp_request.", op, ": ", harp_req_last_error(), " (status ", rc, ")");
+}
+hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+int code(at::ScalarType t) { return t == at::kFloat ? HARP_REQ_F32 : HARP_REQ_BF16; }
+int int_code(at::ScalarType t) { return t == at::kLong ? HARP_REQ_I64 : HARP_REQ_I32; }
+
+int checked_int(int64_t v, const char* name) {
+  TORCH_CHECK(v <= 0x7fffffff, name, " of ", v, " is 2^31 or more");
+  return (int)v;
+}
+void check_device(const at::Tensor& t, const at::Tensor& ref, const char* name) {
+  TORCH_CHECK(t.device() == ref.device(), name, " must be on ", ref.device(), ", got ", t.device());
+}
+at::Tensor plain(const at::Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
+bool capturing() { return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None; }
+
+// ---------------------------------------------------------------------------
+// rotary positions
+// ---------------------------------------------------------------------------
+struct Axes {
+  harp_req_axes_t a{};
+  int64_t D = 0;
+};
+Axes axes_of(at::IntArrayRef widths, at::ArrayRef<double> theta, bool half) {
+  Axes r;
+  TORCH_CHECK(widths.size() >= 1 && widths.size() <= HARP_REQ_MAX_AXES && theta.size() == widths.size(),
+              "one to four axes with a theta each, got ", widths.size(), " and ", theta.size());
+  r.a.n = (int)widths.size();
+  r.a.half = half;
+  for (size_t i = 0; i < widths.size(); ++i) {
+    TORCH_CHECK(widths[i] >= 2 && widths[i] <= 256 && widths[i] % 2 == 0, "an axis' width must be even, 2 to 256, got ",
+                widths[i]);
+    r.a.width[i] = (int)widths[i];
+    r.a.theta[i] = theta[i];
+    r.D += widths[i];
+  }
+  return r;
+}
+
+// positions [S, n] or [B or 1, S, n]
+struct Positions {
+  at::Tensor t;
+  harp_req_positions_t p{};
+};
+Positions positions_of(const at::Tensor& pos, int64_t n, int64_t B, int64_t S) {
+  Positions r;
+  const auto ty = pos.scalar_type();
+  TORCH_CHECK(ty == at::kInt || ty == at::kLong || ty == at::kFloat, "positions must be int32, int64 or float32, got ", ty);
+  TORCH_CHECK(pos.dim() == 2 || pos.dim() == 3, "positions must be [S, axes] or [B, S, axes], got ", pos.sizes());
+  TORCH_CHECK(pos.size(-1) == n && pos.size(-2) == S && (pos.dim() == 2 || pos.size(0) == B || pos.size(0) == 1),
+              "positions must be [", S, ", ", n, "], or [", B, " or 1, ", S, ", ", n, "], got ", pos.sizes());
+  r.t = plain(pos);
+  r.p.p = r.t.const_data_ptr();
+  r.p.dtype = ty == at::kFloat ? HARP_REQ_F32 : int_code(ty);
+  r.p.stride_b = pos.dim() == 3 && pos.size(0) > 1 ? r.t.stride(0) : 0;
+  r.p.stride_s = r.t.stride(-2);
+  r.p.stride_a = r.t.stride(-1);
+  return r;
+}
+
+// [B, H, S, D] views the kernels read: unit stride along D, the others multiples of 8, 16-byte aligned
+bool readable(const at::Tensor& t) {
+  if (t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) % 8 || (i && t.stride(i) > 0x7fffffff))) return false;
+  return true;
+}
+at::Tensor heads_of(const at::Tensor& t) {
+  const at::Tensor r = plain(t);
+  return r.numel() == 0 || readable(r) ? r : r.contiguous();
+}
+at::Tensor like(const at::Tensor& x) {  // x's layout where it is one without holes
+  return x.is_non_overlapping_and_dense() ? at::empty_strided(x.sizes(), x.strides(), x.options())
+                                          : at::empty(x.sizes(), x.options());
+}
+void strides_of(const at::Tensor& t, int64_t (&st)[3]) {
+  const int order[3] = {0, 1, 2};
+  for (int i : order) st[i] = t.size(i) > 1 ? t.stride(i) : 0;
+}
+
+at::Tensor weight_of(const OptTensor& w, const at::Tensor& x, const char* name) {
+  if (!given(w)) return {};
+  check_device(*w, x, name);
+  TORCH_CHECK(w->scalar_type() == at::kBFloat16 || w->scalar_type() == at::kFloat, name,
+              " must be bfloat16 or float32, got ", w->scalar_type());
+  TORCH_CHECK(w->dim() == 1 && w->size(0) == x.size(3), name, " must be a vector of ", x.size(3), " elements, got ",
+              w->sizes());
+  return plain(*w).contiguous();
+}
+
+struct RopeCall {
+  Axes axes;
+  std::vector<double> eps;  // of q and k; negative: no norm
+};
+RopeCall rope_call(at::IntArrayRef widths, at::ArrayRef<double> theta, bool half, at::ArrayRef<double> eps) {
+  RopeCall c{axes_of(widths, theta, half), eps.vec()};
+  TORCH_CHECK(c.eps.size() == 2, "eps must be two values, got ", c.eps.size());
+  return c;
+}
+
+void check_qk(const at::Tensor& q, const OptTensor& k, const at::Tensor& positions, const RopeCall& c,
+              const OptTensor& qw, const OptTensor& kw) {
+  TORCH_CHECK(q.is_cuda(), "harp_request.qk_norm_rope: tensors must be on a HIP device");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kFloat, "q must be bfloat16 or float32, got ",
+              q.scalar_type());
+  TORCH_CHECK(q.dim() == 4, "q must be [B, heads, S, D], got ", q.sizes());
+  TORCH_CHECK(q.size(3) == c.axes.D, "q has heads of ", q.size(3), " features, the axes ", c.axes.D);
+  TORCH_CHECK(c.axes.D % 8 == 0 && c.axes.D <= 256, "heads must have a multiple of 8 features, at most 256, got ", c.axes.D);
+  if (given(k)) {
+    check_device(*k, q, "k");
+    TORCH_CHECK(k->scalar_type() == q.scalar_type(), "k must be ", q.scalar_type(), " as q, got ", k->scalar_type());
+    TORCH_CHECK(k->dim() == 4 && k->size(0) == q.size(0) && k->size(2) == q.size(2) && k->size(3) == q.size(3),
+                "k must be [", q.size(0), ", heads, ", q.size(2), ", ", q.size(3), "], got ", k->sizes());
+  }
+  check_device(positions, q, "positions");
+  TORCH_CHECK((!given(qw) || c.eps[0] >= 0) && (!given(kw) || c.eps[1] >= 0), "a weight needs its norm: eps is missing");
+  TORCH_CHECK(!given(kw) || given(k), "k_weight without k");
+  checked_int(q.size(0), "batch");
+  checked_int(q.size(1), "heads");
+  checked_int(q.size(2), "seq");
+}
+
+std::tuple<at::Tensor, at::Tensor> rope_forward(const at::Tensor& q, const OptTensor& k, const at::Tensor& positions,
+                                                const RopeCall& c, const OptTensor& qw, const OptTensor& kw) {
+  check_qk(q, k, positions, c, qw, kw);
+  const c10::DeviceGuard guard(q.device());
+  const Positions pos = positions_of(positions, c.axes.a.n, q.size(0), q.size(2));
+  harp_req_heads_t heads[2] = {};
+  at::Tensor x[2], y[2], w[2];
+  for (int i = 0; i < 2; ++i) {
+    if (i && !given(k)) break;
+    x[i] = heads_of(i ? *k : q);
+    y[i] = like(x[i]);
+    w[i] = weight_of(i ? kw : qw, q, i ? "k_weight" : "q_weight");
+    harp_req_heads_t& h = heads[i];
+    h.x = x[i].const_data_ptr();
+    strides_of(x[i], h.x_stride);
+    h.y = y[i].data_ptr();
+    strides_of(y[i], h.y_stride);
+    h.heads = checked_int(x[i].size(1), "heads");
+    h.norm = c.eps[i] >= 0;
+    if (w[i].defined()) {
+      h.weight = w[i].const_data_ptr();
+      h.weight_dtype = code(w[i].scalar_type());
+    }
+    h.eps = (float)c.eps[i];
+  }
+  check_status(harp_req_qk_norm_rope_forward(&c.axes.a, &pos.p, heads, (int)q.size(0), (int)q.size(2),
+                                             code(q.scalar_type()), stream_of(q)),
+               "qk_norm_rope");
+  return {y[0], y[1]};
+}
+
+// the gradients of (q, k, q_weight, k_weight); undefined where dy is (its tensor took no part) or not wanted
+std::vector<at::Tensor> rope_backward(const at::Tensor (&dy)[2], const at::Tensor (&x)[2], const at::Tensor (&w)[2],
+                                      const at::Tensor& positions, const RopeCall& c, const bool (&want_w)[2]) {
+  const at::Tensor& ref = dy[0].defined() ? dy[0] : dy[1];
+  const c10::DeviceGuard guard(ref.device());
+  const Positions pos = positions_of(positions, c.axes.a.n, ref.size(0), ref.size(2));
+  harp_req_heads_t heads[2] = {};
+  std::vector<at::Tensor> out(4);
+  at::Tensor d[2], xs[2], ws[2], work;
+  int normed[2] = {0, 0};
+  bool any = false;
+  for (int i = 0; i < 2; ++i) {
+    if (!dy[i].defined()) continue;
+    d[i] = heads_of(dy[i]);
+    harp_req_heads_t& h = heads[i];
+    h.heads = (int)d[i].size(1);
+    h.norm = c.eps[i] >= 0;
+    if (h.norm) {
+      xs[i] = heads_of(x[i]);
+      h.x = xs[i].const_data_ptr();
+      strides_of(xs[i], h.x_stride);
+      normed[i] = h.heads;
+      if (w[i].defined()) {
+        ws[i] = plain(w[i]).contiguous();
+        h.weight = ws[i].const_data_ptr();
+        h.weight_dtype = code(ws[i].scalar_type());
+        if (want_w[i]) {
+          out[2 + i] = d[i].numel() ? at::empty_like(ws[i]) : at::zeros_like(ws[i]);
+          h.grad_weight = out[2 + i].data_ptr();
+          any = true;
+        }
+      }
+    }
+    out[i] = like(h.norm ? xs[i] : d[i]);
+    h.y = out[i].data_ptr();
+    strides_of(out[i], h.y_stride);
+    h.dy = d[i].const_data_ptr();
+    strides_of(d[i], h.dy_stride);
+    h.eps = (float)c.eps[i];
+  }
+  size_t bytes = 0;
+  if (any && ref.size(0) * ref.size(2)) {
+    bytes = harp_req_qk_backward_workspace_bytes((int)ref.size(0), (int)ref.size(2), (int)c.axes.D, normed[0], normed[1]);
+    TORCH_CHECK(bytes != (size_t)-1, "harp_request.qk_norm_rope: ", harp_req_last_error());
+    work = at::empty({(int64_t)(bytes / 4)}, ref.options().dtype(at::kFloat));
+  }
+  check_status(harp_req_qk_norm_rope_backward(&c.axes.a, &pos.p, heads, (int)ref.size(0), (int)ref.size(2),
+                                              code(ref.scalar_type()), work.defined() ? work.data_ptr() : nullptr, bytes,
+                                              stream_of(ref)),
+               "qk_norm_rope (backward)");
+  return out;
+}
+
+class QkNormRope : public torch::autograd::Function<QkNormRope> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                const OptTensor& k, const at::Tensor& positions,
+                                                std::vector<int64_t> widths, std::vector<double> theta, bool half,
+                                                const OptTensor& qw, const OptTensor& kw, std::vector<double> eps) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const RopeCall c = rope_call(widths, theta, half, eps);
+    auto [yq, yk] = rope_forward(q, k, positions, c, qw, kw);
+    ctx->set_materialize_grads(false);
+    const at::Tensor none;
+    auto wants = [](const OptTensor& t) { return given(t) && t->requires_grad(); };
+    ctx->saved_data["widths"] = widths;
+    ctx->saved_data["theta"] = theta;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["flags"] =
+        (int64_t)half + 2 * q.requires_grad() + 4 * wants(k) + 8 * wants(qw) + 16 * wants(kw);
+    // (a rotation alone needs no input for its gradient)
+    ctx->save_for_backward({c.eps[0] >= 0 ? q : none, given(k) && c.eps[1] >= 0 ? *k : none, given(qw) ? *qw : none,
+                            given(kw) ? *kw : none, positions});
+    if (!given(k)) return {yq};
+    return {yq, yk};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    for (const auto& t : grads) harp_torch::refuse_tangent(t, "harp_request", "qk_norm_rope (backward)");
+    const bool want[2] = {(flags & 2) != 0, (flags & 4) != 0}, want_w[2] = {(flags & 8) != 0, (flags & 16) != 0};
+    torch::autograd::variable_list out(9);
+    at::Tensor dy[2];
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (want[i] || want_w[i]) dy[i] = grads[i];
+    if (dy[0].defined() || dy[1].defined()) {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      const RopeCall c = rope_call(ctx->saved_data["widths"].toIntVector(), ctx->saved_data["theta"].toDoubleVector(),
+                                   flags & 1, ctx->saved_data["eps"].toDoubleVector());
+      const at::Tensor x[2] = {saved[0], saved[1]}, w[2] = {saved[2], saved[3]};
+      auto g = rope_backward(dy, x, w, saved[4], c, want_w);
+      if (want[0]) out[0] = g[0];
+      if (want[1]) out[1] = g[1];
+      out[6] = g[2];
+      out[7] = g[3];
+    }
+    harp_torch::once_only(out, "qk_norm_rope");
+    return out;
+  }
+};
+
+void refuse_grad(const OptTensor& t, const char* op, const char* name) {
+  TORCH_CHECK(!given(t) || !t->requires_grad() || !at::GradMode::is_enabled(), "harp_request.", op, ": ", name,
+              " has no gradient here: pass it detached");
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const OptTensor& k, const at::Tensor& positions,
+                                                at::IntArrayRef widths, at::ArrayRef<double> theta, bool half,
+                                                const OptTensor& qw, const OptTensor& kw, at::ArrayRef<double> eps) {
+  return rope_forward(q, k, positions, rope_call(widths, theta, half, eps), qw, kw);
+}
+
+void refuse_rope(const at::Tensor& q, const OptTensor& k, const at::Tensor& positions, const OptTensor& qw,
+                 const OptTensor& kw) {
+  for (const OptTensor& t : {OptTensor(q), k, OptTensor(positions), qw, kw})
+    if (given(t)) harp_torch::refuse_tangent(*t, "harp_request", "qk_norm_rope");
+  refuse_grad(positions, "qk_norm_rope", "positions");
+}
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& q, const OptTensor& k,
+                                                         const at::Tensor& positions, at::IntArrayRef widths,
+                                                         at::ArrayRef<double> theta, bool half, const OptTensor& qw,
+                                                         const OptTensor& kw, at::ArrayRef<double> eps) {
+  refuse_rope(q, k, positions, qw, kw);
+  const OptTensor leaves[] = {q, k, qw, kw};
+  bool record = false;
+  for (const auto& t : leaves) record |= given(t) && t->requires_grad();
+  if (!record || !at::GradMode::is_enabled()) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return qk_norm_rope(q, k, positions, widths, theta, half, qw, kw, eps);
+  }
+  const c10::DeviceGuard guard(q.device());
+  if (capturing()) {
+    const c10::Stream current = c10::hip::getCurrentHIPStream(q.get_device()).unwrap();
+    const char* const names[] = {"q", "k", "q_weight", "k_weight"};
+    for (int i = 0; i < 4; ++i) harp_torch::check_capture(leaves[i], current, "qk_norm_rope", names[i]);
+  }
+  auto out = QkNormRope::apply(q, k, positions, widths.vec(), theta.vec(), half, qw, kw, eps.vec());
+  return {out[0], given(k) ? out[1] : at::Tensor()};
+}
+
+at::Tensor rope_table(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta) {
+  TORCH_CHECK(positions.is_cuda(), "harp_request.rope_table: this library runs on a HIP device only");
+  TORCH_CHECK(positions.dim() == 2 || positions.dim() == 3, "positions must be [S, axes] or [B, S, axes], got ",
+              positions.sizes());
+  const Axes ax = axes_of(widths, theta, false);
+  const c10::DeviceGuard guard(positions.device());
+  const int64_t B = positions.dim() == 3 ? positions.size(0) : 1, S = positions.size(-2);
+  const Positions pos = positions_of(positions, ax.a.n, B, S);
+  std::vector<int64_t> shape(positions.sizes().begin(), positions.sizes().end());
+  shape.back() = ax.D / 2;
+  at::Tensor out = at::empty(shape, positions.options().dtype(at::kComplexFloat));
+  check_status(harp_req_rope_table(&ax.a, &pos.p, checked_int(B, "batch"), checked_int(S, "seq"),
+                                   (float*)out.data_ptr(), stream_of(positions)),
+               "rope_table");
+  return out;
+}
+at::Tensor rope_table_autograd(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta) {
+  harp_torch::refuse_tangent(positions, "harp_request", "rope_table");
+  refuse_grad(positions, "rope_table", "positions");
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rope_table(positions, widths, theta);
+}
+
+// ---------------------------------------------------------------------------
+// adapters
+// ---------------------------------------------------------------------------
+// [.., C] tensors as rows; leading dimensions that are no single row stride are copied
+struct Rows {
+  at::Tensor t;
+  const void* p = nullptr;
+  int64_t ld = 0;
+  int rows = 0, cols = 0;
+};
+Rows rows_of(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.dim() >= 1 && t.size(-1) >= 1, name, " must have a last dimension of at least 1, got ", t.sizes());
+  Rows r;
+  r.cols = checked_int(t.size(-1), "columns");
+  r.rows = checked_int(t.numel() / t.size(-1), "rows");
+  r.t = plain(t);
+  if (r.t.stride(-1) != 1) r.t = r.t.contiguous();
+  if (r.t.dim() != 2) r.t = r.t.reshape({r.rows, r.cols});
+  r.p = r.t.const_data_ptr();
+  r.ld = r.rows > 1 ? r.t.stride(0) : r.cols;
+  return r;
+}
+
+void check_ints(const at::Tensor& t, const at::Tensor& ref, const char* name) {
+  check_device(t, ref, name);
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ",
+              t.scalar_type());
+  TORCH_CHECK(t.dim() == 1, name, " must be a vector, got ", t.sizes());
+}
+
+struct AdapterCall {
+  Rows x;
+  at::Tensor a, b, scales, index, offsets;
+  harp_req_adapters_t adapters{};
+  harp_req_requests_t requests{};
+  int N = 0;
+};
+AdapterCall adapter_call(const at::Tensor& x, const at::Tensor& a, const at::Tensor& b, const OptTensor& scales,
+                         const at::Tensor& index, const OptTensor& offsets) {
+  TORCH_CHECK(x.is_cuda(), "harp_request.add_adapters: tensors must be on a HIP device");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16, "x must be bfloat16, got ", x.scalar_type());
+  AdapterCall c;
+  c.x = rows_of(x, "x");
+  for (const auto* t : {&a, &b}) {
+    check_device(*t, x, t == &a ? "a" : "b");
+    TORCH_CHECK(t->scalar_type() == at::kBFloat16 && t->dim() == 3, t == &a ? "a" : "b",
+                " must be a bfloat16 [adapters, .., ..] tensor, got ", t->scalar_type(), " ", t->sizes());
+  }
+  TORCH_CHECK(a.size(2) == c.x.cols, "a must be [adapters, rank, ", c.x.cols, "], got ", a.sizes());
+  TORCH_CHECK(b.size(0) == a.size(0) && b.size(2) == a.size(1), "b must be [", a.size(0), ", features, ", a.size(1),
+              "], got ", b.sizes());
+  TORCH_CHECK(a.size(0) >= 1 && a.size(1) >= 1 && b.size(1) >= 1, "adapters need a rank and features, got a ", a.sizes(),
+              ", b ", b.sizes());
+  c.a = plain(a).contiguous();
+  c.b = plain(b).contiguous();
+  c.N = checked_int(b.size(1), "features");
+  if (given(scales)) {
+    check_device(*scales, x, "scales");
+    TORCH_CHECK(scales->scalar_type() == at::kFloat && scales->dim() == 1 && scales->size(0) == a.size(0),
+                "scales must be float32 [", a.size(0), "], got ", scales->scalar_type(), " ", scales->sizes());
+    c.scales = plain(*scales).contiguous();
+  }
+  check_ints(index, x, "index");
+  TORCH_CHECK(index.size(0) >= 1, "index must hold an adapter for at least one request");
+  c.index = index.contiguous();
+  if (given(offsets)) {
+    check_ints(*offsets, x, "offsets");
+    TORCH_CHECK(offsets->size(0) == index.size(0) + 1, "offsets must be ", index.size(0) + 1,
+                " values (one more than requests), got ", offsets->size(0));
+    c.offsets = offsets->contiguous();
+  } else {
+    TORCH_CHECK(c.x.rows % index.size(0) == 0, c.x.rows, " tokens are not ", index.size(0),
+                " requests of one length: pass their offsets");
+  }
+  c.adapters = harp_req_adapters_t{c.a.const_data_ptr(), c.b.const_data_ptr(),
+                                   c.scales.defined() ? c.scales.const_data_ptr<float>() : nullptr,
+                                   checked_int(a.size(0), "adapters"), checked_int(a.size(1), "rank")};
+  c.requests = harp_req_requests_t{c.index.const_data_ptr(), int_code(index.scalar_type()),
+                                   c.offsets.defined() ? c.offsets.const_data_ptr() : nullptr,
+                                   c.offsets.defined() ? int_code(c.offsets.scalar_type()) : HARP_REQ_I32,
+                                   checked_int(index.size(0), "requests")};
+  return c;
+}
+
+// (out, t)
+std::tuple<at::Tensor, at::Tensor> adapters_forward(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
+                                                    const at::Tensor& b, const OptTensor& scales,
+                                                    const at::Tensor& index, const OptTensor& offsets) {
+  const AdapterCall c = adapter_call(x, a, b, scales, index, offsets);
+  check_device(base, x, "base");
+  TORCH_CHECK(base.scalar_type() == at::kBFloat16 || base.scalar_type() == at::kFloat,
+              "base must be bfloat16 or float32, got ", base.scalar_type());
+  TORCH_CHECK(base.dim() == x.dim() && base.size(-1) == c.N && base.sizes().slice(0, base.dim() - 1) ==
+                                                                   x.sizes().slice(0, x.dim() - 1),
+              "base must be x's shape with ", c.N, " features, got ", base.sizes(), " for x ", x.sizes());
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor out = at::empty(base.sizes(), base.options()), t;
+  const int cols = harp_req_adapter_columns(c.adapters.rank);
+  TORCH_CHECK(cols > 0, "harp_request.add_adapters: ", harp_req_last_error());
+  t = at::empty({c.x.rows, cols}, x.options().dtype(at::kFloat));
+  if (c.x.rows) {
+    const Rows br = rows_of(base, "base");
+    check_status(harp_req_add_adapters_forward(c.x.p, c.x.ld, br.p, br.ld, out.data_ptr(), c.N,
+                                               code(base.scalar_type()), &c.adapters, &c.requests, t.data_ptr<float>(),
+                                               c.x.rows, c.x.cols, c.N, stream_of(x)),
+                 "add_adapters");
+  }
+  return {out, t};
+}
+
+// gradients of (x, a, b), undefined where not wanted
+std::tuple<at::Tensor, at::Tensor, at::Tensor> adapters_backward(const at::Tensor& dy, const at::Tensor& x,
+                                                                 const at::Tensor& a, const at::Tensor& b,
+                                                                 const OptTensor& scales, const at::Tensor& index,
+                                                                 const OptTensor& offsets, const at::Tensor& t,
+                                                                 bool want_x, bool want_a, bool want_b) {
+  const AdapterCall c = adapter_call(x, a, b, scales, index, offsets);
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor dx, da, db, work;
+  const bool none = c.x.rows == 0;
+  if (want_x) dx = at::empty(x.sizes(), x.options());
+  if (want_a) da = none ? at::zeros(a.sizes(), a.options()) : at::empty(a.sizes(), a.options());
+  if (want_b) db = none ? at::zeros(b.sizes(), b.options()) : at::empty(b.sizes(), b.options());
+  if (none) return {dx, da, db};
+  const Rows d = rows_of(dy, "dy");
+  const size_t bytes = harp_req_adapter_backward_workspace_bytes(c.x.rows, c.x.cols, c.N, c.adapters.n, c.adapters.rank,
+                                                                 c.requests.count, want_a, want_b);
+  TORCH_CHECK(bytes != (size_t)-1, "harp_request.add_adapters: ", harp_req_last_error());
+  work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+  check_status(harp_req_add_adapters_backward(
+                   d.p, d.ld, c.x.p, c.x.ld, t.const_data_ptr<float>(), &c.adapters, &c.requests,
+                   want_x ? dx.data_ptr() : nullptr, c.x.cols, 0, want_a ? da.data_ptr() : nullptr,
+                   want_b ? db.data_ptr() : nullptr, c.x.rows, c.x.cols, c.N, work.data_ptr(), bytes, stream_of(x)),
+               "add_adapters (backward)");
+  return {dx, da, db};
+}
+
+class AddAdapters : public torch::autograd::Function<AddAdapters> {
+ public:
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& base, const at::Tensor& x,
+                            const at::Tensor& a, const at::Tensor& b, const OptTensor& scales, const at::Tensor& index,
+                            const OptTensor& offsets) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    auto [out, t] = adapters_forward(base, x, a, b, scales, index, offsets);
+    ctx->saved_data["wanted"] = (int64_t)(base.requires_grad() + 2 * x.requires_grad() + 4 * a.requires_grad() +
+                                          8 * b.requires_grad());
+    const at::Tensor none;
+    ctx->save_for_backward({x, a, b, given(scales) ? *scales : none, index, given(offsets) ? *offsets : none, t});
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const int64_t wanted = ctx->saved_data["wanted"].toInt();
+    const at::Tensor& dy = grads[0];
+    harp_torch::refuse_tangent(dy, "harp_request", "add_adapters (backward)");
+    torch::autograd::variable_list out(7);
+    if (dy.defined()) {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      if (wanted & 1) out[0] = dy;
+      if (wanted & ~1) {
+        auto opt = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+        auto [dx, da, db] = adapters_backward(dy, s[0], s[1], s[2], opt(s[3]), s[4], opt(s[5]), s[6], wanted & 2,
+                                              wanted & 4, wanted & 8);
+        out[1] = dx;
+        out[2] = da;
+        out[3] = db;
+      }
+    }
+    harp_torch::once_only(out, "add_adapters");
+    return out;
+  }
+};
+
+at::Tensor add_adapters(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                        const OptTensor& scales, const at::Tensor& index, const OptTensor& offsets) {
+  return std::get<0>(adapters_forward(base, x, a, b, scales, index, offsets));
+}
+
+void refuse_adapters(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                     const OptTensor& scales) {
+  for (const OptTensor& t : {OptTensor(base), OptTensor(x), OptTensor(a), OptTensor(b), scales})
+    if (given(t)) harp_torch::refuse_tangent(*t, "harp_request", "add_adapters");
+  refuse_grad(scales, "add_adapters", "scales");
+}
+
+at::Tensor add_adapters_autograd(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                                 const OptTensor& scales, const at::Tensor& index, const OptTensor& offsets) {
+  refuse_adapters(base, x, a, b, scales);
+  const at::Tensor* const leaves[] = {&base, &x, &a, &b};
+  bool record = false;
+  for (const auto* t : leaves) record |= t->requires_grad();
+  if (!record || !at::GradMode::is_enabled()) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return add_adapters(base, x, a, b, scales, index, offsets);
+  }
+  TORCH_CHECK(base.scalar_type() == at::kBFloat16, "harp_request.add_adapters: gradients need a bfloat16 base, got ",
+              base.scalar_type());
+  const c10::DeviceGuard guard(x.device());
+  if (capturing()) {
+    const c10::Stream current = c10::hip::getCurrentHIPStream(x.get_device()).unwrap();
+    const char* const names[] = {"base", "x", "a", "b"};
+    for (int i = 0; i < 4; ++i) harp_torch::check_capture(*leaves[i], current, "add_adapters", names[i]);
+  }
+  return AddAdapters::apply(base, x, a, b, scales, index, offsets);
+}
+
+// For an autograd Function in Python: the leaves of a call that is being captured
+void check_capture(const std::vector<at::Tensor>& leaves) {
+  for (const auto& t : leaves) {
+    if (!t.is_cuda()) continue;
+    const c10::DeviceGuard guard(t.device());
+    if (!capturing()) continue;
+    harp_torch::check_capture(t, c10::hip::getCurrentHIPStream(t.get_device()).unwrap(), "harp_request", "an argument");
+  }
+}
+
+[[noreturn]] void no_cpu(const char* op) {
+  TORCH_CHECK(false, "harp_request.", op, ": this library runs on a HIP device only (CPU tensors given)");
+}
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_cpu(const at::Tensor&, const OptTensor&, const at::Tensor&,
+                                                    at::IntArrayRef, at::ArrayRef<double>, bool, const OptTensor&,
+                                                    const OptTensor&, at::ArrayRef<double>) {
+  no_cpu("qk_norm_rope");
+}
+at::Tensor rope_table_cpu(const at::Tensor&, at::IntArrayRef, at::ArrayRef<double>) { no_cpu("rope_table"); }
+at::Tensor add_adapters_cpu(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const OptTensor&, const at::Tensor&, const OptTensor&) {
+  no_cpu("add_adapters");
+}
+std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd_cpu(const at::Tensor& q, const OptTensor& k,
+                                                             const at::Tensor& positions, at::IntArrayRef,
+                                                             at::ArrayRef<double>, bool, const OptTensor& qw,
+                                                             const OptTensor& kw, at::ArrayRef<double>) {
+  refuse_rope(q, k, positions, qw, kw);
+  no_cpu("qk_norm_rope");
+}
+at::Tensor add_adapters_autograd_cpu(const at::Tensor& base, const at::Tensor& x, const at::Tensor& a,
+                                     const at::Tensor& b, const OptTensor& scales, const at::Tensor&,
+                                     const OptTensor&) {
+  refuse_adapters(base, x, a, b, scales);
+  no_cpu("add_adapters");
+}
+
+}  // namespace
+
+TORCH_LIBRARY(harp_request, m) {
+  m.def(
+      "qk_norm_rope(Tensor q, Tensor? k, Tensor positions, int[] widths, float[] theta, bool half, Tensor? q_weight, "
+      "Tensor? k_weight, float[] eps) -> (Tensor, Tensor)");
+  m.def("rope_table(Tensor positions, int[] widths, float[] theta) -> Tensor");
+  m.def(
+      "add_adapters(Tensor base, Tensor x, Tensor a, Tensor b, Tensor? scales, Tensor index, Tensor? offsets) -> "
+      "Tensor");
+  m.def("check_capture(Tensor[] leaves) -> ()", &check_capture);
+}
+
+TORCH_LIBRARY_IMPL(harp_request, AutogradCUDA, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope_autograd);
+  m.impl("rope_table", &rope_table_autograd);
+  m.impl("add_adapters", &add_adapters_autograd);
+}
+
+TORCH_LIBRARY_IMPL(harp_request, AutogradCPU, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope_autograd_cpu);
+  m.impl("rope_table", &rope_table_autograd);
+  m.impl("add_adapters", &add_adapters_autograd_cpu);
+}
+
+TORCH_LIBRARY_IMPL(harp_request, CUDA, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope);
+  m.impl("rope_table", &rope_table);
+  m.impl("add_adapters", &add_adapters);
+}
+
+TORCH_LIBRARY_IMPL(harp_request, CPU, m) {
+  m.impl("qk_norm_rope", &qk_norm_rope_cpu);
+  m.impl("rope_table", &rope_table_cpu);
+  m.impl("add_adapters", &add_adapters_cpu);
+}
