@@ -214,6 +214,12 @@ class ReqAdapters(ctypes.Structure):
     _fields_ = [("a", _p), ("b", _p), ("scales", _p), ("n", _i), ("rank", _i)]
 
 
+class ReqBackwardSet(ctypes.Structure):
+    """harp_req_backward_set_t of include/harp_request_ops.h (one projection's gradients)."""
+
+    _fields_ = [("adapters", ReqAdapters), ("t", _p), ("dy", _p), ("ld_dy", _i64), ("da", _p), ("db", _p)]
+
+
 _axes_p, _pos_p, _heads_p = (ctypes.POINTER(t) for t in (ReqAxes, ReqPositions, ReqHeads))
 _req_p, _adapters_p = ctypes.POINTER(ReqRequests), ctypes.POINTER(ReqAdapters)
 
@@ -225,9 +231,12 @@ REQ_PROTOTYPES = {
     "harp_req_rope_table": (_i, [_axes_p, _pos_p, _i, _i, _p, _p]),
     "harp_req_adapter_columns": (_i, [_i]),
     "harp_req_add_adapters_forward": (_i, [_p, _i64, _p, _i64, _p, _i64, _i, _adapters_p, _req_p, _p, _i, _i, _i, _p]),
-    "harp_req_add_adapters_backward": (_i, [_p, _i64, _p, _i64, _p, _adapters_p, _req_p, _p, _i64, _i, _p, _p, _i, _i,
-                                            _i, _p, _sz, _p]),
-    "harp_req_adapter_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "harp_req_add_adapters_backward": (_i, [ctypes.POINTER(ReqBackwardSet), _i, _p, _i64, _req_p, _p, _i64, _p, _i64,
+                                            _i, _i, _i, _p, _sz, _p]),
+    "harp_req_adapter_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "harp_req_qkv_project": (_i, [_p, _i64, _i, _i, _i, _i, _p, _i64, _i64, ctypes.POINTER(QkvOut), _adapters_p, _i,
+                                  _req_p, _pp, _p, _sz, _p]),
+    "harp_req_qkv_workspace_bytes": (_sz, [_i, _i, _i]),
     "harp_req_last_error": (ctypes.c_char_p, []),
 }
 

@@ -38,7 +38,8 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import nn
 
-from .adapters import AdapterRequests, add_adapters, is_adapted
+from .adapters import (AdapterRequests, add_adapters, fused_adapters_supported, is_adapted,
+                       project_qkv_adapters)
 from .int8 import Int8Linear, Int8Rows, fused_int8_supported, is_int8, project_qkv_int8, quantize_int8
 from .ops import RingAttention
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn
@@ -76,8 +77,11 @@ def _norm_axial_rope(attn, query: torch.Tensor, key: torch.Tensor, freqs: AxialP
 
 
 def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: Freqs,
-                     requests: Optional[AdapterRequests]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                     fused: bool, requests: Optional[AdapterRequests]
+                     ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """project_qkv of a module with adapters."""
+    if fused and requests is not None and fused_adapters_supported(attn, hidden_states, freqs, requests):
+        return project_qkv_adapters(attn, hidden_states, freqs, requests)
     x, heads, rows = hidden_states, attn.heads, None
     bases = [m.base if is_adapted(m) else m for m in (attn.to_q, attn.to_k, attn.to_v)]
     int8 = [isinstance(m, Int8Linear) for m in bases]
@@ -122,7 +126,7 @@ def project_qkv(attn: nn.Module, hidden_states: Union[torch.Tensor, Int8Rows], f
     if requests is not None and not adapted and not _adapted_out(attn):
         raise ValueError("requests need an attention module with adapters (harp_amd.adapt_attention)")
     if adapted:
-        return _project_adapted(attn, hidden_states, freqs_cis, requests)
+        return _project_adapted(attn, hidden_states, freqs_cis, fused, requests)
     axial = freqs_cis if isinstance(freqs_cis, AxialPositions) else None
     if axial is not None:
         # the one-launch forms: neighbouring pairs of heads of 128 features

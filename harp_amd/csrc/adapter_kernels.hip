@@ -12,18 +12,11 @@
 // bf16 (three for an fp32 result) whose products are added in fp32: 2^-17 (2^-25)
 // of a value is left out, far below the result's own rounding, and the
 // second product costs nothing beside the memory these kernels wait for.
-//
-// Requests are ranges of tokens of any length, known on the device only.  A
-// kernel that works in tiles of M tokens is launched with T / M + R + 2 slots;
-// segment i (the tokens in front of the first request, each request, the tokens
-// behind the last) starts at slot a_i / M + i, where its first token is a_i:
-// floor(b / M) + i + 1 - (floor(a / M) + i) is never less than the ceil((b - a) / M)
-// tiles it needs, so no tile is shared by two requests, nothing is counted
-// beforehand, and a block finds its segment by one or two 64-way searches.
-// What the arrays hold is clamped before it is used as an index.
+// Which tokens a block works on: req_device.h.
 #include <algorithm>
 
 #include "ra_common.h"
+#include "req_device.h"
 #include "req_kernels.h"
 
 namespace harp_req {
@@ -44,66 +37,6 @@ typedef u32x2 u32x2u __attribute__((aligned(2)));
 constexpr int kThreads = 256;
 
 // ---------------------------------------------------------------------------
-// Which tokens, which adapter
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ int64_t load_int(const void* p, int is64, int64_t i) {
-  return is64 ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
-}
-// first token of request i (0 .. count), within 0 .. tokens
-__device__ __forceinline__ int token_of(const Requests& q, int i) {
-  const int64_t v = q.offsets ? load_int(q.offsets, q.offsets64, i) : (int64_t)i * q.len;
-  return (int)min(max(v, (int64_t)0), (int64_t)q.tokens);
-}
-// adapter of request i, -1: none
-__device__ __forceinline__ int adapter_of(const Requests& q, int i) {
-  const int64_t v = load_int(q.index, q.index64, i);
-  return v >= 0 && v < q.n ? (int)v : -1;
-}
-// first token of segment i: 0 in front of the requests, request i - 1, behind them
-__device__ __forceinline__ int segment_start(const Requests& q, int i) {
-  if (i <= 0) return 0;
-  return i > q.count + 1 ? q.tokens : token_of(q, i - 1);
-}
-
-// The largest i <= count + 1 whose segment starts at or before `slot`, M tokens a slot
-template <int M>
-__device__ __forceinline__ int segment_at(const Requests& q, int slot) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, hi = q.count + 2;  // lo's start is <= slot; hi's is above, or hi is behind the last
-  while (hi - lo > 1) {          // (uniform: hi - lo shrinks 64-fold)
-    const int step = (hi - lo + 63) / 64;
-    const int i = lo + lane * step;
-    const bool at = i < hi && segment_start(q, i) / M + i <= slot;
-    // the last lane of the leading run; lane 0 (lo itself) is in it
-    const uint64_t b = __ballot(at) | 1;
-    const int last = __ffsll((unsigned long long)~b) - 2;
-    const int k = b == ~0ull ? 63 : last;
-    hi = min(hi, lo + (k + 1) * step);
-    lo = lo + k * step;
-  }
-  return __builtin_amdgcn_readfirstlane(lo);
-}
-
-// A tile: rows first .. first + rows - 1 (rows <= M) with one adapter (-1: none)
-struct Tile {
-  int first, rows, adapter;
-};
-template <int M>
-__device__ __forceinline__ Tile tile_at(const Requests& q, int slot) {
-  const int i = segment_at<M>(q, slot);
-  const int a = segment_start(q, i), b = segment_start(q, i + 1);
-  Tile t;
-  t.first = a + (slot - (a / M + i)) * M;
-  t.rows = min(M, b - t.first);
-  t.adapter = i >= 1 && i <= q.count ? adapter_of(q, i - 1) : -1;
-  t.first = __builtin_amdgcn_readfirstlane(t.first);
-  t.rows = __builtin_amdgcn_readfirstlane(t.rows);
-  t.adapter = __builtin_amdgcn_readfirstlane(t.adapter);
-  return t;
-}
-int64_t slots_of(const Requests& q, int M) { return (int64_t)q.tokens / M + q.count + 2; }
-
-// ---------------------------------------------------------------------------
 // Fragments
 // ---------------------------------------------------------------------------
 // n (<= 8) bf16 at p, zeros behind them
@@ -116,17 +49,16 @@ __device__ __forceinline__ bf16x8 load_some(const bf16* p, int n) {
 }
 __device__ __forceinline__ bf16x8 load_full(const bf16* p) { return __builtin_bit_cast(bf16x8, *(const u32x4u*)p); }
 
-__device__ __forceinline__ float high_part(float f) { return (float)(bf16)f; }
-
 }  // namespace
 
 // ---------------------------------------------------------------------------
-// Shrink.  A block takes a tile of 16 TB tokens and 16 RB ranks of one adapter;
-// its WAVES waves take every WAVES-th 64 columns of K and their sums are added
-// in LDS in the order of the waves.  v_mfma_f32_16x16x32_bf16 with A's rows as
-// the first operand: a lane ends with four neighbouring ranks of one token.
-// Fragments come straight from memory: a 64-column step reads whole 128-byte
-// lines of x and of A, and nothing of x is used twice by a block.
+// Shrink.  A block takes a tile of 16 TB tokens and RB blocks of 16 ranks (of the
+// sets one after the other) of one adapter; its WAVES waves take every WAVES-th
+// 64 columns of K and their sums are added in LDS in the order of the waves.
+// v_mfma_f32_16x16x32_bf16 with A's rows as the first operand: a lane ends with
+// four neighbouring ranks of one token.  Fragments come straight from memory: a
+// 64-column step reads whole 128-byte lines of x and of A, and nothing of x is
+// used twice by a block.
 // ---------------------------------------------------------------------------
 template <int TB, int RB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
@@ -134,26 +66,35 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
   __shared__ f32x4 sums[WAVES][TB * RB][64];
   const Tile tile = tile_at<M>(p.req, (int)blockIdx.x);
   if (tile.rows <= 0 || tile.adapter < 0) return;
-  const int which = blockIdx.z, r0 = (int)blockIdx.y * 16 * RB;
-  const ShrinkSet set = which == 0 ? p.set[0] : which == 1 ? p.set[1] : p.set[2];
+  // this block's entries e0 .. e0 + RB - 1 (before e_end) of the sets' rank blocks; those of sets with an x of
+  // their own are not shared
+  const int per = p.rp / 16, groups = (per + RB - 1) / RB, own = (int)blockIdx.y / groups;
+  const int e0 = p.apart ? own * per + ((int)blockIdx.y - own * groups) * RB : (int)blockIdx.y * RB;
+  const int e_end = p.apart ? (own + 1) * per : per * p.sets;
   const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  // (constant indices: a kernel-argument array indexed at run time would be copied to scratch memory)
+  auto set_of = [&](int e) { return min(e, e_end - 1) / per; };
+  auto a_of = [&](int i) { return (const bf16*)(i == 0 ? p.set[0].a : i == 1 ? p.set[1].a : p.set[2].a); };
+  const int s0 = set_of(e0);
+  const bf16* const x = (const bf16*)(s0 == 0 ? p.set[0].x : s0 == 1 ? p.set[1].x : p.set[2].x);
+  const int64_t ldx = s0 == 0 ? p.set[0].ldx : s0 == 1 ? p.set[1].ldx : p.set[2].ldx;
   const bf16* xr[TB];
   const bf16* ar[RB];
   // rows behind the tile and ranks behind r repeat the last one; their sums are dropped
 #pragma unroll
-  for (int i = 0; i < TB; ++i)
-    xr[i] = (const bf16*)p.x + (int64_t)(tile.first + min(16 * i + l16, tile.rows - 1)) * p.ldx + 8 * g;
+  for (int i = 0; i < TB; ++i) xr[i] = x + (int64_t)(tile.first + min(16 * i + l16, tile.rows - 1)) * ldx + 8 * g;
 #pragma unroll
-  for (int j = 0; j < RB; ++j)
-    ar[j] = (const bf16*)set.a + ((int64_t)tile.adapter * p.r + min(r0 + 16 * j + l16, p.r - 1)) * p.K + 8 * g;
+  for (int j = 0; j < RB; ++j) {
+    const int set = set_of(e0 + j), rank = 16 * (min(e0 + j, e_end - 1) - set * per) + l16;
+    ar[j] = a_of(set) + ((int64_t)tile.adapter * p.r + min(rank, p.r - 1)) * p.K + 8 * g;
+  }
   f32x4 acc[RB][TB];
 #pragma unroll
   for (int j = 0; j < RB; ++j)
 #pragma unroll
     for (int i = 0; i < TB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int full = p.K / 64;
-#pragma unroll 2
   for (int c = wave; c < full; c += WAVES) {
     bf16x8 xf[2][TB], af[2][RB];
 #pragma unroll
@@ -189,27 +130,28 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
 #pragma unroll
     for (int i = 0; i < TB; ++i) sums[wave][j * TB + i][lane] = acc[j][i];
   __syncthreads();
-  const float scale = set.scale ? set.scale[tile.adapter] : 1.f;
   for (int e = threadIdx.x; e < TB * RB * 64; e += 64 * WAVES) {
     const int at = e >> 6, l = e & 63, j = at / TB, i = at % TB;
     f32x4 s = sums[0][at][l];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) s += sums[w][at][l];
-    const int row = 16 * i + (l & 15), rank = r0 + 16 * j + 4 * (l >> 4);
-    if (row >= tile.rows || rank >= p.rp) continue;
+    const int row = 16 * i + (l & 15);
+    if (row >= tile.rows || e0 + j >= e_end) continue;
+    const int which = (e0 + j) / per, rank = 16 * (e0 + j - which * per) + 4 * (l >> 4);
+    const ShrinkSet set = which == 0 ? p.set[0] : which == 1 ? p.set[1] : p.set[2];
+    const float scale = set.scale ? set.scale[tile.adapter] : 1.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) s[k] = rank + k < p.r ? s[k] * scale : 0.f;
     const int64_t m = tile.first + row;
-    if (!p.pairs) {
-      *(f32x4*)((float*)set.t + m * p.ldt + rank) = s;
-    } else {
+    if (set.t) *(f32x4*)(set.t + m * p.ldt + rank) = s;
+    if (set.pairs) {
       bf16 hi[4], lo[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         hi[k] = (bf16)s[k];
         lo[k] = (bf16)(s[k] - (float)hi[k]);
       }
-      bf16* t = (bf16*)set.t + m * p.ldt + rank;
+      bf16* t = (bf16*)set.pairs + m * 2 * p.rp + rank;
       *(u32x2*)t = *(const u32x2*)hi;
       *(u32x2*)(t + p.rp) = *(const u32x2*)lo;
     }
@@ -218,70 +160,78 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
 
 // ---------------------------------------------------------------------------
 // Expand.  A wave takes 32 tokens and walks 64 features at a time:
-// v_mfma_f32_32x32x16_bf16 with B's rows as the first operand, its row q of a
-// 32-feature block reading feature 32 g + 16 block + r of the 64, so that a lane
-// (token l % 32, half g) ends with 2 x 16 neighbouring features and the
-// wave's base and out accesses are whole 128-byte lines of a row.  t's fragments
-// stay in registers over the walk.
+// v_mfma_f32_32x32x16_bf16 with B's rows as the first operand, so that a lane
+// ends with runs of four features of one token.  Those go through the wave's
+// 8 KB of LDS (16-byte chunk c of row r at c ^ (r % 16): no bank conflict either
+// way), so that base is read and out written in whole 128-byte lines, 16 bytes a
+// lane: straight from the accumulators' layout each access touched 64 rows'
+// pieces and the kernel ran at half the rate.  t's fragments stay in registers
+// over the walk.
 // ---------------------------------------------------------------------------
 namespace {
 
-// 16 (bf16: 32 bytes, fp32: 64 bytes) values of a row from column f on, columns below N
-template <bool F32>
-__device__ __forceinline__ void load16(const void* row, int f, int N, float (&v)[16]) {
+constexpr int kNoBase = 0, kBaseBf16 = 1, kBaseF32 = 2;
+
+template <int E>
+struct Run {
+  float v[E];
+};
+// E values of a row from column c on as they are in memory, those below N
+template <bool F32, int E>
+struct RawRun {
+  u32x4 u[E * (F32 ? 4 : 2) / 16];
+};
+template <bool F32, int E>
+__device__ __forceinline__ RawRun<F32, E> load_run(const char* row, int c, int N) {
+  constexpr int es = F32 ? 4 : 2, kWords = E * es / 16;
+  RawRun<F32, E> r;
+  if (c + E <= N) {
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int c = f + 8 * q;
-    if (c + 8 <= N) {
-      if constexpr (F32) {
+    for (int h = 0; h < kWords; ++h) r.u[h] = *(const u32x4u*)(row + (int64_t)c * es + 16 * h);
+  } else {
+    uint32_t w[4 * kWords] = {};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 u = *(const f32x4u*)((const float*)row + c + 4 * h);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[8 * q + 4 * h + k] = u[k];
-        }
-      } else {
-        const u32x4 u = *(const u32x4u*)((const bf16*)row + c);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          v[8 * q + 2 * k] = __uint_as_float(u[k] << 16);
-          v[8 * q + 2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u);
-        }
+    for (int k = 0; k < E; ++k)
+      if (c + k < N) {
+        if constexpr (F32) w[k] = ((const uint32_t*)row)[c + k];
+        else w[k / 2] |= (uint32_t)((const uint16_t*)row)[c + k] << (16 * (k & 1));
       }
-    } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        v[8 * q + k] = 0.f;
-        if (c + k < N) v[8 * q + k] = F32 ? ((const float*)row)[c + k] : (float)((const bf16*)row)[c + k];
-      }
-    }
+    for (int h = 0; h < kWords; ++h) r.u[h] = u32x4{w[4 * h], w[4 * h + 1], w[4 * h + 2], w[4 * h + 3]};
   }
+  return r;
 }
-template <bool F32>
-__device__ __forceinline__ void store16(void* row, int f, int N, const float (&v)[16]) {
+template <bool F32, int E>
+__device__ __forceinline__ Run<E> values(const RawRun<F32, E>& r) {
+  Run<E> v;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int c = f + 8 * q;
-    if (c + 8 <= N) {
-      if constexpr (F32) {
+  for (int k = 0; k < E; ++k) {
+    if constexpr (F32) v.v[k] = __uint_as_float(r.u[k / 4][k % 4]);
+    else v.v[k] = __uint_as_float((k & 1) ? r.u[k / 8][k / 2 % 4] & 0xffff0000u : r.u[k / 8][k / 2 % 4] << 16);
+  }
+  return v;
+}
+template <bool F32, int E>
+__device__ __forceinline__ void store_run(char* row, int c, int N, const Run<E>& r) {
+  if (c + E <= N) {
+    if constexpr (F32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *(f32x4u*)((float*)row + c + 4 * h) =
-              f32x4{v[8 * q + 4 * h], v[8 * q + 4 * h + 1], v[8 * q + 4 * h + 2], v[8 * q + 4 * h + 3]};
-      } else {
-        bf16x8 o;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k] = (bf16)v[8 * q + k];
-        *(u32x4u*)((bf16*)row + c) = __builtin_bit_cast(u32x4, o);
-      }
+      for (int h = 0; h < E / 4; ++h)
+        *(f32x4u*)((float*)row + c + 4 * h) = f32x4{r.v[4 * h], r.v[4 * h + 1], r.v[4 * h + 2], r.v[4 * h + 3]};
     } else {
+      static_assert(E == 8);
+      bf16x8 o;
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c + k < N) {
-          if constexpr (F32) ((float*)row)[c + k] = v[8 * q + k];
-          else ((bf16*)row)[c + k] = (bf16)v[8 * q + k];
-        }
+      for (int k = 0; k < 8; ++k) o[k] = (bf16)r.v[k];
+      *(u32x4u*)((bf16*)row + c) = __builtin_bit_cast(u32x4, o);
     }
+  } else {
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+      if (c + k < N) {
+        if constexpr (F32) ((float*)row)[c + k] = r.v[k];
+        else ((bf16*)row)[c + k] = (bf16)r.v[k];
+      }
   }
 }
 
@@ -289,30 +239,31 @@ __device__ __forceinline__ void store16(void* row, int f, int N, const float (&v
 
 // RS: 16-rank steps (rp / 16); WT: waves of a block along the tokens (the other
 // 4 / WT along the features); a block walks `span` features
-template <bool F32, int RS, int WT>
+template <int BASE, bool F32, int RS, int WT>
 __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int span) {
   constexpr int M = 32 * WT, WF = 4 / WT, PARTS = F32 ? 3 : 2;
+  constexpr int E = F32 ? 4 : 8;             // features of a lane's access: 16 bytes of out
+  constexpr int kLanes = 64 / E, kPass = 32 / E;  // lanes of a row, passes over the 32 rows
+  __shared__ f32x4 tiles[4][32 * 16];
   const Tile tile = tile_at<M>(p.req, (int)blockIdx.x);
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int row = 32 * (wave % WT) + l32;
-  if (tile.rows <= 32 * (wave % WT)) return;
-  const bool mine = row < tile.rows;
-  const int64_t m = tile.first + (mine ? row : 0);
+  const int row0 = 32 * (wave % WT), rows = min(32, tile.rows - row0);
+  if (rows <= 0) return;
+  const int64_t m0 = tile.first + row0;
+  f32x4* const lds = tiles[wave];
   const int f_end = min(p.N, ((int)blockIdx.y + 1) * span);
-  constexpr int es = F32 ? 4 : 2;
-  const char* const base = p.base ? (const char*)p.base + m * p.ld_base * es : nullptr;
-  char* const out = (char*)p.out + m * p.ld_out * es;
+  constexpr int es = F32 ? 4 : 2, bs = BASE == kBaseF32 ? 4 : 2;
 
   bf16x8 tf[RS][PARTS];
   if (tile.adapter >= 0) {
+    const float* const t = p.t + (m0 + min(l32, rows - 1)) * p.ldt + 8 * g;
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
-      const float* t = p.t + m * p.ldt + 16 * s + 8 * g;
       float v[8];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const f32x4 u = *(const f32x4*)(t + 4 * h);
+        const f32x4 u = *(const f32x4*)(t + 16 * s + 4 * h);
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[4 * h + k] = u[k];
       }
@@ -326,26 +277,23 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int sp
         }
     }
   }
-  // the B row of operand row l32 in block q: feature 32 g' + 16 q + 4 a + b for l32 = 8 a + 4 g' + b
-  const int feat = 32 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);
   const bool whole = p.r % 8 == 0;
+  const int r_in = lane / kLanes, c_in = E * (lane % kLanes);  // this lane's row and columns of a pass
   for (int f0 = (int)blockIdx.y * span + 64 * (wave / WT); f0 < f_end; f0 += 64 * WF) {
-    float v[2][16];
+    RawRun<BASE == kBaseF32, E> raw[kPass];
+    if constexpr (BASE != kNoBase) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      if (base) {
-        load16<F32>(base, f0 + 32 * g + 16 * q, p.N, v[q]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[q][k] = 0.f;
+      for (int i = 0; i < kPass; ++i) {
+        const int row = i * E + r_in;
+        if (row < rows)
+          raw[i] = load_run<BASE == kBaseF32, E>((const char*)p.base + (m0 + row) * p.ld_base * bs, f0 + c_in, p.N);
       }
     }
     if (tile.adapter >= 0) {
-      f32x16 acc[2];
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
-        const bf16* b = (const bf16*)p.b + ((int64_t)tile.adapter * p.N + min(f0 + feat + 16 * q, p.N - 1)) * p.r + 8 * g;
-        acc[q] = harp_ra::zero16();
+        const bf16* b = (const bf16*)p.b + ((int64_t)tile.adapter * p.N + min(f0 + 32 * q + l32, p.N - 1)) * p.r + 8 * g;
+        f32x16 acc = harp_ra::zero16();
 #pragma unroll
         for (int s = 0; s < RS; ++s) {
           const int n = p.r - 16 * s - 8 * g;  // ranks this lane has left: 8 or more but in the last step
@@ -353,142 +301,253 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int sp
                             : whole              ? harp_ra::zero8()
                                                  : load_some(b + 16 * s, n);
 #pragma unroll
-          for (int part = 0; part < PARTS; ++part) acc[q] = harp_ra::mfma32x32x16(bf, tf[s][part], acc[q]);
+          for (int part = 0; part < PARTS; ++part) acc = harp_ra::mfma32x32x16(bf, tf[s][part], acc);
+        }
+        // registers 4 a .. + 3: features 32 q + 8 a + 4 g .. + 3 of token l32
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          lds[l32 * 16 + ((8 * q + 2 * a + g) ^ (l32 & 15))] =
+              f32x4{acc[4 * a], acc[4 * a + 1], acc[4 * a + 2], acc[4 * a + 3]};
+      }
+    }
+    // (the wave's own LDS, whose operations stay in order)
+#pragma unroll
+    for (int i = 0; i < kPass; ++i) {
+      const int row = i * E + r_in;
+      Run<E> v{};
+      if constexpr (BASE != kNoBase) v = values<BASE == kBaseF32, E>(raw[i]);
+      if (tile.adapter >= 0) {
+#pragma unroll
+        for (int h = 0; h < E / 4; ++h) {
+          const f32x4 d = lds[row * 16 + ((c_in / 4 + h) ^ (row & 15))];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v.v[4 * h + k] += d[k];
         }
       }
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int k = 0; k < 16; ++k) v[q][k] += acc[q][k];
-    }
-    if (mine) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) store16<F32>(out, f0 + 32 * g + 16 * q, p.N, v[q]);
+      if (row < rows) store_run<F32, E>((char*)p.out + (m0 + row) * p.ld_out * es, f0 + c_in, p.N, v);
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Gradients of A and B: for each adapter the sum over its tokens of
-// v[m]^T x[m], 16 RB ranks x 128 columns a block.  The WAVES waves take every
-// WAVES-th four tokens; v_mfma_f32_16x16x4_f32 takes them as they lie in
-// memory (a lane holds rank l % 16, or 8 columns 8 (l % 16) .., of token l / 16),
-// so nothing is transposed and v keeps its 32 bits.  The waves' sums are
-// added in LDS in order.  Where the blocks of all adapters would not fill the
-// chip, each request's tokens are taken in `splits` parts whose sums a second
-// kernel adds, in order too.
+// Gradients of A and B: for each adapter the sum over its tokens of v[m]^T x[m].
+// A block takes 128 columns and 32 RK ranks of one adapter, its four waves 32
+// columns each, and walks the adapter's tokens 64 at a time: the step's x (bf16)
+// and v (taken apart into two bf16) lie in LDS as they come, and
+// ds_read_b64_tr_b16 reads both transposed, tokens along the contraction of
+// v_mfma_f32_32x32x16_bf16.  The next step's loads are on their way meanwhile.
+// (v_mfma_f32_16x16x4_f32 takes the values without a transpose, and runs at a
+// sixteenth of the rate: rank 64 over 8192 tokens took 119 us.)  Where the
+// blocks of all adapters would not fill the chip, each request's tokens are taken
+// in `splits` parts whose sums a second kernel adds in order.
 // ---------------------------------------------------------------------------
-constexpr int kGradWaves = 8, kGradCols = 128;
+namespace {
+constexpr int kGradCols = 128, kGradStep = 64;
 
-template <int RB>
-__global__ __launch_bounds__(64 * kGradWaves) void grad_kernel(GradParams p) {
-  __shared__ f32x4 sums[kGradWaves][RB * 2][64];
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int c0_blocks = p.part[0].out ? (p.part[0].C + kGradCols - 1) / kGradCols : 0;
-  const bool second = (int)blockIdx.x >= c0_blocks;
-  const GradPart part = second ? p.part[1] : p.part[0];
-  const int c0 = ((int)blockIdx.x - (second ? c0_blocks : 0)) * kGradCols;
-  const int rgroups = (p.r + 16 * RB - 1) / (16 * RB);
-  const int adapter = (int)blockIdx.y / rgroups, r0 = (int)blockIdx.y % rgroups * 16 * RB;
+// Rows of 128 bf16: 16-byte chunk c of row r at c ^ swz(r).  Row reads and the
+// transposed reads below are free of bank conflicts.
+__device__ __forceinline__ int grad_slot(int r, int c) { return r * 128 + ((c ^ harp_ra::swz(r)) << 3); }
+
+// T[r0 + {4 g .. + 3, 8 + 4 g .. + 3}][32 db + l32]: of two lanes with one g each
+// register holds one token, the same for both operands.  In each group of 16
+// lanes, lane i's value s is element i % 4 of the 8 bytes that lane 4 s + i / 4 addresses.
+__device__ __forceinline__ bf16x8 tr_frag(const bf16* t, int r0, int db) {
+  const int lane = threadIdx.x & 63, g = lane >> 5, s = (lane >> 2) & 3, m = lane & 3;
+  const int c = 4 * db + 2 * ((lane >> 4) & 1) + (m >> 1);
+  const int ra = r0 + 4 * g + s, rb = ra + 8;
+  const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((harp_ra::lds_bf16x4*)(t + grad_slot(ra, c) + 4 * (m & 1)));
+  const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((harp_ra::lds_bf16x4*)(t + grad_slot(rb, c) + 4 * (m & 1)));
+  bf16x8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = lo[i];
+    r[i + 4] = hi[i];
+  }
+  return r;
+}
+
+// The steps of an adapter's tokens: those of its requests one after the other
+struct Steps {
+  int i0;         // requests i0 .. i0 + 63 are in `todo`
+  uint64_t todo;  // those of the adapter that are left
+  int m, end;     // the next step's first token, the end of the request's part
+};
+
+}  // namespace
+
+template <int RK>
+__global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
+  __shared__ __attribute__((aligned(16))) bf16 xs[kGradStep * 128], vs[2][kGradStep * 128];
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // this block's part and columns (constant indices: see the shrink kernel)
+  GradPart part = p.part[0];
+  int cb = blockIdx.x;
+  int64_t at = 0;  // of the part's values among all
+  const int64_t per = (int64_t)p.req.n * p.r;
+#pragma unroll
+  for (int i = 1; i < kMaxGradParts; ++i) {
+    const int blocks = (part.C + kGradCols - 1) / kGradCols;
+    if (i < p.parts && cb >= blocks) {
+      cb -= blocks;
+      at += per * part.C;
+      part = p.part[i];
+    } else {
+      break;
+    }
+  }
+  const int c0 = cb * kGradCols;
+  const int rgroups = (p.rp + 32 * RK - 1) / (32 * RK);
+  const int adapter = (int)blockIdx.y / rgroups, r0 = (int)blockIdx.y % rgroups * 32 * RK;
   const int split = blockIdx.z;
-  const int col = c0 + 8 * l16;
-  const int ncol = min(8, part.C - col);  // <= 0: no column of this lane
 
-  f32x4 acc[RB][8];
+  f32x16 acc[RK];
 #pragma unroll
-  for (int j = 0; j < RB; ++j)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) acc[j][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < RK; ++j) acc[j] = harp_ra::zero16();
 
-  for (int i0 = 0; i0 < p.req.count; i0 += 64) {
-    const bool hit = i0 + lane < p.req.count && adapter_of(p.req, min(i0 + lane, p.req.count - 1)) == adapter;
-    for (uint64_t todo = __ballot(hit); todo; todo &= todo - 1) {
-      const int i = i0 + __ffsll((unsigned long long)todo) - 1;
+  Steps st{-64, 0, 0, 0};
+  auto next = [&]() {  // whether there is another step; its tokens are st.m .. min(st.m + 64, st.end) - 1
+    while (st.m >= st.end) {
+      while (!st.todo) {
+        st.i0 += 64;
+        if (st.i0 >= p.req.count) return false;
+        const int i = st.i0 + lane;
+        st.todo = __ballot(i < p.req.count && adapter_of(p.req, min(i, p.req.count - 1)) == adapter);
+      }
+      const int i = st.i0 + __ffsll((unsigned long long)st.todo) - 1;
+      st.todo &= st.todo - 1;
       const int a = token_of(p.req, i), n = max(token_of(p.req, i + 1) - a, 0);
-      const int begin = a + (int)((int64_t)n * split / p.splits), end = a + (int)((int64_t)n * (split + 1) / p.splits);
-      for (int m0 = begin + 4 * wave; m0 < end; m0 += 4 * kGradWaves) {
-        const int m = m0 + g;
-        const bool in = m < end;
-        bf16x8 xv = harp_ra::zero8();
-        float vv[RB];
-        if (in) {
-          const bf16* x = (const bf16*)part.x + (int64_t)m * part.ldx + col;
-          if (ncol == 8) xv = load_full(x);
-          else if (ncol > 0) xv = load_some(x, ncol);
-        }
+      st.m = a + (int)((int64_t)n * split / p.splits);
+      st.end = a + (int)((int64_t)n * (split + 1) / p.splits);
+    }
+    return true;
+  };
+
+  // a thread's share of a step: x row tid / 16 + 16 k, 8 columns; v row tid / (4 RK)
+  // + 64 / RK k, 8 ranks
+  constexpr int kVLanes = 4 * RK, kVRows = kThreads / kVLanes, kVPass = kGradStep / kVRows;
+  bf16x8 xv[4];
+  f32x4 vv[kVPass][2];
+  const int xr = tid >> 4, xc = tid & 15, vr = tid / kVLanes, vc = tid % kVLanes;
+  auto load = [&](int m, int n) {
 #pragma unroll
-        for (int j = 0; j < RB; ++j)
-          vv[j] = in && r0 + 16 * j < p.rp ? part.v[(int64_t)m * part.ldv + r0 + 16 * j + l16] : 0.f;
-#pragma unroll
-        for (int j = 0; j < RB; ++j)
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            acc[j][k] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv[j], (float)xv[k], acc[j][k], 0, 0, 0);
+    for (int k = 0; k < 4; ++k) {
+      const int row = xr + 16 * k, left = part.C - c0 - 8 * xc;
+      xv[k] = harp_ra::zero8();
+      if (row < n && left > 0) {
+        const bf16* x = (const bf16*)part.x + (int64_t)(m + row) * part.ldx + c0 + 8 * xc;
+        xv[k] = left >= 8 ? load_full(x) : load_some(x, left);
       }
     }
+#pragma unroll
+    for (int k = 0; k < kVPass; ++k) {
+      const int row = vr + kVRows * k;
+      vv[k][0] = vv[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (row < n && r0 + 8 * vc < p.rp) {
+        const float* v = part.v + (int64_t)(m + row) * part.ldv + r0 + 8 * vc;
+        vv[k][0] = *(const f32x4*)v;
+        vv[k][1] = *(const f32x4*)(v + 4);
+      }
+    }
+  };
+  bool more = next();
+  if (more) load(st.m, min(kGradStep, st.end - st.m));
+  while (more) {
+    const int n = min(kGradStep, st.end - st.m);
+    st.m += n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) *(bf16x8*)(xs + grad_slot(xr + 16 * k, xc)) = xv[k];
+#pragma unroll
+    for (int k = 0; k < kVPass; ++k) {
+      bf16x8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = vv[k][e / 4][e % 4];
+        hi[e] = (bf16)f;
+        lo[e] = (bf16)(f - (float)hi[e]);
+      }
+      *(bf16x8*)(vs[0] + grad_slot(vr + kVRows * k, vc)) = hi;
+      *(bf16x8*)(vs[1] + grad_slot(vr + kVRows * k, vc)) = lo;
+    }
+    __syncthreads();
+    more = next();
+    if (more) load(st.m, min(kGradStep, st.end - st.m));
+    const int ksteps = (n + 15) / 16;
+    for (int k = 0; k < ksteps; ++k) {
+      const bf16x8 xf = tr_frag(xs, 16 * k, wave);
+#pragma unroll
+      for (int j = 0; j < RK; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc[j] = harp_ra::mfma32x32x16(xf, tr_frag(vs[h], 16 * k, j), acc[j]);
+    }
+    __syncthreads();
   }
 
-  // columns 8 l16 + 2 h, + 1 of all waves at a time; a lane holds ranks 4 g .. + 3
+  // a lane holds rank r0 + 32 j + l32 and columns 8 a + 4 g .. + 3 of the wave's 32
 #pragma unroll
-  for (int h = 0; h < 4; ++h) {
+  for (int j = 0; j < RK; ++j) {
+    const int rank = r0 + 32 * j + l32;
+    if (rank >= p.r) continue;
 #pragma unroll
-    for (int j = 0; j < RB; ++j)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) sums[wave][2 * j + k][lane] = acc[j][2 * h + k];
-    __syncthreads();
-    for (int e = threadIdx.x; e < RB * 2 * 64; e += 64 * kGradWaves) {
-      const int at = e >> 6, l = e & 63;
-      f32x4 s = sums[0][at][l];
-#pragma unroll
-      for (int w = 1; w < kGradWaves; ++w) s += sums[w][at][l];
-      const int c = c0 + 8 * (l & 15) + 2 * h + (at & 1), rank = r0 + 16 * (at >> 1) + 4 * (l >> 4);
+    for (int e = 0; e < 16; ++e) {
+      const int c = c0 + 32 * wave + harp_ra::c_row(e, g);
       if (c >= part.C) continue;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (rank + k >= p.r) break;
-        const int64_t o = part.cols_first ? ((int64_t)adapter * part.C + c) * p.r + rank + k
-                                          : ((int64_t)adapter * p.r + rank + k) * part.C + c;
-        if (p.splits == 1) ((bf16*)part.out)[o] = (bf16)s[k];
-        else {
-          const int64_t all = (int64_t)p.req.n * p.r * ((p.part[0].out ? p.part[0].C : 0) + (p.part[1].out ? p.part[1].C : 0));
-          p.work[split * all + (second && p.part[0].out ? (int64_t)p.req.n * p.r * p.part[0].C : 0) + o] = s[k];
-        }
-      }
+      const int64_t o = part.cols_first ? ((int64_t)adapter * part.C + c) * p.r + rank
+                                        : ((int64_t)adapter * p.r + rank) * part.C + c;
+      if (p.splits == 1) ((bf16*)part.out)[o] = (bf16)acc[j][e];
+      else p.work[split * grad_values(p) + at + o] = acc[j][e];
     }
-    __syncthreads();
   }
 }
 
-__global__ __launch_bounds__(kThreads) void grad_sum_kernel(const float* work, int splits, int64_t n0, int64_t n1,
-                                                            bf16* out0, bf16* out1) {
-  const int64_t all = n0 + n1;
+// the sum of the splits, in order
+__global__ __launch_bounds__(kThreads) void grad_sum_kernel(GradParams p, int64_t all) {
+  const int64_t per = (int64_t)p.req.n * p.r;
   for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < all; i += (int64_t)gridDim.x * kThreads) {
-    float s = work[i];
-    for (int k = 1; k < splits; ++k) s += work[k * all + i];
-    (i < n0 ? out0[i] : out1[i - n0]) = (bf16)s;
+    float s = p.work[i];
+    for (int k = 1; k < p.splits; ++k) s += p.work[k * all + i];
+    int64_t o = i;
+    void* out = p.part[0].out;
+    int64_t n = per * p.part[0].C;
+#pragma unroll
+    for (int k = 1; k < kMaxGradParts; ++k)
+      if (k < p.parts && o >= n) {
+        o -= n;
+        out = p.part[k].out;
+        n = per * p.part[k].C;
+      }
+    ((bf16*)out)[o] = (bf16)s;
   }
 }
 
 // ---------------------------------------------------------------------------
 // n matrices transposed, 64 x 64 values a block
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(kThreads) void transpose_kernel(TransposeParams p, int tiles0) {
+__global__ __launch_bounds__(kThreads) void transpose_kernel(TransposeParams p) {
   __shared__ uint16_t t[64][65];
-  const bool second = (int)blockIdx.x >= tiles0;
-  const TransposePart part = second ? p.part[1] : p.part[0];
-  const int across = (part.cols + 63) / 64;
-  const int tile = (int)blockIdx.x - (second ? tiles0 : 0);
+  TransposePart part = p.part[0];
+  int tile = blockIdx.x;
+#pragma unroll
+  for (int i = 1; i < 2 * kMaxSets; ++i) {
+    const int tiles = (max(part.rows, part.fill) + 63) / 64 * ((part.cols + 63) / 64);
+    if (i < p.parts && tile >= tiles) {
+      tile -= tiles;
+      part = p.part[i];
+    } else {
+      break;
+    }
+  }
+  const int across = (part.cols + 63) / 64, fill = max(part.rows, part.fill);
   const int r0 = tile / across * 64, c0 = tile % across * 64;
   const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
   for (int i = blockIdx.y; i < p.n; i += gridDim.y) {
     const uint16_t* src = (const uint16_t*)part.src + (int64_t)i * part.rows * part.cols;
-    uint16_t* dst = (uint16_t*)part.dst + (int64_t)i * part.rows * part.cols;
+    uint16_t* dst = (uint16_t*)part.dst + (int64_t)i * part.cols * part.ld;
     for (int y = ty; y < 64; y += 4)
-      if (r0 + y < part.rows && c0 + tx < part.cols) t[y][tx] = src[(int64_t)(r0 + y) * part.cols + c0 + tx];
+      t[y][tx] = r0 + y < part.rows && c0 + tx < part.cols ? src[(int64_t)(r0 + y) * part.cols + c0 + tx] : (uint16_t)0;
     __syncthreads();
     for (int y = ty; y < 64; y += 4)
-      if (c0 + y < part.cols && r0 + tx < part.rows) dst[(int64_t)(c0 + y) * part.rows + r0 + tx] = t[tx][y];
+      if (c0 + y < part.cols && r0 + tx < fill) dst[(int64_t)(c0 + y) * part.ld + r0 + tx] = t[tx][y];
     __syncthreads();
   }
 }
@@ -499,20 +558,27 @@ __global__ __launch_bounds__(kThreads) void transpose_kernel(TransposeParams p, 
 namespace {
 template <int TB, int RB, int WAVES>
 hipError_t shrink_t(const ShrinkParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)slots_of(p.req, 16 * TB), (unsigned)((p.rp + 16 * RB - 1) / (16 * RB)), (unsigned)p.sets);
+  const int per = p.rp / 16;
+  const int groups = p.apart ? p.sets * ((per + RB - 1) / RB) : (per * p.sets + RB - 1) / RB;
+  const dim3 grid((unsigned)slots_of(p.req, 16 * TB), (unsigned)groups);
   hipLaunchKernelGGL((shrink_kernel<TB, RB, WAVES>), grid, dim3(64 * WAVES), 0, st, p);
   return hipGetLastError();
+}
+template <int WAVES>
+hipError_t shrink_w(const ShrinkParams& p, hipStream_t st) {
+  const int total = p.rp / 16 * (p.apart ? 1 : p.sets);
+  if (slots_of(p.req, 16) * (p.rp / 16) * p.sets <= 512 || total == 1) return shrink_t<1, 1, WAVES>(p, st);
+  return total % 4 == 0 || total > 4 ? shrink_t<2, 4, WAVES>(p, st) : shrink_t<2, 2, WAVES>(p, st);
 }
 }  // namespace
 
 hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
-  // few tokens: 16 waves share a tile's K
-  if (slots_of(p.req, 32) * p.sets < 512) return shrink_t<1, 1, 16>(p, st);
-  return p.rp <= 16 ? shrink_t<2, 1, 4>(p, st) : p.rp <= 32 ? shrink_t<2, 2, 4>(p, st) : shrink_t<4, 4, 4>(p, st);
+  // the waves of a block share K: 16 of them where each has a 64-column step
+  return p.K >= 1024 ? shrink_w<16>(p, st) : shrink_w<4>(p, st);
 }
 
 namespace {
-template <bool F32, int RS, int WT>
+template <int BASE, bool F32, int RS, int WT>
 hipError_t expand_t(const ExpandParams& p, hipStream_t st) {
   const int64_t slots = slots_of(p.req, 32 * WT);
   // enough blocks for the chip, in multiples of a block's 64-feature steps
@@ -520,72 +586,71 @@ hipError_t expand_t(const ExpandParams& p, hipStream_t st) {
   const int steps = (p.N + step - 1) / step;
   const int64_t want = std::max<int64_t>(1, 2048 / slots);
   const int each = (int)std::max<int64_t>(1, steps / std::min<int64_t>(want, steps));
-  hipLaunchKernelGGL((expand_kernel<F32, RS, WT>), dim3((unsigned)slots, (unsigned)((steps + each - 1) / each)),
+  hipLaunchKernelGGL((expand_kernel<BASE, F32, RS, WT>), dim3((unsigned)slots, (unsigned)((steps + each - 1) / each)),
                      dim3(kThreads), 0, st, p, each * step);
   return hipGetLastError();
 }
-template <bool F32, int RS>
+template <int BASE, bool F32, int RS>
 hipError_t expand_w(const ExpandParams& p, hipStream_t st) {
   // requests of 64 tokens and more on the average fill a block's waves along the tokens
-  return p.req.tokens / std::max(p.req.count, 1) >= 64 ? expand_t<F32, RS, 4>(p, st) : expand_t<F32, RS, 1>(p, st);
+  return p.req.tokens / std::max(p.req.count, 1) >= 64 ? expand_t<BASE, F32, RS, 4>(p, st)
+                                                       : expand_t<BASE, F32, RS, 1>(p, st);
 }
-template <bool F32>
+template <int BASE, bool F32>
 hipError_t expand_r(const ExpandParams& p, hipStream_t st) {
   switch (p.rp / 16) {
-    case 1: return expand_w<F32, 1>(p, st);
-    case 2: return expand_w<F32, 2>(p, st);
-    case 3: return expand_w<F32, 3>(p, st);
-    case 4: return expand_w<F32, 4>(p, st);
-    case 5: return expand_w<F32, 5>(p, st);
-    case 6: return expand_w<F32, 6>(p, st);
-    case 7: return expand_w<F32, 7>(p, st);
-    default: return expand_w<F32, 8>(p, st);
+    case 1: return expand_w<BASE, F32, 1>(p, st);
+    case 2: return expand_w<BASE, F32, 2>(p, st);
+    case 3: return expand_w<BASE, F32, 3>(p, st);
+    case 4: return expand_w<BASE, F32, 4>(p, st);
+    case 5: return expand_w<BASE, F32, 5>(p, st);
+    case 6: return expand_w<BASE, F32, 6>(p, st);
+    case 7: return expand_w<BASE, F32, 7>(p, st);
+    default: return expand_w<BASE, F32, 8>(p, st);
   }
 }
 }  // namespace
-hipError_t launch_expand(const ExpandParams& p, hipStream_t st) { return p.f32 ? expand_r<true>(p, st) : expand_r<false>(p, st); }
+hipError_t launch_expand(const ExpandParams& p, hipStream_t st) {
+  if (p.out_f32) return expand_r<kBaseF32, true>(p, st);
+  if (!p.base) return expand_r<kNoBase, false>(p, st);
+  return p.base_f32 ? expand_r<kBaseF32, false>(p, st) : expand_r<kBaseBf16, false>(p, st);
+}
 
 namespace {
-int grad_ranks(const GradParams& p) { return p.rp <= 16 ? 1 : p.rp <= 32 ? 2 : 4; }  // RB
-int grad_cols(const GradParams& p) {
+int grad_blocks(const GradParams& p) {
   int n = 0;
-  for (const GradPart& q : p.part) n += q.out ? (q.C + kGradCols - 1) / kGradCols : 0;
+  for (int i = 0; i < p.parts; ++i) n += (p.part[i].C + kGradCols - 1) / kGradCols;
   return n;
 }
-template <int RB>
+int grad_groups(const GradParams& p) { return (p.rp + 63) / 64; }  // 64 ranks a block (32 where that is all)
+template <int RK>
 hipError_t grad_t(const GradParams& p, hipStream_t st) {
-  const dim3 grid((unsigned)grad_cols(p), (unsigned)(p.req.n * ((p.r + 16 * RB - 1) / (16 * RB))), (unsigned)p.splits);
-  hipLaunchKernelGGL((grad_kernel<RB>), grid, dim3(64 * kGradWaves), 0, st, p);
+  const dim3 grid((unsigned)grad_blocks(p), (unsigned)(p.req.n * ((p.rp + 32 * RK - 1) / (32 * RK))), (unsigned)p.splits);
+  hipLaunchKernelGGL((grad_kernel<RK>), grid, dim3(kThreads), 0, st, p);
   return hipGetLastError();
 }
 }  // namespace
 int grad_splits(const GradParams& p) {
-  const int RB = grad_ranks(p);
-  const int64_t blocks = (int64_t)grad_cols(p) * std::min(p.req.n, p.req.count) * ((p.r + 16 * RB - 1) / (16 * RB));
+  const int64_t blocks = (int64_t)grad_blocks(p) * std::min(p.req.n, p.req.count) * grad_groups(p);
   if (!blocks) return 1;
   const int64_t want = (512 + blocks - 1) / blocks;                               // two blocks a CU
   const int64_t most = std::max<int64_t>(1, p.req.tokens / p.req.count / 128);    // of 128 tokens at least
   return (int)std::min(want, most);
 }
 hipError_t launch_adapter_grad(const GradParams& p, hipStream_t st) {
-  const int RB = grad_ranks(p);
-  const hipError_t e = RB == 1 ? grad_t<1>(p, st) : RB == 2 ? grad_t<2>(p, st) : grad_t<4>(p, st);
+  const hipError_t e = p.rp <= 32 ? grad_t<1>(p, st) : grad_t<2>(p, st);
   if (e != hipSuccess || p.splits == 1) return e;
-  const int64_t per = (int64_t)p.req.n * p.r;
-  const int64_t n0 = p.part[0].out ? per * p.part[0].C : 0, n1 = p.part[1].out ? per * p.part[1].C : 0;
-  const int64_t blocks = std::min<int64_t>((n0 + n1 + kThreads - 1) / kThreads, 4096);
-  hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, (const float*)p.work, p.splits, n0,
-                     n1, (bf16*)p.part[0].out, (bf16*)p.part[1].out);
+  const int64_t all = grad_values(p);
+  const int64_t blocks = std::min<int64_t>((all + kThreads - 1) / kThreads, 4096);
+  hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, st, p, all);
   return hipGetLastError();
 }
 
 hipError_t launch_transpose(const TransposeParams& p, hipStream_t st) {
-  auto tiles = [](const TransposePart& q) {
-    return q.src ? (int64_t)((q.rows + 63) / 64) * ((q.cols + 63) / 64) : 0;
-  };
-  const int64_t t0 = tiles(p.part[0]), t1 = tiles(p.part[1]);
-  hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)(t0 + t1), (unsigned)std::min(p.n, 65535)), dim3(kThreads), 0, st,
-                     p, (int)t0);
+  int64_t tiles = 0;
+  for (int i = 0; i < p.parts; ++i)
+    tiles += (int64_t)((std::max(p.part[i].rows, p.part[i].fill) + 63) / 64) * ((p.part[i].cols + 63) / 64);
+  hipLaunchKernelGGL(transpose_kernel, dim3((unsigned)tiles, (unsigned)std::min(p.n, 65535)), dim3(kThreads), 0, st, p);
   return hipGetLastError();
 }
 

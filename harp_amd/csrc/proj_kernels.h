@@ -6,6 +6,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "../../include/harp_qk_norm_rope.h"
+#include "req_kernels.h"
+
 namespace harp_proj {
 
 constexpr int kHeadDim = 128;       // features of one head (one wave's share)
@@ -48,5 +51,20 @@ struct ProjParams {
 constexpr int kProjLdsBytes = 144 * 1024;
 
 hipError_t launch_proj(const ProjParams& p, hipStream_t stream);
+
+// Low-rank adapters beside the projections: output i of token m gets t[m] B^T of
+// its request's adapter, t as launch_shrink writes its pairs.  The results are
+// rounded once, to nearest, after norm and rotation.
+struct ProjLow {
+  harp_req::Requests req;
+  int r, rp;
+  const uint16_t* t[kMaxOuts];  // [M, 2 rp] bf16 pairs
+  const uint16_t* b[kMaxOuts];  // [n, n_out, r] bf16
+};
+hipError_t launch_proj_low(const ProjParams& p, const ProjLow& low, hipStream_t stream);
+
+// harp_qkv_project's checks (qk_abi.hip): fills p, or returns a status with the message set
+int fill_params(ProjParams& p, const void* x, int64_t ld_x, int batch, int seq, int k_dim, int n_out,
+                const float* freqs, int64_t f_stride_b, int64_t f_stride_s, const harp_qkv_out_t* outs, int n_outs);
 
 }  // namespace harp_proj

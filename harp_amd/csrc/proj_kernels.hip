@@ -44,6 +44,13 @@
 //            where the large blocks fill 45, and reads the 88 MB of weights at
 //            2.6 TB/s: 83 -> 34 us.
 // launch_proj has the rule.
+// Low-rank adapters (LOW): token m of a request with an adapter also takes t[m]
+// B^T, t = x A^T beforehand.  The contraction runs on over it: behind the last
+// tile of K, for each request among the block's tokens a tile of t's two bf16
+// parts (zeros for the other requests' tokens) meets the same columns of B twice.
+// That is one tile per request up to rank 32 against K / 64 of the projection, and
+// no other pass over q, k and v; each result is then rounded once, to nearest,
+// behind the norm and the rotation, in fp32 until there.
 // Pipeline: one barrier per tile, in its last k-step, after which nobody
 // reads tile t's stage any more (its last fragments are in registers) and
 // tile t + 1 is complete; the copies of tile t + stages then go into tile t's
@@ -51,6 +58,7 @@
 // before their tile to land.  Fragment reads run on across tile boundaries.
 #include "proj_kernels.h"
 #include "ra_common.h"
+#include "req_device.h"
 
 namespace harp_proj {
 
@@ -107,6 +115,19 @@ __device__ __forceinline__ float half_wave_sum(float x) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // to nearest
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = {(bf16)lo, (bf16)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+
+template <bool LOW>
+struct LowArg {};
+template <>
+struct LowArg<true> {
+  ProjLow v;
+};
+
 template <int NJ>
 struct Frags {
   bf16x8 a[4];   // W rows: 32 features each (the wave's head)
@@ -117,8 +138,8 @@ struct Frags {
 
 // TPW tokens per wave, HEADS heads per block, STAGES tiles in LDS; TAIL: the
 // blocks are parts (of 128 tokens x HEADS heads) of the main grid's last units
-template <int TPW, int HEADS, int STAGES, bool TAIL>
-__global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(ProjParams p) {
+template <int TPW, int HEADS, int STAGES, bool TAIL, bool LOW>
+__global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(ProjParams p, LowArg<LOW> low) {
   constexpr int kWaves = kTokenGroups * HEADS;
   constexpr int kFeatures = HEADS * kHeadDim;
   constexpr int kWBytes = kFeatures * kRowBytes;          // 16 KB per head
@@ -320,6 +341,47 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
   // the last tiles issued (empty) copies; none may still write the LDS when
   // the workgroup ends
   wait_lds_loads();
+  if constexpr (LOW) {
+    const ProjLow& lo = low.v;
+    const uint16_t* const tb = (y == 0 ? lo.t[0] : y == 1 ? lo.t[1] : lo.t[2]) + (int64_t)m0 * 2 * lo.rp;
+    const uint16_t* const bb = y == 0 ? lo.b[0] : y == 1 ? lo.b[1] : lo.b[2];
+    const int tr = lane >> 3, tc = lane & 7;  // row and position of this lane in a copy's 8 rows
+    const int chunks = lo.rp / 4, half = lo.rp / 8;  // 16-byte chunks of a token's parts, of one part
+    int seg = harp_req::last_segment(lo.req, [&](int i) { return harp_req::segment_start(lo.req, i) <= m0; });
+    for (int start = harp_req::segment_start(lo.req, seg); start < m0 + rows_x && seg <= lo.req.count; ++seg) {
+      const int end = harp_req::segment_start(lo.req, seg + 1);
+      const int first = max(start, m0), adapter = seg ? harp_req::adapter_of(lo.req, seg - 1) : -1;
+      start = end;
+      if (adapter < 0 || first >= end) continue;
+      const rsrc_t tr_rsrc = make_rsrc(tb, (uint32_t)(rows_x * lo.rp * 4));
+      const rsrc_t b_rsrc = make_rsrc(bb + ((int64_t)adapter * p.heads + h0) * kHeadDim * lo.r,
+                                      (uint32_t)(rows_w * lo.r * 2));
+      for (int c0 = 0; c0 < chunks; c0 += 8) {
+        // every wave has read the last tile's fragments
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kXPerWave; ++k) {
+          const int r = (wave + kWaves * k) * 8 + tr, c = c0 + tile_pos(r, tc), m = m0 + r;
+          const bool in = m >= first && m < end && c < chunks;
+          lds_dma_b128(tr_rsrc, lds_wave + kWaves * k * 1024, in ? (uint32_t)(r * lo.rp * 4 + c * 16) : harp_ra::kOOB);
+        }
+#pragma unroll
+        for (int k = 0; k < kWPerWave; ++k) {
+          const int r = (wave + kWaves * k) * 8 + tr, c = c0 + tile_pos(r, tc), cb = c < half ? c : c - half;
+          const bool in = c < chunks && cb * 8 < lo.r;
+          lds_dma_b128(b_rsrc, lds_wave + STAGES * kXBytes + kWaves * k * 1024,
+                       in ? (uint32_t)(r * lo.r * 2 + cb * 16) : harp_ra::kOOB);
+        }
+        wait_lds_loads();
+        __syncthreads();
+        const int steps = min(4, (chunks - c0 + 1) / 2);
+        for (int ks = 0; ks < steps; ++ks) {
+          const Frags<NJ> f = load(0, ks);
+          mma(f, false, {}, {}, 0);
+        }
+      }
+    }
+  }
   if (norm && tid < kHeadDim) norm_wf[tid] = wreg;
   // every wave is past its fragment reads: the stages become staging rows
   __syncthreads();
@@ -329,12 +391,14 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
   const int h = h0 + hh;
   if (h >= p.heads) return;
   const int lane_e = harp_ra::lane_id_fresh(), l32e = lane_e & 31, ge = lane_e >> 5;
+  if constexpr (!LOW) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = round_bf16(acc[i][j][r]);
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = round_bf16(acc[i][j][r]);
+  }
 
   // Output stores go through LDS: the wave's TPW rows of 256 bytes (its
   // head's 128 bf16 features per token), 16-byte chunk c of row r at position
@@ -354,6 +418,8 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
       if (m < p.M) *(uint4*)(base + m * o.ldy + h * kHeadDim + c * 8) = v;
     }
   };
+  // two results: exact in bf16 or truncated to it, or (LOW) rounded to nearest
+  auto pair = [](float a, float b) { return LOW ? pack_bf16(a, b) : bf16_bits(a) | (bf16_bits(b) << 16); };
   auto put_rounded = [&]() {  // the bf16 products
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
@@ -361,8 +427,8 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          stage_put(j, i, q, bf16_bits(acc[i][j][4 * q]) | (bf16_bits(acc[i][j][4 * q + 1]) << 16),
-                    bf16_bits(acc[i][j][4 * q + 2]) | (bf16_bits(acc[i][j][4 * q + 3]) << 16));
+          stage_put(j, i, q, pair(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
+                    pair(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]));
   };
   if (!norm) {
     put_rounded();
@@ -417,8 +483,10 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
         const f32x4 w = *(const f32x4*)(norm_wf + d0);
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          y[e] = bf16_bits_to_f32(f32_to_bf16_trunc(__fmul_rn(__fmul_rn(acc[i][j][4 * q + e], inv), w[e])));
+        for (int e = 0; e < 4; ++e) {
+          y[e] = __fmul_rn(__fmul_rn(acc[i][j][4 * q + e], inv), w[e]);
+          if constexpr (!LOW) y[e] = bf16_bits_to_f32(f32_to_bf16_trunc(y[e]));
+        }
         if (rope) {
           // pairs (d0, d0 + 1) and (d0 + 2, d0 + 3): RoPE pairs d0 / 2 and d0 / 2 + 1
           const f32x4 f = fq[i][q];
@@ -429,8 +497,7 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
             y[e + 1] = __builtin_fmaf(xi, cr, __fmul_rn(xr, ci));
           }
         }
-        stage_put(j, i, q, f32_to_bf16_trunc(y[0]) | (f32_to_bf16_trunc(y[1]) << 16),
-                  f32_to_bf16_trunc(y[2]) | (f32_to_bf16_trunc(y[3]) << 16));
+        stage_put(j, i, q, pair(y[0], y[1]), pair(y[2], y[3]));
       }
   }
   stage_flush(o.y);
@@ -450,26 +517,24 @@ int device_cus() {
 }
 
 // One grid over all outputs, every block TPW * 4 tokens x HEADS heads.
-template <int TPW, int HEADS, int STAGES>
-hipError_t launch_grid(ProjParams p, hipStream_t stream) {
+template <int TPW, int HEADS, int STAGES, bool LOW>
+hipError_t launch_grid(ProjParams p, const LowArg<LOW>& low, hipStream_t stream) {
   constexpr int kTok = kTokenGroups * TPW;
   p.n_lin = ((p.M + kTok - 1) / kTok) * ((p.heads + HEADS - 1) / HEADS);
   p.keep_last = p.tail_bid0 = p.n_lin;
-  hipLaunchKernelGGL((proj_kernel<TPW, HEADS, STAGES, false>), dim3((unsigned)p.n_lin, (unsigned)p.n_outs),
-                     dim3(64 * kTokenGroups * HEADS), 0, stream, p);
+  hipLaunchKernelGGL((proj_kernel<TPW, HEADS, STAGES, false, LOW>), dim3((unsigned)p.n_lin, (unsigned)p.n_outs),
+                     dim3(64 * kTokenGroups * HEADS), 0, stream, p, low);
   return hipGetLastError();
 }
 
 // Parts of the last r units of the 256-token x 2-head grid, as blocks of 128
 // tokens x HEADS heads.
-template <int HEADS, int STAGES>
-hipError_t launch_tail(const ProjParams& p, int r, hipStream_t stream) {
-  hipLaunchKernelGGL((proj_kernel<32, HEADS, STAGES, true>), dim3((unsigned)(4 / HEADS * r)),
-                     dim3(64 * kTokenGroups * HEADS), 0, stream, p);
+template <int HEADS, int STAGES, bool LOW>
+hipError_t launch_tail(const ProjParams& p, const LowArg<LOW>& low, int r, hipStream_t stream) {
+  hipLaunchKernelGGL((proj_kernel<32, HEADS, STAGES, true, LOW>), dim3((unsigned)(4 / HEADS * r)),
+                     dim3(64 * kTokenGroups * HEADS), 0, stream, p, low);
   return hipGetLastError();
 }
-
-}  // namespace
 
 // Which blocks.  Each kind is taken where one round of it covers the whole
 // grid, the smallest first: a round of the 128-token x 1-head blocks takes
@@ -483,24 +548,32 @@ hipError_t launch_tail(const ProjParams& p, int r, hipStream_t stream) {
 // most half full, the last round would idle half the CUs through a whole
 // block).  Against a whole round: 2048 tokens x 24 heads (32 units over) 142
 // -> 116 us, 2048 x 30 (104 over) 181 -> 159.
-hipError_t launch_proj(const ProjParams& p_in, hipStream_t stream) {
+template <bool LOW>
+hipError_t launch_t(const ProjParams& p_in, const LowArg<LOW>& low, hipStream_t stream) {
   ProjParams p = p_in;
   const int64_t cus = device_cus();
   const int64_t tiles128 = (int64_t)p.n_outs * ((p.M + 127) / 128);
-  if (tiles128 * p.heads <= cus) return launch_grid<32, 1, 4>(p, stream);
-  if (tiles128 * ((p.heads + 1) / 2) <= cus) return launch_grid<32, 2, 3>(p, stream);
+  if (tiles128 * p.heads <= cus) return launch_grid<32, 1, 4>(p, low, stream);
+  if (tiles128 * ((p.heads + 1) / 2) <= cus) return launch_grid<32, 2, 3>(p, low, stream);
   const int L = ((p.M + kBlockTokens - 1) / kBlockTokens) * ((p.heads + kBlockHeads - 1) / kBlockHeads);
   const int64_t units = (int64_t)p.n_outs * L;
   const int r = cus > 0 ? (int)(units % cus) : 0;
   const bool split = r > 0 && 2 * r <= cus && units > cus && r <= L;
-  if (!split) return launch_grid<64, 2, 2>(p, stream);
+  if (!split) return launch_grid<64, 2, 2>(p, low, stream);
   p.n_lin = L;
   p.keep_last = p.tail_bid0 = L - r;
-  hipLaunchKernelGGL((proj_kernel<64, 2, 2, false>), dim3((unsigned)L, (unsigned)p.n_outs),
-                     dim3(64 * kTokenGroups * 2), 0, stream, p);
+  hipLaunchKernelGGL((proj_kernel<64, 2, 2, false, LOW>), dim3((unsigned)L, (unsigned)p.n_outs),
+                     dim3(64 * kTokenGroups * 2), 0, stream, p, low);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  return 4 * r <= cus ? launch_tail<1, 4>(p, r, stream) : launch_tail<2, 3>(p, r, stream);
+  return 4 * r <= cus ? launch_tail<1, 4>(p, low, r, stream) : launch_tail<2, 3>(p, low, r, stream);
+}
+
+}  // namespace
+
+hipError_t launch_proj(const ProjParams& p, hipStream_t stream) { return launch_t(p, LowArg<false>{}, stream); }
+hipError_t launch_proj_low(const ProjParams& p, const ProjLow& low, hipStream_t stream) {
+  return launch_t(p, LowArg<true>{low}, stream);
 }
 
 }  // namespace harp_proj

@@ -10,6 +10,7 @@
 #include <utility>
 
 #include "../../include/harp_request_ops.h"
+#include "proj_kernels.h"
 #include "req_kernels.h"
 
 using namespace harp_req;
@@ -225,35 +226,37 @@ int check_matrix(const void* p, int64_t ld, int dtype, int cols, bool output, co
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-// the backward's workspace: u, B and A transposed, partial gradients
+// the backward's workspace: u of all sets, B and A transposed, partial gradients
 struct BackwardPlan {
-  GradParams grad;
+  bool together;  // the sets' parts of dx in one pass, their ranks one after the other
   size_t u, bt, at, part, total;  // offsets
 };
-BackwardPlan backward_plan(int tokens, int K, int N, int n, int rank, int count, bool dx, bool da, bool db) {
+BackwardPlan backward_plan(int tokens, int K, int N, int n, int rank, int count, int sets) {
   BackwardPlan w{};
   const size_t rp = rank_pad(rank);
-  w.grad.req.count = count;
-  w.grad.req.tokens = tokens;
-  w.grad.req.n = n;
-  w.grad.r = rank;
-  w.grad.rp = (int)rp;
-  // (the pointers tell which sums run; only whether they are NULL counts here)
-  w.grad.part[0].C = K;
-  w.grad.part[0].out = da ? (void*)1 : nullptr;
-  w.grad.part[1].C = N;
-  w.grad.part[1].out = db ? (void*)1 : nullptr;
-  w.grad.splits = grad_splits(w.grad);
+  GradParams g{};
+  g.req.count = count;
+  g.req.tokens = tokens;
+  g.req.n = n;
+  g.r = rank;
+  g.rp = (int)rp;
+  g.parts = 2 * sets;
+  for (int i = 0; i < sets; ++i) {
+    g.part[2 * i].C = K;
+    g.part[2 * i + 1].C = N;
+  }
+  w.together = (int)rp * sets <= kMaxRank;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t r = at;
     at += align256(bytes);
     return r;
   };
-  w.u = take(dx || da ? (size_t)tokens * rp * 4 : 0);
-  w.bt = take(dx || da ? (size_t)n * rank * N * 2 : 0);
-  w.at = take(dx ? (size_t)n * rank * K * 2 : 0);
-  w.part = take(w.grad.splits > 1 ? (size_t)w.grad.splits * n * rank * ((da ? K : 0) + (size_t)(db ? N : 0)) * 4 : 0);
+  w.u = take((size_t)tokens * rp * sets * 4);
+  w.bt = take((size_t)sets * n * rank * N * 2);
+  w.at = take((size_t)sets * n * rp * K * 2);
+  const int splits = grad_splits(g);
+  w.part = take(splits > 1 ? (size_t)splits * grad_values(g) * 4 : 0);
   w.total = at;
   return w;
 }
@@ -373,14 +376,12 @@ int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base,
   if (!t || !aligned(t, 16)) return fail(HARP_REQ_EINVAL, "t must be a 16-byte aligned device pointer");
   ShrinkParams s{};
   s.req = q;
-  s.x = x;
-  s.ldx = ld_x;
   s.K = k_dim;
   s.r = adapters->rank;
   s.rp = rank_pad(adapters->rank);
   s.ldt = s.rp;
   s.sets = 1;
-  s.set[0] = ShrinkSet{adapters->a, adapters->scales, t};
+  s.set[0] = ShrinkSet{adapters->a, adapters->scales, x, ld_x, t, nullptr};
   if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
   ExpandParams e{};
   e.req = q;
@@ -391,7 +392,7 @@ int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base,
   e.ld_base = ld_base;
   e.out = out;
   e.ld_out = ld_out;
-  e.f32 = dtype == kF32;
+  e.base_f32 = e.out_f32 = dtype == kF32;
   e.N = n_dim;
   e.r = s.r;
   e.rp = s.rp;
@@ -399,80 +400,176 @@ int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base,
 }
 
 size_t harp_req_adapter_backward_workspace_bytes(int tokens, int k_dim, int n_dim, int n, int rank, int count,
-                                                 int want_da, int want_db) {
+                                                 int n_sets) {
   const harp_req_adapters_t a{nullptr, nullptr, nullptr, n, rank};
   if (check_tokens(tokens) || check_adapters(&a, k_dim, n_dim, false)) return (size_t)-1;
-  if (count < 1 || count > kMaxCount) {
-    fail(HARP_REQ_EINVAL, "count=%d: 1 to 2^20", count);
+  if (count < 1 || count > kMaxCount || n_sets < 1 || n_sets > kMaxSets) {
+    fail(HARP_REQ_EINVAL, "count=%d: 1 to 2^20, n_sets=%d: 1 to %d", count, n_sets, kMaxSets);
     return (size_t)-1;
   }
-  return backward_plan(tokens, k_dim, n_dim, n, rank, count, true, want_da, want_db).total;
+  return backward_plan(tokens, k_dim, n_dim, n, rank, count, n_sets).total;
 }
 
-int harp_req_add_adapters_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, const float* t,
-                                   const harp_req_adapters_t* adapters, const harp_req_requests_t* requests, void* dx,
-                                   int64_t ld_dx, int add_to_dx, void* da, void* db, int tokens, int k_dim, int n_dim,
-                                   void* workspace, size_t workspace_bytes, void* stream) {
+int harp_req_add_adapters_backward(const harp_req_backward_set_t* sets, int n_sets, const void* x, int64_t ld_x,
+                                   const harp_req_requests_t* requests, float* dx_base, int64_t ld_dx_base, void* dx,
+                                   int64_t ld_dx, int tokens, int k_dim, int n_dim, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
   int rc;
   Requests q;
+  if (!sets || n_sets < 1 || n_sets > kMaxSets)
+    return fail(HARP_REQ_EINVAL, "sets must hold 1 to %d projections (got %d)", kMaxSets, n_sets);
   if ((rc = check_tokens(tokens))) return rc;
-  if ((rc = check_adapters(adapters, k_dim, n_dim, tokens > 0))) return rc;
-  if (tokens == 0 || (!dx && !da && !db)) return ok();  // (no token: the gradients of a and b are the caller's zeros)
-  if ((rc = check_requests(requests, tokens, adapters->n, q))) return rc;
-  if ((rc = check_matrix(dy, ld_dy, kBf16, n_dim, false, "dy"))) return rc;
-  if (da && (rc = check_matrix(x, ld_x, kBf16, k_dim, false, "x"))) return rc;
+  const int n = sets[0].adapters.n, r = sets[0].adapters.rank;
+  bool any_da = false, any_db = false;
+  for (int i = 0; i < n_sets; ++i) {
+    const harp_req_backward_set_t& s = sets[i];
+    if ((rc = check_adapters(&s.adapters, k_dim, n_dim, tokens > 0))) return rc;
+    if (s.adapters.n != n || s.adapters.rank != r)
+      return fail(HARP_REQ_EINVAL, "sets[%d]: %d adapters of rank %d, sets[0] has %d of rank %d", i, s.adapters.n,
+                  s.adapters.rank, n, r);
+    any_da |= s.da != nullptr;
+    any_db |= s.db != nullptr;
+  }
+  if (tokens == 0 || (!dx && !any_da && !any_db)) return ok();  // (no token: da and db are the caller's zeros)
+  if ((rc = check_requests(requests, tokens, n, q))) return rc;
+  for (int i = 0; i < n_sets; ++i) {
+    const harp_req_backward_set_t& s = sets[i];
+    if ((rc = check_matrix(s.dy, s.ld_dy, kBf16, n_dim, false, "dy"))) return rc;
+    if (!aligned(s.da, 2) || !aligned(s.db, 2)) return fail(HARP_REQ_EINVAL, "da and db must be aligned to their elements");
+    if (s.db && (!s.t || !aligned(s.t, 16))) return fail(HARP_REQ_EINVAL, "t must be a 16-byte aligned device pointer");
+  }
+  if (any_da && (rc = check_matrix(x, ld_x, kBf16, k_dim, false, "x"))) return rc;
   if (dx && (rc = check_matrix(dx, ld_dx, kBf16, k_dim, true, "dx"))) return rc;
-  if (!aligned(da, 2) || !aligned(db, 2)) return fail(HARP_REQ_EINVAL, "da and db must be aligned to their elements");
-  if (db && (!t || !aligned(t, 16))) return fail(HARP_REQ_EINVAL, "t must be a 16-byte aligned device pointer");
-  const int n = adapters->n, r = adapters->rank, rp = rank_pad(r);
-  BackwardPlan w = backward_plan(tokens, k_dim, n_dim, n, r, q.count, dx, da, db);
-  if (w.total && (!workspace || workspace_bytes < w.total))
+  if (dx && dx_base && (rc = check_matrix(dx_base, ld_dx_base, kF32, k_dim, true, "dx_base"))) return rc;
+  const int rp = rank_pad(r);
+  const BackwardPlan w = backward_plan(tokens, k_dim, n_dim, n, r, q.count, n_sets);
+  if (dx && !dx_base && n_sets > 1 && !w.together)
+    return fail(HARP_REQ_EINVAL, "%d sets of rank %d need a dx_base", n_sets, r);
+  if (!workspace || workspace_bytes < w.total)
     return fail(HARP_REQ_ENOMEM, "workspace of %zu bytes is smaller than the %zu bytes needed",
                 workspace ? workspace_bytes : (size_t)0, w.total);
   if (!aligned(workspace, 16)) return fail(HARP_REQ_EINVAL, "workspace must be 16-byte aligned");
   char* const ws = (char*)workspace;
   float* const u = (float*)(ws + w.u);
+  const int64_t ldu = (int64_t)rp * n_sets;
+  uint16_t* const bt = (uint16_t*)(ws + w.bt);
+  uint16_t* const at = (uint16_t*)(ws + w.at);
+  const size_t bt_set = (size_t)n * r * n_dim, at_set = (size_t)n * rp * k_dim;
   hipStream_t st = (hipStream_t)stream;
-  if (dx || da) {
+  if (dx || any_da) {
     TransposeParams tp{};
-    tp.n = n;
-    tp.part[0] = TransposePart{adapters->b, ws + w.bt, n_dim, r};
-    if (dx) tp.part[1] = TransposePart{adapters->a, ws + w.at, r, k_dim};
-    if ((rc = launched(launch_transpose(tp, st), "adapters' transpose"))) return rc;
     ShrinkParams s{};
+    tp.n = n;
     s.req = q;
-    s.x = dy;
-    s.ldx = ld_dy;
     s.K = n_dim;
     s.r = r;
     s.rp = rp;
-    s.ldt = rp;
-    s.sets = 1;
-    s.set[0] = ShrinkSet{ws + w.bt, adapters->scales, u};
+    s.ldt = ldu;
+    s.sets = n_sets;
+    s.apart = 1;
+    for (int i = 0; i < n_sets; ++i) {
+      const harp_req_backward_set_t& e = sets[i];
+      tp.part[tp.parts++] = TransposePart{e.adapters.b, bt + i * bt_set, n_dim, r, n_dim, 0};
+      if (dx) {
+        // rows of all sets' ranks side by side, or a matrix for each set
+        uint16_t* const to = w.together ? at + (size_t)i * rp : at + i * at_set;
+        tp.part[tp.parts++] = TransposePart{e.adapters.a, to, r, k_dim, w.together ? rp * n_sets : rp, rp};
+      }
+      s.set[i] = ShrinkSet{bt + i * bt_set, e.adapters.scales, e.dy, e.ld_dy, u + (size_t)i * rp, nullptr};
+    }
+    if ((rc = launched(launch_transpose(tp, st), "adapters' transpose"))) return rc;
     if ((rc = launched(launch_shrink(s, st), "adapters (dy B)"))) return rc;
   }
   if (dx) {
     ExpandParams e{};
     e.req = q;
-    e.t = u;
-    e.ldt = rp;
-    e.b = ws + w.at;
-    e.base = add_to_dx ? dx : nullptr;
-    e.ld_base = ld_dx;
-    e.out = dx;
-    e.ld_out = ld_dx;
+    e.ldt = ldu;
     e.N = k_dim;
-    e.r = r;
-    e.rp = rp;
-    if ((rc = launched(launch_expand(e, st), "adapters (u A)"))) return rc;
+    const int passes = w.together ? 1 : n_sets;
+    for (int i = 0; i < passes; ++i) {
+      e.t = u + (size_t)i * rp;
+      e.b = at + (w.together ? 0 : i * at_set);
+      e.r = e.rp = w.together ? rp * n_sets : rp;
+      e.base = dx_base;
+      e.ld_base = ld_dx_base;
+      e.base_f32 = 1;
+      e.out_f32 = i < passes - 1;
+      e.out = e.out_f32 ? (void*)dx_base : dx;
+      e.ld_out = e.out_f32 ? ld_dx_base : ld_dx;
+      if ((rc = launched(launch_expand(e, st), "adapters (u A)"))) return rc;
+    }
   }
-  if (!da && !db) return ok();
-  GradParams& g = w.grad;
+  if (!any_da && !any_db) return ok();
+  GradParams g{};
   g.req = q;
-  g.part[0] = GradPart{x, ld_x, u, rp, k_dim, 0, da};
-  g.part[1] = GradPart{dy, ld_dy, t, rp, n_dim, 1, db};
+  g.r = r;
+  g.rp = rp;
+  for (int i = 0; i < n_sets; ++i) {
+    const harp_req_backward_set_t& e = sets[i];
+    if (e.da) g.part[g.parts++] = GradPart{x, ld_x, u + (size_t)i * rp, ldu, k_dim, 0, e.da};
+    if (e.db) g.part[g.parts++] = GradPart{e.dy, e.ld_dy, e.t, rp, n_dim, 1, e.db};
+  }
+  // (the plan's workspace is for all sums; fewer of them may be split into more parts where it holds those)
+  const size_t room = w.total - w.part, one = (size_t)grad_values(g) * 4;
+  g.splits = grad_splits(g);
+  if ((size_t)g.splits * one > room) g.splits = room / one > 1 ? (int)(room / one) : 1;
   g.work = (float*)(ws + w.part);
   return launched(launch_adapter_grad(g, st), "adapters' gradients");
+}
+
+size_t harp_req_qkv_workspace_bytes(int tokens, int rank, int n_outs) {
+  if (check_tokens(tokens)) return (size_t)-1;
+  if (rank < 1 || rank > kMaxRank || n_outs < 1 || n_outs > kMaxSets) {
+    fail(HARP_REQ_EINVAL, "rank=%d: 1 to %d, n_outs=%d: 1 to %d", rank, kMaxRank, n_outs, kMaxSets);
+    return (size_t)-1;
+  }
+  return n_outs * align256((size_t)tokens * 2 * rank_pad(rank) * 2);
+}
+
+int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_dim, int n_out, const float* freqs,
+                         int64_t f_stride_b, int64_t f_stride_s, const harp_qkv_out_t* outs,
+                         const harp_req_adapters_t* adapters, int n_outs, const harp_req_requests_t* requests,
+                         float* const* t, void* workspace, size_t workspace_bytes, void* stream) {
+  harp_proj::ProjParams p;
+  static_assert(HARP_QK_EINVAL == HARP_REQ_EINVAL && HARP_QK_EUNSUPPORTED == HARP_REQ_EUNSUPPORTED, "status values");
+  int rc = harp_proj::fill_params(p, x, ld_x, batch, seq, k_dim, n_out, freqs, f_stride_b, f_stride_s, outs, n_outs);
+  if (rc) return fail(rc, "%s", harp_qk_last_error());
+  if ((int64_t)batch * seq > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "batch * seq > 2^28");
+  if (!adapters) return fail(HARP_REQ_EINVAL, "adapters is NULL");
+  const int tokens = batch * seq, n = adapters[0].n, r = adapters[0].rank;
+  for (int i = 0; i < n_outs; ++i) {
+    if ((rc = check_adapters(&adapters[i], k_dim, n_out, true))) return rc;
+    if (adapters[i].n != n || adapters[i].rank != r)
+      return fail(HARP_REQ_EINVAL, "adapters[%d]: %d of rank %d, adapters[0] are %d of rank %d", i, adapters[i].n,
+                  adapters[i].rank, n, r);
+    if (r % 8 || !aligned(adapters[i].b, 16))
+      return fail(HARP_REQ_EUNSUPPORTED, "rank=%d must be a multiple of 8, b 16-byte aligned", r);
+    if (t && !aligned(t[i], 16)) return fail(HARP_REQ_EINVAL, "t[%d] must be 16-byte aligned", i);
+  }
+  Requests q;
+  if ((rc = check_requests(requests, tokens, n, q))) return rc;
+  const size_t need = harp_req_qkv_workspace_bytes(tokens, r, n_outs);
+  if (!workspace || workspace_bytes < need)
+    return fail(HARP_REQ_ENOMEM, "workspace of %zu bytes is smaller than the %zu bytes needed",
+                workspace ? workspace_bytes : (size_t)0, need);
+  if (!aligned(workspace, 16)) return fail(HARP_REQ_EINVAL, "workspace must be 16-byte aligned");
+  const int rp = rank_pad(r);
+  ShrinkParams s{};
+  harp_proj::ProjLow low{};
+  s.req = low.req = q;
+  s.K = k_dim;
+  s.r = low.r = r;
+  s.rp = low.rp = rp;
+  s.ldt = rp;
+  s.sets = n_outs;
+  for (int i = 0; i < n_outs; ++i) {
+    uint16_t* const pairs = (uint16_t*)((char*)workspace + i * (need / n_outs));
+    s.set[i] = ShrinkSet{adapters[i].a, adapters[i].scales, x, ld_x, t ? t[i] : nullptr, pairs};
+    low.t[i] = pairs;
+    low.b[i] = (const uint16_t*)adapters[i].b;
+  }
+  if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
+  return launched(harp_proj::launch_proj_low(p, low, (hipStream_t)stream), "qkv projection with adapters");
 }
 
 }  // extern "C"

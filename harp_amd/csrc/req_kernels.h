@@ -93,21 +93,23 @@ struct Requests {
 };
 
 // t[m][0 .. rp - 1] = scale * x A^T of token m's adapter (zeros behind rank r;
-// rows without an adapter are not written), as fp32 or as a bf16 value and the
-// bf16 rounding of what it left out: [high part (rp) | low part (rp)].
+// rows without an adapter are not written), as fp32 (t), and as a bf16 value
+// with the bf16 rounding of what it left out (pairs: [rp high parts | rp low
+// parts] of each token); either may be NULL.  Up to three sets; one read of an x that they share.
 struct ShrinkSet {
   const void* a;       // bf16 [n, r, K]
   const float* scale;  // [n] or NULL (ones)
-  void* t;
+  const void* x;       // bf16 [tokens, K], row stride ldx
+  int64_t ldx;
+  float* t;  // row stride ldt
+  void* pairs;  // bf16, row stride 2 rp
 };
 struct ShrinkParams {
   Requests req;
-  const void* x;  // bf16 [tokens, K]
-  int64_t ldx;
   int K, r, rp;
-  int64_t ldt;  // elements (fp32, or bf16 with pairs)
-  int pairs;
+  int64_t ldt;
   int sets;
+  int apart;  // the sets have an x each
   ShrinkSet set[kMaxSets];
 };
 hipError_t launch_shrink(const ShrinkParams& p, hipStream_t stream);
@@ -115,48 +117,61 @@ hipError_t launch_shrink(const ShrinkParams& p, hipStream_t stream);
 // out[m][j] = base[m][j] + sum over ranks t[m][.] B[j][.]
 struct ExpandParams {
   Requests req;
-  const float* t;  // [tokens, rp]
+  const float* t;  // [tokens, rp], row stride ldt
   int64_t ldt;
   const void* b;  // bf16 [n, N, r]
   const void* base;  // [tokens, N] or NULL (zeros)
   int64_t ld_base;
   void* out;
   int64_t ld_out;
-  int f32;  // base and out are fp32 (bf16 otherwise)
+  int base_f32, out_f32;  // (bf16 otherwise); an fp32 result has an fp32 base
   int N, r, rp;
 };
 hipError_t launch_expand(const ExpandParams& p, hipStream_t stream);
 
-// ga[a][j][c] = sum over the tokens m of adapter a of v[m][j] x[m][c]; stored [n, r, C]
-// (or [n, C, r] with `cols_first`), bf16.  Two such sums run in one launch.
+// For each adapter a the sum over its tokens m of v[m][j] x[m][c]: out [n, r, C],
+// or [n, C, r] with `cols_first`, bf16.  Up to six such sums in one launch.
 struct GradPart {
   const void* x;  // bf16 [tokens, C]
   int64_t ldx;
-  const float* v;  // fp32 [tokens, rp]
+  const float* v;  // [tokens, rp]
   int64_t ldv;
   int C;
   int cols_first;
-  void* out;  // bf16, NULL = not wanted
+  void* out;
 };
+constexpr int kMaxGradParts = 2 * kMaxSets;
 struct GradParams {
   Requests req;
   int r, rp;
-  GradPart part[2];
+  int parts;
+  GradPart part[kMaxGradParts];
   int splits;   // each request's tokens in so many parts (grad_splits)
-  float* work;  // [splits][n][r][C of both parts] partial sums where splits > 1
+  float* work;  // [splits] of all outputs, one after the other, where splits > 1
 };
 int grad_splits(const GradParams& p);
+// values of all outputs
+__host__ __device__ inline int64_t grad_values(const GradParams& p) {
+  int64_t c = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxGradParts; ++i)
+    if (i < p.parts) c += p.part[i].C;
+  return c * p.req.n * p.r;
+}
 hipError_t launch_adapter_grad(const GradParams& p, hipStream_t stream);
 
-// dst[i][c][r] = src[i][r][c], bf16, n matrices of rows x cols; two in one launch
+// dst[i][c][r] = src[i][r][c], bf16, n matrices of rows x cols, dst's rows ld
+// values apart and zero from the source's rows up to `fill`
 struct TransposePart {
   const void* src;
   void* dst;
   int rows, cols;
+  int ld, fill;
 };
 struct TransposeParams {
   int n;
-  TransposePart part[2];
+  int parts;
+  TransposePart part[2 * kMaxSets];
 };
 hipError_t launch_transpose(const TransposeParams& p, hipStream_t stream);
 

@@ -4,7 +4,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
-#include <c10/core/Stream.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
@@ -28,12 +28,14 @@ inline void refuse_tangent(const at::Tensor& t, const char* library, const char*
 // While a graph of an earlier call is alive, a leaf keeps the accumulator node
 // of that graph, with the stream it was made on.  A backward captured on
 // another stream would have the engine wait across the two streams inside the
-// capture, which ends the process: such a call is refused while it can be.
-inline void check_capture(const OptTensor& t, const c10::Stream& current, const char* op, const char* name) {
+// capture, which ends the process: such a call is refused while it can be.  (The
+// current stream is asked for as the node did when it was made.)
+inline void check_capture(const OptTensor& t, const char* op, const char* name) {
   if (!given(t) || !t->requires_grad() || t->grad_fn()) return;
   const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
   if (!node) return;
   const auto made_on = node->stream();
+  const c10::Stream current = c10::impl::VirtualGuardImpl(t->device().type()).getStream(t->device());
   TORCH_CHECK(!made_on || *made_on == current, op, ": ", name,
               " belongs to a live autograd graph of another stream, so its gradient cannot be captured: delete that "
               "graph's tensors (an earlier step's outputs or loss) before the capture");

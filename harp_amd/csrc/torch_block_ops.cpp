@@ -223,8 +223,8 @@ class AddRMSNorm : public torch::autograd::Function<AddRMSNorm> {
   }
 };
 
-void check_capture(const OptTensor& t, const c10::Stream& current, const char* name) {
-  harp_torch::check_capture(t, current, "add_rms_norm", name);
+void check_capture(const OptTensor& t, const char* name) {
+  harp_torch::check_capture(t, "add_rms_norm", name);
 }
 
 void refuse_tangents(const at::Tensor& x, const OptTensor& residual, const OptTensor& weight) {
@@ -245,10 +245,9 @@ std::tuple<at::Tensor, at::Tensor> add_rms_norm_autograd(const at::Tensor& x, co
   }
   const c10::DeviceGuard guard(x.device());  // the capture of x's device
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
-    const c10::Stream current = c10::hip::getCurrentHIPStream(x.get_device()).unwrap();
-    check_capture(x, current, "x");
-    check_capture(residual, current, "residual");
-    check_capture(weight, current, "weight");
+    check_capture(x, "x");
+    check_capture(residual, "residual");
+    check_capture(weight, "weight");
   }
   auto out = AddRMSNorm::apply(x, residual, weight, eps);
   return {out[0], given(residual) ? out[1] : at::Tensor()};

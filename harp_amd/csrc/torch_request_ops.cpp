@@ -4,13 +4,15 @@
 //   qk_norm_rope    RMSNorm and rotation of queries and keys by their positions
 //   rope_table      the rotation's table
 //   add_adapters    low-rank adapters beside a projection's result
-//   check_capture   refuses leaves whose gradients cannot be captured
+//   qkv_adapters    the q/k/v producer with adapters beside its projections
 // The operators allocate their results and workspaces from PyTorch's allocator
 // and run on the current HIP stream of the input's device.  Implementations are
 // registered for the CUDA dispatch key (HIP tensors carry it); the CPU key
 // raises.  qk_norm_rope and add_adapters are differentiable (once, in reverse
-// mode); an argument with a forward-mode tangent raises.
+// mode), and so is qkv_adapters where its rotation is given as positions; an argument
+// with a forward-mode tangent raises.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -318,9 +320,8 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& q, co
   }
   const c10::DeviceGuard guard(q.device());
   if (capturing()) {
-    const c10::Stream current = c10::hip::getCurrentHIPStream(q.get_device()).unwrap();
     const char* const names[] = {"q", "k", "q_weight", "k_weight"};
-    for (int i = 0; i < 4; ++i) harp_torch::check_capture(leaves[i], current, "qk_norm_rope", names[i]);
+    for (int i = 0; i < 4; ++i) harp_torch::check_capture(leaves[i], "qk_norm_rope", names[i]);
   }
   auto out = QkNormRope::apply(q, k, positions, widths.vec(), theta.vec(), half, qw, kw, eps.vec());
   return {out[0], given(k) ? out[1] : at::Tensor()};
@@ -475,13 +476,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> adapters_backward(const at::Tenso
   if (none) return {dx, da, db};
   const Rows d = rows_of(dy, "dy");
   const size_t bytes = harp_req_adapter_backward_workspace_bytes(c.x.rows, c.x.cols, c.N, c.adapters.n, c.adapters.rank,
-                                                                 c.requests.count, want_a, want_b);
+                                                                 c.requests.count, 1);
   TORCH_CHECK(bytes != (size_t)-1, "harp_request.add_adapters: ", harp_req_last_error());
   work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
-  check_status(harp_req_add_adapters_backward(
-                   d.p, d.ld, c.x.p, c.x.ld, t.const_data_ptr<float>(), &c.adapters, &c.requests,
-                   want_x ? dx.data_ptr() : nullptr, c.x.cols, 0, want_a ? da.data_ptr() : nullptr,
-                   want_b ? db.data_ptr() : nullptr, c.x.rows, c.x.cols, c.N, work.data_ptr(), bytes, stream_of(x)),
+  const harp_req_backward_set_t set{c.adapters, t.const_data_ptr<float>(), d.p, d.ld, want_a ? da.data_ptr() : nullptr,
+                                    want_b ? db.data_ptr() : nullptr};
+  check_status(harp_req_add_adapters_backward(&set, 1, c.x.p, c.x.ld, &c.requests, nullptr, 0,
+                                              want_x ? dx.data_ptr() : nullptr, c.x.cols, c.x.rows, c.x.cols, c.N,
+                                              work.data_ptr(), bytes, stream_of(x)),
                "add_adapters (backward)");
   return {dx, da, db};
 }
@@ -550,21 +552,302 @@ at::Tensor add_adapters_autograd(const at::Tensor& base, const at::Tensor& x, co
               base.scalar_type());
   const c10::DeviceGuard guard(x.device());
   if (capturing()) {
-    const c10::Stream current = c10::hip::getCurrentHIPStream(x.get_device()).unwrap();
     const char* const names[] = {"base", "x", "a", "b"};
-    for (int i = 0; i < 4; ++i) harp_torch::check_capture(*leaves[i], current, "add_adapters", names[i]);
+    for (int i = 0; i < 4; ++i) harp_torch::check_capture(*leaves[i], "add_adapters", names[i]);
   }
   return AddAdapters::apply(base, x, a, b, scales, index, offsets);
 }
 
-// For an autograd Function in Python: the leaves of a call that is being captured
-void check_capture(const std::vector<at::Tensor>& leaves) {
-  for (const auto& t : leaves) {
-    if (!t.is_cuda()) continue;
-    const c10::DeviceGuard guard(t.device());
-    if (!capturing()) continue;
-    harp_torch::check_capture(t, c10::hip::getCurrentHIPStream(t.get_device()).unwrap(), "harp_request", "an argument");
+// ---------------------------------------------------------------------------
+// the q/k/v producer with adapters
+// ---------------------------------------------------------------------------
+constexpr int64_t kHeadDim = 128;
+
+using Tensors = std::vector<at::Tensor>;
+
+// The rotation of q and k: by a table (complex64 [S, 64] or [B or 1, S, 64]), or by
+// positions along axes of interleaved pairs, or none
+struct QkvCall {
+  AdapterCall first;           // x, requests, adapters[0]
+  harp_req_adapters_t adapters[3];
+  Tensors a, b, scales;        // kept alive
+  at::Tensor freqs;            // fp32 (cos, sin) rows
+  int64_t fsb = 0;
+  Tensors w, nw;               // projections, norm weights (undefined: none)
+  int64_t B = 0, S = 0, K = 0, N = 0, H = 0;
+};
+QkvCall qkv_call(const at::Tensor& x, const Tensors& weights, const Tensors& a, const Tensors& b,
+                 const c10::List<OptTensor>& scales, const at::Tensor& index, const OptTensor& offsets,
+                 const c10::List<OptTensor>& norm_weights, const OptTensor& freqs) {
+  TORCH_CHECK(x.dim() == 3, "x must be [B, S, dim], got ", x.sizes());
+  TORCH_CHECK(weights.size() == 3 && a.size() == 3 && b.size() == 3 && scales.size() == 3 && norm_weights.size() == 2,
+              "three weights with an adapter stack each, and two norm weights (or None)");
+  QkvCall c;
+  c.B = x.size(0);
+  c.S = x.size(1);
+  c.K = x.size(2);
+  c.N = weights[0].size(0);
+  c.H = c.N / kHeadDim;
+  TORCH_CHECK(c.N >= kHeadDim && c.N % kHeadDim == 0, "weights must have heads of 128 features, got ", c.N, " rows");
+  const at::Tensor xc = plain(x).contiguous();  // (its rows are read 16 bytes at a time)
+  c.first = adapter_call(xc, a[0], b[0], scales.get(0), index, offsets);
+  for (int i = 0; i < 3; ++i) {
+    TORCH_CHECK(a[i].sizes() == a[0].sizes() && b[i].sizes() == b[0].sizes(),
+                "adapters of q, k and v must have one number and one rank, got a ", a[0].sizes(), " and ", a[i].sizes());
+    const AdapterCall one = i ? adapter_call(xc, a[i], b[i], scales.get(i), index, offsets) : c.first;
+    TORCH_CHECK(one.N == c.N, "b must be [", a[0].size(0), ", ", c.N, ", ", a[0].size(1), "], got ", b[i].sizes());
+    c.adapters[i] = one.adapters;
+    c.a.push_back(one.a);
+    c.b.push_back(one.b);
+    c.scales.push_back(one.scales);
+    check_device(weights[i], x, "weight");
+    TORCH_CHECK(weights[i].scalar_type() == at::kBFloat16 && weights[i].dim() == 2 && weights[i].size(0) == c.N &&
+                    weights[i].size(1) == c.K && weights[i].stride(1) == 1,
+                "every weight must be a bfloat16 [", c.N, ", ", c.K, "] tensor with unit column stride, got ",
+                weights[i].scalar_type(), " ", weights[i].sizes());
+    c.w.push_back(plain(weights[i]));
+    at::Tensor nw;
+    const OptTensor n = i < 2 ? norm_weights.get(i) : OptTensor();
+    if (given(n)) {
+      check_device(*n, x, "norm weight");
+      TORCH_CHECK((n->scalar_type() == at::kBFloat16 || n->scalar_type() == at::kFloat) && n->dim() == 1 &&
+                      n->size(0) == kHeadDim,
+                  "norm weights must be bfloat16 or float32 [128], got ", n->scalar_type(), " ", n->sizes());
+      nw = plain(*n).contiguous();
+    }
+    c.nw.push_back(nw);
   }
+  if (given(freqs)) {
+    check_device(*freqs, x, "freqs_cis");
+    TORCH_CHECK(freqs->scalar_type() == at::kComplexFloat && (freqs->dim() == 2 || freqs->dim() == 3) &&
+                    freqs->size(-1) == kHeadDim / 2 && freqs->size(-2) == c.S &&
+                    (freqs->dim() == 2 || freqs->size(0) == 1 || freqs->size(0) == c.B),
+                "freqs_cis must be complex64 [S, 64] or [B, S, 64] with S=", c.S, ", got ", freqs->sizes());
+    c.freqs = at::view_as_real(freqs->resolve_conj()).contiguous();
+    c.fsb = freqs->dim() == 3 && freqs->size(0) > 1 ? c.freqs.stride(0) : 0;
+  }
+  return c;
+}
+
+struct QkvResult {
+  Tensors y;     // q, k, v [B, H, S, 128], token-major
+  Tensors lin;   // of q and k before the norm [B, S, N], with keep
+  Tensors t;     // x A^T of the three, with keep
+};
+QkvResult qkv_forward(const QkvCall& c, const at::Tensor& x, const std::vector<double>& eps, bool keep) {
+  TORCH_CHECK(eps.size() == 2, "eps must be two values, got ", eps.size());
+  const c10::DeviceGuard guard(x.device());
+  QkvResult r;
+  harp_qkv_out_t outs[3] = {};
+  float* t[3] = {};
+  for (int i = 0; i < 3; ++i) {
+    r.y.push_back(at::empty({c.B, c.S, c.N}, x.options()));
+    harp_qkv_out_t& o = outs[i];
+    o.weight = c.w[i].const_data_ptr();
+    o.ld_weight = c.w[i].stride(0);
+    o.y = r.y[i].data_ptr();
+    o.ld_y = c.N;
+    if (c.nw[i].defined()) {
+      o.norm_weight = c.nw[i].const_data_ptr();
+      o.norm_weight_dtype = c.nw[i].scalar_type() == at::kFloat ? HARP_QK_F32 : HARP_QK_BF16;
+      o.eps = (float)eps[i];
+      if (keep) {
+        r.lin.push_back(at::empty({c.B, c.S, c.N}, x.options()));
+        o.y_lin = r.lin.back().data_ptr();
+      }
+    } else {
+      TORCH_CHECK(!c.freqs.defined() || i == 2, "a rotation without its RMSNorm is the separate operator's");
+    }
+    if (keep) {
+      r.t.push_back(at::empty({c.B * c.S, harp_req_adapter_columns(c.adapters[0].rank)}, x.options().dtype(at::kFloat)));
+      t[i] = r.t[i].data_ptr<float>();
+    }
+  }
+  if (c.B * c.S) {
+    const size_t bytes = harp_req_qkv_workspace_bytes(c.first.x.rows, c.adapters[0].rank, 3);
+    TORCH_CHECK(bytes != (size_t)-1, "harp_request.qkv_adapters: ", harp_req_last_error());
+    const at::Tensor work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    check_status(
+        harp_req_qkv_project(c.first.x.p, c.first.x.ld, checked_int(c.B, "batch"), checked_int(c.S, "seq"),
+                             checked_int(c.K, "dim"), checked_int(c.N, "features"),
+                             c.freqs.defined() ? c.freqs.const_data_ptr<float>() : nullptr, c.fsb, kHeadDim, outs,
+                             c.adapters, 3, &c.first.requests, keep ? t : nullptr, work.data_ptr(), bytes, stream_of(x)),
+        "qkv_adapters");
+  }
+  for (auto& y : r.y) y = y.unflatten(-1, {c.H, kHeadDim}).transpose(1, 2);
+  return r;
+}
+
+at::Tensor table_of(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta,
+                    const at::Tensor& x) {
+  TORCH_CHECK(x.dim() == 3, "x must be [B, S, dim], got ", x.sizes());
+  check_device(positions, x, "positions");
+  positions_of(positions, (int64_t)widths.size(), x.size(0), x.size(1));  // (their shape)
+  int64_t D = 0;
+  for (int64_t w : widths) D += w;
+  TORCH_CHECK(D == kHeadDim, "the axes' widths must add up to 128, got ", widths);
+  return rope_table(positions, widths, theta);
+}
+
+Tensors qkv_adapters(const at::Tensor& x, const Tensors& weights, const Tensors& a, const Tensors& b,
+                     const c10::List<OptTensor>& scales, const at::Tensor& index, const OptTensor& offsets,
+                     const c10::List<OptTensor>& norm_weights, const std::vector<double>& eps, const OptTensor& freqs,
+                     const OptTensor& positions, const std::vector<int64_t>& widths, const std::vector<double>& theta) {
+  TORCH_CHECK(x.is_cuda(), "harp_request.qkv_adapters: tensors must be on a HIP device");
+  TORCH_CHECK(!given(freqs) || !given(positions), "one rotation: freqs_cis or positions");
+  const OptTensor table = given(positions) ? OptTensor(table_of(*positions, widths, theta, x)) : freqs;
+  return qkv_forward(qkv_call(x, weights, a, b, scales, index, offsets, norm_weights, table), x, eps, false).y;
+}
+
+// Differentiable arguments in this order: x, three weights, two norm weights, three a, three b
+class QkvAdapters : public torch::autograd::Function<QkvAdapters> {
+ public:
+  static constexpr int kLeaves = 12;
+
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                const at::Tensor& wq, const at::Tensor& wk, const at::Tensor& wv,
+                                                const at::Tensor& nq, const at::Tensor& nk, const at::Tensor& aq,
+                                                const at::Tensor& ak, const at::Tensor& av, const at::Tensor& bq,
+                                                const at::Tensor& bk, const at::Tensor& bv,
+                                                c10::List<OptTensor> scales, const at::Tensor& index,
+                                                const OptTensor& offsets, std::vector<double> eps,
+                                                const at::Tensor& positions, std::vector<int64_t> widths,
+                                                std::vector<double> theta) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    c10::List<OptTensor> norms;
+    norms.push_back(nq);
+    norms.push_back(nk);
+    const at::Tensor table = table_of(positions, widths, theta, x);
+    const QkvCall c = qkv_call(x, {wq, wk, wv}, {aq, ak, av}, {bq, bk, bv}, scales, index, offsets, norms, table);
+    const QkvResult r = qkv_forward(c, x, eps, true);
+    int64_t wanted = 0;
+    const at::Tensor* const leaves[] = {&x, &wq, &wk, &wv, &nq, &nk, &aq, &ak, &av, &bq, &bk, &bv};
+    for (int i = 0; i < kLeaves; ++i) wanted |= (int64_t)leaves[i]->requires_grad() << i;
+    ctx->saved_data["wanted"] = wanted;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["widths"] = widths;
+    ctx->saved_data["theta"] = theta;
+    auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
+    ctx->save_for_backward({x, wq, wk, wv, nq, nk, aq, ak, av, bq, bk, bv, or_none(scales.get(0)),
+                            or_none(scales.get(1)), or_none(scales.get(2)), index, or_none(offsets), positions,
+                            r.lin[0], r.lin[1], r.t[0], r.t[1], r.t[2]});
+    return {r.y[0], r.y[1], r.y[2]};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const int64_t wanted = ctx->saved_data["wanted"].toInt();
+    auto want = [&](int i) { return (wanted >> i & 1) != 0; };
+    for (const auto& t : grads) harp_torch::refuse_tangent(t, "harp_request", "qkv_adapters (backward)");
+    torch::autograd::variable_list out(19);
+    {
+      at::AutoDispatchBelowADInplaceOrView guard;
+      const at::Tensor &x = s[0], &index = s[15];
+      const c10::DeviceGuard device(x.device());
+      const int64_t B = x.size(0), S = x.size(1), K = x.size(2), N = s[1].size(0), H = N / kHeadDim, M = B * S;
+      // through the rotation and the norm: the gradients of the three products [M, N]
+      const RopeCall rope = rope_call(ctx->saved_data["widths"].toIntVector(),
+                                      ctx->saved_data["theta"].toDoubleVector(), false,
+                                      ctx->saved_data["eps"].toDoubleVector());
+      auto heads = [&](const at::Tensor& t) { return t.unflatten(-1, {H, kHeadDim}).transpose(1, 2); };
+      const at::Tensor d[2] = {grads[0], grads[1]}, lin[2] = {heads(s[18]), heads(s[19])}, nw[2] = {s[4], s[5]};
+      const bool want_nw[2] = {want(4), want(5)};
+      auto g = rope_backward(d, lin, nw, s[17], rope, want_nw);
+      out[4] = g[2];
+      out[5] = g[3];
+      auto rows = [&](const at::Tensor& t) { return t.transpose(1, 2).reshape({M, N}); };
+      const at::Tensor gy[3] = {rows(g[0]), rows(g[1]), rows(plain(grads[2]))};
+      const at::Tensor x2 = plain(x).reshape({M, K});
+      for (int i = 0; i < 3; ++i)
+        if (want(1 + i)) out[1 + i] = at::mm(gy[i].t(), x2);
+      bool low = want(0);
+      for (int i = 6; i < kLeaves; ++i) low |= want(i);
+      if (low) {
+        harp_req_backward_set_t sets[3];
+        std::vector<AdapterCall> calls;
+        std::vector<Rows> dys;
+        for (int i = 0; i < 3; ++i) {
+          const at::Tensor &a = s[6 + i], &b = s[9 + i];
+          calls.push_back(adapter_call(x, a, b, s[12 + i].defined() ? OptTensor(s[12 + i]) : OptTensor(), index,
+                                       s[16].defined() ? OptTensor(s[16]) : OptTensor()));
+          dys.push_back(rows_of(gy[i], "dy"));
+          // (without a token the sums are empty)
+          if (want(6 + i)) out[6 + i] = M ? at::empty(a.sizes(), a.options()) : at::zeros(a.sizes(), a.options());
+          if (want(9 + i)) out[9 + i] = M ? at::empty(b.sizes(), b.options()) : at::zeros(b.sizes(), b.options());
+          sets[i] = {calls[i].adapters,
+                     s[20 + i].const_data_ptr<float>(),
+                     dys[i].p,
+                     dys[i].ld,
+                     want(6 + i) ? out[6 + i].data_ptr() : nullptr,
+                     want(9 + i) ? out[9 + i].data_ptr() : nullptr};
+        }
+        at::Tensor dx, base;
+        if (want(0)) {
+          // the projections' part, added up in 32 bits; the adapters' kernel adds its own and rounds
+          dx = at::empty({B, S, K}, x.options());
+          if (M) {
+            base = at::mm(gy[0], s[1], at::kFloat);
+            for (int i = 1; i < 3; ++i) base = at::addmm(base, gy[i], s[1 + i], at::kFloat);
+          }
+        }
+        if (M) {
+          const size_t bytes = harp_req_adapter_backward_workspace_bytes(
+              (int)M, (int)K, (int)N, calls[0].adapters.n, calls[0].adapters.rank, calls[0].requests.count, 3);
+          TORCH_CHECK(bytes != (size_t)-1, "harp_request.qkv_adapters: ", harp_req_last_error());
+          const at::Tensor work = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+          check_status(harp_req_add_adapters_backward(sets, 3, calls[0].x.p, calls[0].x.ld, &calls[0].requests,
+                                                      base.defined() ? base.data_ptr<float>() : nullptr, K,
+                                                      dx.defined() ? dx.data_ptr() : nullptr, K, (int)M, (int)K, (int)N,
+                                                      work.data_ptr(), bytes, stream_of(x)),
+                       "qkv_adapters (backward)");
+        }
+        out[0] = dx;
+      }
+    }
+    harp_torch::once_only(out, "qkv_adapters");
+    return out;
+  }
+};
+
+Tensors qkv_adapters_autograd(const at::Tensor& x, const Tensors& weights, const Tensors& a, const Tensors& b,
+                              const c10::List<OptTensor>& scales, const at::Tensor& index, const OptTensor& offsets,
+                              const c10::List<OptTensor>& norm_weights, const std::vector<double>& eps,
+                              const OptTensor& freqs, const OptTensor& positions, const std::vector<int64_t>& widths,
+                              const std::vector<double>& theta) {
+  Tensors leaves = {x};
+  leaves.insert(leaves.end(), weights.begin(), weights.end());
+  for (size_t i = 0; i < norm_weights.size(); ++i) leaves.push_back(given(norm_weights.get(i)) ? *norm_weights.get(i) : at::Tensor());
+  leaves.insert(leaves.end(), a.begin(), a.end());
+  leaves.insert(leaves.end(), b.begin(), b.end());
+  for (const auto& t : leaves) harp_torch::refuse_tangent(t, "harp_request", "qkv_adapters");
+  for (size_t i = 0; i < scales.size(); ++i) {
+    if (given(scales.get(i))) harp_torch::refuse_tangent(*scales.get(i), "harp_request", "qkv_adapters");
+    refuse_grad(scales.get(i), "qkv_adapters", "scales");
+  }
+  for (const OptTensor& t : {freqs, positions}) {
+    if (given(t)) harp_torch::refuse_tangent(*t, "harp_request", "qkv_adapters");
+    refuse_grad(t, "qkv_adapters", "the rotation");
+  }
+  bool record = false;
+  for (const auto& t : leaves) record |= t.defined() && t.requires_grad();
+  if (!record || !at::GradMode::is_enabled()) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("harp_request::qkv_adapters", "")
+                               .typed<decltype(qkv_adapters)>();
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return op.call(x, weights, a, b, scales, index, offsets, norm_weights, eps, freqs, positions, widths, theta);
+  }
+  TORCH_CHECK(x.is_cuda(), "harp_request.qkv_adapters: this library runs on a HIP device only (CPU tensors given)");
+  TORCH_CHECK(leaves.size() == QkvAdapters::kLeaves && given(positions) && leaves[4].defined() && leaves[5].defined(),
+              "harp_request.qkv_adapters: gradients need both norm weights, and the rotation as positions");
+  const c10::DeviceGuard guard(x.device());
+  if (capturing()) {
+    for (const auto& t : leaves) harp_torch::check_capture(t, "qkv_adapters", "an argument");
+  }
+  const Tensors& l = leaves;
+  return QkvAdapters::apply(l[0], l[1], l[2], l[3], l[4], l[5], l[6], l[7], l[8], l[9], l[10], l[11], scales, index,
+                            offsets, eps, *positions, widths, theta);
 }
 
 [[noreturn]] void no_cpu(const char* op) {
@@ -579,6 +862,11 @@ at::Tensor rope_table_cpu(const at::Tensor&, at::IntArrayRef, at::ArrayRef<doubl
 at::Tensor add_adapters_cpu(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                             const OptTensor&, const at::Tensor&, const OptTensor&) {
   no_cpu("add_adapters");
+}
+Tensors qkv_adapters_cpu(const at::Tensor&, const Tensors&, const Tensors&, const Tensors&, const c10::List<OptTensor>&,
+                         const at::Tensor&, const OptTensor&, const c10::List<OptTensor>&, const std::vector<double>&,
+                         const OptTensor&, const OptTensor&, const std::vector<int64_t>&, const std::vector<double>&) {
+  no_cpu("qkv_adapters");
 }
 std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd_cpu(const at::Tensor& q, const OptTensor& k,
                                                              const at::Tensor& positions, at::IntArrayRef,
@@ -604,29 +892,36 @@ TORCH_LIBRARY(harp_request, m) {
   m.def(
       "add_adapters(Tensor base, Tensor x, Tensor a, Tensor b, Tensor? scales, Tensor index, Tensor? offsets) -> "
       "Tensor");
-  m.def("check_capture(Tensor[] leaves) -> ()", &check_capture);
+  m.def(
+      "qkv_adapters(Tensor x, Tensor[] weights, Tensor[] a, Tensor[] b, Tensor?[] scales, Tensor index, Tensor? "
+      "offsets, Tensor?[] norm_weights, float[] eps, Tensor? freqs_cis, Tensor? positions, int[] widths, float[] "
+      "theta) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(harp_request, AutogradCUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_autograd);
   m.impl("rope_table", &rope_table_autograd);
   m.impl("add_adapters", &add_adapters_autograd);
+  m.impl("qkv_adapters", &qkv_adapters_autograd);
 }
 
 TORCH_LIBRARY_IMPL(harp_request, AutogradCPU, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_autograd_cpu);
   m.impl("rope_table", &rope_table_autograd);
   m.impl("add_adapters", &add_adapters_autograd_cpu);
+  m.impl("qkv_adapters", &qkv_adapters_autograd);
 }
 
 TORCH_LIBRARY_IMPL(harp_request, CUDA, m) {
   m.impl("qk_norm_rope", &qk_norm_rope);
   m.impl("rope_table", &rope_table);
   m.impl("add_adapters", &add_adapters);
+  m.impl("qkv_adapters", &qkv_adapters);
 }
 
 TORCH_LIBRARY_IMPL(harp_request, CPU, m) {
   m.impl("qk_norm_rope", &qk_norm_rope_cpu);
   m.impl("rope_table", &rope_table_cpu);
   m.impl("add_adapters", &add_adapters_cpu);
+  m.impl("qkv_adapters", &qkv_adapters_cpu);
 }

@@ -26,6 +26,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "harp_qk_norm_rope.h"
+
 #ifndef HARP_REQ_API
 #define HARP_REQ_API __attribute__((visibility("default")))
 #endif
@@ -151,18 +153,47 @@ HARP_REQ_API int harp_req_add_adapters_forward(const void* x, int64_t ld_x, cons
                                                int n_dim, void* stream);
 
 /*
- * From dy bf16 [tokens, N] and the forward's t: dx bf16 [tokens, K] (zeros for the tokens without an
- * adapter), da and db of a's and b's shapes (zeros for adapters without a token); each NULL = not wanted.
- * (The gradient of base is dy.)  add_to_dx: dx holds a gradient already, which the adapters' part is added to.
- * workspace: harp_req_adapter_backward_workspace_bytes, 16-byte aligned.
+ * The gradients of one to three projections of one x, each with adapters of one n
+ * and one rank: from dy bf16 [tokens, N] and the forward's t of each, da and db of a's
+ * and b's shapes (zeros for adapters without a token; NULL = not wanted), and dx bf16
+ * [tokens, K], the sum of all of them plus dx_base (NULL: zeros), or NULL.  (The
+ * gradient of base is dy.)  dx_base: fp32 [tokens, K], written over where the ranks (rounded up
+ * to 16) of all sets exceed 128 together; such calls with more than one set need it.  workspace:
+ * harp_req_adapter_backward_workspace_bytes, 16-byte aligned, free again when the launches
+ * behind this call have run.
  */
-HARP_REQ_API int harp_req_add_adapters_backward(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x,
-                                                const float* t, const harp_req_adapters_t* adapters,
-                                                const harp_req_requests_t* requests, void* dx, int64_t ld_dx,
-                                                int add_to_dx, void* da, void* db, int tokens, int k_dim, int n_dim,
-                                                void* workspace, size_t workspace_bytes, void* stream);
+typedef struct {
+  harp_req_adapters_t adapters;
+  const float* t;
+  const void* dy;
+  int64_t ld_dy;
+  void* da;
+  void* db;
+} harp_req_backward_set_t;
+
+HARP_REQ_API int harp_req_add_adapters_backward(const harp_req_backward_set_t* sets, int n_sets, const void* x,
+                                                int64_t ld_x, const harp_req_requests_t* requests, float* dx_base,
+                                                int64_t ld_dx_base, void* dx, int64_t ld_dx, int tokens, int k_dim,
+                                                int n_dim, void* workspace, size_t workspace_bytes, void* stream);
 HARP_REQ_API size_t harp_req_adapter_backward_workspace_bytes(int tokens, int k_dim, int n_dim, int n, int rank,
-                                                              int count, int want_da, int want_db);
+                                                              int count, int n_sets);
+
+/*
+ * harp_qkv_project (harp_qk_norm_rope.h) with low-rank adapters beside its
+ * projections, in one launch behind the one for x A^T: adapters[i] goes with outs[i]
+ * (a [n, rank, k_dim], b [n, n_out, rank]; one n and one rank, a multiple of 8 up to
+ * 128).  Arithmetic is fp32 from the products to the result, rounded once, to nearest
+ * (harp_qkv_project truncates behind the norm and the rotation); y_lin is the rounded
+ * product with its adapter.  t (n_outs pointers, or NULL): each fp32 [tokens,
+ * harp_req_adapter_columns(rank)], as for harp_req_add_adapters_forward.  workspace:
+ * harp_req_qkv_workspace_bytes, 16-byte aligned.  batch * seq up to 2^28.
+ */
+HARP_REQ_API int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_dim, int n_out,
+                                      const float* freqs, int64_t f_stride_b, int64_t f_stride_s,
+                                      const harp_qkv_out_t* outs, const harp_req_adapters_t* adapters, int n_outs,
+                                      const harp_req_requests_t* requests, float* const* t, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+HARP_REQ_API size_t harp_req_qkv_workspace_bytes(int tokens, int rank, int n_outs);
 
 HARP_REQ_API const char* harp_req_last_error(void);
 

@@ -41,7 +41,7 @@ def test_structures_have_the_header_s_layout(tmp_path):
     """sizeof and the last member's offset of each structure, from a C compiler."""
     pairs = {"harp_req_axes_t": (_lib.ReqAxes, "half"), "harp_req_positions_t": (_lib.ReqPositions, "stride_a"),
              "harp_req_heads_t": (_lib.ReqHeads, "grad_weight"), "harp_req_requests_t": (_lib.ReqRequests, "count"),
-             "harp_req_adapters_t": (_lib.ReqAdapters, "rank")}
+             "harp_req_adapters_t": (_lib.ReqAdapters, "rank"), "harp_req_backward_set_t": (_lib.ReqBackwardSet, "db")}
     body = "".join(f'printf("%zu %zu\\n", sizeof({c}), offsetof({c}, {m}));' for c, (_, m) in pairs.items())
     src = tmp_path / "s.c"
     src.write_text(f'#include <stdio.h>\n#include "{HEADER}"\nint main(void) {{ {body} return 0; }}\n')
@@ -176,11 +176,17 @@ def _add(**over):
         a["x"], a["ldx"], a["base"], a["ldb"], a["out"], a["ldo"], a["dtype"], ad, rq, a["t"], a["T"], a["K"], a["N"], None)
 
 
-def _back(dy=FAKE, lddy=96, dx=FAKE, lddx=64, add=0, da=FAKE, db=FAKE, ws=FAKE, wsb=1 << 30, **over):
+def _back(dy=FAKE, lddy=96, dx=FAKE, lddx=64, base=None, ldb=64, da=FAKE, db=FAKE, ws=FAKE, wsb=1 << 30, sets=1,
+          second=None, **over):
     a = {**ADD, **over}
     ad, rq = _adapters(a)
+    arr = (_lib.ReqBackwardSet * 3)()
+    for i in range(3):
+        arr[i] = _lib.ReqBackwardSet(ad, a["t"], dy, lddy, da, db)
+    if second is not None:
+        arr[1].adapters.rank = second
     return harp_amd.load_abi().harp_req_add_adapters_backward(
-        dy, lddy, a["x"], a["ldx"], a["t"], ad, rq, dx, lddx, add, da, db, a["T"], a["K"], a["N"], ws, wsb, None)
+        arr if sets else None, sets, a["x"], a["ldx"], rq, base, ldb, dx, lddx, a["T"], a["K"], a["N"], ws, wsb, None)
 
 
 BOTH = [
@@ -241,10 +247,57 @@ def test_adapters_forward_refuses(over, code, msg):
     (dict(ws=None), ENOMEM, "workspace"),
     (dict(wsb=64), ENOMEM, "workspace"),
     (dict(ws=FAKE + 8), EINVAL, "workspace"),
+    (dict(sets=0), EINVAL, "1 to 3"),
+    (dict(sets=4), EINVAL, "1 to 3"),
+    (dict(sets=2, second=8), EINVAL, "sets[1]"),
+    (dict(sets=3, rank=48), EINVAL, "dx_base"),
+    (dict(base=FAKE + 2), EINVAL, "dx_base must be aligned"),
+    (dict(base=FAKE, ldb=63), EINVAL, "dx_base row stride"),
 ])
 def test_adapters_backward_refuses(over, code, msg):
     rc = _back(**over)
     assert rc == code and msg in _err(), (rc, _err())
+
+
+def _qkv(x=FAKE, ldx=128, B=1, S=6, K=128, N=256, n_outs=3, ws=FAKE, wsb=1 << 30, t=None, adapters=True, odd=None,
+         weight=FAKE, **over):
+    a = {**ADD, **over}
+    ad, rq = _adapters(a)
+    ads = (_lib.ReqAdapters * 3)(ad, ad, ad)
+    if odd is not None:
+        ads[2].rank = odd
+    outs = (_lib.QkvOut * 3)()
+    for o in outs:
+        o.weight, o.ld_weight, o.y, o.ld_y = weight, K, FAKE, N
+    ts = None if t is None else (ctypes.c_void_p * 3)(*[t] * 3)
+    return harp_amd.load_abi().harp_req_qkv_project(x, ldx, B, S, K, N, None, 0, 128, outs, ads if adapters else None,
+                                                    n_outs, rq, ts, ws, wsb, None)
+
+
+@pytest.mark.parametrize("over,code,msg", [
+    (dict(x=None), EINVAL, "x must be"),
+    (dict(weight=FAKE + 8), EINVAL, "weight"),
+    (dict(K=100), EUNSUPPORTED, "k_dim=100"),
+    (dict(N=100), EUNSUPPORTED, "n_out=100"),
+    (dict(n_outs=4), EINVAL, "1 to 3"),
+    (dict(B=1 << 14, S=(1 << 14) + 1), EUNSUPPORTED, "2^28"),
+    (dict(adapters=False), EINVAL, "adapters is NULL"),
+    (dict(rank=0), EINVAL, "rank=0"),
+    (dict(rank=12), EUNSUPPORTED, "multiple of 8"),
+    (dict(b=FAKE + 8), EUNSUPPORTED, "16-byte"),
+    (dict(odd=8), EINVAL, "adapters[2]"),
+    (dict(index=None), EINVAL, "index is NULL"),
+    (dict(offsets=None, count=4), EINVAL, "one length"),
+    (dict(t=FAKE + 4), EINVAL, "t[0]"),
+    (dict(ws=None), ENOMEM, "workspace"),
+    (dict(wsb=100), ENOMEM, "workspace"),
+    (dict(ws=FAKE + 8), EINVAL, "workspace"),
+])
+def test_qkv_refuses(over, code, msg):
+    rc = _qkv(**over)
+    assert rc == code and msg in _err(), (rc, _err())
+    size = harp_amd.load_abi().harp_req_qkv_workspace_bytes
+    assert size(6, 16, 3) >= 3 * 6 * 64 and size(6, 0, 3) == size(6, 16, 4) == size(-1, 16, 1) == ctypes.c_size_t(-1).value
 
 
 def test_adapters_sizes_and_empty_calls():
@@ -253,9 +306,11 @@ def test_adapters_sizes_and_empty_calls():
     assert lib.harp_req_adapter_columns(0) == -1 and lib.harp_req_adapter_columns(129) == -1
     size = lib.harp_req_adapter_backward_workspace_bytes
     # u, and a and b transposed, at least
-    assert size(6, 64, 96, 2, 16, 2, 1, 1) >= 6 * 64 + 2 * 16 * (64 + 96) * 2
+    assert size(6, 64, 96, 2, 16, 2, 1) >= 6 * 64 + 2 * 16 * (64 + 96) * 2
     for bad in ((-1, 64, 96, 2, 16, 2), (6, 0, 96, 2, 16, 2), (6, 64, 96, 0, 16, 2), (6, 64, 96, 2, 200, 2), (6, 64, 96, 2, 16, 0)):
-        assert size(*bad, 1, 1) == ctypes.c_size_t(-1).value
+        assert size(*bad, 1) == ctypes.c_size_t(-1).value
+    assert size(6, 64, 96, 2, 16, 2, 0) == size(6, 64, 96, 2, 16, 2, 4) == ctypes.c_size_t(-1).value
+    assert size(6, 64, 96, 2, 16, 2, 3) > size(6, 64, 96, 2, 16, 2, 1)
     assert _add(T=0, x=None, base=None, out=None, t=None) == 0 and _back(T=0, dy=None, ws=None, wsb=0) == 0
     assert _back(dx=None, da=None, db=None, ws=None, wsb=0) == 0
 
