@@ -14,6 +14,7 @@
 // second product costs nothing beside the memory these kernels wait for.
 // Which tokens a block works on: req_device.h.
 #include <algorithm>
+#include <type_traits>
 
 #include "ra_common.h"
 #include "req_device.h"
@@ -49,6 +50,40 @@ __device__ __forceinline__ bf16x8 load_some(const bf16* p, int n) {
 }
 __device__ __forceinline__ bf16x8 load_full(const bf16* p) { return __builtin_bit_cast(bf16x8, *(const u32x4u*)p); }
 
+}  // namespace
+
+namespace {
+// t of a block's tile from its waves' sums: sum_of(wave, rank block * TB + token block, lane)
+template <int TB, int RB, int WAVES, class F>
+__device__ __forceinline__ void shrink_store(const ShrinkParams& p, const Tile& tile, int e0, int e_end, F sum_of) {
+  const int per = p.rp / 16;
+  for (int e = threadIdx.x; e < TB * RB * 64; e += 64 * WAVES) {
+    const int at = e >> 6, l = e & 63, j = at / TB, i = at % TB;
+    f32x4 s = sum_of(0, at, l);
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += sum_of(w, at, l);
+    const int row = 16 * i + (l & 15);
+    if (row >= tile.rows || e0 + j >= e_end) continue;
+    const int which = (e0 + j) / per, rank = 16 * (e0 + j - which * per) + 4 * (l >> 4);
+    const ShrinkSet set = which == 0 ? p.set[0] : which == 1 ? p.set[1] : p.set[2];
+    const float scale = set.scale ? set.scale[tile.adapter] : 1.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = rank + k < p.r ? s[k] * scale : 0.f;
+    const int64_t m = tile.first + row;
+    if (set.t) *(f32x4*)(set.t + m * p.ldt + rank) = s;
+    if (set.pairs) {
+      bf16 hi[4], lo[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        hi[k] = (bf16)s[k];
+        lo[k] = (bf16)(s[k] - (float)hi[k]);
+      }
+      bf16* t = (bf16*)set.pairs + m * 2 * p.rp + rank;
+      *(u32x2*)t = *(const u32x2*)hi;
+      *(u32x2*)(t + p.rp) = *(const u32x2*)lo;
+    }
+  }
+}
 }  // namespace
 
 // ---------------------------------------------------------------------------
@@ -130,32 +165,129 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
 #pragma unroll
     for (int i = 0; i < TB; ++i) sums[wave][j * TB + i][lane] = acc[j][i];
   __syncthreads();
-  for (int e = threadIdx.x; e < TB * RB * 64; e += 64 * WAVES) {
-    const int at = e >> 6, l = e & 63, j = at / TB, i = at % TB;
-    f32x4 s = sums[0][at][l];
+  shrink_store<TB, RB, WAVES>(p, tile, e0, e_end, [&](int w, int at, int l) { return sums[w][at][l]; });
+}
+
+// The same where x's and A's rows are 16-byte aligned.  Fragments read straight
+// from memory touch 16 rows with every 16 lanes, and the caches serve those one
+// after the other; here each wave copies its 64 columns of the tile's rows to LDS
+// (buffer_load ... lds, eight whole 128-byte lines an instruction) and reads the
+// fragments from there.  A wave has STAGES such steps of its own, so the loop has
+// no barrier: it waits for its oldest copies, reads, multiplies and sends the next
+// copies into the same place.
+template <int TB, int RB, int WAVES, int STAGES>
+__global__ __launch_bounds__(64 * WAVES) void shrink_lds_kernel(ShrinkParams p) {
+  constexpr int M = 16 * TB;
+  constexpr int kCopies = 2 * (TB + RB);  // of 8 rows each, x's rows and then A's
+  constexpr int kStage = 1024 * kCopies;  // bytes
+  constexpr int kTiles = WAVES * STAGES * kStage, kSums = WAVES * TB * RB * 64 * 16;
+  __shared__ __attribute__((aligned(16))) char lds[kTiles > kSums ? kTiles : kSums];
+  const Tile tile = tile_at<M>(p.req, (int)blockIdx.x);
+  if (tile.rows <= 0 || tile.adapter < 0) return;
+  // this block's entries e0 .. e0 + RB - 1 (before e_end) of the sets' rank blocks; those of sets with an x of
+  // their own are not shared
+  const int per = p.rp / 16, groups = (per + RB - 1) / RB, own = (int)blockIdx.y / groups;
+  const int e0 = p.apart ? own * per + ((int)blockIdx.y - own * groups) * RB : (int)blockIdx.y * RB;
+  const int e_end = p.apart ? (own + 1) * per : per * p.sets;
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int s0 = __builtin_amdgcn_readfirstlane(min(e0, e_end - 1) / per);
+  const bf16* const x = (const bf16*)(s0 == 0 ? p.set[0].x : s0 == 1 ? p.set[1].x : p.set[2].x);
+  const int64_t ldx = s0 == 0 ? p.set[0].ldx : s0 == 1 ? p.set[1].ldx : p.set[2].ldx;
+  // copy j takes rows 8 j + lane / 8, the 16-byte chunk that sits at position lane % 8 of its row: chunk c of
+  // row r at c ^ ((r >> 1) & 7), so that 16 rows' reads of one chunk hit every bank once
+  const int row8 = lane >> 3, chunk = (lane & 7) ^ ((row8 >> 1) & 7);
+  const harp_ra::rsrc_t xr =
+      harp_ra::make_rsrc(x + (int64_t)tile.first * ldx, (uint32_t)(((int64_t)(tile.rows - 1) * ldx + p.K) * 2));
+  uint32_t xsrc[2 * TB], asrc[2 * RB];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s += sums[w][at][l];
-    const int row = 16 * i + (l & 15);
-    if (row >= tile.rows || e0 + j >= e_end) continue;
-    const int which = (e0 + j) / per, rank = 16 * (e0 + j - which * per) + 4 * (l >> 4);
-    const ShrinkSet set = which == 0 ? p.set[0] : which == 1 ? p.set[1] : p.set[2];
-    const float scale = set.scale ? set.scale[tile.adapter] : 1.f;
+  for (int j = 0; j < 2 * TB; ++j) {
+    const int r = 8 * j + row8;
+    xsrc[j] = r < tile.rows ? (uint32_t)(r * ldx * 2 + (chunk ^ (4 * (j & 1))) * 16) : harp_ra::kOOB;
+  }
+  const bf16* ab[RB];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s[k] = rank + k < p.r ? s[k] * scale : 0.f;
-    const int64_t m = tile.first + row;
-    if (set.t) *(f32x4*)(set.t + m * p.ldt + rank) = s;
-    if (set.pairs) {
-      bf16 hi[4], lo[4];
+  for (int j = 0; j < RB; ++j) {
+    const int e = min(e0 + j, e_end - 1), set = e / per;
+    const void* a = set == 0 ? p.set[0].a : set == 1 ? p.set[1].a : p.set[2].a;
+    ab[j] = (const bf16*)a + ((int64_t)tile.adapter * p.r + 16 * (e - set * per)) * p.K;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        hi[k] = (bf16)s[k];
-        lo[k] = (bf16)(s[k] - (float)hi[k]);
-      }
-      bf16* t = (bf16*)set.pairs + m * 2 * p.rp + rank;
-      *(u32x2*)t = *(const u32x2*)hi;
-      *(u32x2*)(t + p.rp) = *(const u32x2*)lo;
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * h + row8;
+      asrc[2 * j + h] = 16 * (e - set * per) + r < p.r ? (uint32_t)(r * p.K * 2 + (chunk ^ (4 * h)) * 16) : harp_ra::kOOB;
     }
   }
+  const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(harp_ra::lds_void*)lds) +
+                        (uint32_t)(wave * STAGES * kStage);
+  const char* const mine = lds + wave * STAGES * kStage;
+  // the copies of columns 64 c .. 64 c + 63 into stage s; columns behind K are zeros (`live` false: all of them)
+  auto copy = [&](int s, int c, bool live) {
+    const int left = live ? p.K - 64 * c : 0;  // columns
+#pragma unroll
+    for (int j = 0; j < 2 * TB; ++j) {
+      const bool in = 8 * (chunk ^ (4 * (j & 1))) < left;
+      harp_ra::lds_dma_b128(xr, base + s * kStage + 1024 * j, in ? xsrc[j] + 128 * c : harp_ra::kOOB);
+    }
+#pragma unroll
+    for (int j = 0; j < RB; ++j) {
+      const harp_ra::rsrc_t arr = harp_ra::make_rsrc(ab[j], 16u * (uint32_t)p.K * 2u);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool in = 8 * (chunk ^ (4 * h)) < left;
+        harp_ra::lds_dma_b128(arr, base + s * kStage + 1024 * (2 * TB + 2 * j + h),
+                              in ? asrc[2 * j + h] + 128 * c : harp_ra::kOOB);
+      }
+    }
+  };
+  f32x4 acc[RB][TB];
+#pragma unroll
+  for (int j = 0; j < RB; ++j)
+#pragma unroll
+    for (int i = 0; i < TB; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (p.K + 63) / 64;
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s) copy(s, wave + WAVES * s, wave + WAVES * s < steps);
+  auto step = [&](auto SC, int c) {
+    constexpr int S = decltype(SC)::value;
+    harp_ra::wait_lds_loads_but<(STAGES - 1) * kCopies>();
+    bf16x8 xf[2][TB], af[2][RB];
+    const char* const t = mine + S * kStage;
+    auto frag = [&](int r, int h) {  // row r (16 of them in a block), columns 32 h + 8 g ..
+      return *(const bf16x8*)(t + r * 128 + (((4 * h + g) ^ ((r >> 1) & 7)) << 4));
+    };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < TB; ++i) xf[h][i] = frag(16 * i + l16, h);
+#pragma unroll
+      for (int j = 0; j < RB; ++j) af[h][j] = frag(16 * (TB + j) + l16, h);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < RB; ++j)
+#pragma unroll
+        for (int i = 0; i < TB; ++i) acc[j][i] = harp_ra::mfma16x16x32(af[h][j], xf[h][i], acc[j][i]);
+    // the fragments are in registers: the stage is free
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    copy(S, c + STAGES * WAVES, c + STAGES * WAVES < steps);
+  };
+  for (int c = wave; c < steps; c += STAGES * WAVES) {
+    step(std::integral_constant<int, 0>{}, c);
+    if constexpr (STAGES > 1)
+      if (c + WAVES < steps) step(std::integral_constant<int, 1>{}, c + WAVES);
+    if constexpr (STAGES > 2)
+      if (c + 2 * WAVES < steps) step(std::integral_constant<int, 2>{}, c + 2 * WAVES);
+  }
+  harp_ra::wait_lds_loads();  // (the empty copies too: the sums go over the stages)
+  __syncthreads();
+  f32x4* const sums = (f32x4*)lds;
+#pragma unroll
+  for (int j = 0; j < RB; ++j)
+#pragma unroll
+    for (int i = 0; i < TB; ++i) sums[(wave * TB * RB + j * TB + i) * 64 + lane] = acc[j][i];
+  __syncthreads();
+  shrink_store<TB, RB, WAVES>(p, tile, e0, e_end, [&](int w, int at, int l) { return sums[(w * TB * RB + at) * 64 + l]; });
 }
 
 // ---------------------------------------------------------------------------
@@ -237,27 +369,38 @@ __device__ __forceinline__ void store_run(char* row, int c, int N, const Run<E>&
 
 }  // namespace
 
-// RS: 16-rank steps (rp / 16); WT: waves of a block along the tokens (the other
-// 4 / WT along the features); a block walks `span` features
-template <int BASE, bool F32, int RS, int WT>
-__global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int span) {
-  constexpr int M = 32 * WT, WF = 4 / WT, PARTS = F32 ? 3 : 2;
-  constexpr int E = F32 ? 4 : 8;             // features of a lane's access: 16 bytes of out
-  constexpr int kLanes = 64 / E, kPass = 32 / E;  // lanes of a row, passes over the 32 rows
-  __shared__ f32x4 tiles[4][32 * 16];
-  const Tile tile = tile_at<M>(p.req, (int)blockIdx.x);
-  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int row0 = 32 * (wave % WT), rows = min(32, tile.rows - row0);
-  if (rows <= 0) return;
-  const int64_t m0 = tile.first + row0;
-  f32x4* const lds = tiles[wave];
-  const int f_end = min(p.N, ((int)blockIdx.y + 1) * span);
-  constexpr int es = F32 ? 4 : 2, bs = BASE == kBaseF32 ? 4 : 2;
+namespace {
 
-  bf16x8 tf[RS][PARTS];
-  if (tile.adapter >= 0) {
-    const float* const t = p.t + (m0 + min(l32, rows - 1)) * p.ldt + 8 * g;
+// What both kernels below share: a wave's 32 rows of a tile, its 8 KB of LDS
+template <int BASE, bool F32, int RS>
+struct Expand {
+  static constexpr int PARTS = F32 ? 3 : 2;
+  static constexpr int E = F32 ? 4 : 8;                   // features of a lane's access: 16 bytes of out
+  static constexpr int kLanes = 64 / E, kPass = 32 / E;   // lanes of a row, passes over the 32 rows
+  static constexpr int es = F32 ? 4 : 2, bs = BASE == kBaseF32 ? 4 : 2;
+  typedef RawRun<BASE == kBaseF32, E> Raw;
+  typedef Raw Raws[kPass];
+  typedef bf16x8 Frags[RS][PARTS];
+  const ExpandParams& p;
+  f32x4* lds;
+  int64_t m0;
+  int rows, adapter;
+  int l32, g, r_in, c_in;  // r_in, c_in: this lane's row and columns of a pass
+
+  __device__ __forceinline__ Expand(const ExpandParams& p_, f32x4* lds_, const Tile& tile, int row0)
+      : p(p_), lds(lds_), m0(tile.first + row0), rows(min(32, tile.rows - row0)), adapter(tile.adapter) {
+    const int lane = threadIdx.x & 63;
+    l32 = lane & 31;
+    g = lane >> 5;
+    r_in = lane / kLanes;
+    c_in = E * (lane % kLanes);
+  }
+  // t as parts of bf16, from this lane's token's row of it
+  __device__ __forceinline__ void load_t(Frags& tf) const {
+    if (adapter >= 0) load_t(tf, p.t + (m0 + min(l32, rows - 1)) * p.ldt);
+  }
+  __device__ __forceinline__ void load_t(Frags& tf, const float* t) const {
+    t += 8 * g;
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
       float v[8];
@@ -277,10 +420,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int sp
         }
     }
   }
-  const bool whole = p.r % 8 == 0;
-  const int r_in = lane / kLanes, c_in = E * (lane % kLanes);  // this lane's row and columns of a pass
-  for (int f0 = (int)blockIdx.y * span + 64 * (wave / WT); f0 < f_end; f0 += 64 * WF) {
-    RawRun<BASE == kBaseF32, E> raw[kPass];
+  __device__ __forceinline__ void load_base(Raws& raw, int f0) const {
     if constexpr (BASE != kNoBase) {
 #pragma unroll
       for (int i = 0; i < kPass; ++i) {
@@ -289,34 +429,22 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int sp
           raw[i] = load_run<BASE == kBaseF32, E>((const char*)p.base + (m0 + row) * p.ld_base * bs, f0 + c_in, p.N);
       }
     }
-    if (tile.adapter >= 0) {
+  }
+  // features 32 q .. + 31 of the 64: registers 4 a .. + 3 are features 8 a + 4 g .. + 3 of token l32
+  __device__ __forceinline__ void put(int q, const f32x16& acc) const {
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const bf16* b = (const bf16*)p.b + ((int64_t)tile.adapter * p.N + min(f0 + 32 * q + l32, p.N - 1)) * p.r + 8 * g;
-        f32x16 acc = harp_ra::zero16();
-#pragma unroll
-        for (int s = 0; s < RS; ++s) {
-          const int n = p.r - 16 * s - 8 * g;  // ranks this lane has left: 8 or more but in the last step
-          const bf16x8 bf = s < RS - 1 || n >= 8 ? load_full(b + 16 * s)
-                            : whole              ? harp_ra::zero8()
-                                                 : load_some(b + 16 * s, n);
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) acc = harp_ra::mfma32x32x16(bf, tf[s][part], acc);
-        }
-        // registers 4 a .. + 3: features 32 q + 8 a + 4 g .. + 3 of token l32
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-          lds[l32 * 16 + ((8 * q + 2 * a + g) ^ (l32 & 15))] =
-              f32x4{acc[4 * a], acc[4 * a + 1], acc[4 * a + 2], acc[4 * a + 3]};
-      }
-    }
-    // (the wave's own LDS, whose operations stay in order)
+    for (int a = 0; a < 4; ++a)
+      lds[l32 * 16 + ((8 * q + 2 * a + g) ^ (l32 & 15))] =
+          f32x4{acc[4 * a], acc[4 * a + 1], acc[4 * a + 2], acc[4 * a + 3]};
+  }
+  // base + what put() left (the wave's own LDS, whose operations stay in order)
+  __device__ __forceinline__ void store(const Raws& raw, int f0) const {
 #pragma unroll
     for (int i = 0; i < kPass; ++i) {
       const int row = i * E + r_in;
       Run<E> v{};
       if constexpr (BASE != kNoBase) v = values<BASE == kBaseF32, E>(raw[i]);
-      if (tile.adapter >= 0) {
+      if (adapter >= 0) {
 #pragma unroll
         for (int h = 0; h < E / 4; ++h) {
           const f32x4 d = lds[row * 16 + ((c_in / 4 + h) ^ (row & 15))];
@@ -327,6 +455,252 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int sp
       if (row < rows) store_run<F32, E>((char*)p.out + (m0 + row) * p.ld_out * es, f0 + c_in, p.N, v);
     }
   }
+};
+
+}  // namespace
+
+// Long requests: a block's four waves take 128 tokens and walk `span` features
+// together.  64 rows of B at a time are copied to LDS, whole lines, for all four
+// (fragments read straight from memory touch a row's line with every lane: rank 64
+// took 33 us for 63 MB of results), XOR-swizzled as the row length asks.  A step's
+// copies and base loads go out one step ahead, before the stores of the step
+// before: behind them they would wait for the stores to be done.
+template <int BASE, bool F32, int RS>
+__global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int span) {
+  typedef Expand<BASE, F32, RS> X;
+  constexpr int kChunks = RS == 1 ? 2 : RS == 2 ? 4 : RS <= 4 ? 8 : 16;  // 16-byte chunks of a row of B in LDS
+  constexpr int kRows = 16 / kChunks;                                  // rows of B in 256 bytes
+  __shared__ f32x4 tiles[4][32 * 16];
+  __shared__ __attribute__((aligned(16))) char bs[2][64 * kChunks * 16];
+  const Tile tile = tile_at<128>(p.req, (int)blockIdx.x);
+  if (tile.rows <= 0) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const X x(p, tiles[wave], tile, 32 * wave);  // (rows <= 0: the wave only helps to copy)
+  const int f_begin = (int)blockIdx.y * span, f_end = min(p.N, f_begin + span);
+  auto pos = [](int r, int c) { return c ^ (r / kRows & (kChunks - 1)); };  // of chunk c in row r
+  const harp_ra::rsrc_t br = harp_ra::make_rsrc((const bf16*)p.b + (int64_t)max(tile.adapter, 0) * p.N * p.r,
+                                                (uint32_t)p.N * (uint32_t)p.r * 2u);
+  const uint32_t b_lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(harp_ra::lds_void*)bs);
+  auto copy_b = [&](int f0, int stage) {
+#pragma unroll
+    for (int j = wave; j < kChunks; j += 4) {  // 64 chunks each
+      const int slot = 64 * j + lane, r = slot / kChunks, c = pos(r, slot % kChunks);
+      const bool in = f0 + r < p.N && 8 * c < p.r;
+      harp_ra::lds_dma_b128(br, b_lds + stage * (64 * kChunks * 16) + 1024 * j,
+                            in ? (uint32_t)((f0 + r) * p.r * 2 + 16 * c) : harp_ra::kOOB);
+    }
+  };
+  typename X::Frags tf;
+  typename X::Raws raw, cur;
+  // (loads come back in order: once `tick` is there, the copies before it are too)
+  uint32_t tick = 0;
+  auto load_step = [&](int f0, int stage) {
+    if (tile.adapter >= 0) {
+      copy_b(f0, stage);
+      tick = ((const uint16_t*)p.b)[((int64_t)tile.adapter * p.N + f0) * p.r + (lane & 7)];  // (r is 8 or more)
+    }
+    if (x.rows > 0) x.load_base(raw, f0);
+  };
+  if (x.rows > 0) x.load_t(tf);
+  load_step(f_begin, 0);
+  int stage = 0;
+  for (int f0 = f_begin; f0 < f_end; f0 += 64, stage ^= 1) {
+    asm volatile("" : "+v"(tick)::"memory");
+    if (tile.adapter >= 0) {
+      __syncthreads();
+      if (x.rows > 0) {
+        const char* const t = bs[stage];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          f32x16 acc = harp_ra::zero16();
+#pragma unroll
+          for (int s = 0; s < RS; ++s) {
+            const int r = 32 * q + x.l32;
+            const bf16x8 bf = *(const bf16x8*)(t + (r * kChunks + pos(r, 2 * s + x.g)) * 16);
+#pragma unroll
+            for (int part = 0; part < X::PARTS; ++part) acc = harp_ra::mfma32x32x16(bf, tf[s][part], acc);
+          }
+          x.put(q, acc);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < X::kPass; ++i) cur[i] = raw[i];
+    if (f0 + 64 < f_end) load_step(f0 + 64, stage ^ 1);
+    if (x.rows > 0) x.store(cur, f0);
+  }
+  harp_ra::wait_lds_loads();
+}
+
+// Short requests, and ranks whose rows of B are not 16-byte aligned: a tile of 32
+// tokens, each wave 64 features of its own, B's fragments straight from memory.
+template <int BASE, bool F32, int RS>
+__global__ __launch_bounds__(kThreads) void expand_short_kernel(ExpandParams p, int span) {
+  typedef Expand<BASE, F32, RS> X;
+  __shared__ f32x4 tiles[4][32 * 16];
+  const Tile tile = tile_at<32>(p.req, (int)blockIdx.x);
+  if (tile.rows <= 0) return;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const X x(p, tiles[wave], tile, 0);
+  const int f_end = min(p.N, ((int)blockIdx.y + 1) * span);
+  const bool whole = p.r % 8 == 0;
+  typename X::Frags tf;
+  typename X::Raws raw, cur;
+  bf16x8 bf[2][RS];
+  auto load_step = [&](int f0) {
+    if (tile.adapter >= 0) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const bf16* b =
+            (const bf16*)p.b + ((int64_t)tile.adapter * p.N + min(f0 + 32 * q + x.l32, p.N - 1)) * p.r + 8 * x.g;
+#pragma unroll
+        for (int s = 0; s < RS; ++s) {
+          const int n = p.r - 16 * s - 8 * x.g;  // ranks this lane has left: 8 or more but in the last step
+          bf[q][s] = s < RS - 1 || n >= 8 ? load_full(b + 16 * s) : whole ? harp_ra::zero8() : load_some(b + 16 * s, n);
+        }
+      }
+    }
+    x.load_base(raw, f0);
+  };
+  int f0 = (int)blockIdx.y * span + 64 * wave;
+  if (f0 >= f_end) return;
+  load_step(f0);
+  x.load_t(tf);
+  for (; f0 < f_end; f0 += 256) {
+    if (tile.adapter >= 0) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        f32x16 acc = harp_ra::zero16();
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+          for (int part = 0; part < X::PARTS; ++part) acc = harp_ra::mfma32x32x16(bf[q][s], tf[s][part], acc);
+        x.put(q, acc);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < X::kPass; ++i) cur[i] = raw[i];
+    if (f0 + 256 < f_end) load_step(f0 + 256);
+    x.store(cur, f0);
+  }
+}
+
+// One to four tokens to a request: both products in one launch, in fp32 on the
+// vector units.  What counts is how long a block waits, not what it computes: every
+// block forms t of its tokens anew (a wave sums 2 RS ranks with its lanes along K, so
+// that each load is one run of 1 KB; fragments of the matrix instructions would touch
+// 16 rows with every 16 lanes, and A's 123 KB of rank 16 over 3840 columns then took a
+// CU 3.6 us), and its threads take a feature each, whose row of B and base were on their
+// way meanwhile.
+constexpr int kFewFeatures = 512;  // of a block: a thread each
+
+__device__ __forceinline__ float wave_sum(float v) {
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));  // row_ror:8
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xf, 0xf, true));  // row_ror:4
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4e, 0xf, 0xf, true));   // quad_perm:[2,3,0,1]
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xb1, 0xf, 0xf, true));   // quad_perm:[1,0,3,2]
+  v += __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401f));              // lane ^ 16
+  return harp_ra::wave_half_sum(v);
+}
+
+template <bool F32, int RS, int M>
+__global__ __launch_bounds__(kFewFeatures) void few_kernel(ExpandParams p, FewParams q) {
+  constexpr int kWaves = kFewFeatures / 64, RJ = 16 * RS / kWaves;  // ranks of a wave
+  __shared__ __attribute__((aligned(16))) float ts[M][16 * RS];
+  const Tile tile = tile_at<M>(p.req, (int)blockIdx.x);
+  if (tile.rows <= 0) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int f = (int)blockIdx.y * kFewFeatures + (int)threadIdx.x, fc = min(f, p.N - 1);
+  float base[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    const int64_t o = (int64_t)(tile.first + min(m, tile.rows - 1)) * p.ld_base + fc;
+    base[m] = F32 ? ((const float*)p.base)[o] : (float)((const bf16*)p.base)[o];
+  }
+  if (tile.adapter >= 0) {  // (the same in every thread)
+    const bool whole = p.r % 8 == 0;
+    const bf16* const b = (const bf16*)p.b + ((int64_t)tile.adapter * p.N + fc) * p.r;
+    bf16x8 bv[2 * RS];
+#pragma unroll
+    for (int s = 0; s < 2 * RS; ++s) {
+      const int n = p.r - 8 * s;
+      bv[s] = n >= 8 ? load_full(b + 8 * s) : whole ? harp_ra::zero8() : load_some(b + 8 * s, n);
+    }
+    const bf16* xr[M];
+    const bf16* ar[RJ];
+    float acc[RJ][M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) xr[m] = (const bf16*)q.x + (int64_t)(tile.first + min(m, tile.rows - 1)) * q.ldx;
+#pragma unroll
+    for (int j = 0; j < RJ; ++j) {
+      ar[j] = (const bf16*)q.a + ((int64_t)tile.adapter * p.r + min(RJ * wave + j, p.r - 1)) * q.K;
+#pragma unroll
+      for (int m = 0; m < M; ++m) acc[j][m] = 0.f;
+    }
+    auto add = [&](const bf16x8(&xv)[M], const bf16x8(&av)[RJ]) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int j = 0; j < RJ; ++j)
+#pragma unroll
+          for (int m = 0; m < M; ++m) acc[j][m] = __builtin_fmaf((float)av[j][k], (float)xv[m][k], acc[j][m]);
+    };
+    int k = 8 * lane;
+    constexpr int U = RS * M <= 4 ? 4 : RS * M <= 8 ? 2 : 1;  // loads on their way, as the registers allow
+#pragma unroll U
+    for (; k + 8 <= q.K; k += 512) {
+      bf16x8 xv[M], av[RJ];
+#pragma unroll
+      for (int m = 0; m < M; ++m) xv[m] = load_full(xr[m] + k);
+#pragma unroll
+      for (int j = 0; j < RJ; ++j) av[j] = load_full(ar[j] + k);
+      add(xv, av);
+    }
+    if (k < q.K) {
+      bf16x8 xv[M], av[RJ];
+#pragma unroll
+      for (int m = 0; m < M; ++m) xv[m] = load_some(xr[m] + k, q.K - k);
+#pragma unroll
+      for (int j = 0; j < RJ; ++j) av[j] = load_some(ar[j] + k, q.K - k);
+      add(xv, av);
+    }
+    const float scale = q.scale ? q.scale[tile.adapter] : 1.f;
+#pragma unroll
+    for (int j = 0; j < RJ; ++j)
+#pragma unroll
+      for (int m = 0; m < M; ++m) {
+        const float v = wave_sum(acc[j][m]);
+        if (lane == 0) ts[m][RJ * wave + j] = RJ * wave + j < p.r ? v * scale : 0.f;
+      }
+    __syncthreads();
+    if (q.t && blockIdx.y == 0)
+      for (int e = threadIdx.x; e < 16 * RS * min(M, tile.rows); e += kFewFeatures)
+        q.t[(int64_t)(tile.first + e / (16 * RS)) * p.ldt + e % (16 * RS)] = ts[e / (16 * RS)][e % (16 * RS)];
+    float y[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) y[m] = 0.f;
+#pragma unroll
+    for (int s = 0; s < 2 * RS; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const f32x4 t = *(const f32x4*)&ts[m][8 * s + 4 * h];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[m] = __builtin_fmaf(t[e], (float)bv[s][4 * h + e], y[m]);
+        }
+#pragma unroll
+    for (int m = 0; m < M; ++m) base[m] += y[m];
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+    if (f < p.N && m < tile.rows) {
+      const int64_t o = (int64_t)(tile.first + m) * p.ld_out + f;
+      if constexpr (F32) ((float*)p.out)[o] = base[m];
+      else ((bf16*)p.out)[o] = (bf16)base[m];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -556,45 +930,58 @@ __global__ __launch_bounds__(kThreads) void transpose_kernel(TransposeParams p) 
 // Launchers
 // ---------------------------------------------------------------------------
 namespace {
+template <int RB>
+unsigned shrink_groups(const ShrinkParams& p) {
+  const int per = p.rp / 16;
+  return (unsigned)(p.apart ? p.sets * ((per + RB - 1) / RB) : (per * p.sets + RB - 1) / RB);
+}
 template <int TB, int RB, int WAVES>
 hipError_t shrink_t(const ShrinkParams& p, hipStream_t st) {
-  const int per = p.rp / 16;
-  const int groups = p.apart ? p.sets * ((per + RB - 1) / RB) : (per * p.sets + RB - 1) / RB;
-  const dim3 grid((unsigned)slots_of(p.req, 16 * TB), (unsigned)groups);
-  hipLaunchKernelGGL((shrink_kernel<TB, RB, WAVES>), grid, dim3(64 * WAVES), 0, st, p);
+  hipLaunchKernelGGL((shrink_kernel<TB, RB, WAVES>), dim3((unsigned)slots_of(p.req, 16 * TB), shrink_groups<RB>(p)),
+                     dim3(64 * WAVES), 0, st, p);
   return hipGetLastError();
 }
-template <int WAVES>
-hipError_t shrink_w(const ShrinkParams& p, hipStream_t st) {
-  const int total = p.rp / 16 * (p.apart ? 1 : p.sets);
-  if (slots_of(p.req, 16) * (p.rp / 16) * p.sets <= 512 || total == 1) return shrink_t<1, 1, WAVES>(p, st);
-  return total % 4 == 0 || total > 4 ? shrink_t<2, 4, WAVES>(p, st) : shrink_t<2, 2, WAVES>(p, st);
+template <int TB, int RB, int WAVES>
+hipError_t shrink_lds_t(const ShrinkParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((shrink_lds_kernel<TB, RB, WAVES, 3>),
+                     dim3((unsigned)slots_of(p.req, 16 * TB), shrink_groups<RB>(p)), dim3(64 * WAVES), 0, st, p);
+  return hipGetLastError();
 }
 }  // namespace
 
 hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
+  bool aligned = p.K % 8 == 0;
+  for (int i = 0; i < p.sets; ++i) {
+    const ShrinkSet& s = p.set[i];
+    aligned &= s.ldx % 8 == 0 && s.ldx < (1 << 24) && (uintptr_t)s.x % 16 == 0 && (uintptr_t)s.a % 16 == 0;
+  }
+  // few tokens: a block for every 16 ranks
+  const bool few = slots_of(p.req, 16) * (p.rp / 16) * p.sets <= 512;
+  const int total = p.rp / 16 * (p.apart ? 1 : p.sets);
+  if (aligned) {
+    if (few) return shrink_lds_t<1, 1, 8>(p, st);
+    return total == 1 ? shrink_lds_t<2, 1, 4>(p, st) : total == 2 ? shrink_lds_t<2, 2, 4>(p, st) : shrink_lds_t<2, 4, 4>(p, st);
+  }
   // the waves of a block share K: 16 of them where each has a 64-column step
-  return p.K >= 1024 ? shrink_w<16>(p, st) : shrink_w<4>(p, st);
+  if (p.K < 1024) return few ? shrink_t<1, 1, 4>(p, st) : shrink_t<2, 4, 4>(p, st);
+  return few || total == 1 ? shrink_t<1, 1, 16>(p, st) : shrink_t<2, 4, 16>(p, st);
 }
 
 namespace {
-template <int BASE, bool F32, int RS, int WT>
-hipError_t expand_t(const ExpandParams& p, hipStream_t st) {
-  const int64_t slots = slots_of(p.req, 32 * WT);
-  // enough blocks for the chip, in multiples of a block's 64-feature steps
-  constexpr int step = 64 * (4 / WT);
-  const int steps = (p.N + step - 1) / step;
-  const int64_t want = std::max<int64_t>(1, 2048 / slots);
-  const int each = (int)std::max<int64_t>(1, steps / std::min<int64_t>(want, steps));
-  hipLaunchKernelGGL((expand_kernel<BASE, F32, RS, WT>), dim3((unsigned)slots, (unsigned)((steps + each - 1) / each)),
-                     dim3(kThreads), 0, st, p, each * step);
-  return hipGetLastError();
-}
 template <int BASE, bool F32, int RS>
 hipError_t expand_w(const ExpandParams& p, hipStream_t st) {
   // requests of 64 tokens and more on the average fill a block's waves along the tokens
-  return p.req.tokens / std::max(p.req.count, 1) >= 64 ? expand_t<BASE, F32, RS, 4>(p, st)
-                                                       : expand_t<BASE, F32, RS, 1>(p, st);
+  const bool tall = p.req.tokens / std::max(p.req.count, 1) >= 64 && p.r % 8 == 0 && (uintptr_t)p.b % 16 == 0;
+  const int64_t slots = slots_of(p.req, tall ? 128 : 32);
+  // blocks in multiples of their steps: of the long requests' three fit a CU at a time, and no more than that
+  // keeps what a block does before its first step small (rank 64, 8192 x 3840: 22 us, with 2048 blocks 27)
+  const int step = tall ? 64 : 256, steps = (p.N + step - 1) / step;
+  const int64_t want = std::max<int64_t>(1, (tall ? 768 : 2048) / slots);
+  const int each = (int)std::max<int64_t>(1, steps / std::min<int64_t>(want, steps));
+  const dim3 grid((unsigned)slots, (unsigned)((steps + each - 1) / each));
+  if (tall) hipLaunchKernelGGL((expand_kernel<BASE, F32, RS>), grid, dim3(kThreads), 0, st, p, each * step);
+  else hipLaunchKernelGGL((expand_short_kernel<BASE, F32, RS>), grid, dim3(kThreads), 0, st, p, each * step);
+  return hipGetLastError();
 }
 template <int BASE, bool F32>
 hipError_t expand_r(const ExpandParams& p, hipStream_t st) {
@@ -614,6 +1001,42 @@ hipError_t launch_expand(const ExpandParams& p, hipStream_t st) {
   if (p.out_f32) return expand_r<kBaseF32, true>(p, st);
   if (!p.base) return expand_r<kNoBase, false>(p, st);
   return p.base_f32 ? expand_r<kBaseF32, false>(p, st) : expand_r<kBaseBf16, false>(p, st);
+}
+
+namespace {
+constexpr int64_t kFewBytes = 32 << 20;  // of A that all blocks together read
+constexpr int kFewSteps4 = 3;            // 16-rank steps of four tokens' sums that fit the registers
+
+int64_t few_blocks(const ExpandParams& p) { return (p.N + kFewFeatures - 1) / kFewFeatures; }
+
+template <bool F32, int RS>
+hipError_t few_t(const ExpandParams& p, const FewParams& q, hipStream_t st) {
+  if (p.req.tokens <= p.req.count)
+    hipLaunchKernelGGL((few_kernel<F32, RS, 1>), dim3((unsigned)slots_of(p.req, 1), (unsigned)few_blocks(p)),
+                       dim3(kFewFeatures), 0, st, p, q);
+  else if constexpr (RS <= kFewSteps4)
+    hipLaunchKernelGGL((few_kernel<F32, RS, 4>), dim3((unsigned)slots_of(p.req, 4), (unsigned)few_blocks(p)),
+                       dim3(kFewFeatures), 0, st, p, q);
+  return hipGetLastError();
+}
+template <bool F32>
+hipError_t few_r(const ExpandParams& p, const FewParams& q, hipStream_t st) {
+  switch (p.rp / 16) {
+    case 1: return few_t<F32, 1>(p, q, st);
+    case 2: return few_t<F32, 2>(p, q, st);
+    case 3: return few_t<F32, 3>(p, q, st);
+    default: return few_t<F32, 4>(p, q, st);
+  }
+}
+}  // namespace
+bool few_tokens(const ExpandParams& p, int K) {
+  const int64_t tiles = std::min<int64_t>(p.req.tokens, p.req.tokens / 4 + p.req.count);  // that have tokens
+  const int most = p.req.tokens <= p.req.count ? 4 : kFewSteps4;
+  return p.rp <= 16 * most && p.base && p.base_f32 == p.out_f32 && p.req.tokens <= 4 * (int64_t)p.req.count &&
+         tiles * few_blocks(p) * p.r * K * 2 <= kFewBytes;
+}
+hipError_t launch_few(const ExpandParams& p, const FewParams& q, hipStream_t st) {
+  return p.out_f32 ? few_r<true>(p, q, st) : few_r<false>(p, q, st);
 }
 
 namespace {

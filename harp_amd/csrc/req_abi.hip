@@ -374,19 +374,12 @@ int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base,
   if ((rc = check_matrix(out, ld_out, dtype, n_dim, true, "out"))) return rc;
   if (base == out && ld_base != ld_out) return fail(HARP_REQ_EINVAL, "out in base's place needs base's row stride");
   if (!t || !aligned(t, 16)) return fail(HARP_REQ_EINVAL, "t must be a 16-byte aligned device pointer");
-  ShrinkParams s{};
-  s.req = q;
-  s.K = k_dim;
-  s.r = adapters->rank;
-  s.rp = rank_pad(adapters->rank);
-  s.ldt = s.rp;
-  s.sets = 1;
-  s.set[0] = ShrinkSet{adapters->a, adapters->scales, x, ld_x, t, nullptr};
-  if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
   ExpandParams e{};
   e.req = q;
+  e.r = adapters->rank;
+  e.rp = rank_pad(e.r);
   e.t = t;
-  e.ldt = s.rp;
+  e.ldt = e.rp;
   e.b = adapters->b;
   e.base = base;
   e.ld_base = ld_base;
@@ -394,8 +387,18 @@ int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base,
   e.ld_out = ld_out;
   e.base_f32 = e.out_f32 = dtype == kF32;
   e.N = n_dim;
-  e.r = s.r;
-  e.rp = s.rp;
+  if (few_tokens(e, k_dim))
+    return launched(launch_few(e, FewParams{adapters->a, adapters->scales, x, ld_x, k_dim, t}, (hipStream_t)stream),
+                    "adapters (few tokens)");
+  ShrinkParams s{};
+  s.req = q;
+  s.K = k_dim;
+  s.r = e.r;
+  s.rp = e.rp;
+  s.ldt = e.rp;
+  s.sets = 1;
+  s.set[0] = ShrinkSet{adapters->a, adapters->scales, x, ld_x, t, nullptr};
+  if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
   return launched(launch_expand(e, (hipStream_t)stream), "adapters (t B^T)");
 }
 

@@ -129,6 +129,19 @@ struct ExpandParams {
 };
 hipError_t launch_expand(const ExpandParams& p, hipStream_t stream);
 
+// Both of the above in one launch, for few tokens to a request: t is formed from x
+// and A (as ShrinkSet's) where it is needed, and written if it is wanted.
+struct FewParams {
+  const void* a;
+  const float* scale;
+  const void* x;
+  int64_t ldx;
+  int K;
+  float* t;  // row stride ldt of the other parameters, or NULL
+};
+bool few_tokens(const ExpandParams& p, int K);  // whether it is for this call
+hipError_t launch_few(const ExpandParams& p, const FewParams& q, hipStream_t stream);
+
 // For each adapter a the sum over its tokens m of v[m][j] x[m][c]: out [n, r, C],
 // or [n, C, r] with `cols_first`, bf16.  Up to six such sums in one launch.
 struct GradPart {

@@ -117,6 +117,14 @@ CASES = [
     (2, 301, 67, 61, 127, 3, F32, True),
     (3, 260, 50, 1, 80, 2, B16, True),
     (1, 77, 1, 40, 5, 1, B16, False),
+    (9, 20, 1000, 1100, 16, 4, B16, True),    # up to four tokens to a request, one launch
+    (40, 120, 515, 520, 64, 9, F32, False),
+    (17, 17, 515, 600, 50, 9, B16, False),
+    (12, 40, 136, 700, 33, 5, B16, True),
+    (3, 2000, 1088, 72, 16, 2, B16, True),    # whole lines through LDS: one, two and more blocks of ranks
+    (3, 2000, 520, 200, 24, 2, B16, True),
+    (2, 1700, 72, 456, 72, 2, F32, True),
+    (2, 8192, 40, 136, 120, 2, B16, False),
     (6, 4100, 160, 128, 40, 3, B16, True),   # blocks that share K between four waves
     (6, 9000, 64, 96, 96, 3, F32, True),
     (5, 8192, 128, 64, 16, 2, B16, True),
