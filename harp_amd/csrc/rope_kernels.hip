@@ -14,10 +14,15 @@
 // 1.8e-9 and (pi/4)^10 / 10! = 2.5e-8).
 //
 // Layout: LPR lanes (8, 16 or 32 for D <= 64, 128, 256) hold a row, 8 values
-// (four pairs) each, so a lane's pairs are the same in every row: their four
-// rates are formed once per thread and their angles once per token, for R heads
-// of that token.  The kernels are bound by memory; the angles' arithmetic runs
-// while the rows' loads are on their way, and no table is read.
+// (four pairs) each.  The angles of the few tokens that a block's rows are of are
+// formed by all its threads while the rows' loads are on their way, and shared
+// through LDS (each lane its own four, their rates' powers in 64 bits among them, the
+// arithmetic took longer than the memory: 62 us for 8192 tokens x 60 heads).  No
+// table is read.
+//
+// Bound by memory: at 8192 tokens x 60 heads of 128 in bf16 the forward moves 252 MB in
+// 52 us (4.8 TB/s) and the backward, which reads x and dy, 377 MB in 85 us (4.4 TB/s),
+// where a large copy moves 5.1 TB/s.  A call of few tokens is bound by its launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -199,31 +204,24 @@ __device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
 
 // Workgroups are dealt to the 8 XCDs round-robin: each XCD takes one contiguous
 // range of the work, so that what its L2 holds is one window of memory.
-__device__ __forceinline__ int64_t xcd_block(uint32_t bid, uint32_t blocks) {
+__device__ __forceinline__ uint32_t xcd_block(uint32_t bid, uint32_t blocks) {
   const uint32_t q = blocks / 8, r = blocks % 8, x = bid % 8, local = bid / 8;
   return x < r ? x * (q + 1) + local : r * (q + 1) + (x - r) * q + local;
 }
 
-// A launch's blocks: those of q, then those of k (so a block's tensor is
-// uniform).  The heads of a token are dealt to J groups of lanes, R to each.
-struct Range {
-  int64_t first;  // of the tensor's blocks
-  int n;
-};
-struct Ranges {
-  Range q, k;
+// A launch's blocks: those of q, then those of k.  The heads of a token are dealt
+// to J groups of lanes, R to each.
+struct Blocks {
+  int q, k;
+  uint32_t q_steps, k_steps;  // of a block (the last one's may be fewer)
 };
 struct Unit {
   uint32_t b, s;
   int j;
 };
-__device__ __forceinline__ Unit unit_at(int S, int J, int64_t unit) {
-  Unit u;
-  const int64_t tok = unit / J;
-  u.j = (int)(unit - tok * J);
-  u.b = (uint32_t)(tok / S);
-  u.s = (uint32_t)(tok - (int64_t)u.b * S);
-  return u;
+__device__ __forceinline__ Unit unit_at(uint32_t S, uint32_t J, uint32_t unit) {
+  const uint32_t tok = unit / J, b = tok / S;
+  return Unit{b, tok - b * S, (int)(unit - tok * J)};
 }
 // n units on, in 32 bits (n is a block's groups)
 __device__ __forceinline__ Unit unit_after(uint32_t S, uint32_t J, const Unit& u, uint32_t n) {
@@ -234,25 +232,45 @@ __device__ __forceinline__ int64_t offset_of(const RopeStrides& st, const Unit& 
   return u.b * st.b + (int64_t)h * st.h + (int64_t)u.s * st.s;
 }
 
+// The angles of a block's step: its kGroups units, one after the other, are of a
+// few tokens (kGroups at most).  A thread keeps one pair, whose rate it forms
+// once, and forms the angles of every 256 / kPairs-th token for all of them.
+template <int LPR>
 struct Angles {
-  double rate[4];
-  int64_t axis[4];  // offsets of the pairs' axes in a token's position
-  __device__ __forceinline__ void init(const RopeParams& p, int sub) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      int a;
-      rate[k] = rate_of(p.axes, min(4 * sub + k, p.D / 2 - 1), a);
-      axis[k] = a * p.pos.sa;
+  static constexpr int kPairs = 4 * LPR, kGroups = kThreads / LPR;
+  typedef float2 Buf[kGroups][kPairs];
+  double rate;
+  int64_t axis;  // offset of the pair's axis in a token's position
+  int pair, at;
+  __device__ __forceinline__ explicit Angles(const RopeParams& p) {
+    pair = threadIdx.x % kPairs;
+    at = threadIdx.x / kPairs;
+    int a;
+    rate = rate_of(p.axes, min(pair, p.D / 2 - 1), a);
+    axis = a * p.pos.sa;
+  }
+  // of the tokens from `first` (of unit u) on
+  __device__ __forceinline__ void form(const RopeParams& p, const Unit& u, int tokens, float sign, Buf& buf) const {
+    if (2 * pair >= p.D) return;
+    for (int k = at; k < tokens; k += kThreads / kPairs) {
+      const uint32_t s = u.s + k, db = s / (uint32_t)p.S;
+      const int64_t off[1] = {axis};
+      double v[1];
+      load_pos(p.pos, (int64_t)(u.b + db) * p.pos.sb + (int64_t)(s - db * (uint32_t)p.S) * p.pos.ss, off, v);
+      float2 cs;
+      cos_sin(v[0] * rate, cs.x, cs.y);
+      cs.y *= sign;
+      buf[k][pair] = cs;
     }
   }
-  __device__ __forceinline__ void at(const RopeParams& p, const Unit& u, float sign, float (&c)[4], float (&s)[4]) const {
-    const int64_t base = (int64_t)u.b * p.pos.sb + (int64_t)u.s * p.pos.ss;
-    double pos[4];
-    load_pos(p.pos, base, axis, pos);
+  static __device__ __forceinline__ void read(const Buf& buf, int token, int sub, float (&c)[4], float (&s)[4]) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      cos_sin(pos[k] * rate[k], c[k], s[k]);
-      s[k] *= sign;
+    for (int k = 0; k < 4; k += 2) {
+      const f32x4 v = *(const f32x4*)&buf[token][4 * sub + k];
+      c[k] = v[0];
+      s[k] = v[1];
+      c[k + 1] = v[2];
+      s[k + 1] = v[3];
     }
   }
 };
@@ -280,41 +298,113 @@ __device__ __forceinline__ float inv_rms(float ss, int D, float eps) {
 // ---------------------------------------------------------------------------
 // Forward, and (sign -1, no norm) the rotation's own backward
 // ---------------------------------------------------------------------------
-template <bool F32, bool HALF, int LPR, int R>
-__global__ __launch_bounds__(kThreads) void rope_forward_kernel(RopeParams p, Ranges ranges) {
-  constexpr int es = F32 ? 4 : 2;
-  const int grp = threadIdx.x / LPR, sub = threadIdx.x % LPR;
-  const bool is_k = (int)blockIdx.x >= ranges.q.n;
-  const RopeHeads t = is_k ? p.t[1] : p.t[0];
-  const Range rg = is_k ? ranges.k : ranges.q;
-  const int64_t blk = rg.first + xcd_block(blockIdx.x - (is_k ? ranges.q.n : 0), rg.n);
-  const int J = (t.H + R - 1) / R;
-  const int64_t unit = blk * (kThreads / LPR) + grp;
-  if (unit >= (int64_t)p.B * p.S * J) return;  // whole groups
-  const Unit u = unit_at(p.S, J, unit);
-  const bool live = 8 * sub < p.D;
-  const int lane = live ? sub : 0;  // lanes behind D repeat the first values and store nothing
-  Raw<F32> raw[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-    raw[i] = load_raw<F32, HALF>((const char*)t.x + offset_of(t.sx, u, min(u.j + J * i, t.H - 1)) * es, lane, p.D);
-  Angles ang;
-  ang.init(p, lane);
-  float c[4], s[4], w[8];
-  ang.at(p, u, p.sign, c, s);
-  load_weight<HALF>(t.w, t.w_f32, lane, p.D, w);
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    const int h = u.j + J * i;
-    float v[8];
-    unpack<F32, HALF>(raw[i], v);
-    if (t.norm) {
-      const float inv = inv_rms(group_sum<LPR>(live ? dot8(v, v) : 0.f), p.D, t.eps);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = v[k] * inv * w[k];
+namespace {
+
+// A block's share bid of `blocks` of a tensor's steps, kGroups units each (a unit: R
+// heads of one token): where each group of lanes is in them.
+template <int LPR, int R>
+struct Walk {
+  static constexpr int kGroups = kThreads / LPR;
+  uint32_t units, step, end, S;  // (at most 2^31 units: 64-bit divisions took a microsecond of a short call)
+  int J, grp, groups, token;  // groups: that have a unit in this step; token: this one's among the step's
+  Unit u0, u;                 // the step's first unit, this group's
+  __device__ __forceinline__ Walk(const RopeParams& p, const RopeHeads& t, uint32_t bid, int blocks, uint32_t each) {
+    J = (t.H + R - 1) / R;
+    S = (uint32_t)p.S;
+    grp = threadIdx.x / LPR;
+    units = (uint32_t)p.B * S * (uint32_t)J;
+    step = xcd_block(bid, blocks) * each;
+    end = min(step + each, (units + kGroups - 1) / kGroups);
+    if (step < end) {
+      u0 = unit_at(p.S, J, step * kGroups);
+      place();
     }
-    rotate(v, c, s);
-    if (live && h < t.H) store_row<F32, HALF>((char*)t.y + offset_of(t.sy, u, h) * es, lane, p.D, v);
+  }
+  // a group behind the last unit repeats it (and counts for nothing)
+  __device__ __forceinline__ void place() {
+    groups = (int)min((uint32_t)kGroups, units - step * kGroups);
+    const int at = min(grp, groups - 1);
+    token = (u0.j + at) / J;
+    u = unit_after(S, J, u0, at);
+  }
+  __device__ __forceinline__ int tokens() const { return (u0.j + groups - 1) / J + 1; }
+  __device__ __forceinline__ bool next() {
+    if (++step >= end) return false;
+    u0 = unit_after(S, J, u0, kGroups);
+    place();
+    return true;
+  }
+};
+
+// Forward: the blocks of long calls (four heads a group) walk their steps, a short one's have a
+// step each (with the walk's second buffer and copies, 1024 tokens x 30 heads of 72 in fp32 took
+// 12.2 us instead of 11.3 and one token's heads 7.2 instead of 4.5)
+template <int R>
+constexpr bool kWalk = R == 4;
+
+template <bool F32, bool HALF, int LPR, int R>
+__device__ __forceinline__ void forward_share(const RopeParams& p, const RopeHeads& t, const Angles<LPR>& ang,
+                                              uint32_t bid, int blocks, uint32_t each,
+                                              typename Angles<LPR>::Buf (&angles)[kWalk<R> ? 2 : 1]) {
+  constexpr int es = F32 ? 4 : 2;
+  const int sub = threadIdx.x % LPR;
+  const bool lane_in = 8 * sub < p.D;
+  const int lane = lane_in ? sub : 0;  // lanes behind D repeat the first values and store nothing
+  Walk<LPR, R> at(p, t, bid, blocks, each);
+  if (at.step >= at.end) return;
+  float w[8];
+  load_weight<HALF>(t.w, t.w_f32, lane, p.D, w);
+  Raw<F32> raw[R];
+  auto load = [&]() {
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      raw[i] = load_raw<F32, HALF>((const char*)t.x + offset_of(t.sx, at.u, min(at.u.j + at.J * i, t.H - 1)) * es, lane, p.D);
+  };
+  load();
+  bool more = true;
+  for (int odd = 0; more; odd ^= 1) {
+    ang.form(p, at.u0, at.tokens(), p.sign, angles[odd]);
+    __syncthreads();  // (the other buffer's readers are past the barrier of the step before)
+    float c[4], s[4];
+    Angles<LPR>::read(angles[odd], at.token, lane, c, s);
+    const Unit u = at.u;
+    const bool in = lane_in && at.grp < at.groups;
+    Raw<F32> cur[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) cur[i] = raw[i];
+    more = kWalk<R> && at.next();
+    if (more) load();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int h = u.j + at.J * i;
+      float v[8];
+      unpack<F32, HALF>(cur[i], v);
+      if (t.norm) {
+        const float inv = inv_rms(group_sum<LPR>(lane_in ? dot8(v, v) : 0.f), p.D, t.eps);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = v[k] * inv * w[k];
+      }
+      rotate(v, c, s);
+      if (in && h < t.H) store_row<F32, HALF>((char*)t.y + offset_of(t.sy, u, h) * es, lane, p.D, v);
+    }
+  }
+}
+
+}  // namespace
+
+template <bool F32, bool HALF, int LPR, int R>
+__global__ __launch_bounds__(kThreads) void rope_forward_kernel(RopeParams p, Blocks n) {
+  __shared__ __attribute__((aligned(16))) typename Angles<LPR>::Buf angles[kWalk<R> ? 2 : 1];
+  const Angles<LPR> ang(p);
+  harp_ra::sched_fence();
+  const bool is_k = (int)blockIdx.x >= n.q;
+  if constexpr (kWalk<R>) {
+    // (two copies of the walk: both tensors' strides side by side do not fit the scalar registers)
+    if (!is_k) forward_share<F32, HALF, LPR, R>(p, p.t[0], ang, blockIdx.x, n.q, n.q_steps, angles);
+    else forward_share<F32, HALF, LPR, R>(p, p.t[1], ang, blockIdx.x - n.q, n.k, n.k_steps, angles);
+  } else {
+    const RopeHeads t = is_k ? p.t[1] : p.t[0];
+    forward_share<F32, HALF, LPR, R>(p, t, ang, blockIdx.x - (is_k ? n.q : 0), is_k ? n.k : n.q, 1, angles);
   }
 }
 
@@ -324,48 +414,59 @@ __global__ __launch_bounds__(kThreads) void rope_forward_kernel(RopeParams p, Ra
 // adds those in a fixed order.
 // ---------------------------------------------------------------------------
 namespace {
-// The block's share blk of `blocks` of one tensor, t
+// The block's share of one tensor, t: the next step's loads are on their way while one is worked on
 template <bool F32, bool HALF, int LPR, int R>
-__device__ __forceinline__ void backward_share(const RopeParams& p, const RopeHeads& t, const Angles& ang, uint32_t bid,
-                                               int blocks, float (&part)[kThreads / LPR][LPR * 8 + 4]) {
-  constexpr int es = F32 ? 4 : 2, kGroups = kThreads / LPR;
-  const int grp = threadIdx.x / LPR, sub = threadIdx.x % LPR;
-  const int64_t blk = xcd_block(bid, blocks);
-  const int J = (t.H + R - 1) / R;
-  const int64_t units = (int64_t)p.B * p.S * J, steps = (units + kGroups - 1) / kGroups;
-  const int64_t begin = steps * blk / blocks, end = steps * (blk + 1) / blocks;
-  const bool live = 8 * sub < p.D;
-  const int lane = live ? sub : 0;
-  float wg[8], w[8];
+__device__ __forceinline__ void backward_share(const RopeParams& p, const RopeHeads& t, const Angles<LPR>& ang,
+                                               uint32_t bid, int blocks, uint32_t each,
+                                               typename Angles<LPR>::Buf (&angles)[2],
+                                               float (&wg)[8]) {
+  constexpr int es = F32 ? 4 : 2;
+  const int sub = threadIdx.x % LPR;
+  const bool lane_in = 8 * sub < p.D;
+  const int lane = lane_in ? sub : 0;
+  Walk<LPR, R> at(p, t, bid, blocks, each);
+  if (at.step >= at.end) return;
+  float w[8];
   load_weight<HALF>(t.w, t.w_f32, lane, p.D, w);
-#pragma unroll
-  for (int k = 0; k < 8; ++k) wg[k] = 0.f;
-  Unit u = unit_at(p.S, J, begin * kGroups + grp);
-  // (only the last step of all is short, by whole groups)
-  int left = (int)(end - begin) - (begin < end && (end - 1) * kGroups + grp >= units);
-  for (; left > 0; --left, u = unit_after(p.S, J, u, kGroups)) {
-    Raw<F32> rx[R], rd[R];
+  Raw<F32> rx[R], rd[R];
+  auto load = [&]() {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int h = min(u.j + J * i, t.H - 1);
-      rd[i] = load_raw<F32, HALF>((const char*)t.dy + offset_of(t.sdy, u, h) * es, lane, p.D);
-      rx[i] = load_raw<F32, HALF>((const char*)t.x + offset_of(t.sx, u, h) * es, lane, p.D);
+      const int h = min(at.u.j + at.J * i, t.H - 1);
+      rd[i] = load_raw<F32, HALF>((const char*)t.dy + offset_of(t.sdy, at.u, h) * es, lane, p.D);
+      rx[i] = load_raw<F32, HALF>((const char*)t.x + offset_of(t.sx, at.u, h) * es, lane, p.D);
     }
+  };
+  load();
+  bool more = true;
+  for (int odd = 0; more; odd ^= 1) {
+    ang.form(p, at.u0, at.tokens(), -1.f, angles[odd]);
+    __syncthreads();  // (the other buffer's readers are past the barrier of the step before)
     float c[4], s[4];
-    ang.at(p, u, -1.f, c, s);
+    Angles<LPR>::read(angles[odd], at.token, lane, c, s);
+    const Unit u = at.u;
+    const bool in = lane_in && at.grp < at.groups;
+    Raw<F32> cx[R], cd[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int h = u.j + J * i;
-      const bool mine = live && h < t.H;
+      cx[i] = rx[i];
+      cd[i] = rd[i];
+    }
+    more = at.next();
+    if (more) load();
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int h = u.j + at.J * i;
+      const bool mine = in && h < t.H;
       float x[8], g[8];
-      unpack<F32, HALF>(rd[i], g);
-      unpack<F32, HALF>(rx[i], x);
+      unpack<F32, HALF>(cd[i], g);
+      unpack<F32, HALF>(cx[i], x);
       rotate(g, c, s);
-      const float inv = inv_rms(group_sum<LPR>(live ? dot8(x, x) : 0.f), p.D, t.eps);
+      const float inv = inv_rms(group_sum<LPR>(lane_in ? dot8(x, x) : 0.f), p.D, t.eps);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        x[k] = mine ? x[k] * inv : 0.f;  // a row past H repeats the last one and counts for nothing
-        wg[k] = __builtin_fmaf(g[k], x[k], wg[k]);
+        x[k] = lane_in ? x[k] * inv : 0.f;
+        wg[k] = __builtin_fmaf(mine ? g[k] : 0.f, x[k], wg[k]);
         g[k] *= w[k];
       }
       const float mean = __fdiv_rn(group_sum<LPR>(dot8(g, x)), (float)p.D);
@@ -374,24 +475,24 @@ __device__ __forceinline__ void backward_share(const RopeParams& p, const RopeHe
       if (mine) store_row<F32, HALF>((char*)t.y + offset_of(t.sy, u, h) * es, lane, p.D, g);
     }
   }
-#pragma unroll
-  for (int k = 0; k < 8; ++k) part[grp][8 * sub + k] = wg[k];
 }
 }  // namespace
 
 template <bool F32, bool HALF, int LPR, int R>
-__global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p, Ranges ranges) {
+__global__ __launch_bounds__(kThreads) void rope_backward_kernel(RopeParams p, Blocks n) {
   constexpr int kGroups = kThreads / LPR;
+  __shared__ __attribute__((aligned(16))) typename Angles<LPR>::Buf angles[2];
   __shared__ float part[kGroups][LPR * 8 + 4];
-  Angles ang;
-  ang.init(p, 8 * (threadIdx.x % LPR) < p.D ? threadIdx.x % LPR : 0);
+  float wg[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) wg[k] = 0.f;
+  const Angles<LPR> ang(p);
   harp_ra::sched_fence();
-  // (two copies of the walk: both tensors' strides side by side do not fit the scalar registers)
-  if ((int)blockIdx.x < ranges.q.n)
-    backward_share<F32, HALF, LPR, R>(p, p.t[0], ang, blockIdx.x, ranges.q.n, part);
-  else
-    backward_share<F32, HALF, LPR, R>(p, p.t[1], ang, blockIdx.x - ranges.q.n, ranges.k.n, part);
+  if ((int)blockIdx.x < n.q) backward_share<F32, HALF, LPR, R>(p, p.t[0], ang, blockIdx.x, n.q, n.q_steps, angles, wg);
+  else backward_share<F32, HALF, LPR, R>(p, p.t[1], ang, blockIdx.x - n.q, n.k, n.k_steps, angles, wg);
   if (!p.wpart) return;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) part[threadIdx.x / LPR][8 * (threadIdx.x % LPR) + k] = wg[k];
   __syncthreads();
   // value 2 k + e of the partial row is element e of pair k
   if ((int)threadIdx.x < p.D) {
@@ -466,9 +567,11 @@ namespace {
 
 int lanes_per_row(int D) { return D > 128 ? 32 : D > 64 ? 16 : 8; }
 
-constexpr int kFillBlocks = 1024;    // four blocks for each of 256 CUs
-constexpr int kBwdMaxBlocks = 1024;
-constexpr int64_t kLaunchBlocks = 1 << 22;  // of q and of k, 256 threads each: below 2^32 threads a launch
+constexpr int kFillBlocks = 1024;  // four blocks for each of 256 CUs
+// A long call's blocks walk their steps, four of them at a time on a CU, all in one round.  8192 tokens x 60
+// heads of 128: forward 52 us (58 with 1536 blocks), backward 85 (95 with 1280).
+constexpr int kMaxBlocks = 1024;
+constexpr int kOneStep = 1 << 30;  // no limit: a step to a block
 
 int64_t blocks_of(const RopeParams& p, const RopeHeads& t, int R) {
   const int per = kThreads / lanes_per_row(p.D);
@@ -482,7 +585,7 @@ int heads_per_group(const RopeParams& p, int most) {
   return 1;
 }
 template <template <bool, bool, int, int> class K>
-hipError_t dispatch(const RopeParams& p, int R, const Ranges& r, hipStream_t st) {
+hipError_t dispatch(const RopeParams& p, int R, const Blocks& r, hipStream_t st) {
   auto heads = [&](auto f32, auto half, auto l) {
     constexpr bool F = decltype(f32)::value, H = decltype(half)::value;
     constexpr int L = decltype(l)::value;
@@ -502,48 +605,49 @@ hipError_t dispatch(const RopeParams& p, int R, const Ranges& r, hipStream_t st)
 }
 template <bool F, bool H, int L, int R>
 struct Forward {
-  static void launch(const RopeParams& p, const Ranges& r, hipStream_t st) {
-    hipLaunchKernelGGL((rope_forward_kernel<F, H, L, R>), dim3((unsigned)(r.q.n + r.k.n)), dim3(kThreads), 0, st, p, r);
+  static void launch(const RopeParams& p, const Blocks& r, hipStream_t st) {
+    hipLaunchKernelGGL((rope_forward_kernel<F, H, L, R>), dim3((unsigned)(r.q + r.k)), dim3(kThreads), 0, st, p, r);
   }
 };
 constexpr int kBwdHeads = 2;  // rows of x and dy of four heads would leave a CU half the waves
 template <bool F, bool H, int L, int R>
 struct Backward {
-  static void launch(const RopeParams& p, const Ranges& r, hipStream_t st) {
+  static void launch(const RopeParams& p, const Blocks& r, hipStream_t st) {
     constexpr int B = R > kBwdHeads ? kBwdHeads : R;
-    hipLaunchKernelGGL((rope_backward_kernel<F, H, L, B>), dim3((unsigned)(r.q.n + r.k.n)), dim3(kThreads), 0, st, p, r);
+    hipLaunchKernelGGL((rope_backward_kernel<F, H, L, B>), dim3((unsigned)(r.q + r.k)), dim3(kThreads), 0, st, p, r);
   }
 };
 
-// at most kBwdMaxBlocks, as few as leave the busiest one no more steps
-int bwd_blocks(const RopeParams& p, const RopeHeads& t, int most) {
-  const int64_t steps = blocks_of(p, t, heads_per_group(p, kBwdHeads));
-  const int64_t each = (steps + most - 1) / most;
-  return each ? (int)((steps + each - 1) / each) : 0;
+// each tensor's share of at most `most` blocks, as few as leave the busiest one no more steps
+Blocks shares(const RopeParams& p, int R, int most) {
+  auto share = [&](const RopeHeads& t, int& blocks, uint32_t& each) {
+    const int64_t steps = blocks_of(p, t, R);
+    if (!steps) return;
+    const int64_t mine = std::max<int64_t>(1, (int64_t)most * t.H / (p.t[0].H + p.t[1].H));
+    each = (uint32_t)((steps + mine - 1) / mine);
+    blocks = (int)((steps + each - 1) / each);
+  };
+  Blocks n{};
+  share(p.t[0], n.q, n.q_steps);
+  share(p.t[1], n.k, n.k_steps);
+  return n;
 }
 
 }  // namespace
 
 hipError_t launch_rope_forward(const RopeParams& p, hipStream_t stream) {
   const int R = heads_per_group(p, 4);
-  const int64_t total[2] = {blocks_of(p, p.t[0], R), blocks_of(p, p.t[1], R)};
-  for (int64_t first = 0; first < std::max(total[0], total[1]); first += kLaunchBlocks) {
-    auto part = [&](int64_t n) { return Range{first, (int)std::max((int64_t)0, std::min(n - first, kLaunchBlocks))}; };
-    const hipError_t e = dispatch<Forward>(p, R, Ranges{part(total[0]), part(total[1])}, stream);
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
+  return dispatch<Forward>(p, R, shares(p, R, R == 4 ? kMaxBlocks : kOneStep), stream);
 }
 
 void rope_bwd_blocks(const RopeParams& p, int blocks[2]) {
-  const int rows = p.t[0].H + p.t[1].H;
-  for (int i = 0; i < 2; ++i)  // each tensor's share of the blocks
-    blocks[i] = p.t[i].H ? bwd_blocks(p, p.t[i], std::max(1, (int)((int64_t)kBwdMaxBlocks * p.t[i].H / rows))) : 0;
+  const Blocks n = shares(p, heads_per_group(p, kBwdHeads), kMaxBlocks);
+  blocks[0] = n.q;
+  blocks[1] = n.k;
 }
 hipError_t launch_rope_backward(const RopeParams& p, hipStream_t stream) {
-  int n[2];
-  rope_bwd_blocks(p, n);
-  return dispatch<Backward>(p, heads_per_group(p, kBwdHeads), Ranges{Range{0, n[0]}, Range{0, n[1]}}, stream);
+  const int R = heads_per_group(p, kBwdHeads);
+  return dispatch<Backward>(p, R, shares(p, R, kMaxBlocks), stream);
 }
 
 hipError_t launch_rope_wgrad(const float* wpart, const int blocks[2], int D, void* const gw[2], const int gw_f32[2],

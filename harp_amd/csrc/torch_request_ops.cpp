@@ -18,8 +18,10 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
 
+#include <cstring>
 #include <string>
 #include <tuple>
+#include <type_traits>
 #include <vector>
 
 #include "harp_request_ops.h"
@@ -124,11 +126,21 @@ at::Tensor weight_of(const OptTensor& w, const at::Tensor& x, const char* name) 
 
 struct RopeCall {
   Axes axes;
-  std::vector<double> eps;  // of q and k; negative: no norm
+  double eps[2];      // of q and k; negative: no norm
+  bool want[4] = {};  // of the gradients of q, k and their weights
 };
 RopeCall rope_call(at::IntArrayRef widths, at::ArrayRef<double> theta, bool half, at::ArrayRef<double> eps) {
-  RopeCall c{axes_of(widths, theta, half), eps.vec()};
-  TORCH_CHECK(c.eps.size() == 2, "eps must be two values, got ", c.eps.size());
+  TORCH_CHECK(eps.size() == 2, "eps must be two values, got ", eps.size());
+  return RopeCall{axes_of(widths, theta, half), {eps[0], eps[1]}};
+}
+// as one saved value (four lists of a call would cost the host some microseconds)
+std::string saved(const RopeCall& c) {
+  static_assert(std::is_trivially_copyable_v<RopeCall>);
+  return std::string(reinterpret_cast<const char*>(&c), sizeof(c));
+}
+RopeCall restored(const std::string& s) {
+  RopeCall c;
+  std::memcpy(&c, s.data(), sizeof(c));
   return c;
 }
 
@@ -241,20 +253,15 @@ std::vector<at::Tensor> rope_backward(const at::Tensor (&dy)[2], const at::Tenso
 class QkNormRope : public torch::autograd::Function<QkNormRope> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
-                                                const OptTensor& k, const at::Tensor& positions,
-                                                std::vector<int64_t> widths, std::vector<double> theta, bool half,
-                                                const OptTensor& qw, const OptTensor& kw, std::vector<double> eps) {
+                                                const OptTensor& k, const at::Tensor& positions, const OptTensor& qw,
+                                                const OptTensor& kw, RopeCall c) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    const RopeCall c = rope_call(widths, theta, half, eps);
     auto [yq, yk] = rope_forward(q, k, positions, c, qw, kw);
     ctx->set_materialize_grads(false);
     const at::Tensor none;
-    auto wants = [](const OptTensor& t) { return given(t) && t->requires_grad(); };
-    ctx->saved_data["widths"] = widths;
-    ctx->saved_data["theta"] = theta;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["flags"] =
-        (int64_t)half + 2 * q.requires_grad() + 4 * wants(k) + 8 * wants(qw) + 16 * wants(kw);
+    const OptTensor leaves[] = {q, k, qw, kw};
+    for (int i = 0; i < 4; ++i) c.want[i] = given(leaves[i]) && leaves[i]->requires_grad();
+    ctx->saved_data["call"] = saved(c);
     // (a rotation alone needs no input for its gradient)
     ctx->save_for_backward({c.eps[0] >= 0 ? q : none, given(k) && c.eps[1] >= 0 ? *k : none, given(qw) ? *qw : none,
                             given(kw) ? *kw : none, positions});
@@ -265,23 +272,21 @@ class QkNormRope : public torch::autograd::Function<QkNormRope> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const int64_t flags = ctx->saved_data["flags"].toInt();
+    const RopeCall c = restored(ctx->saved_data["call"].toStringRef());
     for (const auto& t : grads) harp_torch::refuse_tangent(t, "harp_request", "qk_norm_rope (backward)");
-    const bool want[2] = {(flags & 2) != 0, (flags & 4) != 0}, want_w[2] = {(flags & 8) != 0, (flags & 16) != 0};
-    torch::autograd::variable_list out(9);
+    torch::autograd::variable_list out(6);
     at::Tensor dy[2];
     for (size_t i = 0; i < grads.size(); ++i)
-      if (want[i] || want_w[i]) dy[i] = grads[i];
+      if (c.want[i] || c.want[2 + i]) dy[i] = grads[i];
     if (dy[0].defined() || dy[1].defined()) {
       at::AutoDispatchBelowADInplaceOrView guard;
-      const RopeCall c = rope_call(ctx->saved_data["widths"].toIntVector(), ctx->saved_data["theta"].toDoubleVector(),
-                                   flags & 1, ctx->saved_data["eps"].toDoubleVector());
       const at::Tensor x[2] = {saved[0], saved[1]}, w[2] = {saved[2], saved[3]};
+      const bool want_w[2] = {c.want[2], c.want[3]};
       auto g = rope_backward(dy, x, w, saved[4], c, want_w);
-      if (want[0]) out[0] = g[0];
-      if (want[1]) out[1] = g[1];
-      out[6] = g[2];
-      out[7] = g[3];
+      if (c.want[0]) out[0] = g[0];
+      if (c.want[1]) out[1] = g[1];
+      out[3] = g[2];
+      out[4] = g[3];
     }
     harp_torch::once_only(out, "qk_norm_rope");
     return out;
@@ -323,15 +328,14 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rope_autograd(const at::Tensor& q, co
     const char* const names[] = {"q", "k", "q_weight", "k_weight"};
     for (int i = 0; i < 4; ++i) harp_torch::check_capture(leaves[i], "qk_norm_rope", names[i]);
   }
-  auto out = QkNormRope::apply(q, k, positions, widths.vec(), theta.vec(), half, qw, kw, eps.vec());
+  auto out = QkNormRope::apply(q, k, positions, qw, kw, rope_call(widths, theta, half, eps));
   return {out[0], given(k) ? out[1] : at::Tensor()};
 }
 
-at::Tensor rope_table(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta) {
+at::Tensor table(const at::Tensor& positions, const Axes& ax) {
   TORCH_CHECK(positions.is_cuda(), "harp_request.rope_table: this library runs on a HIP device only");
   TORCH_CHECK(positions.dim() == 2 || positions.dim() == 3, "positions must be [S, axes] or [B, S, axes], got ",
               positions.sizes());
-  const Axes ax = axes_of(widths, theta, false);
   const c10::DeviceGuard guard(positions.device());
   const int64_t B = positions.dim() == 3 ? positions.size(0) : 1, S = positions.size(-2);
   const Positions pos = positions_of(positions, ax.a.n, B, S);
@@ -342,6 +346,9 @@ at::Tensor rope_table(const at::Tensor& positions, at::IntArrayRef widths, at::A
                                    (float*)out.data_ptr(), stream_of(positions)),
                "rope_table");
   return out;
+}
+at::Tensor rope_table(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta) {
+  return table(positions, axes_of(widths, theta, false));
 }
 at::Tensor rope_table_autograd(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta) {
   harp_torch::refuse_tangent(positions, "harp_request", "rope_table");
@@ -634,8 +641,7 @@ struct QkvResult {
   Tensors lin;   // of q and k before the norm [B, S, N], with keep
   Tensors t;     // x A^T of the three, with keep
 };
-QkvResult qkv_forward(const QkvCall& c, const at::Tensor& x, const std::vector<double>& eps, bool keep) {
-  TORCH_CHECK(eps.size() == 2, "eps must be two values, got ", eps.size());
+QkvResult qkv_forward(const QkvCall& c, const at::Tensor& x, const double (&eps)[2], bool keep) {
   const c10::DeviceGuard guard(x.device());
   QkvResult r;
   harp_qkv_out_t outs[3] = {};
@@ -678,15 +684,12 @@ QkvResult qkv_forward(const QkvCall& c, const at::Tensor& x, const std::vector<d
   return r;
 }
 
-at::Tensor table_of(const at::Tensor& positions, at::IntArrayRef widths, at::ArrayRef<double> theta,
-                    const at::Tensor& x) {
+at::Tensor table_of(const at::Tensor& positions, const RopeCall& c, const at::Tensor& x) {
   TORCH_CHECK(x.dim() == 3, "x must be [B, S, dim], got ", x.sizes());
   check_device(positions, x, "positions");
-  positions_of(positions, (int64_t)widths.size(), x.size(0), x.size(1));  // (their shape)
-  int64_t D = 0;
-  for (int64_t w : widths) D += w;
-  TORCH_CHECK(D == kHeadDim, "the axes' widths must add up to 128, got ", widths);
-  return rope_table(positions, widths, theta);
+  positions_of(positions, c.axes.a.n, x.size(0), x.size(1));  // (their shape)
+  TORCH_CHECK(c.axes.D == kHeadDim, "the axes' widths must add up to 128, got ", c.axes.D);
+  return table(positions, c.axes);
 }
 
 Tensors qkv_adapters(const at::Tensor& x, const Tensors& weights, const Tensors& a, const Tensors& b,
@@ -695,8 +698,11 @@ Tensors qkv_adapters(const at::Tensor& x, const Tensors& weights, const Tensors&
                      const OptTensor& positions, const std::vector<int64_t>& widths, const std::vector<double>& theta) {
   TORCH_CHECK(x.is_cuda(), "harp_request.qkv_adapters: tensors must be on a HIP device");
   TORCH_CHECK(!given(freqs) || !given(positions), "one rotation: freqs_cis or positions");
-  const OptTensor table = given(positions) ? OptTensor(table_of(*positions, widths, theta, x)) : freqs;
-  return qkv_forward(qkv_call(x, weights, a, b, scales, index, offsets, norm_weights, table), x, eps, false).y;
+  TORCH_CHECK(eps.size() == 2, "eps must be two values, got ", eps.size());
+  const double both[2] = {eps[0], eps[1]};
+  const OptTensor table =
+      given(positions) ? OptTensor(table_of(*positions, rope_call(widths, theta, false, eps), x)) : freqs;
+  return qkv_forward(qkv_call(x, weights, a, b, scales, index, offsets, norm_weights, table), x, both, false).y;
 }
 
 // Differentiable arguments in this order: x, three weights, two norm weights, three a, three b
@@ -710,23 +716,19 @@ class QkvAdapters : public torch::autograd::Function<QkvAdapters> {
                                                 const at::Tensor& ak, const at::Tensor& av, const at::Tensor& bq,
                                                 const at::Tensor& bk, const at::Tensor& bv,
                                                 c10::List<OptTensor> scales, const at::Tensor& index,
-                                                const OptTensor& offsets, std::vector<double> eps,
-                                                const at::Tensor& positions, std::vector<int64_t> widths,
-                                                std::vector<double> theta) {
+                                                const OptTensor& offsets, const at::Tensor& positions, RopeCall call) {
     at::AutoDispatchBelowADInplaceOrView guard;
     c10::List<OptTensor> norms;
     norms.push_back(nq);
     norms.push_back(nk);
-    const at::Tensor table = table_of(positions, widths, theta, x);
+    const at::Tensor table = table_of(positions, call, x);
     const QkvCall c = qkv_call(x, {wq, wk, wv}, {aq, ak, av}, {bq, bk, bv}, scales, index, offsets, norms, table);
-    const QkvResult r = qkv_forward(c, x, eps, true);
+    const QkvResult r = qkv_forward(c, x, call.eps, true);
     int64_t wanted = 0;
     const at::Tensor* const leaves[] = {&x, &wq, &wk, &wv, &nq, &nk, &aq, &ak, &av, &bq, &bk, &bv};
     for (int i = 0; i < kLeaves; ++i) wanted |= (int64_t)leaves[i]->requires_grad() << i;
     ctx->saved_data["wanted"] = wanted;
-    ctx->saved_data["eps"] = eps;
-    ctx->saved_data["widths"] = widths;
-    ctx->saved_data["theta"] = theta;
+    ctx->saved_data["call"] = saved(call);
     auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
     ctx->save_for_backward({x, wq, wk, wv, nq, nk, aq, ak, av, bq, bk, bv, or_none(scales.get(0)),
                             or_none(scales.get(1)), or_none(scales.get(2)), index, or_none(offsets), positions,
@@ -740,16 +742,14 @@ class QkvAdapters : public torch::autograd::Function<QkvAdapters> {
     const int64_t wanted = ctx->saved_data["wanted"].toInt();
     auto want = [&](int i) { return (wanted >> i & 1) != 0; };
     for (const auto& t : grads) harp_torch::refuse_tangent(t, "harp_request", "qkv_adapters (backward)");
-    torch::autograd::variable_list out(19);
+    torch::autograd::variable_list out(17);
     {
       at::AutoDispatchBelowADInplaceOrView guard;
       const at::Tensor &x = s[0], &index = s[15];
       const c10::DeviceGuard device(x.device());
       const int64_t B = x.size(0), S = x.size(1), K = x.size(2), N = s[1].size(0), H = N / kHeadDim, M = B * S;
       // through the rotation and the norm: the gradients of the three products [M, N]
-      const RopeCall rope = rope_call(ctx->saved_data["widths"].toIntVector(),
-                                      ctx->saved_data["theta"].toDoubleVector(), false,
-                                      ctx->saved_data["eps"].toDoubleVector());
+      const RopeCall rope = restored(ctx->saved_data["call"].toStringRef());
       auto heads = [&](const at::Tensor& t) { return t.unflatten(-1, {H, kHeadDim}).transpose(1, 2); };
       const at::Tensor d[2] = {grads[0], grads[1]}, lin[2] = {heads(s[18]), heads(s[19])}, nw[2] = {s[4], s[5]};
       const bool want_nw[2] = {want(4), want(5)};
@@ -847,7 +847,7 @@ Tensors qkv_adapters_autograd(const at::Tensor& x, const Tensors& weights, const
   }
   const Tensors& l = leaves;
   return QkvAdapters::apply(l[0], l[1], l[2], l[3], l[4], l[5], l[6], l[7], l[8], l[9], l[10], l[11], scales, index,
-                            offsets, eps, *positions, widths, theta);
+                            offsets, *positions, rope_call(widths, theta, false, eps));
 }
 
 [[noreturn]] void no_cpu(const char* op) {

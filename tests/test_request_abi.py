@@ -143,6 +143,7 @@ def test_rope_backward_refuses(over, code, msg):
 
 
 def test_rope_does_nothing_without_tokens():
+    assert harp_amd.load_abi().harp_req_qk_backward_workspace_bytes(1, 4, 128, 0, 0) == 0
     assert _rope(batch=0) == 0 and _rope(True, seq=0, ws=None, wsb=0) == 0 and _rope(q=_heads(heads=0)) == 0
 
 
