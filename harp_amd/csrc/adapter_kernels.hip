@@ -36,6 +36,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2u __attribute__((aligned(2)));
 
 constexpr int kThreads = 256;
+constexpr int kCUs = 256;
 
 // ---------------------------------------------------------------------------
 // Fragments
@@ -705,32 +706,38 @@ __global__ __launch_bounds__(kFewFeatures) void few_kernel(ExpandParams p, FewPa
 
 // ---------------------------------------------------------------------------
 // Gradients of A and B: for each adapter the sum over its tokens of v[m]^T x[m].
-// A block takes 128 columns and 32 RK ranks of one adapter, its four waves 32
-// columns each, and walks the adapter's tokens 64 at a time: the step's x (bf16)
-// and v (taken apart into two bf16) lie in LDS as they come, and
+// A block takes 128 columns and 32 RK ranks of one adapter.  Its four groups of four
+// waves (32 columns each) walk the adapter's tokens, 64 in a group's step: the step's x
+// (bf16) and v (taken apart into two bf16) lie in LDS as they come, and
 // ds_read_b64_tr_b16 reads both transposed, tokens along the contraction of
-// v_mfma_f32_32x32x16_bf16.  The next step's loads are on their way meanwhile.
+// v_mfma_f32_32x32x16_bf16.  The next step's loads are on their way meanwhile, and the
+// groups' sums are added in LDS in their order.
 // (v_mfma_f32_16x16x4_f32 takes the values without a transpose, and runs at a
 // sixteenth of the rate: rank 64 over 8192 tokens took 119 us.)  Where the
 // blocks of all adapters would not fill the chip, each request's tokens are taken
 // in `splits` parts whose sums a second kernel adds in order.
 // ---------------------------------------------------------------------------
 namespace {
-constexpr int kGradCols = 128, kGradStep = 64;
+constexpr int kGradCols = 128, kGradStep = 64, kGradGroups = 4, kGradThreads = kThreads * kGradGroups;
 
-// Rows of 128 bf16: 16-byte chunk c of row r at c ^ swz(r).  Row reads and the
-// transposed reads below are free of bank conflicts.
-__device__ __forceinline__ int grad_slot(int r, int c) { return r * 128 + ((c ^ harp_ra::swz(r)) << 3); }
+// Rows of W (128, 64 or 32) bf16: 16-byte chunk c of row r.  Row writes and the transposed reads below
+// (64 bytes of each of four rows at a time) are free of bank conflicts.
+template <int W>
+__device__ __forceinline__ int grad_slot(int r, int c) {
+  const int x = W == 128 ? harp_ra::swz(r) : W == 64 ? (r & 2) << 1 : 0;
+  return r * W + ((c ^ x) << 3);
+}
 
 // T[r0 + {4 g .. + 3, 8 + 4 g .. + 3}][32 db + l32]: of two lanes with one g each
 // register holds one token, the same for both operands.  In each group of 16
 // lanes, lane i's value s is element i % 4 of the 8 bytes that lane 4 s + i / 4 addresses.
+template <int W>
 __device__ __forceinline__ bf16x8 tr_frag(const bf16* t, int r0, int db) {
   const int lane = threadIdx.x & 63, g = lane >> 5, s = (lane >> 2) & 3, m = lane & 3;
   const int c = 4 * db + 2 * ((lane >> 4) & 1) + (m >> 1);
   const int ra = r0 + 4 * g + s, rb = ra + 8;
-  const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((harp_ra::lds_bf16x4*)(t + grad_slot(ra, c) + 4 * (m & 1)));
-  const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((harp_ra::lds_bf16x4*)(t + grad_slot(rb, c) + 4 * (m & 1)));
+  const auto lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((harp_ra::lds_bf16x4*)(t + grad_slot<W>(ra, c) + 4 * (m & 1)));
+  const auto hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((harp_ra::lds_bf16x4*)(t + grad_slot<W>(rb, c) + 4 * (m & 1)));
   bf16x8 r;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -750,10 +757,15 @@ struct Steps {
 }  // namespace
 
 template <int RK>
-__global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
-  __shared__ __attribute__((aligned(16))) bf16 xs[kGradStep * 128], vs[2][kGradStep * 128];
-  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+__global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_t all) {
+  constexpr int kRanks = 32 * RK, kPitch = kGradCols + 4;  // of the sums (a lane writes 4 columns of its rank)
+  constexpr int kX = kGradStep * kGradCols, kV = kGradStep * kRanks, kGroup = 2 * (kX + 2 * kV), kSums = kRanks * kPitch * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kGradGroups * (kGroup > kSums ? kGroup : kSums)];
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, tid = threadIdx.x % kThreads;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kThreads);
+  bf16* const xs = (bf16*)(lds + group * kGroup);
+  bf16* const vs = xs + kX;  // the parts one after the other
   // this block's part and columns (constant indices: see the shrink kernel)
   GradPart part = p.part[0];
   int cb = blockIdx.x;
@@ -771,9 +783,10 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
     }
   }
   const int c0 = cb * kGradCols;
-  const int rgroups = (p.rp + 32 * RK - 1) / (32 * RK);
-  const int adapter = (int)blockIdx.y / rgroups, r0 = (int)blockIdx.y % rgroups * 32 * RK;
+  const int rgroups = (p.rp + kRanks - 1) / kRanks;
+  const int adapter = (int)blockIdx.y / rgroups, r0 = (int)blockIdx.y % rgroups * kRanks;
   const int split = blockIdx.z;
+  harp_ra::sched_fence();  // (the parts' arguments and the walk's beside each other do not fit the scalar registers)
 
   f32x16 acc[RK];
 #pragma unroll
@@ -796,6 +809,23 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
     }
     return true;
   };
+  // the next step of every group, and whether there was one for the first; this group's is n tokens (or 0) from m on
+  int m = 0, n = 0;
+  auto deal = [&]() {
+    bool any = false;
+    n = 0;
+#pragma unroll 1
+    for (int q = 0; q < kGradGroups && next(); ++q) {
+      any = true;
+      const int rows = min(kGradStep, st.end - st.m);
+      if (q == group) {
+        m = st.m;
+        n = rows;
+      }
+      st.m += rows;
+    }
+    return any;
+  };
 
   // a thread's share of a step: x row tid / 16 + 16 k, 8 columns; v row tid / (4 RK)
   // + 64 / RK k, 8 ranks
@@ -803,7 +833,7 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
   bf16x8 xv[4];
   f32x4 vv[kVPass][2];
   const int xr = tid >> 4, xc = tid & 15, vr = tid / kVLanes, vc = tid % kVLanes;
-  auto load = [&](int m, int n) {
+  auto load = [&]() {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int row = xr + 16 * k, left = part.C - c0 - 8 * xc;
@@ -824,13 +854,12 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
       }
     }
   };
-  bool more = next();
-  if (more) load(st.m, min(kGradStep, st.end - st.m));
+  bool more = deal();
+  load();
   while (more) {
-    const int n = min(kGradStep, st.end - st.m);
-    st.m += n;
+    const int ksteps = (n + 15) / 16;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) *(bf16x8*)(xs + grad_slot(xr + 16 * k, xc)) = xv[k];
+    for (int k = 0; k < 4; ++k) *(bf16x8*)(xs + grad_slot<kGradCols>(xr + 16 * k, xc)) = xv[k];
 #pragma unroll
     for (int k = 0; k < kVPass; ++k) {
       bf16x8 hi, lo;
@@ -840,37 +869,44 @@ __global__ __launch_bounds__(kThreads) void grad_kernel(GradParams p) {
         hi[e] = (bf16)f;
         lo[e] = (bf16)(f - (float)hi[e]);
       }
-      *(bf16x8*)(vs[0] + grad_slot(vr + kVRows * k, vc)) = hi;
-      *(bf16x8*)(vs[1] + grad_slot(vr + kVRows * k, vc)) = lo;
+      *(bf16x8*)(vs + grad_slot<kRanks>(vr + kVRows * k, vc)) = hi;
+      *(bf16x8*)(vs + kV + grad_slot<kRanks>(vr + kVRows * k, vc)) = lo;
     }
     __syncthreads();
-    more = next();
-    if (more) load(st.m, min(kGradStep, st.end - st.m));
-    const int ksteps = (n + 15) / 16;
+    more = deal();
+    load();
     for (int k = 0; k < ksteps; ++k) {
-      const bf16x8 xf = tr_frag(xs, 16 * k, wave);
+      const bf16x8 xf = tr_frag<kGradCols>(xs, 16 * k, wave);
 #pragma unroll
       for (int j = 0; j < RK; ++j)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) acc[j] = harp_ra::mfma32x32x16(xf, tr_frag(vs[h], 16 * k, j), acc[j]);
+        for (int h = 0; h < 2; ++h)
+          acc[j] = harp_ra::mfma32x32x16(xf, tr_frag<kRanks>(vs + h * kV, 16 * k, j), acc[j]);
     }
     __syncthreads();
   }
 
-  // a lane holds rank r0 + 32 j + l32 and columns 8 a + 4 g .. + 3 of the wave's 32
+  // a lane holds rank 32 j + l32 and columns 8 a + 4 g .. + 3 of the wave's 32
+  float* const sums = (float*)lds;
 #pragma unroll
-  for (int j = 0; j < RK; ++j) {
-    const int rank = r0 + 32 * j + l32;
-    if (rank >= p.r) continue;
+  for (int j = 0; j < RK; ++j)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int c = c0 + 32 * wave + harp_ra::c_row(e, g);
-      if (c >= part.C) continue;
-      const int64_t o = part.cols_first ? ((int64_t)adapter * part.C + c) * p.r + rank
-                                        : ((int64_t)adapter * p.r + rank) * part.C + c;
-      if (p.splits == 1) ((bf16*)part.out)[o] = (bf16)acc[j][e];
-      else p.work[split * grad_values(p) + at + o] = acc[j][e];
-    }
+    for (int e = 0; e < 16; e += 4)
+      *(f32x4*)(sums + (group * kRanks + 32 * j + l32) * kPitch + 32 * wave + harp_ra::c_row(e, g)) =
+          f32x4{acc[j][e], acc[j][e + 1], acc[j][e + 2], acc[j][e + 3]};
+  __syncthreads();
+  // out as it lies in memory, one value a thread
+  const int ranks = min(kRanks, p.r - r0), cols = min(kGradCols, part.C - c0);
+  for (int i = threadIdx.x; i < kRanks * kGradCols; i += kGradThreads) {
+    const int rank = part.cols_first ? i % kRanks : i / kGradCols, c = part.cols_first ? i / kRanks : i % kGradCols;
+    if (rank >= ranks || c >= cols) continue;
+    float sum = sums[rank * kPitch + c];
+#pragma unroll
+    for (int q = 1; q < kGradGroups; ++q) sum += sums[(q * kRanks + rank) * kPitch + c];
+    const int64_t o = part.cols_first ? ((int64_t)adapter * part.C + c0 + c) * p.r + r0 + rank
+                                      : ((int64_t)adapter * p.r + r0 + rank) * part.C + c0 + c;
+    if (p.splits == 1) ((bf16*)part.out)[o] = (bf16)sum;
+    else p.work[split * all + at + o] = sum;
   }
 }
 
@@ -917,9 +953,17 @@ __global__ __launch_bounds__(kThreads) void transpose_kernel(TransposeParams p) 
   for (int i = blockIdx.y; i < p.n; i += gridDim.y) {
     const uint16_t* src = (const uint16_t*)part.src + (int64_t)i * part.rows * part.cols;
     uint16_t* dst = (uint16_t*)part.dst + (int64_t)i * part.cols * part.ld;
-    for (int y = ty; y < 64; y += 4)
-      t[y][tx] = r0 + y < part.rows && c0 + tx < part.cols ? src[(int64_t)(r0 + y) * part.cols + c0 + tx] : (uint16_t)0;
+    uint16_t v[16];  // (all of them on their way at once)
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int r = r0 + ty + 4 * k, c = c0 + tx;
+      v[k] = src[(int64_t)min(r, part.rows - 1) * part.cols + min(c, part.cols - 1)];
+      if (r >= part.rows || c >= part.cols) v[k] = 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t[ty + 4 * k][tx] = v[k];
     __syncthreads();
+#pragma unroll
     for (int y = ty; y < 64; y += 4)
       if (c0 + y < part.cols && r0 + tx < fill) dst[(int64_t)(c0 + y) * part.ld + r0 + tx] = t[tx][y];
     __syncthreads();
@@ -941,9 +985,9 @@ hipError_t shrink_t(const ShrinkParams& p, hipStream_t st) {
                      dim3(64 * WAVES), 0, st, p);
   return hipGetLastError();
 }
-template <int TB, int RB, int WAVES>
+template <int TB, int RB, int WAVES, int STAGES>
 hipError_t shrink_lds_t(const ShrinkParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((shrink_lds_kernel<TB, RB, WAVES, 3>),
+  hipLaunchKernelGGL((shrink_lds_kernel<TB, RB, WAVES, STAGES>),
                      dim3((unsigned)slots_of(p.req, 16 * TB), shrink_groups<RB>(p)), dim3(64 * WAVES), 0, st, p);
   return hipGetLastError();
 }
@@ -959,8 +1003,18 @@ hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
   const bool few = slots_of(p.req, 16) * (p.rp / 16) * p.sets <= 512;
   const int total = p.rp / 16 * (p.apart ? 1 : p.sets);
   if (aligned) {
-    if (few) return shrink_lds_t<1, 1, 8>(p, st);
-    return total == 1 ? shrink_lds_t<2, 1, 4>(p, st) : total == 2 ? shrink_lds_t<2, 2, 4>(p, st) : shrink_lds_t<2, 4, 4>(p, st);
+    if (few) return shrink_lds_t<1, 1, 8, 3>(p, st);
+    // Tiles of 64 tokens read A half as often and leave half as many blocks, one to a CU: they win where 32 tokens a
+    // tile take more than one round.  K = 3840, rank 64: 16384 tokens 42 -> 36 us, 12000 tokens 38 -> 31, but 8192
+    // tokens 22.5 -> 28; rank 32: 35 -> 29.5, 31 -> 28, 18 -> 22.
+    if (p.req.tokens > 32 * kCUs && p.req.tokens / std::max(p.req.count, 1) >= 64)
+      return total == 1   ? shrink_lds_t<4, 1, 4, 3>(p, st)
+             : total == 2 ? shrink_lds_t<4, 2, 4, 3>(p, st)
+                          : shrink_lds_t<4, 4, 4, 2>(p, st);
+    // (96 KB and more of LDS each: blocks that leave room for a second one land on one CU in twos: 16 us, with half 22)
+    return total == 1   ? shrink_lds_t<2, 1, 8, 2>(p, st)
+           : total == 2 ? shrink_lds_t<2, 2, 4, 3>(p, st)
+                        : shrink_lds_t<2, 4, 4, 3>(p, st);
   }
   // the waves of a block share K: 16 of them where each has a 64-column step
   if (p.K < 1024) return few ? shrink_t<1, 1, 4>(p, st) : shrink_t<2, 4, 4>(p, st);
@@ -1049,16 +1103,17 @@ int grad_groups(const GradParams& p) { return (p.rp + 63) / 64; }  // 64 ranks a
 template <int RK>
 hipError_t grad_t(const GradParams& p, hipStream_t st) {
   const dim3 grid((unsigned)grad_blocks(p), (unsigned)(p.req.n * ((p.rp + 32 * RK - 1) / (32 * RK))), (unsigned)p.splits);
-  hipLaunchKernelGGL((grad_kernel<RK>), grid, dim3(kThreads), 0, st, p);
+  hipLaunchKernelGGL((grad_kernel<RK>), grid, dim3(kGradThreads), 0, st, p,
+                     grad_values(p));
   return hipGetLastError();
 }
 }  // namespace
 int grad_splits(const GradParams& p) {
   const int64_t blocks = (int64_t)grad_blocks(p) * std::min(p.req.n, p.req.count) * grad_groups(p);
   if (!blocks) return 1;
-  const int64_t want = (512 + blocks - 1) / blocks;                               // two blocks a CU
-  const int64_t most = std::max<int64_t>(1, p.req.tokens / p.req.count / 128);    // of 128 tokens at least
-  return (int)std::min(want, most);
+  const int64_t want = (kCUs + blocks / 2) / blocks;  // a block to a CU, more or less
+  const int64_t most = p.req.tokens / p.req.count / (kGradStep * kGradGroups);  // a step for every group at least
+  return (int)std::max<int64_t>(1, std::min(want, most));
 }
 hipError_t launch_adapter_grad(const GradParams& p, hipStream_t st) {
   const hipError_t e = p.rp <= 32 ? grad_t<1>(p, st) : grad_t<2>(p, st);

@@ -7,7 +7,7 @@
 // behind the last) starts at slot a_i / M + i, where its first token is a_i:
 // floor(b / M) + i + 1 - (floor(a / M) + i) is never less than the ceil((b - a) / M)
 // tiles it needs, so no tile is shared by two requests, nothing is counted
-// beforehand, and a block finds its segment by one or two 64-way searches.
+// beforehand, and a block finds its segment by a 64-way search.
 // What the arrays hold is clamped before it is used as an index.
 #pragma once
 
@@ -35,12 +35,12 @@ __device__ __forceinline__ int segment_start(const Requests& q, int i) {
   return i > q.count + 1 ? q.tokens : token_of(q, i - 1);
 }
 
-// The largest segment i (0 .. count + 1) with at(i), which holds for 0 and, in order, for no others than a first run
+// at(i) holds for segment 0 and, in order, for no others than a first run of the segments 0 .. count + 1.
+// at(lo) holds, hi is behind the last segment or at(hi) does not: narrows both to at most `most` apart.
 template <class F>
-__device__ __forceinline__ int last_segment(const Requests& q, F at) {
+__device__ __forceinline__ void narrow(int& lo, int& hi, int most, F at) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, hi = q.count + 2;  // at(lo) holds; hi is behind the last segment or at(hi) does not hold
-  while (hi - lo > 1) {          // (uniform, and hi - lo shrinks 64-fold)
+  while (hi - lo > most) {  // (uniform, and hi - lo shrinks 64-fold)
     const int step = (hi - lo + 63) / 64;
     const int i = lo + lane * step;
     const uint64_t b = __ballot(i < hi && at(i)) | 1;
@@ -48,24 +48,37 @@ __device__ __forceinline__ int last_segment(const Requests& q, F at) {
     hi = min(hi, lo + (k + 1) * step);
     lo = lo + k * step;
   }
-  return __builtin_amdgcn_readfirstlane(lo);
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  hi = __builtin_amdgcn_readfirstlane(hi);
+}
+// The largest segment i with at(i)
+template <class F>
+__device__ __forceinline__ int last_segment(const Requests& q, F at) {
+  int lo = 0, hi = q.count + 2;
+  narrow(lo, hi, 1, at);
+  return lo;
 }
 
 // A tile: rows first .. first + rows - 1 (rows <= M, or not positive) with one adapter (-1: none)
 struct Tile {
   int first, rows, adapter;
 };
+// (the last 62 candidates' starts and adapters come with one load each, one in every lane: each load that
+// waits for another costs a short call most of a microsecond)
 template <int M>
 __device__ __forceinline__ Tile tile_at(const Requests& q, int slot) {
-  const int i = last_segment(q, [&](int s) { return segment_start(q, s) / M + s <= slot; });
-  const int a = segment_start(q, i), b = segment_start(q, i + 1);
+  const int lane = threadIdx.x & 63;
+  int lo = 0, hi = q.count + 2;
+  narrow(lo, hi, 63, [&](int s) { return segment_start(q, s) / M + s <= slot; });
+  const int i = lo + lane, start = segment_start(q, i);
+  const int adapter = i >= 1 && i <= q.count ? adapter_of(q, i - 1) : -1;
+  const uint64_t in = __ballot(i < hi && start / M + i <= slot) | 1;
+  const int k = __ffsll((unsigned long long)~in) - 2;  // (0 .. 62: the segment is lo + k)
   Tile t;
-  t.first = a + (slot - (a / M + i)) * M;
+  const int a = __builtin_amdgcn_readlane(start, k), b = __builtin_amdgcn_readlane(start, k + 1);
+  t.first = a + (slot - (a / M + lo + k)) * M;
   t.rows = min(M, b - t.first);
-  t.adapter = i >= 1 && i <= q.count ? adapter_of(q, i - 1) : -1;
-  t.first = __builtin_amdgcn_readfirstlane(t.first);
-  t.rows = __builtin_amdgcn_readfirstlane(t.rows);
-  t.adapter = __builtin_amdgcn_readfirstlane(t.adapter);
+  t.adapter = __builtin_amdgcn_readlane(adapter, k);
   return t;
 }
 inline int64_t slots_of(const Requests& q, int M) { return (int64_t)q.tokens / M + q.count + 2; }

@@ -112,6 +112,7 @@ QKV = [
     (1, 1500, 2, 128, 128, 2, [0, 700, 1400]),
     (4, 1, 2, 128, 16, 4, None),
     (1, 5000, 10, 64, 16, 2, [0, 1, 2, 3, 4000, 5000]),     # the large blocks
+    (3, 235, 30, 128, 72, 3, None),                         # whole blocks, a third of the CUs without one
     (1, 4300, 30, 128, 40, 3, [0, 2200, 4300]),             # and the second launch of smaller ones
 ]
 
