@@ -788,7 +788,7 @@ class QkvAdapters : public torch::autograd::Function<QkvAdapters> {
           dx = at::empty({B, S, K}, x.options());
           if (M) {
             base = at::mm(gy[0], s[1], at::kFloat);
-            for (int i = 1; i < 3; ++i) base = at::addmm(base, gy[i], s[1 + i], at::kFloat);
+            for (int i = 1; i < 3; ++i) at::addmm_out(base, base, gy[i], s[1 + i], at::kFloat);
           }
         }
         if (M) {
