@@ -132,51 +132,60 @@ def adapt_attention(attn, to_q: Optional[Adapters] = None, to_k: Optional[Adapte
     return AdaptedAttention(attn, to_q=to_q, to_k=to_k, to_v=to_v, to_out=to_out)
 
 
-def fused_adapters_supported(attn, hidden_states: torch.Tensor, freqs, requests: AdapterRequests) -> bool:
-    """True when :func:`project_qkv_adapters` takes this module and input: adapters of one number and one rank, a
-    multiple of 8, beside bfloat16 projections without a bias, heads of 128 features, norms of both q and k with a
-    rotation, positions along interleaved axes where a gradient is recorded, and requests of 32 tokens or more on
-    the average, or few of them."""
+def fused_adapters_arguments(attn, hidden_states: torch.Tensor, freqs, requests: AdapterRequests) -> Optional[tuple]:
+    """What :func:`project_qkv_adapters` takes for this module and input, or None where it does not: adapters of one
+    number and one rank, a multiple of 8, beside bfloat16 projections without a bias, heads of 128 features, norms of
+    both q and k with a rotation, positions along interleaved axes where a gradient is recorded, and requests of 8
+    tokens or more on the average, or few of them."""
     lins = (attn.to_q, attn.to_k, attn.to_v)
-    if not all(is_adapted(m) for m in lins) or any(isinstance(m.base, Int8Linear) for m in lins):
-        return False
-    axial = isinstance(freqs, AxialPositions)
-    if not isinstance(hidden_states, torch.Tensor) or not (axial or freqs is None or freqs.dtype == torch.complex64):
-        return False
-    if any(m.a.shape != lins[0].a.shape or m.b.shape != lins[0].b.shape for m in lins) or lins[0].a.size(1) % 8:
-        return False
-    if any(not (t.is_contiguous() and t.dtype == torch.bfloat16 and t.device == hidden_states.device
-                and t.data_ptr() % 16 == 0) for m in lins for t in (m.a, m.b)):
-        return False
+    if not all(is_adapted(m) for m in lins) or not isinstance(hidden_states, torch.Tensor):
+        return None
+    bases = [m.base for m in lins]
+    if any(isinstance(m, Int8Linear) for m in bases):
+        return None
+    a, b = [m.a for m in lins], [m.b for m in lins]
+    if a[1].shape != a[0].shape or a[2].shape != a[0].shape or a[0].size(1) % 8:
+        return None
+    if b[1].shape != b[0].shape or b[2].shape != b[0].shape:
+        return None
+    device = hidden_states.device
+    for t in (*a, *b):
+        if not t.is_contiguous() or t.dtype != torch.bfloat16 or t.device != device or t.data_ptr() % 16:
+            return None
     tokens = hidden_states.numel() // max(hidden_states.size(-1), 1)
-    if requests.index.numel() > 16 and tokens < 32 * requests.index.numel():
-        return False  # a tile of the contraction for each request among 128 or 256 tokens
-    norms = [getattr(attn, n, None) for n in ("norm_q", "norm_k")]
-    weights = [getattr(n, "weight", None) for n in norms]
-    if axial and (freqs.rope.layout != "interleaved" or freqs.rope.dim != HEAD_DIM):
-        return False
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (
-            hidden_states, *weights, *(t for m in lins for t in (m.a, m.b, m.base.weight)))):
-        if not axial or any(w is None for w in weights):
-            return False
-    bare = SimpleNamespace(heads=attn.heads, norm_q=norms[0], norm_k=norms[1], to_q=lins[0].base, to_k=lins[1].base,
-                           to_v=lins[2].base)
-    if axial and any(w is None for w in weights):
-        return False
-    return fused_supported(bare, hidden_states, None if axial else freqs)
+    count = requests.index.numel()
+    # The contraction takes a tile more for each request among a block's tokens, 128 or 256 of them.  30 heads from
+    # 3840 features, rank 16, one launch and parts: 32 requests of 8 tokens 65 and 93 us, of one token 79 and 61;
+    # 16 of one token 60 and 53, 8 of one token 51 and 51.
+    if count > 8 and tokens < 8 * count:
+        return None
+    norms = [getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)]
+    norm_weights = [getattr(n, "weight", None) for n in norms]
+    axial = isinstance(freqs, AxialPositions)
+    if axial:
+        rope = freqs.rope
+        if rope.layout != "interleaved" or rope.dim != HEAD_DIM or norm_weights[0] is None or norm_weights[1] is None:
+            return None
+    elif freqs is not None and freqs.dtype != torch.complex64:
+        return None
+    bare = SimpleNamespace(heads=attn.heads, norm_q=norms[0], norm_k=norms[1], to_q=bases[0], to_k=bases[1],
+                           to_v=bases[2])
+    if not fused_supported(bare, hidden_states, None if axial else freqs):
+        return None
+    weights = [m.weight for m in bases]
+    if not axial and torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (hidden_states, *norm_weights, *a, *b, *weights)):
+        return None
+    eps = [0.0 if n is None else float(n.eps) for n in norms]
+    rotation = (None, freqs.positions, rope.axes_dims, rope.theta) if axial else (freqs, None, (), ())
+    return (hidden_states, weights, a, b, [m.scales for m in lins], requests.index, requests.offsets, norm_weights, eps,
+            *rotation)
 
 
-def project_qkv_adapters(attn, hidden_states: torch.Tensor, freqs, requests: AdapterRequests):
+def project_qkv_adapters(arguments: tuple):
     """q, k, v [B, H, S, 128] (token-major strides) of a module with adapters beside all three projections: one
     launch for x A^T, one for the products, the adapters, the QK RMSNorm and the rotation."""
-    lins = (attn.to_q, attn.to_k, attn.to_v)
-    norms = [getattr(attn, n, None) for n in ("norm_q", "norm_k")]
-    axial = isinstance(freqs, AxialPositions)
-    q, k, v = _ops().qkv_adapters(
-        hidden_states, [m.base.weight for m in lins], [m.a for m in lins], [m.b for m in lins],
-        [m.scales for m in lins], requests.index, requests.offsets, [None if n is None else n.weight for n in norms],
-        [0.0 if n is None else float(n.eps) for n in norms], None if axial else freqs,
-        freqs.positions if axial else None, freqs.rope.axes_dims if axial else (), freqs.rope.theta if axial else ())
+    q, k, v = _ops().qkv_adapters(*arguments)
     return q, k, v
 
 

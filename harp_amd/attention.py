@@ -38,7 +38,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import nn
 
-from .adapters import (AdapterRequests, add_adapters, fused_adapters_supported, is_adapted,
+from .adapters import (AdapterRequests, add_adapters, fused_adapters_arguments, is_adapted,
                        project_qkv_adapters)
 from .int8 import Int8Linear, Int8Rows, fused_int8_supported, is_int8, project_qkv_int8, quantize_int8
 from .ops import RingAttention
@@ -80,8 +80,10 @@ def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: 
                      fused: bool, requests: Optional[AdapterRequests]
                      ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """project_qkv of a module with adapters."""
-    if fused and requests is not None and fused_adapters_supported(attn, hidden_states, freqs, requests):
-        return project_qkv_adapters(attn, hidden_states, freqs, requests)
+    if fused and requests is not None:
+        arguments = fused_adapters_arguments(attn, hidden_states, freqs, requests)
+        if arguments is not None:
+            return project_qkv_adapters(arguments)
     x, heads, rows = hidden_states, attn.heads, None
     bases = [m.base if is_adapted(m) else m for m in (attn.to_q, attn.to_k, attn.to_v)]
     int8 = [isinstance(m, Int8Linear) for m in bases]
