@@ -49,6 +49,11 @@ __device__ __forceinline__ bf16x8 load_some(const bf16* p, int n) {
     if (i < n) v[i] = p[i];
   return v;
 }
+// what the rounding b left of v; nothing behind an infinity, whose difference would be NaN
+__device__ __forceinline__ float rest(float v, bf16 b) {
+  constexpr float kMost = 0x1.fep127f;  // of bf16
+  return __builtin_amdgcn_fmed3f(v, -kMost, kMost) - __builtin_amdgcn_fmed3f((float)b, -kMost, kMost);
+}
 __device__ __forceinline__ bf16x8 load_full(const bf16* p) { return __builtin_bit_cast(bf16x8, *(const u32x4u*)p); }
 
 }  // namespace
@@ -77,7 +82,7 @@ __device__ __forceinline__ void shrink_store(const ShrinkParams& p, const Tile& 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         hi[k] = (bf16)s[k];
-        lo[k] = (bf16)(s[k] - (float)hi[k]);
+        lo[k] = (bf16)rest(s[k], hi[k]);
       }
       bf16* t = (bf16*)set.pairs + m * 2 * p.rp + rank;
       *(u32x2*)t = *(const u32x2*)hi;
@@ -417,7 +422,7 @@ struct Expand {
         for (int k = 0; k < 8; ++k) {
           const bf16 b = (bf16)v[k];
           tf[s][part][k] = b;
-          v[k] -= (float)b;
+          v[k] = rest(v[k], b);
         }
     }
   }
@@ -786,6 +791,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
   const int rgroups = (p.rp + kRanks - 1) / kRanks;
   const int adapter = (int)blockIdx.y / rgroups, r0 = (int)blockIdx.y % rgroups * kRanks;
   const int split = blockIdx.z;
+  float* const work = p.work + split * all + at;
   harp_ra::sched_fence();  // (the parts' arguments and the walk's beside each other do not fit the scalar registers)
 
   f32x16 acc[RK];
@@ -867,7 +873,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
       for (int e = 0; e < 8; ++e) {
         const float f = vv[k][e / 4][e % 4];
         hi[e] = (bf16)f;
-        lo[e] = (bf16)(f - (float)hi[e]);
+        lo[e] = (bf16)(f - (float)hi[e]);  // (an infinite t or u has no gradient to give: NaN)
       }
       *(bf16x8*)(vs + grad_slot<kRanks>(vr + kVRows * k, vc)) = hi;
       *(bf16x8*)(vs + kV + grad_slot<kRanks>(vr + kVRows * k, vc)) = lo;
@@ -906,7 +912,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
     const int64_t o = part.cols_first ? ((int64_t)adapter * part.C + c0 + c) * p.r + r0 + rank
                                       : ((int64_t)adapter * p.r + r0 + rank) * part.C + c0 + c;
     if (p.splits == 1) ((bf16*)part.out)[o] = (bf16)sum;
-    else p.work[split * all + at + o] = sum;
+    else work[o] = sum;
   }
 }
 

@@ -353,12 +353,12 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
       const int first = max(start, m0), adapter = seg ? harp_req::adapter_of(lo.req, seg - 1) : -1;
       start = end;
       if (adapter < 0 || first >= end) continue;
-      const rsrc_t tr_rsrc = make_rsrc(tb, (uint32_t)(rows_x * lo.rp * 4));
-      const rsrc_t b_rsrc = make_rsrc(bb + ((int64_t)adapter * p.heads + h0) * kHeadDim * lo.r,
-                                      (uint32_t)(rows_w * lo.r * 2));
       for (int c0 = 0; c0 < chunks; c0 += 8) {
         // every wave has read the last tile's fragments
         __syncthreads();
+        const rsrc_t tr_rsrc = make_rsrc(tb, (uint32_t)(rows_x * lo.rp * 4));
+        const rsrc_t b_rsrc = make_rsrc(bb + ((int64_t)adapter * p.heads + h0) * kHeadDim * lo.r,
+                                        (uint32_t)(rows_w * lo.r * 2));
 #pragma unroll
         for (int k = 0; k < kXPerWave; ++k) {
           const int r = (wave + kWaves * k) * 8 + tr, c = c0 + tile_pos(r, tc), m = m0 + r;
@@ -374,14 +374,37 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
         }
         wait_lds_loads();
         __syncthreads();
+        // into sums of their own, taken for the request's tokens only: to the others, an infinity
+        // or NaN in this adapter's B times the zeros is NaN (a second loop for blocks of one request's
+        // tokens does not fit the registers; its fewer LDS reads are worth 1.5% at rank 16)
         const int steps = min(4, (chunks - c0 + 1) / 2);
-        for (int ks = 0; ks < steps; ++ks) {
-          const Frags<NJ> f = load(0, ks);
-          mma(f, false, {}, {}, 0);
+        const char* const xs = Xs(0) + tg * TPW * kRowBytes;
+        const char* const ws = Ws(0) + hh * kHeadDim * kRowBytes;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int m = m0 + TPW * tg + 32 * j + l32;
+          const bool mine = m >= first && m < end;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f32x16 d = zero16();
+#pragma unroll 1
+            for (int ks = 0; ks < steps; ++ks) {
+              const int at = l32 * kRowBytes + (tile_pos(l32, 2 * ks + g) << 4);  // (foff[ks])
+              d = mfma32x32x16(*(const bf16x8*)(ws + 32 * i * kRowBytes + at),
+                               *(const bf16x8*)(xs + 32 * j * kRowBytes + at), d);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] += mine ? d[r] : 0.f;
+            asm volatile("" : "+v"(acc[i][j]));  // (one tile at a time: more of them do not fit the registers)
+          }
         }
       }
     }
   }
+  // (LOW: the output's arguments read again here, or they and the requests' do not fit the scalar registers)
+  int ye = y;
+  if constexpr (LOW) asm volatile("" : "+s"(ye));
+  const ProjOut oe = LOW ? (ye == 0 ? p.out[0] : (ye == 1 ? p.out[1] : p.out[2])) : o;
   if (norm && tid < kHeadDim) norm_wf[tid] = wreg;
   // every wave is past its fragment reads: the stages become staging rows
   __syncthreads();
@@ -415,7 +438,7 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
       const int r = 4 * k + (lane_e >> 4), c = lane_e & 15;
       const uint4 v = *(const uint4*)(stg + r * 256 + ((c ^ (r & 15)) << 4));
       const int64_t m = m0 + TPW * tg + r;
-      if (m < p.M) *(uint4*)(base + m * o.ldy + h * kHeadDim + c * 8) = v;
+      if (m < p.M) *(uint4*)(base + m * oe.ldy + h * kHeadDim + c * 8) = v;
     }
   };
   // two results: exact in bf16 or truncated to it, or (LOW) rounded to nearest
@@ -432,7 +455,7 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
   };
   if (!norm) {
     put_rounded();
-    stage_flush(o.y);
+    stage_flush(oe.y);
     return;
   }
 
@@ -452,9 +475,9 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
   };
   // loaded before any store (a load issued after a store would wait for it)
   if (rope) load_freqs(0);
-  if (o.y_lin) {
+  if (oe.y_lin) {
     put_rounded();
-    stage_flush(o.y_lin);
+    stage_flush(oe.y_lin);
   }
 
   // RMSNorm: sum of squares over the head's 128 features = this lane's 64 +
@@ -468,12 +491,12 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
 #pragma unroll
       for (int r = 0; r < 16; ++r) ss = __builtin_fmaf(acc[i][j][r], acc[i][j][r], ss);
     ss = half_wave_sum(ss);
-    const float rms = __fsqrt_rn(__fdiv_rn(ss, (float)kHeadDim) + o.eps);
+    const float rms = __fsqrt_rn(__fdiv_rn(ss, (float)kHeadDim) + oe.eps);
     const float inv = __fdiv_rn(1.f, rms);
     const int64_t m = m0 + TPW * tg + 32 * j + l32e;
-    if (ge == 0 && o.rms && m < p.M) {
+    if (ge == 0 && oe.rms && m < p.M) {
       const int b = (int)(m / p.S), s = (int)(m % p.S);
-      o.rms[((int64_t)b * p.heads + h) * p.S + s] = rms;
+      oe.rms[((int64_t)b * p.heads + h) * p.S + s] = rms;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -500,7 +523,7 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
         stage_put(j, i, q, pair(y[0], y[1]), pair(y[2], y[3]));
       }
   }
-  stage_flush(o.y);
+  stage_flush(oe.y);
 }
 
 namespace {

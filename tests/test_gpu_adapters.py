@@ -341,3 +341,47 @@ def test_refusals():
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             f(base, torch.autograd.forward_ad.make_dual(x, x), low, ok)
+
+
+def _same_where_not_finite(got, want, signs):
+    """An infinite t stays an infinity of its sign.  An infinity in B may become NaN: t is taken apart into hi + lo,
+    lo is zero or of either sign, and hi inf + lo inf is then NaN."""
+    assert torch.equal(torch.isfinite(got), torch.isfinite(want))
+    if signs:
+        for f in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(f(got), f(want)), f
+
+
+@pytest.mark.parametrize("T,r,dtype", [(3, 16, B16), (9, 16, B16), (60, 16, B16), (60, 40, F32), (600, 32, B16), (600, 16, F32)])
+def test_infinities_stay_with_their_request_and_stay_infinities(T, r, dtype):
+    """Three requests; the second's adapter sums to infinities (in t, or in B), the others' rows are as without it."""
+    g = _gen(T + r)
+    K, N, n = 64, 96, 3
+    base, x = _rand(g, T, N, dtype=dtype), _rand(g, T, K)
+    low = _low(g, n, r, K, N)
+    requests = harp_amd.AdapterRequests(torch.tensor([0, 1, 2], device=DEV))
+    clean = harp_amd.add_adapters(base, x, low, requests)
+    part = slice(T // 3, 2 * (T // 3))
+    for which in ("a", "b", "nan"):
+        a, b = low.a.clone(), low.b.clone()
+        if which == "a":  # one rank's t is an infinity of x's sign; the other ranks add finite values
+            a[1] = 0
+            a[1, 0, 5] = float("inf")
+            a[1, 0, :5] = a[1, 0, 6:] = 0
+            b[1, :, 1:] = 0
+            x = x.clone()
+            x[part, 5] = torch.where(x[part, 5] == 0, torch.ones_like(x[part, 5]), x[part, 5])
+        else:
+            b[1, 7, 0] = float("inf") if which == "b" else float("nan")
+        out = harp_amd.add_adapters(base, x, harp_amd.Adapters(a, b, low.scales), requests)
+        t = low.scales[1].double() * (x[part].double() @ a[1].double().t())
+        if which == "a":
+            t = torch.where(torch.arange(r, device=DEV) == 0, t, 0.0)
+        want = base[part].double() + t @ b[1].double().t()
+        _same_where_not_finite(out[part].double(), want, which == "a")
+        assert not bool(torch.isfinite(want).all())
+        others = torch.ones(T, dtype=torch.bool, device=DEV)
+        others[part] = False
+        if which != "a":
+            assert torch.equal(out[others], clean[others])
+        assert bool(torch.isfinite(out[others]).all())

@@ -452,3 +452,28 @@ def test_a_weight_shared_by_two_captured_calls():
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+def test_a_broken_adapter_stays_with_its_request():
+    """Infinities and NaN in one adapter's B reach no token of the requests in the same block of the one launch."""
+    for r, S, heads in ((16, 24, 2), (72, 40, 2), (16, 900, 30)):
+        g = _gen(r + S)
+        attn = harp_amd.adapt_attention(_attention(g, 128, heads), **{t: _low(g, 3, r, 128, heads * 128) for t in ("to_q", "to_k", "to_v")})
+        x, pos = _rand(g, 3, S, 128), _positions(g, 3, S, ROPE)
+        for index in ([0, 1, 2], [2, 1, -1], [1, 0, 5]):
+            requests = harp_amd.AdapterRequests(torch.tensor(index, device=DEV))
+            with torch.no_grad():
+                clean = harp_amd.project_qkv(attn, x, pos, requests=requests)
+                kept = [m.b.clone() for m in (attn.to_q, attn.to_k, attn.to_v)]
+                for m in (attn.to_q, attn.to_k, attn.to_v):
+                    m.b[1, 3::7] = float("inf")
+                    m.b[1, 4::9, 0] = float("nan")
+                broken = harp_amd.project_qkv(attn, x, pos, requests=requests)
+                for m, b in zip((attn.to_q, attn.to_k, attn.to_v), kept):
+                    m.b.copy_(b)
+            for a, b in zip(broken, clean):
+                for i, which in enumerate(index):
+                    if which == 1:
+                        assert not bool(torch.isfinite(a[i]).all())
+                    else:
+                        assert torch.equal(a[i], b[i])
