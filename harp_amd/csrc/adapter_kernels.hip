@@ -1005,7 +1005,8 @@ hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
     const ShrinkSet& s = p.set[i];
     aligned &= s.ldx % 8 == 0 && s.ldx < (1 << 24) && (uintptr_t)s.x % 16 == 0 && (uintptr_t)s.a % 16 == 0;
   }
-  // few tokens: a block for every 16 ranks
+  // Few tokens: a block for every 16 ranks.  K = 3840, such blocks and the others (with t B^T): rank 64, 256 tokens 12.3
+  // and 15.5 us, 1024 tokens 15.1 and 18.7, 2048 tokens 21.4 and 19.1; rank 16, 4096 tokens 14.4 and 14.6.
   const bool few = slots_of(p.req, 16) * (p.rp / 16) * p.sets <= 512;
   const int total = p.rp / 16 * (p.apart ? 1 : p.sets);
   if (aligned) {
@@ -1022,16 +1023,19 @@ hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
            : total == 2 ? shrink_lds_t<2, 2, 4, 3>(p, st)
                         : shrink_lds_t<2, 4, 4, 3>(p, st);
   }
-  // the waves of a block share K: 16 of them where each has a 64-column step
-  if (p.K < 1024) return few ? shrink_t<1, 1, 4>(p, st) : shrink_t<2, 4, 4>(p, st);
+  // The waves of a block share K.  16 of them and 4: rank 64, 4096 tokens, K = 2052 25.1 and 30.8 us (with t B^T),
+  // K = 324 17.2 and 18.3, K = 130 15.3 and 15.0; rank 128, 8192 tokens, K = 66 32.2 and 27.1.
+  if (p.K < 256) return few ? shrink_t<1, 1, 4>(p, st) : shrink_t<2, 4, 4>(p, st);
   return few || total == 1 ? shrink_t<1, 1, 16>(p, st) : shrink_t<2, 4, 16>(p, st);
 }
 
 namespace {
 template <int BASE, bool F32, int RS>
 hipError_t expand_w(const ExpandParams& p, hipStream_t st) {
-  // requests of 64 tokens and more on the average fill a block's waves along the tokens
-  const bool tall = p.req.tokens / std::max(p.req.count, 1) >= 64 && p.r % 8 == 0 && (uintptr_t)p.b % 16 == 0;
+  // Requests of 128 tokens and more on the average fill a block's waves along the tokens.  To 3840 features, tall
+  // and short: 32 requests of 256 tokens with rank 64 45 and 62 us, of 128 tokens 36 and 36, of 32 tokens 21.7 and
+  // 22.3, with rank 16 13.4 and 13.7; of 16 tokens with rank 16 11.1 and 9.5.
+  const bool tall = p.req.tokens / std::max(p.req.count, 1) >= 128 && p.r % 8 == 0 && (uintptr_t)p.b % 16 == 0;
   const int64_t slots = slots_of(p.req, tall ? 128 : 32);
   // blocks in multiples of their steps: of the long requests' three fit a CU at a time, and no more than that
   // keeps what a block does before its first step small (rank 64, 8192 x 3840: 22 us, with 2048 blocks 27)
@@ -1064,8 +1068,14 @@ hipError_t launch_expand(const ExpandParams& p, hipStream_t st) {
 }
 
 namespace {
-constexpr int64_t kFewBytes = 32 << 20;  // of A that all blocks together read
-constexpr int kFewSteps4 = 3;            // 16-rank steps of four tokens' sums that fit the registers
+// One launch and two, K = 3840.  Of a token a request, rank 16: one request to 10240 features 4.7 and 8.6 us; to 3840
+// features 16 requests (15.7 MB of A read by all blocks) 7.1 and 9.0, 24 requests (23.6 MB) 7.6 and 9.3, 64 requests
+// 17.5 and 13.1; 32 requests from 256 to 15360 features 8.9 and 14.5.  Rank 64 (491 KB of A a block): 12.3 and 9.7.
+// Of four tokens a request, rank 16: 4 requests (3.9 MB) 7.5 and 8.7, 8 (7.9 MB) 8.9 and 8.8, 16 (15.7 MB) 10.8
+// and 9.1; rank 48 15.1 and 9.0.
+constexpr int64_t kFewBytes = 24 << 20, kFewBytes4 = 8 << 20;  // of A that all blocks together read
+constexpr int64_t kFewBlockBytes = 256 << 10;                  // and one of them
+constexpr int kFewSteps4 = 3;  // 16-rank steps of four tokens' sums that fit the registers
 
 int64_t few_blocks(const ExpandParams& p) { return (p.N + kFewFeatures - 1) / kFewFeatures; }
 
@@ -1091,9 +1101,11 @@ hipError_t few_r(const ExpandParams& p, const FewParams& q, hipStream_t st) {
 }  // namespace
 bool few_tokens(const ExpandParams& p, int K) {
   const int64_t tiles = std::min<int64_t>(p.req.tokens, p.req.tokens / 4 + p.req.count);  // that have tokens
-  const int most = p.req.tokens <= p.req.count ? 4 : kFewSteps4;
-  return p.rp <= 16 * most && p.base && p.base_f32 == p.out_f32 && p.req.tokens <= 4 * (int64_t)p.req.count &&
-         tiles * few_blocks(p) * p.r * K * 2 <= kFewBytes;
+  const bool one = p.req.tokens <= p.req.count;
+  const int64_t bytes = (int64_t)p.r * K * 2;
+  return p.rp <= 16 * (one ? 4 : kFewSteps4) && p.base && p.base_f32 == p.out_f32 &&
+         p.req.tokens <= 4 * (int64_t)p.req.count && bytes <= kFewBlockBytes &&
+         tiles * few_blocks(p) * bytes <= (one ? kFewBytes : kFewBytes4);
 }
 hipError_t launch_few(const ExpandParams& p, const FewParams& q, hipStream_t st) {
   return p.out_f32 ? few_r<true>(p, q, st) : few_r<false>(p, q, st);
