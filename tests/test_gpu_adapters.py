@@ -128,6 +128,11 @@ CASES = [
     (6, 4100, 160, 128, 40, 3, B16, True),   # blocks that share K between four waves
     (6, 9000, 64, 96, 96, 3, F32, True),
     (5, 8192, 128, 64, 16, 2, B16, True),
+    (3, 8300, 136, 72, 16, 2, B16, True),    # tiles of 64 tokens
+    (2, 8450, 72, 65, 24, 2, B16, False),
+    (61, 300, 64, 72, 16, 4, B16, True),     # segments found at once, and after one and two searches
+    (62, 300, 64, 72, 16, 4, B16, True),
+    (5000, 6001, 64, 72, 8, 7, B16, True),
 ]
 
 
