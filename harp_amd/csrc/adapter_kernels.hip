@@ -99,7 +99,8 @@ __device__ __forceinline__ void shrink_store(const ShrinkParams& p, const Tile& 
 // v_mfma_f32_16x16x32_bf16 with A's rows as the first operand: a lane ends with
 // four neighbouring ranks of one token.  Fragments come straight from memory: a
 // 64-column step reads whole 128-byte lines of x and of A, and nothing of x is
-// used twice by a block.
+// used twice by a block.  Bound by its start and the latency of its loads: 8 us for
+// 1333 tokens x 2570 columns, rank 12, whose rows are 4-byte aligned.
 // ---------------------------------------------------------------------------
 template <int TB, int RB, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
@@ -181,6 +182,10 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
 // fragments from there.  A wave has STAGES such steps of its own, so the loop has
 // no barrier: it waits for its oldest copies, reads, multiplies and sends the next
 // copies into the same place.
+// Bound by the read of x: 8192 tokens x 3840 columns, rank 32, 18 us (3.5 TB/s;
+// 4.7 TB/s from one K to the next, and 6 us to start and end), 23.5 behind a kernel whose
+// 168 MB of results are still on their way to memory.  Other waves, stages and LDS
+// sizes of 96 KB and more came within 1 us of it.
 template <int TB, int RB, int WAVES, int STAGES>
 __global__ __launch_bounds__(64 * WAVES) void shrink_lds_kernel(ShrinkParams p) {
   constexpr int M = 16 * TB;
@@ -304,7 +309,8 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_lds_kernel(ShrinkParams p) 
 // way), so that base is read and out written in whole 128-byte lines, 16 bytes a
 // lane: straight from the accumulators' layout each access touched 64 rows'
 // pieces and the kernel ran at half the rate.  t's fragments stay in registers
-// over the walk.
+// over the walk.  Bound by base and out: 8192 tokens x 10240 features, rank 32, 336 MB in
+// 70.5 us (4.8 TB/s); 3840 features, rank 64, 126 MB in 42 us, without a base 63 MB in 22.
 // ---------------------------------------------------------------------------
 namespace {
 
@@ -541,6 +547,7 @@ __global__ __launch_bounds__(kThreads) void expand_kernel(ExpandParams p, int sp
 
 // Short requests, and ranks whose rows of B are not 16-byte aligned: a tile of 32
 // tokens, each wave 64 features of its own, B's fragments straight from memory.
+// 1333 tokens x 1001 features in fp32, rank 12: 9.6 us, a third of it the start.
 template <int BASE, bool F32, int RS>
 __global__ __launch_bounds__(kThreads) void expand_short_kernel(ExpandParams p, int span) {
   typedef Expand<BASE, F32, RS> X;
@@ -598,7 +605,9 @@ __global__ __launch_bounds__(kThreads) void expand_short_kernel(ExpandParams p, 
 // that each load is one run of 1 KB; fragments of the matrix instructions would touch
 // 16 rows with every 16 lanes, and A's 123 KB of rank 16 over 3840 columns then took a
 // CU 3.6 us), and its threads take a feature each, whose row of B and base were on their
-// way meanwhile.
+// way meanwhile.  One token from 3840 to 10240 features, rank 16: 4.8 us, of which an
+// empty launch is half; 32 tokens with an adapter each from 256 to 15360 features, 16 MB of
+// B: 9 us.
 constexpr int kFewFeatures = 512;  // of a block: a thread each
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -721,6 +730,10 @@ __global__ __launch_bounds__(kFewFeatures) void few_kernel(ExpandParams p, FewPa
 // sixteenth of the rate: rank 64 over 8192 tokens took 119 us.)  Where the
 // blocks of all adapters would not fill the chip, each request's tokens are taken
 // in `splits` parts whose sums a second kernel adds in order.
+// Four adapters of rank 64 over 8192 tokens, 3840 columns of x and of dy: 42 us for
+// 126 MB of them and as much of v again, out of the caches (7.9 TB/s into the CUs).  With
+// one group a block and 12 waves of three blocks a CU the same took 48 us, and 8 more for
+// the sum of its three splits.
 // ---------------------------------------------------------------------------
 namespace {
 constexpr int kGradCols = 128, kGradStep = 64, kGradGroups = 4, kGradThreads = kThreads * kGradGroups;
@@ -937,7 +950,8 @@ __global__ __launch_bounds__(kThreads) void grad_sum_kernel(GradParams p, int64_
 }
 
 // ---------------------------------------------------------------------------
-// n matrices transposed, 64 x 64 values a block
+// n matrices transposed, 64 x 64 values a block, all of a thread's loads on their way at
+// once (8 matrices of 64 x 3840: 5 us; one after the other 9.4)
 // ---------------------------------------------------------------------------
 __global__ __launch_bounds__(kThreads) void transpose_kernel(TransposeParams p) {
   __shared__ uint16_t t[64][65];

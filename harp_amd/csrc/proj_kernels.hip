@@ -50,7 +50,9 @@
 // parts (zeros for the other requests' tokens) meets the same columns of B twice.
 // That is one tile per request up to rank 32 against K / 64 of the projection, and
 // no other pass over q, k and v; each result is then rounded once, to nearest,
-// behind the norm and the rotation, in fp32 until there.
+// behind the norm and the rotation, in fp32 until there.  768 tokens x 30 heads of
+// 3840 columns, rank 16, three requests: 109 us, without adapters 100; 32 requests of 8
+// tokens 65, one after the other in parts 93.
 // Pipeline: one barrier per tile, in its last k-step, after which nobody
 // reads tile t's stage any more (its last fragments are in registers) and
 // tile t + 1 is complete; the copies of tile t + stages then go into tile t's
