@@ -3,7 +3,7 @@
 An adapter of rank r adds ``scale * (x A^T) B^T`` to a projection's result, A [r, in] and
 B [out, r].  A batch holds many requests with an adapter each, or none, of n that are kept
 stacked (:class:`Adapters`); :class:`AdapterRequests` says which tokens are whose.
-:func:`add_adapters` adds each token's own adapter in two launches, differentiable
+:func:`add_adapters` adds each token's own adapter in one or two launches, differentiable
 (any number of the adapters may be trained at once, the projection's weight stays
 frozen or trains by itself).  :class:`AdaptedLinear` puts adapters beside an
 ``nn.Linear`` or an :class:`harp_amd.Int8Linear`, :func:`adapt_attention` beside
@@ -12,6 +12,8 @@ and :class:`harp_amd.RingZAttention` then run with ``requests``.
 
 Which request takes which adapter is read on the GPU only: a call neither waits for
 the device nor depends on the values, so a captured graph may be replayed with others.
+
+An infinity or a NaN in one adapter reaches no token of the requests that do not take it.
 
 Tokens and adapters are bfloat16; a projection's result is bfloat16, or float32 where no
 gradient is taken.  Sums are float32, the result is rounded once.  There is no CPU path.

@@ -44,7 +44,8 @@ int launched(hipError_t e, const char* what) {
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 constexpr int64_t kMaxRows = (int64_t)1 << 31;
-constexpr int kMaxTokens = 1 << 28, kMaxDim = 1 << 22, kMaxCount = 1 << 20, kMaxAdapters = 1 << 14;
+// (tokens: the smallest tiles' grids stay below 2^32 threads)
+constexpr int kMaxTokens = 1 << 25, kMaxDim = 1 << 22, kMaxCount = 1 << 20, kMaxAdapters = 1 << 14;
 
 // ---------------------------------------------------------------------------
 // Rope
@@ -191,7 +192,7 @@ int check_adapters(const harp_req_adapters_t* a, int K, int N, bool pointers) {
 }
 int check_tokens(int tokens) {
   if (tokens < 0) return fail(HARP_REQ_EINVAL, "tokens=%d must not be negative", tokens);
-  if (tokens > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "tokens=%d > 2^28", tokens);
+  if (tokens > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "tokens=%d > 2^25", tokens);
   return HARP_REQ_OK;
 }
 int check_requests(const harp_req_requests_t* r, int tokens, int n, Requests& q) {
@@ -537,7 +538,7 @@ int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_
   static_assert(HARP_QK_EINVAL == HARP_REQ_EINVAL && HARP_QK_EUNSUPPORTED == HARP_REQ_EUNSUPPORTED, "status values");
   int rc = harp_proj::fill_params(p, x, ld_x, batch, seq, k_dim, n_out, freqs, f_stride_b, f_stride_s, outs, n_outs);
   if (rc) return fail(rc, "%s", harp_qk_last_error());
-  if ((int64_t)batch * seq > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "batch * seq > 2^28");
+  if ((int64_t)batch * seq > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "batch * seq > 2^25");
   if (!adapters) return fail(HARP_REQ_EINVAL, "adapters is NULL");
   const int tokens = batch * seq, n = adapters[0].n, r = adapters[0].rank;
   for (int i = 0; i < n_outs; ++i) {

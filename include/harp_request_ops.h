@@ -118,6 +118,8 @@ HARP_REQ_API int harp_req_rope_table(const harp_req_axes_t* axes, const harp_req
  * is not 0 .. n - 1 takes none, nor do the tokens in front of the first request and
  * behind the last.  offsets NULL: each request is tokens / count tokens.  Both I32
  * or I64, each its own.  Values outside 0 .. tokens are read as the nearest of them.
+ * An infinity or a NaN in one adapter reaches its own requests' tokens only (and from
+ * b may come out as NaN).
  */
 typedef struct {
   const void* index;
@@ -144,7 +146,7 @@ HARP_REQ_API int harp_req_adapter_columns(int rank);
  * out may be base itself, and no other input.  t: fp32 [tokens,
  * harp_req_adapter_columns(rank)] contiguous, 16-byte aligned: written with scale x A^T
  * for the tokens that have an adapter, to be kept for the backward call.  rank 1 to
- * 128; K and N 1 to 2^22, tokens up to 2^28, count up to 2^20, n up to 2^14.
+ * 128; K and N 1 to 2^22, tokens up to 2^25, count up to 2^20, n up to 2^14.
  */
 HARP_REQ_API int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base, int64_t ld_base,
                                                void* out, int64_t ld_out, int dtype,
@@ -186,7 +188,7 @@ HARP_REQ_API size_t harp_req_adapter_backward_workspace_bytes(int tokens, int k_
  * (harp_qkv_project truncates behind the norm and the rotation); y_lin is the rounded
  * product with its adapter.  t (n_outs pointers, or NULL): each fp32 [tokens,
  * harp_req_adapter_columns(rank)], as for harp_req_add_adapters_forward.  workspace:
- * harp_req_qkv_workspace_bytes, 16-byte aligned.  batch * seq up to 2^28.
+ * harp_req_qkv_workspace_bytes, 16-byte aligned.  batch * seq up to 2^25.
  */
 HARP_REQ_API int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_dim, int n_out,
                                       const float* freqs, int64_t f_stride_b, int64_t f_stride_s,

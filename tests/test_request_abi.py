@@ -192,7 +192,7 @@ def _back(dy=FAKE, lddy=96, dx=FAKE, lddx=64, base=None, ldb=64, da=FAKE, db=FAK
 
 BOTH = [
     (dict(T=-1), EINVAL, "tokens"),
-    (dict(T=(1 << 28) + 1), EUNSUPPORTED, "2^28"),
+    (dict(T=(1 << 25) + 1), EUNSUPPORTED, "2^25"),
     (dict(n=0), EINVAL, "n=0"),
     (dict(rank=0), EINVAL, "rank=0"),
     (dict(rank=129), EUNSUPPORTED, "rank=129"),
@@ -281,7 +281,7 @@ def _qkv(x=FAKE, ldx=128, B=1, S=6, K=128, N=256, n_outs=3, ws=FAKE, wsb=1 << 30
     (dict(K=100), EUNSUPPORTED, "k_dim=100"),
     (dict(N=100), EUNSUPPORTED, "n_out=100"),
     (dict(n_outs=4), EINVAL, "1 to 3"),
-    (dict(B=1 << 14, S=(1 << 14) + 1), EUNSUPPORTED, "2^28"),
+    (dict(B=1 << 13, S=(1 << 12) + 1), EUNSUPPORTED, "2^25"),
     (dict(adapters=False), EINVAL, "adapters is NULL"),
     (dict(rank=0), EINVAL, "rank=0"),
     (dict(rank=12), EUNSUPPORTED, "multiple of 8"),
