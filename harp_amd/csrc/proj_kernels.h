@@ -47,8 +47,8 @@ struct ProjParams {
 
 // LDS bytes the tiles of one block may take: two stages of the 256-token x
 // 2-head x and W tiles, or three or four of the smaller blocks' tiles, beside
-// the norm weight in the CU's 160 KB
-constexpr int kProjLdsBytes = 144 * 1024;
+// the norm weight and a spare 1 KB in the CU's 160 KB
+constexpr int kProjLdsBytes = 156 * 1024;
 
 hipError_t launch_proj(const ProjParams& p, hipStream_t stream);
 

@@ -33,10 +33,16 @@
 //   k-tile = 64 elements: x tile 256 x 64 and W tile 256 x 64 (32 KB each),
 //            copied global -> LDS by buffer_load ... lds into two stages.
 // These blocks are MFMA- and LDS-bound and the fastest per token once the CUs
-// are full (393 us, 1180 TFLOP/s, at 8192 tokens x 24 heads x 3).  Two smaller
-// ones, bit for bit the same arithmetic, serve grids that leave CUs idle and
-// the last round of the CUs; there a tile's few MFMAs don't cover the memory's
-// latency with one tile of lead, so more stages are in flight:
+// are full (393 us, 1180 TFLOP/s, at 8192 tokens x 24 heads x 3).  Three smaller
+// ones, bit for bit the same arithmetic, serve grids that leave CUs idle and (the
+// last two) the last round of the CUs; there a tile's few MFMAs don't cover the
+// memory's latency with one tile of lead, so more stages are in flight (a CU takes
+// in 41 KB/us with two stages of 64 KB, 44 with three of 48, 56 with four of 32):
+//   32 tokens per wave, 2 heads, five waves along the tokens: 160 tokens x 2
+//            heads, 52 KB a tile, three stages, the most that 160 KB hold.  The
+//            32 copies of a W tile go to ten waves: eight of them send their
+//            fourth to a spare place.  768 tokens x 30 heads: 102 -> 79 us (192
+//            tokens with two stages: 94, with six waves or with four);
 //   32 tokens per wave, 2 heads: 128 tokens x 2 heads, 48 KB a tile, three
 //            stages (two stages: 10-13 us slower at 256 tokens x 24 or 30 heads);
 //   32 tokens per wave, 1 head: 4 waves, 128 tokens x 1 head, 32 KB a tile,
@@ -51,7 +57,7 @@
 // That is one tile per request up to rank 32 against K / 64 of the projection, and
 // no other pass over q, k and v; each result is then rounded once, to nearest,
 // behind the norm and the rotation, in fp32 until there.  768 tokens x 30 heads of
-// 3840 columns, rank 16, three requests: 109 us, without adapters 100; 32 requests of 8
+// 3840 columns, rank 16, three requests: 90 us, as without an adapter; 32 requests of 8
 // tokens 65, one after the other in parts 93.
 // Pipeline: one barrier per tile, in its last k-step, after which nobody
 // reads tile t's stage any more (its last fragments are in registers) and
@@ -138,26 +144,29 @@ struct Frags {
 
 }  // namespace
 
-// TPW tokens per wave, HEADS heads per block, STAGES tiles in LDS; TAIL: the
-// blocks are parts (of 128 tokens x HEADS heads) of the main grid's last units
-template <int TPW, int HEADS, int STAGES, bool TAIL, bool LOW>
-__global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(ProjParams p, LowArg<LOW> low) {
-  constexpr int kWaves = kTokenGroups * HEADS;
+// TG waves of TPW tokens per head, HEADS heads per block, STAGES tiles in LDS; TAIL:
+// the blocks are parts (of 128 tokens x HEADS heads) of the main grid's last units
+template <int TG, int TPW, int HEADS, int STAGES, bool TAIL, bool LOW>
+__global__ __launch_bounds__(64 * TG * HEADS, 1) void proj_kernel(ProjParams p, LowArg<LOW> low) {
+  constexpr int kWaves = TG * HEADS;
   constexpr int kFeatures = HEADS * kHeadDim;
   constexpr int kWBytes = kFeatures * kRowBytes;          // 16 KB per head
-  constexpr int kWPerWave = kWBytes / 1024 / kWaves;      // 1 KB copy instructions per wave and tile: 4
+  constexpr int kWCopies = kWBytes / 1024;                // 1 KB copy instructions per tile
+  constexpr int kWPerWave = (kWCopies + kWaves - 1) / kWaves;  // of a wave: 4
+  constexpr bool kSpare = kWCopies % kWaves != 0;         // the last waves have one less: theirs copies nothing, to `spare`
   constexpr int NJ = TPW / 32;                            // 32-token blocks per wave
-  constexpr int kTok = kTokenGroups * TPW;                // tokens per block
+  constexpr int kTok = TG * TPW;                          // tokens per block
   constexpr int kXBytes = kTok * kRowBytes;               // 32 or 16 KB
   constexpr int kXPerWave = kXBytes / 1024 / kWaves;      // 4 or 2
   constexpr int kDmaPerWave = kXPerWave + kWPerWave;      // 8 or 6 copies per tile
   constexpr int kMfma = 4 * NJ;                           // MFMAs per k-step
-  static_assert(kXBytes % (1024 * kWaves) == 0 && kWBytes % (1024 * kWaves) == 0, "copies split evenly");
+  static_assert(kXBytes % (1024 * kWaves) == 0, "copies split evenly");
   static_assert(STAGES * (kXBytes + kWBytes) <= kProjLdsBytes, "LDS budget");
   // the stages: x tiles, then W tiles; after the main loop each wave's
   // TPW x 256 bytes serve as its staging rows for the output stores
   __shared__ __attribute__((aligned(16))) char lds[STAGES * (kXBytes + kWBytes)];
   __shared__ float norm_wf[kHeadDim];  // RMSNorm weight as fp32
+  __shared__ __attribute__((aligned(16))) char spare[kSpare ? 1024 : 16];
   static_assert(kWaves * TPW * 2 * kHeadDim <= STAGES * (kXBytes + kWBytes), "staging fits the stages");
   auto Xs = [&](int s) { return lds + s * kXBytes; };
   auto Ws = [&](int s) { return lds + STAGES * kXBytes + s * kWBytes; };
@@ -210,8 +219,8 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
   const uint32_t x_bytes = (uint32_t)((int64_t)rows_x * p.ldx * 2);
   const uint32_t w_bytes = (uint32_t)((int64_t)rows_w * o.ldw * 2);
 
-  // this wave's copy instructions: x tile instructions wave + 8k, W tile
-  // instructions wave + 8k (1 KB of LDS each)
+  // this wave's copy instructions: x tile instructions wave + kWaves k, W tile
+  // instructions wave + kWaves k (1 KB of LDS each)
   uint32_t xsrc[kXPerWave], wsrc[kWPerWave];
 #pragma unroll
   for (int k = 0; k < kXPerWave; ++k) xsrc[k] = slot_src((wave + kWaves * k) * 64 + lane, p.ldx);
@@ -232,9 +241,14 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
   // from `base`, the LDS address of the wave's first copy
   const uint32_t lds_wave =
       __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)(lds + wave * 1024));
+  const bool last_w = wave + kWaves * (kWPerWave - 1) < kWCopies;
+  const uint32_t spare_lds = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)spare);
   auto dma = [&](uint32_t base, const rsrc_t& xr, const rsrc_t& wr, int s, int j) {
     if (j < kXPerWave)
       lds_dma_b128(xr, base + s * kXBytes + kWaves * j * 1024, xsrc[j]);
+    else if (kSpare && j == kDmaPerWave - 1)
+      lds_dma_b128(wr, last_w ? base + STAGES * kXBytes + s * kWBytes + kWaves * (j - kXPerWave) * 1024 : spare_lds,
+                   wsrc[j - kXPerWave]);
     else
       lds_dma_b128(wr, base + STAGES * kXBytes + s * kWBytes + kWaves * (j - kXPerWave) * 1024,
                    wsrc[j - kXPerWave]);
@@ -371,7 +385,8 @@ __global__ __launch_bounds__(64 * kTokenGroups * HEADS, 1) void proj_kernel(Proj
         for (int k = 0; k < kWPerWave; ++k) {
           const int r = (wave + kWaves * k) * 8 + tr, c = c0 + tile_pos(r, tc), cb = c < half ? c : c - half;
           const bool in = c < chunks && cb * 8 < lo.r;
-          lds_dma_b128(b_rsrc, lds_wave + STAGES * kXBytes + kWaves * k * 1024,
+          const bool spared = kSpare && k == kWPerWave - 1 && !last_w;
+          lds_dma_b128(b_rsrc, spared ? spare_lds : lds_wave + STAGES * kXBytes + kWaves * k * 1024,
                        in ? (uint32_t)(r * lo.r * 2 + cb * 16) : harp_ra::kOOB);
         }
         wait_lds_loads();
@@ -541,14 +556,14 @@ int device_cus() {
   return cached[dev];
 }
 
-// One grid over all outputs, every block TPW * 4 tokens x HEADS heads.
-template <int TPW, int HEADS, int STAGES, bool LOW>
+// One grid over all outputs, every block TG * TPW tokens x HEADS heads.
+template <int TG, int TPW, int HEADS, int STAGES, bool LOW>
 hipError_t launch_grid(ProjParams p, const LowArg<LOW>& low, hipStream_t stream) {
-  constexpr int kTok = kTokenGroups * TPW;
+  constexpr int kTok = TG * TPW;
   p.n_lin = ((p.M + kTok - 1) / kTok) * ((p.heads + HEADS - 1) / HEADS);
   p.keep_last = p.tail_bid0 = p.n_lin;
-  hipLaunchKernelGGL((proj_kernel<TPW, HEADS, STAGES, false, LOW>), dim3((unsigned)p.n_lin, (unsigned)p.n_outs),
-                     dim3(64 * kTokenGroups * HEADS), 0, stream, p, low);
+  hipLaunchKernelGGL((proj_kernel<TG, TPW, HEADS, STAGES, false, LOW>), dim3((unsigned)p.n_lin, (unsigned)p.n_outs),
+                     dim3(64 * TG * HEADS), 0, stream, p, low);
   return hipGetLastError();
 }
 
@@ -556,17 +571,18 @@ hipError_t launch_grid(ProjParams p, const LowArg<LOW>& low, hipStream_t stream)
 // tokens x HEADS heads.
 template <int HEADS, int STAGES, bool LOW>
 hipError_t launch_tail(const ProjParams& p, const LowArg<LOW>& low, int r, hipStream_t stream) {
-  hipLaunchKernelGGL((proj_kernel<32, HEADS, STAGES, true, LOW>), dim3((unsigned)(4 / HEADS * r)),
+  hipLaunchKernelGGL((proj_kernel<kTokenGroups, 32, HEADS, STAGES, true, LOW>), dim3((unsigned)(4 / HEADS * r)),
                      dim3(64 * kTokenGroups * HEADS), 0, stream, p, low);
   return hipGetLastError();
 }
 
 // Which blocks.  Each kind is taken where one round of it covers the whole
 // grid, the smallest first: a round of the 128-token x 1-head blocks takes
-// 27-35 us at K = 3072 and 3840 (256 tokens), one of 128 x 2 heads 42-59 us
-// (300-768 tokens), one of 256 x 2 heads 70-102 us.  In two rounds the smaller
-// blocks lose: 900 tokens x 24 heads takes 72 us in large blocks and 78-81 in
-// the others, 300 tokens x 30 heads 48 us in 128 x 2 and 61 in 128 x 1.
+// 27-35 us at K = 3072 and 3840 (256 tokens), one of 128 x 2 heads 42-68 us
+// (300-768 tokens), one of 160 x 2 heads 79 (768 x 30 heads; 1120 x 24 of K = 2048
+// 48, in the large blocks 54), one of 256 x 2 heads 70-102 us.  In two rounds the smaller
+// blocks lose: 900 tokens x 24 heads took 72 us in large blocks and 78-81 in
+// two rounds of the 128-token ones, 300 tokens x 30 heads 48 us in 128 x 2 and 61 in 128 x 1.
 // Beyond one round of the large blocks, the units left over for the last one
 // run in a second launch as parts, when one round holds all of them: four
 // parts of 1 head up to a quarter of the CUs, two of 2 heads up to half (at
@@ -578,16 +594,18 @@ hipError_t launch_t(const ProjParams& p_in, const LowArg<LOW>& low, hipStream_t 
   ProjParams p = p_in;
   const int64_t cus = device_cus();
   const int64_t tiles128 = (int64_t)p.n_outs * ((p.M + 127) / 128);
-  if (tiles128 * p.heads <= cus) return launch_grid<32, 1, 4>(p, low, stream);
-  if (tiles128 * ((p.heads + 1) / 2) <= cus) return launch_grid<32, 2, 3>(p, low, stream);
+  if (tiles128 * p.heads <= cus) return launch_grid<4, 32, 1, 4>(p, low, stream);
+  if (tiles128 * ((p.heads + 1) / 2) <= cus) return launch_grid<4, 32, 2, 3>(p, low, stream);
+  const int64_t tiles160 = (int64_t)p.n_outs * ((p.M + 159) / 160);
+  if (tiles160 * ((p.heads + 1) / 2) <= cus) return launch_grid<5, 32, 2, 3>(p, low, stream);
   const int L = ((p.M + kBlockTokens - 1) / kBlockTokens) * ((p.heads + kBlockHeads - 1) / kBlockHeads);
   const int64_t units = (int64_t)p.n_outs * L;
   const int r = cus > 0 ? (int)(units % cus) : 0;
   const bool split = r > 0 && 2 * r <= cus && units > cus && r <= L;
-  if (!split) return launch_grid<64, 2, 2>(p, low, stream);
+  if (!split) return launch_grid<4, 64, 2, 2>(p, low, stream);
   p.n_lin = L;
   p.keep_last = p.tail_bid0 = L - r;
-  hipLaunchKernelGGL((proj_kernel<64, 2, 2, false, LOW>), dim3((unsigned)L, (unsigned)p.n_outs),
+  hipLaunchKernelGGL((proj_kernel<kTokenGroups, 64, 2, 2, false, LOW>), dim3((unsigned)L, (unsigned)p.n_outs),
                      dim3(64 * kTokenGroups * 2), 0, stream, p, low);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
