@@ -234,8 +234,8 @@ REQ_PROTOTYPES = {
     "harp_req_add_adapters_backward": (_i, [ctypes.POINTER(ReqBackwardSet), _i, _p, _i64, _req_p, _p, _i64, _p, _i64,
                                             _i, _i, _i, _p, _sz, _p]),
     "harp_req_adapter_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
-    "harp_req_qkv_project": (_i, [_p, _i64, _i, _i, _i, _i, _p, _i64, _i64, ctypes.POINTER(QkvOut), _adapters_p, _i,
-                                  _req_p, _pp, _p, _sz, _p]),
+    "harp_req_qkv_project": (_i, [_p, _i64, _i, _i, _i, _i, _p, _i64, _i64, _axes_p, _pos_p, _p, ctypes.POINTER(QkvOut),
+                                  _adapters_p, _i, _req_p, _pp, _p, _sz, _p]),
     "harp_req_qkv_workspace_bytes": (_sz, [_i, _i, _i]),
     "harp_req_last_error": (ctypes.c_char_p, []),
 }

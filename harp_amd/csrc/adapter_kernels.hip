@@ -19,6 +19,7 @@
 #include "ra_common.h"
 #include "req_device.h"
 #include "req_kernels.h"
+#include "rope_device.h"
 
 namespace harp_req {
 
@@ -186,8 +187,22 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_kernel(ShrinkParams p) {
 // 4.7 TB/s from one K to the next, and 6 us to start and end), 23.5 behind a kernel whose
 // 168 MB of results are still on their way to memory.  Other waves, stages and LDS
 // sizes of 96 KB and more came within 1 us of it.
-template <int TB, int RB, int WAVES, int STAGES>
-__global__ __launch_bounds__(64 * WAVES) void shrink_lds_kernel(ShrinkParams p) {
+// TABLE: the blocks behind the slots write the rotary table that the next launch reads.
+template <bool TABLE>
+struct TableArg {};
+template <>
+struct TableArg<true> {
+  RopeTable v;
+  int first;  // block
+};
+template <int TB, int RB, int WAVES, int STAGES, bool TABLE>
+__global__ __launch_bounds__(64 * WAVES) void shrink_lds_kernel(ShrinkParams p, TableArg<TABLE> table) {
+  if constexpr (TABLE) {
+    if ((int)blockIdx.x >= table.first) {
+      if (blockIdx.y == 0) table_share(table.v, (int)blockIdx.x - table.first, (int)gridDim.x - table.first, 64 * WAVES);
+      return;
+    }
+  }
   constexpr int M = 16 * TB;
   constexpr int kCopies = 2 * (TB + RB);  // of 8 rows each, x's rows and then A's
   constexpr int kStage = 1024 * kCopies;  // bytes
@@ -1007,13 +1022,14 @@ hipError_t shrink_t(const ShrinkParams& p, hipStream_t st) {
 }
 template <int TB, int RB, int WAVES, int STAGES>
 hipError_t shrink_lds_t(const ShrinkParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((shrink_lds_kernel<TB, RB, WAVES, STAGES>),
-                     dim3((unsigned)slots_of(p.req, 16 * TB), shrink_groups<RB>(p)), dim3(64 * WAVES), 0, st, p);
+  hipLaunchKernelGGL((shrink_lds_kernel<TB, RB, WAVES, STAGES, false>),
+                     dim3((unsigned)slots_of(p.req, 16 * TB), shrink_groups<RB>(p)), dim3(64 * WAVES), 0, st, p,
+                     TableArg<false>{});
   return hipGetLastError();
 }
 }  // namespace
 
-hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
+hipError_t launch_shrink(const ShrinkParams& p, const RopeTable* table, hipStream_t st) {
   bool aligned = p.K % 8 == 0;
   for (int i = 0; i < p.sets; ++i) {
     const ShrinkSet& s = p.set[i];
@@ -1023,6 +1039,19 @@ hipError_t launch_shrink(const ShrinkParams& p, hipStream_t st) {
   // and 15.5 us, 1024 tokens 15.1 and 18.7, 2048 tokens 21.4 and 19.1; rank 16, 4096 tokens 14.4 and 14.6.
   const bool few = slots_of(p.req, 16) * (p.rp / 16) * p.sets <= 512;
   const int total = p.rp / 16 * (p.apart ? 1 : p.sets);
+  if (table) {
+    // The table beside few tokens' blocks, two pairs a thread, where both leave each other their CUs: 768 tokens, ranks of
+    // 16 of three projections, 9.8 us against 9.0 and 5.2; at 8192 tokens 33 against 24 and 6.
+    const int64_t slots = slots_of(p.req, 16);
+    const int64_t more = (table->tokens * table->pairs + 2 * 512 - 1) / (2 * 512);
+    if (aligned && few && slots * shrink_groups<1>(p) + more <= kCUs) {
+      hipLaunchKernelGGL((shrink_lds_kernel<1, 1, 8, 3, true>), dim3((unsigned)(slots + more), shrink_groups<1>(p)),
+                         dim3(512), 0, st, p, TableArg<true>{*table, (int)slots});
+      return hipGetLastError();
+    }
+    const hipError_t e = launch_rope_table(*table, st);
+    if (e != hipSuccess) return e;
+  }
   if (aligned) {
     if (few) return shrink_lds_t<1, 1, 8, 3>(p, st);
     // Tiles of 64 tokens read A half as often and leave half as many blocks, one to a CU: they win where 32 tokens a

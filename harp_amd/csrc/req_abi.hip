@@ -348,7 +348,8 @@ int harp_req_rope_table(const harp_req_axes_t* axes, const harp_req_positions_t*
   if (!((int64_t)batch * seq)) return ok();
   if ((rc = check_positions(positions, pos))) return rc;
   if (!table || !aligned(table, 8)) return fail(HARP_REQ_EINVAL, "table must be an 8-byte aligned device pointer");
-  return launched(launch_rope_table(ax, pos, batch, seq, D, table, (hipStream_t)stream), "rotary table");
+  return launched(launch_rope_table(RopeTable{ax, pos, seq, D / 2, (int64_t)batch * seq, (float2*)table}, (hipStream_t)stream),
+                  "rotary table");
 }
 
 int harp_req_adapter_columns(int rank) {
@@ -399,7 +400,7 @@ int harp_req_add_adapters_forward(const void* x, int64_t ld_x, const void* base,
   s.ldt = e.rp;
   s.sets = 1;
   s.set[0] = ShrinkSet{adapters->a, adapters->scales, x, ld_x, t, nullptr};
-  if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
+  if ((rc = launched(launch_shrink(s, nullptr, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
   return launched(launch_expand(e, (hipStream_t)stream), "adapters (t B^T)");
 }
 
@@ -482,7 +483,7 @@ int harp_req_add_adapters_backward(const harp_req_backward_set_t* sets, int n_se
       s.set[i] = ShrinkSet{bt + i * bt_set, e.adapters.scales, e.dy, e.ld_dy, u + (size_t)i * rp, nullptr};
     }
     if ((rc = launched(launch_transpose(tp, st), "adapters' transpose"))) return rc;
-    if ((rc = launched(launch_shrink(s, st), "adapters (dy B)"))) return rc;
+    if ((rc = launched(launch_shrink(s, nullptr, st), "adapters (dy B)"))) return rc;
   }
   if (dx) {
     ExpandParams e{};
@@ -531,12 +532,31 @@ size_t harp_req_qkv_workspace_bytes(int tokens, int rank, int n_outs) {
 }
 
 int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_dim, int n_out, const float* freqs,
-                         int64_t f_stride_b, int64_t f_stride_s, const harp_qkv_out_t* outs,
+                         int64_t f_stride_b, int64_t f_stride_s, const harp_req_axes_t* axes,
+                         const harp_req_positions_t* positions, float* table, const harp_qkv_out_t* outs,
                          const harp_req_adapters_t* adapters, int n_outs, const harp_req_requests_t* requests,
                          float* const* t, void* workspace, size_t workspace_bytes, void* stream) {
   harp_proj::ProjParams p;
   static_assert(HARP_QK_EINVAL == HARP_REQ_EINVAL && HARP_QK_EUNSUPPORTED == HARP_REQ_EUNSUPPORTED, "status values");
-  int rc = harp_proj::fill_params(p, x, ld_x, batch, seq, k_dim, n_out, freqs, f_stride_b, f_stride_s, outs, n_outs);
+  int rc;
+  RopeTable tab{};
+  if (positions) {
+    int D;
+    if (freqs) return fail(HARP_REQ_EINVAL, "one rotation: freqs or positions");
+    if ((rc = check_axes(axes, tab.axes, D)) || (rc = check_batch(batch, seq)) || (rc = check_positions(positions, tab.pos)))
+      return rc;
+    if (D != 128 || axes->half)
+      return fail(HARP_REQ_EUNSUPPORTED, "the axes' widths must add up to 128 (got %d), of neighbouring pairs", D);
+    if (!table || !aligned(table, 16)) return fail(HARP_REQ_EINVAL, "table must be a 16-byte aligned device pointer");
+    tab.S = seq;
+    tab.pairs = D / 2;
+    tab.tokens = tab.pos.sb ? (int64_t)batch * seq : seq;
+    tab.out = (float2*)table;
+    freqs = table;
+    f_stride_s = D;
+    f_stride_b = tab.pos.sb ? (int64_t)seq * D : 0;
+  }
+  rc = harp_proj::fill_params(p, x, ld_x, batch, seq, k_dim, n_out, freqs, f_stride_b, f_stride_s, outs, n_outs);
   if (rc) return fail(rc, "%s", harp_qk_last_error());
   if ((int64_t)batch * seq > kMaxTokens) return fail(HARP_REQ_EUNSUPPORTED, "batch * seq > 2^25");
   if (!adapters) return fail(HARP_REQ_EINVAL, "adapters is NULL");
@@ -572,7 +592,7 @@ int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_
     low.t[i] = pairs;
     low.b[i] = (const uint16_t*)adapters[i].b;
   }
-  if ((rc = launched(launch_shrink(s, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
+  if ((rc = launched(launch_shrink(s, positions ? &tab : nullptr, (hipStream_t)stream), "adapters (x A^T)"))) return rc;
   return launched(harp_proj::launch_proj_low(p, low, (hipStream_t)stream), "qkv projection with adapters");
 }
 

@@ -67,9 +67,15 @@ hipError_t launch_rope_backward(const RopeParams& p, hipStream_t stream);
 // gw[i] (i: q, k; NULL = not wanted) = sum over the tensor's blocks of wpart
 hipError_t launch_rope_wgrad(const float* wpart, const int blocks[2], int D, void* const gw[2], const int gw_f32[2],
                              hipStream_t stream);
-// fp32 (cos, sin) pairs [B, S, D / 2, 2]
-hipError_t launch_rope_table(const RopeAxes& axes, const RopePos& pos, int B, int S, int D, float* out,
-                             hipStream_t stream);
+// (cos, sin) of every pair's angle: out[token][pair], the tokens of B batches of S one after the other
+struct RopeTable {
+  RopeAxes axes;
+  RopePos pos;
+  int S, pairs;
+  int64_t tokens;
+  float2* out;
+};
+hipError_t launch_rope_table(const RopeTable& t, hipStream_t stream);
 
 // ---------------------------------------------------------------------------
 // Low-rank adapters
@@ -112,7 +118,8 @@ struct ShrinkParams {
   int apart;  // the sets have an x each
   ShrinkSet set[kMaxSets];
 };
-hipError_t launch_shrink(const ShrinkParams& p, hipStream_t stream);
+// (table: written as well, by blocks of the same launch or by a launch in front; or NULL)
+hipError_t launch_shrink(const ShrinkParams& p, const RopeTable* table, hipStream_t stream);
 
 // out[m][j] = base[m][j] + sum over ranks t[m][.] B[j][.]
 struct ExpandParams {

@@ -28,6 +28,7 @@
 
 #include "ra_common.h"
 #include "req_kernels.h"
+#include "rope_device.h"
 
 namespace harp_req {
 
@@ -153,53 +154,6 @@ __device__ __forceinline__ void load_weight(const void* w, int w_f32, int sub, i
     v[2 * k] = w_f32 ? ((const float*)w)[e0] : __uint_as_float((uint32_t)((const uint16_t*)w)[e0] << 16);
     v[2 * k + 1] = w_f32 ? ((const float*)w)[e1] : __uint_as_float((uint32_t)((const uint16_t*)w)[e1] << 16);
   }
-}
-
-// turns per unit of position of pair p, and its axis
-__device__ __forceinline__ double rate_of(const RopeAxes& ax, int p, int& axis) {
-  double c0 = ax.c0[0], c1 = ax.c1[0];
-  axis = 0;
-#pragma unroll
-  for (int a = 1; a < kMaxAxes; ++a)
-    if (a < ax.n && p >= ax.end[a - 1]) {
-      axis = a;
-      c0 = ax.c0[a];
-      c1 = ax.c1[a];
-    }
-  return exp2(__builtin_fma(c1, (double)p, c0));
-}
-// the elements at base + off[k]
-template <int N>
-__device__ __forceinline__ void load_pos(const RopePos& q, int64_t base, const int64_t (&off)[N], double (&v)[N]) {
-  if (q.dtype == kI32) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = (double)((const int32_t*)q.p + base)[off[k]];
-  } else if (q.dtype == kI64) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = (double)((const int64_t*)q.p + base)[off[k]];
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = (double)((const float*)q.p + base)[off[k]];
-  }
-}
-// cos and sin of `turns` turns
-__device__ __forceinline__ void cos_sin(double turns, float& c, float& s) {
-  turns -= __builtin_rint(turns);                // within half a turn, exact
-  const double q = __builtin_rint(4.0 * turns);  // quarters: -2 .. 2
-  const float x = (float)__builtin_fma(4.0, turns, -q) * 1.57079632679489662f;  // within pi / 4
-  const int n = (int)q;
-  const float x2 = x * x;
-  // x - x^3/3! + x^5/5! - x^7/7! + x^9/9!, and 1 - x^2/2! + x^4/4! - x^6/6! + x^8/8!
-  const float sp = __builtin_fmaf(
-      x * x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f),
-      x);
-  const float cp = __builtin_fmaf(
-      x2, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, 1.f / 40320.f, -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
-  const bool odd = n & 1;
-  s = odd ? cp : sp;
-  c = odd ? sp : cp;
-  if (n == 2 || n == -2 || n == -1) s = -s;
-  if (n == 2 || n == -2 || n == 1) c = -c;
 }
 
 // Workgroups are dealt to the 8 XCDs round-robin: each XCD takes one contiguous
@@ -540,24 +494,10 @@ __global__ __launch_bounds__(kWgCols* kWgLanes) void rope_wgrad_kernel(const flo
 }
 
 // ---------------------------------------------------------------------------
-// The table: a thread keeps one pair and walks the tokens
+// The table (table_share)
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(kThreads) void rope_table_kernel(RopeAxes axes, RopePos pos, int S, int64_t tokens,
-                                                              int pairs, float2* out) {
-  const int per = kThreads / pairs;  // tokens of a block's step
-  const int p = threadIdx.x % pairs, at = threadIdx.x / pairs;
-  if (at >= per) return;
-  int axis;
-  const double rate = rate_of(axes, p, axis);
-  for (int64_t tok = (int64_t)blockIdx.x * per + at; tok < tokens; tok += (int64_t)gridDim.x * per) {
-    const int64_t b = tok / S, s = tok - b * S;
-    const int64_t off[1] = {axis * pos.sa};
-    double v[1];
-    load_pos(pos, b * pos.sb + s * pos.ss, off, v);
-    float2 cs;
-    cos_sin(v[0] * rate, cs.x, cs.y);
-    out[tok * pairs + p] = cs;
-  }
+__global__ __launch_bounds__(kThreads) void rope_table_kernel(RopeTable t) {
+  table_share(t, (int)blockIdx.x, (int)gridDim.x, kThreads);
 }
 
 // ---------------------------------------------------------------------------
@@ -657,13 +597,10 @@ hipError_t launch_rope_wgrad(const float* wpart, const int blocks[2], int D, voi
   return hipGetLastError();
 }
 
-hipError_t launch_rope_table(const RopeAxes& axes, const RopePos& pos, int B, int S, int D, float* out,
-                             hipStream_t stream) {
-  const int pairs = D / 2, per = kThreads / pairs;
-  const int64_t tokens = (int64_t)B * S, need = (tokens + per - 1) / per;
-  const int64_t blocks = need < 2048 ? need : 2048;
-  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(kThreads), 0, stream, axes, pos, S, tokens, pairs,
-                     (float2*)out);
+hipError_t launch_rope_table(const RopeTable& t, hipStream_t stream) {
+  const int per = kThreads / t.pairs;
+  const int64_t need = (t.tokens + per - 1) / per;
+  hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)std::min<int64_t>(need, 2048)), dim3(kThreads), 0, stream, t);
   return hipGetLastError();
 }
 

@@ -578,8 +578,11 @@ struct QkvCall {
   AdapterCall first;           // x, requests, adapters[0]
   harp_req_adapters_t adapters[3];
   Tensors a, b, scales;        // kept alive
-  at::Tensor freqs;            // fp32 (cos, sin) rows
+  at::Tensor freqs;            // fp32 (cos, sin) rows, written by the call where it has positions
   int64_t fsb = 0;
+  bool axial = false;
+  Axes axes;
+  Positions pos;
   Tensors w, nw;               // projections, norm weights (undefined: none)
   int64_t B = 0, S = 0, K = 0, N = 0, H = 0;
 };
@@ -676,7 +679,9 @@ QkvResult qkv_forward(const QkvCall& c, const at::Tensor& x, const double (&eps)
     check_status(
         harp_req_qkv_project(c.first.x.p, c.first.x.ld, checked_int(c.B, "batch"), checked_int(c.S, "seq"),
                              checked_int(c.K, "dim"), checked_int(c.N, "features"),
-                             c.freqs.defined() ? c.freqs.const_data_ptr<float>() : nullptr, c.fsb, kHeadDim, outs,
+                             c.freqs.defined() && !c.axial ? c.freqs.const_data_ptr<float>() : nullptr, c.fsb,
+                             kHeadDim, c.axial ? &c.axes.a : nullptr, c.axial ? &c.pos.p : nullptr,
+                             c.axial ? c.freqs.data_ptr<float>() : nullptr, outs,
                              c.adapters, 3, &c.first.requests, keep ? t : nullptr, work.data_ptr(), bytes, stream_of(x)),
         "qkv_adapters");
   }
@@ -684,12 +689,15 @@ QkvResult qkv_forward(const QkvCall& c, const at::Tensor& x, const double (&eps)
   return r;
 }
 
-at::Tensor table_of(const at::Tensor& positions, const RopeCall& c, const at::Tensor& x) {
-  TORCH_CHECK(x.dim() == 3, "x must be [B, S, dim], got ", x.sizes());
+// the rotation by positions, whose table the call writes
+void set_positions(QkvCall& c, const at::Tensor& positions, const RopeCall& rope, const at::Tensor& x) {
   check_device(positions, x, "positions");
-  positions_of(positions, c.axes.a.n, x.size(0), x.size(1));  // (their shape)
-  TORCH_CHECK(c.axes.D == kHeadDim, "the axes' widths must add up to 128, got ", c.axes.D);
-  return table(positions, c.axes);
+  TORCH_CHECK(rope.axes.D == kHeadDim, "the axes' widths must add up to 128, got ", rope.axes.D);
+  c.axial = true;
+  c.axes = rope.axes;
+  c.pos = positions_of(positions, c.axes.a.n, c.B, c.S);
+  const c10::DeviceGuard guard(x.device());
+  c.freqs = at::empty({c.pos.p.stride_b ? c.B : 1, c.S, kHeadDim / 2, 2}, x.options().dtype(at::kFloat));
 }
 
 Tensors qkv_adapters(const at::Tensor& x, const Tensors& weights, const Tensors& a, const Tensors& b,
@@ -700,9 +708,9 @@ Tensors qkv_adapters(const at::Tensor& x, const Tensors& weights, const Tensors&
   TORCH_CHECK(!given(freqs) || !given(positions), "one rotation: freqs_cis or positions");
   TORCH_CHECK(eps.size() == 2, "eps must be two values, got ", eps.size());
   const double both[2] = {eps[0], eps[1]};
-  const OptTensor table =
-      given(positions) ? OptTensor(table_of(*positions, rope_call(widths, theta, false, eps), x)) : freqs;
-  return qkv_forward(qkv_call(x, weights, a, b, scales, index, offsets, norm_weights, table), x, both, false).y;
+  QkvCall c = qkv_call(x, weights, a, b, scales, index, offsets, norm_weights, freqs);
+  if (given(positions)) set_positions(c, *positions, rope_call(widths, theta, false, eps), x);
+  return qkv_forward(c, x, both, false).y;
 }
 
 // Differentiable arguments in this order: x, three weights, two norm weights, three a, three b
@@ -721,8 +729,8 @@ class QkvAdapters : public torch::autograd::Function<QkvAdapters> {
     c10::List<OptTensor> norms;
     norms.push_back(nq);
     norms.push_back(nk);
-    const at::Tensor table = table_of(positions, call, x);
-    const QkvCall c = qkv_call(x, {wq, wk, wv}, {aq, ak, av}, {bq, bk, bv}, scales, index, offsets, norms, table);
+    QkvCall c = qkv_call(x, {wq, wk, wv}, {aq, ak, av}, {bq, bk, bv}, scales, index, offsets, norms, OptTensor());
+    set_positions(c, positions, call, x);
     const QkvResult r = qkv_forward(c, x, call.eps, true);
     int64_t wanted = 0;
     const at::Tensor* const leaves[] = {&x, &wq, &wk, &wv, &nq, &nk, &aq, &ak, &av, &bq, &bk, &bv};

@@ -189,10 +189,16 @@ HARP_REQ_API size_t harp_req_adapter_backward_workspace_bytes(int tokens, int k_
  * product with its adapter.  t (n_outs pointers, or NULL): each fp32 [tokens,
  * harp_req_adapter_columns(rank)], as for harp_req_add_adapters_forward.  workspace:
  * harp_req_qkv_workspace_bytes, 16-byte aligned.  batch * seq up to 2^25.
+ *
+ * The rotation: freqs as harp_qkv_project takes it, or NULL and positions along axes of
+ * 128 features together, of neighbouring pairs; then table, fp32 [batch, seq, 64, 2] ([1, seq,
+ * 64, 2] where stride_b is 0), 16-byte aligned, is written with their table.
  */
 HARP_REQ_API int harp_req_qkv_project(const void* x, int64_t ld_x, int batch, int seq, int k_dim, int n_out,
                                       const float* freqs, int64_t f_stride_b, int64_t f_stride_s,
-                                      const harp_qkv_out_t* outs, const harp_req_adapters_t* adapters, int n_outs,
+                                      const harp_req_axes_t* axes, const harp_req_positions_t* positions,
+                                      float* table, const harp_qkv_out_t* outs,
+                                      const harp_req_adapters_t* adapters, int n_outs,
                                       const harp_req_requests_t* requests, float* const* t, void* workspace,
                                       size_t workspace_bytes, void* stream);
 HARP_REQ_API size_t harp_req_qkv_workspace_bytes(int tokens, int rank, int n_outs);

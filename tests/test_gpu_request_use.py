@@ -153,6 +153,24 @@ def test_qkv_with_adapters(B, S, heads, dim, r, n, offsets):
             assert _rel(a, b) <= 3.5e-3, (i, _rel(a, b))
 
 
+@pytest.mark.parametrize("B,S,heads,dim", [(3, 40, 2, 128), (1, 1, 3, 64), (2, 300, 2, 64), (2, 3000, 2, 64)])
+def test_the_one_launch_takes_positions_of_all_or_of_each(B, S, heads, dim):
+    """Positions of the whole batch, of each sample, as columns of a longer array, and their table: one result."""
+    g = _gen(B * S)
+    attn = harp_amd.adapt_attention(_attention(g, dim, heads), **{t: _low(g, 2, 16, dim, heads * 128) for t in ("to_q", "to_k", "to_v")})
+    x = _rand(g, B, S, dim)
+    requests = harp_amd.AdapterRequests(torch.arange(B, device=DEV) % 2)
+    for dtype in (torch.int32, torch.int64, torch.float32):
+        wide = torch.randint(0, 300, (S, 5), generator=g).to(dtype).to(DEV)
+        p = wide[:, 1:4]
+        forms = [p, p.contiguous()[None], p.expand(B, S, 3), p.expand(B, S, 3).contiguous(), wide.t().contiguous().t()[:, 1:4]]
+        with torch.no_grad():
+            want = harp_amd.project_qkv(attn, x, ROPE.table(p), requests=requests)
+            for f in forms:
+                for a, b in zip(harp_amd.project_qkv(attn, x, harp_amd.AxialPositions(f, ROPE), requests=requests), want):
+                    assert torch.equal(a, b)
+
+
 def test_qkv_without_the_one_launch():
     """The separate parts (here for pairs of the other layout, a bias, heads of 64, few-token requests) agree
     with 64 bits within a rounding of each part: three of 2^-8 / sqrt(3) at most, under 0.6%."""

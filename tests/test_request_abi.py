@@ -52,8 +52,9 @@ def test_structures_have_the_header_s_layout(tmp_path):
         assert (ctypes.sizeof(t), getattr(t, m).offset) == tuple(int(v) for v in line.split())
 
 
-def _axes(width=(32, 48, 48), theta=256.0, n=None):
+def _axes(width=(32, 48, 48), theta=256.0, n=None, half=0):
     a = _lib.ReqAxes()
+    a.half = half
     a.n = len(width) if n is None else n
     for i, w in enumerate(width):
         a.width[i], a.theta[i] = w, theta
@@ -261,7 +262,7 @@ def test_adapters_backward_refuses(over, code, msg):
 
 
 def _qkv(x=FAKE, ldx=128, B=1, S=6, K=128, N=256, n_outs=3, ws=FAKE, wsb=1 << 30, t=None, adapters=True, odd=None,
-         weight=FAKE, **over):
+         weight=FAKE, freqs=None, axes=None, pos=None, table=FAKE, **over):
     a = {**ADD, **over}
     ad, rq = _adapters(a)
     ads = (_lib.ReqAdapters * 3)(ad, ad, ad)
@@ -271,8 +272,8 @@ def _qkv(x=FAKE, ldx=128, B=1, S=6, K=128, N=256, n_outs=3, ws=FAKE, wsb=1 << 30
     for o in outs:
         o.weight, o.ld_weight, o.y, o.ld_y = weight, K, FAKE, N
     ts = None if t is None else (ctypes.c_void_p * 3)(*[t] * 3)
-    return harp_amd.load_abi().harp_req_qkv_project(x, ldx, B, S, K, N, None, 0, 128, outs, ads if adapters else None,
-                                                    n_outs, rq, ts, ws, wsb, None)
+    return harp_amd.load_abi().harp_req_qkv_project(x, ldx, B, S, K, N, freqs, 0, 128, axes, pos, table, outs,
+                                                    ads if adapters else None, n_outs, rq, ts, ws, wsb, None)
 
 
 @pytest.mark.parametrize("over,code,msg", [
@@ -290,6 +291,14 @@ def _qkv(x=FAKE, ldx=128, B=1, S=6, K=128, N=256, n_outs=3, ws=FAKE, wsb=1 << 30
     (dict(index=None), EINVAL, "index is NULL"),
     (dict(offsets=None, count=4), EINVAL, "one length"),
     (dict(t=FAKE + 4), EINVAL, "t[0]"),
+    (dict(axes=_axes(), pos=_positions(), freqs=FAKE), EINVAL, "one rotation"),
+    (dict(axes=None, pos=_positions()), EINVAL, "axes is NULL"),
+    (dict(axes=_axes((32, 32)), pos=_positions()), EUNSUPPORTED, "add up to 128"),
+    (dict(axes=_axes(half=1), pos=_positions()), EUNSUPPORTED, "neighbouring pairs"),
+    (dict(axes=_axes(), pos=_positions(dtype=BF16)), EINVAL, "positions dtype"),
+    (dict(axes=_axes(), pos=_positions(), table=None), EINVAL, "table"),
+    (dict(axes=_axes(), pos=_positions(), table=FAKE + 8), EINVAL, "table"),
+    (dict(axes=_axes(), pos=_positions(), ws=None), ENOMEM, "workspace"),
     (dict(ws=None), ENOMEM, "workspace"),
     (dict(wsb=100), ENOMEM, "workspace"),
     (dict(ws=FAKE + 8), EINVAL, "workspace"),
