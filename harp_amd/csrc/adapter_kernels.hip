@@ -735,7 +735,7 @@ __global__ __launch_bounds__(kFewFeatures) void few_kernel(ExpandParams p, FewPa
 
 // ---------------------------------------------------------------------------
 // Gradients of A and B: for each adapter the sum over its tokens of v[m]^T x[m].
-// A block takes 128 columns and 32 RK ranks of one adapter.  Its four groups of four
+// A block takes 128 columns and 32 RK ranks of one adapter.  Its G groups of four
 // waves (32 columns each) walk the adapter's tokens, 64 in a group's step: the step's x
 // (bf16) and v (taken apart into two bf16) lie in LDS as they come, and
 // ds_read_b64_tr_b16 reads both transposed, tokens along the contraction of
@@ -747,11 +747,11 @@ __global__ __launch_bounds__(kFewFeatures) void few_kernel(ExpandParams p, FewPa
 // in `splits` parts whose sums a second kernel adds in order.
 // Four adapters of rank 64 over 8192 tokens, 3840 columns of x and of dy: 42 us for
 // 126 MB of them and as much of v again, out of the caches (7.9 TB/s into the CUs).  With
-// one group a block and 12 waves of three blocks a CU the same took 48 us, and 8 more for
-// the sum of its three splits.
+// one group a block and three splits, 12 waves of three blocks a CU, the same took 48 us,
+// and 8 more for the sum of the splits.
 // ---------------------------------------------------------------------------
 namespace {
-constexpr int kGradCols = 128, kGradStep = 64, kGradGroups = 4, kGradThreads = kThreads * kGradGroups;
+constexpr int kGradCols = 128, kGradStep = 64, kGradGroups = 4;
 
 // Rows of W (128, 64 or 32) bf16: 16-byte chunk c of row r.  Row writes and the transposed reads below
 // (64 bytes of each of four rows at a time) are free of bank conflicts.
@@ -789,11 +789,11 @@ struct Steps {
 
 }  // namespace
 
-template <int RK>
-__global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_t all) {
+template <int RK, int G>
+__global__ __launch_bounds__(kThreads* G) void grad_kernel(GradParams p, int64_t all) {
   constexpr int kRanks = 32 * RK, kPitch = kGradCols + 4;  // of the sums (a lane writes 4 columns of its rank)
   constexpr int kX = kGradStep * kGradCols, kV = kGradStep * kRanks, kGroup = 2 * (kX + 2 * kV), kSums = kRanks * kPitch * 4;
-  __shared__ __attribute__((aligned(16))) char lds[kGradGroups * (kGroup > kSums ? kGroup : kSums)];
+  __shared__ __attribute__((aligned(16))) char lds[G * (kGroup > kSums ? kGroup : kSums)];
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, tid = threadIdx.x % kThreads;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kThreads);
@@ -801,16 +801,14 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
   bf16* const vs = xs + kX;  // the parts one after the other
   // this block's part and columns (constant indices: see the shrink kernel)
   GradPart part = p.part[0];
-  int cb = blockIdx.x;
-  int64_t at = 0;  // of the part's values among all
-  const int64_t per = (int64_t)p.req.n * p.r;
+  int cb = blockIdx.x, which = 0;
 #pragma unroll
   for (int i = 1; i < kMaxGradParts; ++i) {
     const int blocks = (part.C + kGradCols - 1) / kGradCols;
     if (i < p.parts && cb >= blocks) {
       cb -= blocks;
-      at += per * part.C;
       part = p.part[i];
+      which = i;
     } else {
       break;
     }
@@ -819,7 +817,6 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
   const int rgroups = (p.rp + kRanks - 1) / kRanks;
   const int adapter = (int)blockIdx.y / rgroups, r0 = (int)blockIdx.y % rgroups * kRanks;
   const int split = blockIdx.z;
-  float* const work = p.work + split * all + at;
   harp_ra::sched_fence();  // (the parts' arguments and the walk's beside each other do not fit the scalar registers)
 
   f32x16 acc[RK];
@@ -849,7 +846,7 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
     bool any = false;
     n = 0;
 #pragma unroll 1
-    for (int q = 0; q < kGradGroups && next(); ++q) {
+    for (int q = 0; q < G && next(); ++q) {
       any = true;
       const int rows = min(kGradStep, st.end - st.m);
       if (q == group) {
@@ -929,17 +926,31 @@ __global__ __launch_bounds__(kGradThreads) void grad_kernel(GradParams p, int64_
       *(f32x4*)(sums + (group * kRanks + 32 * j + l32) * kPitch + 32 * wave + harp_ra::c_row(e, g)) =
           f32x4{acc[j][e], acc[j][e + 1], acc[j][e + 2], acc[j][e + 3]};
   __syncthreads();
+  // where the part's values go (found now: kept over the walk, it does not fit the scalar registers either)
+  asm volatile("" : "+s"(which));
+  const int64_t per = (int64_t)p.req.n * p.r;
+  int64_t at = 0;  // of the part's values among all
+  void* out = p.part[0].out;
+  int cols_first = p.part[0].cols_first;
+#pragma unroll
+  for (int i = 1; i < kMaxGradParts; ++i)
+    if (i <= which) {
+      at += per * p.part[i - 1].C;
+      out = p.part[i].out;
+      cols_first = p.part[i].cols_first;
+    }
+  float* const work = p.work + split * all + at;
   // out as it lies in memory, one value a thread
   const int ranks = min(kRanks, p.r - r0), cols = min(kGradCols, part.C - c0);
-  for (int i = threadIdx.x; i < kRanks * kGradCols; i += kGradThreads) {
-    const int rank = part.cols_first ? i % kRanks : i / kGradCols, c = part.cols_first ? i / kRanks : i % kGradCols;
+  for (int i = threadIdx.x; i < kRanks * kGradCols; i += kThreads * G) {
+    const int rank = cols_first ? i % kRanks : i / kGradCols, c = cols_first ? i / kRanks : i % kGradCols;
     if (rank >= ranks || c >= cols) continue;
     float sum = sums[rank * kPitch + c];
 #pragma unroll
-    for (int q = 1; q < kGradGroups; ++q) sum += sums[(q * kRanks + rank) * kPitch + c];
-    const int64_t o = part.cols_first ? ((int64_t)adapter * part.C + c0 + c) * p.r + r0 + rank
+    for (int q = 1; q < G; ++q) sum += sums[(q * kRanks + rank) * kPitch + c];
+    const int64_t o = cols_first ? ((int64_t)adapter * part.C + c0 + c) * p.r + r0 + rank
                                       : ((int64_t)adapter * p.r + r0 + rank) * part.C + c0 + c;
-    if (p.splits == 1) ((bf16*)part.out)[o] = (bf16)sum;
+    if (p.splits == 1) ((bf16*)out)[o] = (bf16)sum;
     else work[o] = sum;
   }
 }
@@ -1161,23 +1172,35 @@ int grad_blocks(const GradParams& p) {
   return n;
 }
 int grad_groups(const GradParams& p) { return (p.rp + 63) / 64; }  // 64 ranks a block (32 where that is all)
-template <int RK>
+// that have tokens (of each split)
+int64_t busy_blocks(const GradParams& p) {
+  return (int64_t)grad_blocks(p) * std::min(p.req.n, p.req.count) * grad_groups(p);
+}
+template <int RK, int G>
 hipError_t grad_t(const GradParams& p, hipStream_t st) {
   const dim3 grid((unsigned)grad_blocks(p), (unsigned)(p.req.n * ((p.rp + 32 * RK - 1) / (32 * RK))), (unsigned)p.splits);
-  hipLaunchKernelGGL((grad_kernel<RK>), grid, dim3(kGradThreads), 0, st, p,
+  hipLaunchKernelGGL((grad_kernel<RK, G>), grid, dim3(kThreads * G), 0, st, p,
                      grad_values(p));
   return hipGetLastError();
 }
+// Four groups of waves where a block has a CU to itself, fewer where more blocks share it.  3840 columns of x and of
+// dy, four, two groups and one: 4 adapters of rank 64 over 8192 tokens (240 blocks) 39, 41 and 54 us; 8 of them (480
+// blocks) 44, 36 and 39; 16 over 2048 tokens (960) 33, 21 and 19; 32 of rank 16 over 4096 tokens (1920) 43, 24 and 20.
+template <int RK>
+hipError_t grad_g(const GradParams& p, hipStream_t st) {
+  const int64_t blocks = busy_blocks(p) * p.splits;
+  return blocks <= kCUs ? grad_t<RK, 4>(p, st) : blocks <= 2 * kCUs ? grad_t<RK, 2>(p, st) : grad_t<RK, 1>(p, st);
+}
 }  // namespace
 int grad_splits(const GradParams& p) {
-  const int64_t blocks = (int64_t)grad_blocks(p) * std::min(p.req.n, p.req.count) * grad_groups(p);
+  const int64_t blocks = busy_blocks(p);
   if (!blocks) return 1;
-  const int64_t want = (kCUs + blocks / 2) / blocks;  // a block to a CU, more or less
+  const int64_t want = kCUs / blocks;  // a CU to a block
   const int64_t most = p.req.tokens / p.req.count / (kGradStep * kGradGroups);  // a step for every group at least
   return (int)std::max<int64_t>(1, std::min(want, most));
 }
 hipError_t launch_adapter_grad(const GradParams& p, hipStream_t st) {
-  const hipError_t e = p.rp <= 32 ? grad_t<1>(p, st) : grad_t<2>(p, st);
+  const hipError_t e = p.rp <= 32 ? grad_g<1>(p, st) : grad_g<2>(p, st);
   if (e != hipSuccess || p.splits == 1) return e;
   const int64_t all = grad_values(p);
   const int64_t blocks = std::min<int64_t>((all + kThreads - 1) / kThreads, 4096);

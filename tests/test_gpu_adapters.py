@@ -133,6 +133,10 @@ CASES = [
     (61, 300, 64, 72, 16, 4, B16, True),     # segments found at once, and after one and two searches
     (62, 300, 64, 72, 16, 4, B16, True),
     (5000, 6001, 64, 72, 8, 7, B16, True),
+    (40, 3000, 520, 1100, 24, 20, B16, True),   # gradients' blocks that share a CU: two and more of them
+    (20, 2000, 520, 1100, 72, 20, B16, False),
+    (64, 4000, 520, 1100, 16, 64, B16, True),
+    (64, 3000, 260, 513, 64, 96, B16, True),
 ]
 
 
