@@ -578,8 +578,8 @@ hipError_t launch_tail(const ProjParams& p, const LowArg<LOW>& low, int r, hipSt
 
 // Which blocks.  Each kind is taken where one round of it covers the whole
 // grid, the smallest first: a round of the 128-token x 1-head blocks takes
-// 27-35 us at K = 3072 and 3840 (256 tokens), one of 128 x 2 heads 42-68 us
-// (300-768 tokens), one of 160 x 2 heads 79 (768 x 30 heads; 1120 x 24 of K = 2048
+// 27-35 us at K = 3072 and 3840 (256 tokens), one of 128 x 2 heads 42-59 us
+// (300-768 tokens; 640 x 30 heads 68), one of 160 x 2 heads 79 (768 x 30 heads; 1120 x 24 of K = 2048
 // 48, in the large blocks 54), one of 256 x 2 heads 70-102 us.  In two rounds the smaller
 // blocks lose: 900 tokens x 24 heads took 72 us in large blocks and 78-81 in
 // two rounds of the 128-token ones, 300 tokens x 30 heads 48 us in 128 x 2 and 61 in 128 x 1.
