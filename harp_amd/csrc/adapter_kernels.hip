@@ -260,8 +260,8 @@ __global__ __launch_bounds__(64 * WAVES) void shrink_lds_kernel(ShrinkParams p, 
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const bool in = 8 * (chunk ^ (4 * h)) < left;
-        harp_ra::lds_dma_b128(arr, base + s * kStage + 1024 * (2 * TB + 2 * j + h),
-                              in ? asrc[2 * j + h] + 128 * c : harp_ra::kOOB);
+        harp_ra::lds_dma_b128_fresh(arr, base + s * kStage + 1024 * (2 * TB + 2 * j + h),
+                                    in ? asrc[2 * j + h] + 128 * c : harp_ra::kOOB);
       }
     }
   };

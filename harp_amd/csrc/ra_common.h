@@ -161,6 +161,22 @@ __device__ __forceinline__ void lds_dma_b128(rsrc_t rs, uint32_t lds, uint32_t v
       : "memory", "m0");
 }
 
+// The same for a descriptor that may have been made just before: five wait states
+// lie between a vector instruction's write of an SGPR (make_rsrc's v_readfirstlane,
+// where the base address is in vector registers) and a vector-memory instruction's
+// read of it, and the compiler does not look into the statement, so they are waited
+// for here.  lds_dma_b128 leaves them out: its descriptors are made well ahead of
+// the copies (a test of the built code follows every path to every copy).
+__device__ __forceinline__ void lds_dma_b128_fresh(rsrc_t rs, uint32_t lds, uint32_t voff) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 3\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen lds"
+      :
+      : "s"(lds), "v"(voff), "s"(rs)
+      : "memory", "m0");
+}
+
 // The same with 4 bytes per lane: lane i's dword lands at lds + 4 * i.
 __device__ __forceinline__ void lds_dma_b32(rsrc_t rs, uint32_t lds, uint32_t voff) {
   asm volatile(
