@@ -103,7 +103,9 @@ bool readable(const at::Tensor& t) {
 }
 at::Tensor heads_of(const at::Tensor& t) {
   const at::Tensor r = plain(t);
-  return r.numel() == 0 || readable(r) ? r : r.contiguous();
+  if (r.numel() == 0 || readable(r)) return r;
+  const at::Tensor c = r.contiguous();
+  return readable(c) ? c : c.clone(at::MemoryFormat::Contiguous);  // (contiguous, from an odd address on)
 }
 at::Tensor like(const at::Tensor& x) {  // x's layout where it is one without holes
   return x.is_non_overlapping_and_dense() ? at::empty_strided(x.sizes(), x.strides(), x.options())

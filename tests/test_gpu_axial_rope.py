@@ -247,6 +247,35 @@ def test_layouts(kind):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("offset", [1, 2, 4])
+@pytest.mark.parametrize("dtype", [B16, F32])
+def test_contiguous_tensors_from_any_address_on(dtype, offset):
+    """q, k and their results' gradients as parts of a packed buffer: contiguous, but not 16-byte aligned."""
+    g = _gen(17 + offset)
+    rope = harp_amd.AxialRope((8, 4, 4), 256.0)
+    B, S, H, D = 2, 9, 3, 16
+    size = B * H * S * D
+
+    def packed(t):
+        store = torch.zeros(size + 8, dtype=dtype, device=DEV)
+        store[offset:offset + size] = t.flatten()
+        return store[offset:offset + size].view(B, H, S, D)
+
+    q, k, dq, dk = (_rand(g, B, H, S, D, dtype=dtype) for _ in range(4))
+    w = (1 + 0.1 * torch.randn(D, generator=g)).to(dtype).to(DEV)
+    pos = _grid(S, g).to(DEV)
+    results = []
+    for form in (lambda t: t.clone(), packed):
+        x = [form(t).requires_grad_() for t in (q, k)]
+        d = [form(t) for t in (dq, dk)]
+        assert all(t.is_contiguous() for t in (*x, *d))
+        for eps in (1e-5, None):
+            out = harp_amd.qk_norm_axial_rope(*x, pos, rope, *((w, w) if eps else ()), eps=eps)
+            results.append((*out, *torch.autograd.grad(out, x, d)))
+    for a, b in zip(results[0] + results[1], results[2] + results[3]):
+        assert torch.equal(a, b)
+
+
 def test_rows_that_are_empty_zero_or_not_finite():
     g = _gen(5)
     rope = harp_amd.AxialRope((32, 48, 48), 256.0)
