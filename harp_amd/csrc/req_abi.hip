@@ -62,9 +62,7 @@ int check_axes(const harp_req_axes_t* in, RopeAxes& ax, int& D) {
       return fail(HARP_REQ_EINVAL, "width[%d]=%d must be even, 2 to %d", a, w, kMaxRopeDim);
     if (!(in->theta[a] > 0.0) || !std::isfinite(in->theta[a]))
       return fail(HARP_REQ_EINVAL, "theta[%d] must be positive and finite", a);
-    // turns: theta^(-2 j / w) / (2 pi) = 2^(c0 + c1 p), j = p - pairs
-    ax.c1[a] = -2.0 / w * std::log2(in->theta[a]);
-    ax.c0[a] = -2.6514961294723187980 - ax.c1[a] * (double)pairs;  // log2(1 / (2 pi))
+    ax.c[a] = -2.0 / w * std::log2(in->theta[a]);  // theta^(-2 j / w) = 2^(c j)
     pairs += w / 2;
     ax.end[a] = (int)pairs;
   }

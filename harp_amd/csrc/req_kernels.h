@@ -17,12 +17,12 @@ constexpr int kF32 = 0, kBf16 = 1, kI32 = 2, kI64 = 3;  // element types
 constexpr int kMaxAxes = 4;
 constexpr int kMaxRopeDim = 256;
 
-// Pair p of a head (p < end[a], not before the axis) turns by
-// 2^(c0[a] + c1[a] * p) turns per unit of its position along axis a.
+// Pair p of a head (p < end[a], not before the axis), the axis' pair j, turns by
+// 2^(c[a] * j) / (2 pi) turns per unit of its position along axis a.
 struct RopeAxes {
   int n;
   int end[kMaxAxes];  // first pair behind the axis; the last one is D / 2
-  double c0[kMaxAxes], c1[kMaxAxes];
+  double c[kMaxAxes];
 };
 
 // positions [B, S, n axes] (element strides, any of them 0)

@@ -8,18 +8,23 @@
 
 namespace harp_req {
 
-// turns per unit of position of pair p, and its axis
+// turns per unit of position of pair p, and its axis.  (The exponent is formed from the pair's place
+// in its axis: from its place in the head, with the axes in front taken off again, it loses bits to
+// them, 2^-18 of a turn at positions of 2^31 where the axes in front are 60 pairs and theta is 1e6;
+// so formed the angle there is within 2^-22.9 of a turn: an ulp of exp2, the roundings of 1 / (2 pi),
+// of the two products and of the exponent, which is small where the rate is not.)
 __device__ __forceinline__ double rate_of(const RopeAxes& ax, int p, int& axis) {
-  double c0 = ax.c0[0], c1 = ax.c1[0];
+  double c = ax.c[0];
+  int first = 0;
   axis = 0;
 #pragma unroll
   for (int a = 1; a < kMaxAxes; ++a)
     if (a < ax.n && p >= ax.end[a - 1]) {
       axis = a;
-      c0 = ax.c0[a];
-      c1 = ax.c1[a];
+      first = ax.end[a - 1];
+      c = ax.c[a];
     }
-  return exp2(__builtin_fma(c1, (double)p, c0));
+  return exp2(c * (double)(p - first)) * 0.15915494309189535;
 }
 // the elements at base + off[k]
 template <int N>

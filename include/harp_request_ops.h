@@ -52,8 +52,9 @@ enum { HARP_REQ_MAX_AXES = 4, HARP_REQ_MAX_RANK = 128 };
  * The axes of a rotary embedding of heads of sum(width) features: axis a takes
  * the next width[a] / 2 pairs, and pair j of it turns by
  * position[a] * theta[a]^(-2 j / width[a]) radians.  Pairs are (2 p, 2 p + 1), or
- * (p, p + D / 2) with half.  Angles are exact to 2^-24 of a turn up to positions
- * of 2^31; a position that is not finite makes its pairs NaN.
+ * (p, p + D / 2) with half.  Angles are off by 2^-22 of a turn at most up
+ * to positions of 2^31, for theta of 1 and more; a position that is not finite makes its
+ * pairs NaN.
  */
 typedef struct {
   int n;                            /* 1 to HARP_REQ_MAX_AXES */

@@ -1,6 +1,7 @@
 """GPU tests of the QK RMSNorm with rotary positions of several axes, forward
 and backward, and of the rotary table, against the formulas in 64 bits."""
 
+import decimal
 import math
 
 import pytest
@@ -195,6 +196,30 @@ def test_far_positions_keep_their_precision():
                      for a in (0, 1)], -1)
     got = rope.table(fine).to(torch.complex128).cpu()
     assert float((got - torch.polar(torch.ones_like(ang), ang)).abs().max()) <= 2.0 ** -21
+
+
+@pytest.mark.parametrize("axes,theta", [((100, 20, 8), 1e6), ((32, 48, 48), 256.0), ((2, 2, 252), 1e6), ((16, 56, 56), 1e4),
+                                        ((128,), 1e4), ((64, 64), (1.0, 1e6))])
+def test_far_positions_along_the_axes_behind_others(axes, theta):
+    """Positions near 2^31 along every axis: the angle is off by 2^-22 of a turn at most, whatever axes are in
+    front.  The angles in whole numbers and 60 digits; 2^-21 is the 32-bit sine's and cosine's own."""
+    rope = harp_amd.AxialRope(axes, theta)
+    values = [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 12345, 2 ** 30 + 7, -1999999999]
+    p = torch.tensor(values)[:, None].expand(-1, len(axes)).to(torch.int32)
+    with decimal.localcontext() as c:
+        c.prec = 60
+        two_pi = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+        want = []
+        for v in values:
+            row = []
+            for d, th in zip(axes, rope.theta):
+                for j in range(d // 2):
+                    turns = v * (decimal.Decimal(th).ln() * (-2 * j) / d).exp() / two_pi
+                    row.append(float((turns - turns.to_integral_value()) * two_pi))
+            want.append(row)
+    ang = torch.tensor(want, dtype=torch.float64)
+    got = rope.table(p.to(DEV)).to(torch.complex128).cpu()
+    assert float((got - torch.polar(torch.ones_like(ang), ang)).abs().max()) <= 2 * math.pi * 2.0 ** -22 + 2.0 ** -21
 
 
 def test_quarter_turns_are_exact():
