@@ -68,7 +68,8 @@ class AdaptedLinear(nn.Module):
 
     ``base``: an ``nn.Linear`` (or a module with its ``weight`` and ``bias``) or an
     :class:`harp_amd.Int8Linear`, shared by all requests.  The adapters' a and b become
-    parameters over the same memory (kept as they are if they are parameters)."""
+    parameters over the same memory (kept as they are if they are parameters); the scales are
+    a buffer that stays float32 where the module is cast to another type."""
 
     def __init__(self, base, adapters: Adapters):
         super().__init__()
@@ -88,6 +89,14 @@ class AdaptedLinear(nn.Module):
 
         self.a, self.b = parameter(a), parameter(b)
         self.register_buffer("scales", scales)
+
+    def _apply(self, fn, *args, **kwargs):
+        scales = self.scales
+        super()._apply(fn, *args, **kwargs)
+        # the scales stay float32 where the module is cast (``module.to(torch.bfloat16)``)
+        if scales is not None and self.scales.dtype != torch.float32:
+            self.scales = scales.to(self.scales.device)
+        return self
 
     @property
     def adapters(self) -> Adapters:

@@ -372,3 +372,15 @@ def test_modules_refuse():
         harp_amd.adapt_attention(attn, to_out=low)
     with pytest.raises(ValueError, match="adapt_attention"):
         harp_amd.project_qkv(attn, x, None, requests=harp_amd.AdapterRequests(torch.zeros(3)))
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.to(torch.bfloat16), lambda m: m.bfloat16(), lambda m: m.half().bfloat16(),
+                                  lambda m: m.double().to("cpu", torch.bfloat16), lambda m: m.to("meta", torch.bfloat16)])
+def test_scales_stay_float32_in_a_cast_module(cast):
+    scales = torch.tensor([0.1, 1.7])  # (no bfloat16 values)
+    lin = harp_amd.AdaptedLinear(nn.Linear(8, 6), harp_amd.Adapters(torch.zeros(2, 4, 8), torch.zeros(2, 6, 4), scales))
+    m = cast(nn.Sequential(lin, harp_amd.AdaptedLinear(nn.Linear(6, 6), harp_amd.Adapters(torch.zeros(2, 4, 6), torch.zeros(2, 6, 4)))))
+    assert all(p.dtype == torch.bfloat16 for p in m.parameters())
+    assert m[0].scales.dtype == torch.float32 and m[0].scales.device == m[0].a.device and m[1].scales is None
+    assert m[0].scales.is_meta or torch.equal(m[0].scales, scales)
+    assert m[0]._buffers["scales"] is m[0].adapters.scales
