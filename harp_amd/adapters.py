@@ -146,8 +146,7 @@ def adapt_attention(attn, to_q: Optional[Adapters] = None, to_k: Optional[Adapte
 def fused_adapters_arguments(attn, hidden_states: torch.Tensor, freqs, requests: AdapterRequests) -> Optional[tuple]:
     """What :func:`project_qkv_adapters` takes for this module and input, or None where it does not: adapters of one
     number and one rank, a multiple of 8, beside bfloat16 projections without a bias, heads of 128 features, norms of
-    both q and k with a rotation, positions along interleaved axes where a gradient is recorded, and requests of 8
-    tokens or more on the average, or few of them."""
+    both q and k with a rotation, and positions along interleaved axes where a gradient is recorded."""
     lins = (attn.to_q, attn.to_k, attn.to_v)
     if not all(is_adapted(m) for m in lins) or not isinstance(hidden_states, torch.Tensor):
         return None
@@ -163,13 +162,6 @@ def fused_adapters_arguments(attn, hidden_states: torch.Tensor, freqs, requests:
     for t in (*a, *b):
         if not t.is_contiguous() or t.dtype != torch.bfloat16 or t.device != device or t.data_ptr() % 16:
             return None
-    tokens = hidden_states.numel() // max(hidden_states.size(-1), 1)
-    count = requests.index.numel()
-    # The contraction takes a tile more for each request among a block's tokens, 128 or 256 of them.  30 heads from
-    # 3840 features, rank 16, one launch and parts: 32 requests of 8 tokens 65 and 93 us, of one token 79 and 61;
-    # 16 of one token 60 and 53, 8 of one token 51 and 51.
-    if count > 8 and tokens < 8 * count:
-        return None
     norms = [getattr(attn, "norm_q", None), getattr(attn, "norm_k", None)]
     norm_weights = [getattr(n, "weight", None) for n in norms]
     axial = isinstance(freqs, AxialPositions)
@@ -198,6 +190,16 @@ def project_qkv_adapters(arguments: tuple):
     launch for x A^T, one for the products, the adapters, the QK RMSNorm and the rotation."""
     q, k, v = _ops().qkv_adapters(*arguments)
     return q, k, v
+
+
+def short_requests(hidden_states: torch.Tensor, requests: AdapterRequests) -> bool:
+    """Whether the parts of the one launch, in float32, serve these requests sooner: more than 8 of them, with fewer
+    than 8 tokens on the average.  The contraction takes a tile more for each request among a block's tokens, 128 or
+    256 of them.  30 heads from 3840 features, one launch and parts: rank 16, 9 requests of one token 64 and 63 us, 32
+    of one token 116 and 78, 64 of four 128 and 124; rank 128, 9 of one token 136 and 85, 64 of four 403 and 242."""
+    tokens = hidden_states.numel() // max(hidden_states.size(-1), 1)
+    count = requests.index.numel()
+    return count > 8 and tokens < 8 * count
 
 
 def is_adapted(module) -> bool:

@@ -39,12 +39,12 @@ import torch
 from torch import nn
 
 from .adapters import (AdapterRequests, add_adapters, fused_adapters_arguments, is_adapted,
-                       project_qkv_adapters)
+                       project_qkv_adapters, short_requests)
 from .int8 import Int8Linear, Int8Rows, fused_int8_supported, is_int8, project_qkv_int8, quantize_int8
 from .ops import RingAttention
 from .qk import ApplyRotaryComplexFn, QKNormRopeFn, RMSNormFn
 from .qkv import HEAD_DIM, ProjectQKVFn, fused_supported, qkv_project
-from .rope import AxialPositions, qk_norm_axial_rope
+from .rope import AxialPositions, AxialRope, qk_norm_axial_rope
 
 
 def _norm_rope(x: torch.Tensor, norm: Optional[nn.Module], freqs_cis: Optional[torch.Tensor]) -> torch.Tensor:
@@ -76,6 +76,43 @@ def _norm_axial_rope(attn, query: torch.Tensor, key: torch.Tensor, freqs: AxialP
                               tuple(None if n is None else float(n.eps) for n in (nq, nk)))
 
 
+def _records_gradient(*tensors: Optional[torch.Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _project_short(attn, x: torch.Tensor, freqs: Freqs, requests: AdapterRequests):
+    """What the one launch with adapters computes, for many short requests and without a gradient: its parts, in
+    float32 to the end and rounded once as there, so that a token's result does not depend on how many requests are
+    served with it."""
+    def project(module):
+        weight = module.base.weight
+        y = torch.mm(x.flatten(0, 1), weight.t(), out_dtype=torch.float32).view(*x.shape[:2], weight.size(0))
+        return add_adapters(y, x, module.adapters, requests).unflatten(-1, (attn.heads, -1)).transpose(1, 2)
+
+    query, key, value = project(attn.to_q), project(attn.to_k), project(attn.to_v)
+    if isinstance(freqs, AxialPositions):
+        query, key = _norm_axial_rope(attn, query, key, freqs)
+    else:  # the norms alone: no token is turned
+        still = torch.zeros((x.size(1), 1), device=x.device)
+
+        def normed(t, norm):
+            if norm is None:
+                return t
+            return qk_norm_axial_rope(t, None, still, AxialRope((HEAD_DIM,), 1.0), norm.weight, eps=float(norm.eps))[0]
+
+        query, key = (normed(t, n) for t, n in zip((query, key), _norms(attn)))
+    if isinstance(freqs, torch.Tensor):
+        turn = freqs.unsqueeze(-3)  # of all heads
+
+        def rotate(t):
+            return torch.view_as_real(torch.view_as_complex(t.unflatten(-1, (-1, 2))) * turn).flatten(-2)
+
+        query, key = rotate(query), rotate(key)
+    # (token-major, as the one launch gives them)
+    return tuple(t.transpose(1, 2).to(torch.bfloat16, memory_format=torch.contiguous_format).transpose(1, 2)
+                 for t in (query, key, value))
+
+
 def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: Freqs,
                      fused: bool, requests: Optional[AdapterRequests]
                      ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -83,6 +120,9 @@ def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: 
     if fused and requests is not None:
         arguments = fused_adapters_arguments(attn, hidden_states, freqs, requests)
         if arguments is not None:
+            x, weights, a, b, _, _, _, norm_weights = arguments[:8]
+            if short_requests(x, requests) and not _records_gradient(x, *weights, *a, *b, *norm_weights):
+                return _project_short(attn, x, freqs, requests)
             return project_qkv_adapters(arguments)
     x, heads, rows = hidden_states, attn.heads, None
     bases = [m.base if is_adapted(m) else m for m in (attn.to_q, attn.to_k, attn.to_v)]

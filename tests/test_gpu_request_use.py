@@ -495,3 +495,75 @@ def test_a_broken_adapter_stays_with_its_request():
                         assert not bool(torch.isfinite(a[i]).all())
                     else:
                         assert torch.equal(a[i], b[i])
+
+
+@pytest.mark.parametrize("r", [8, 16, 128])
+@pytest.mark.parametrize("form,norm", [("positions", True), ("table", True), ("table of each", True), ("none", True),
+                                       ("none", False)])
+def test_a_token_s_rounding_does_not_depend_on_the_batch(r, form, norm):
+    """The same tokens with the same adapter, as two requests (one launch) and as 32 short ones (parts): both are one
+    rounding of 32-bit sums, whose order differs by 2^-20 of a value and moves one of 2^9 results over a border
+    between bf16 values (2^-6 leaves room for small ones); three roundings move every second."""
+    g = _gen(r)
+    attn = harp_amd.adapt_attention(_attention(g, 256, 3), **{t: _low(g, 3, r, 256, 384) for t in ("to_q", "to_k", "to_v")})
+    if not norm:
+        attn.norm_q = attn.norm_k = None
+    B, S = 2, 48
+    x = _rand(g, B, S, 256)
+    pos = _positions(g, B, S, ROPE)
+    freqs = {"positions": pos, "table": ROPE.table(pos.positions[0]), "table of each": pos.table(), "none": None}[form]
+    cuts = torch.linspace(0, B * S, 33).round().to(torch.int32).to(DEV)
+    two = harp_amd.AdapterRequests(torch.tensor([2, 2], device=DEV))
+    many = harp_amd.AdapterRequests(torch.full((32,), 2, device=DEV), cuts)
+    with torch.no_grad():
+        want = harp_amd.project_qkv(attn, x, freqs, requests=two)
+        got = harp_amd.project_qkv(attn, x, freqs, requests=many)
+        each = harp_amd.project_qkv(attn, x, freqs, requests=harp_amd.AdapterRequests(torch.full((96,), 2, device=DEV)))
+    for a, b, c in zip(want, got, each):
+        assert a.stride() == b.stride() == (S * 384, 128, 384, 1) and b.dtype == B16
+        for d in (b, c):
+            assert float((a != d).float().mean()) <= 2.0 ** -6
+            assert float(((a.double() - d.double()).abs() / (a.double().abs() + a.double().abs().mean())).max()) <= 2.0 ** -7
+    if form == "positions":  # with a gradient: the one launch
+        xg = x.clone().requires_grad_()
+        for a, b in zip(want, harp_amd.project_qkv(attn, xg, freqs, requests=many)):
+            assert torch.equal(a, b.detach())
+
+
+def test_short_requests_in_a_captured_graph():
+    g = _gen(71)
+    attn = harp_amd.adapt_attention(_attention(g, 192, 2), **{t: _low(g, 5, 16, 192, 256) for t in ("to_q", "to_k", "to_v")})
+    x, pos = _rand(g, 24, 1, 192), _positions(g, 24, 1, ROPE)
+    index = torch.arange(24, device=DEV) % 6
+    requests = harp_amd.AdapterRequests(index)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad(), torch.cuda.stream(side):
+        for freqs in (pos, pos.table()):
+            harp_amd.project_qkv(attn, x, freqs, requests=requests)
+    torch.cuda.current_stream().wait_stream(side)
+    for freqs in (pos, pos.table()):
+        graph = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(graph):
+            out = harp_amd.project_qkv(attn, x, freqs, requests=requests)
+        for k in range(3):
+            x.copy_(_rand(g, 24, 1, 192))
+            index.copy_((torch.arange(24, device=DEV) * (k + 1)) % 6)
+            graph.replay()
+            with torch.no_grad():
+                want = harp_amd.project_qkv(attn, x, freqs, requests=requests)
+            torch.cuda.synchronize()
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+def test_short_requests_without_a_token():
+    g = _gen(73)
+    attn = harp_amd.adapt_attention(_attention(g, 192, 2), **{t: _low(g, 5, 16, 192, 256) for t in ("to_q", "to_k", "to_v")})
+    requests = harp_amd.AdapterRequests(torch.zeros(9, dtype=torch.int32, device=DEV))
+    for B, S in ((0, 4), (2, 0)):
+        x, pos = _rand(g, B, S, 192), _positions(g, B, S, ROPE)
+        with torch.no_grad():
+            for freqs in (pos, pos.table(), None):
+                for t in harp_amd.project_qkv(attn, x, freqs, requests=requests):
+                    assert t.shape == (B, 2, S, 128) and t.dtype == B16
