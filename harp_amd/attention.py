@@ -33,6 +33,7 @@ low-rank adapters beside its projections (:func:`harp_amd.adapt_attention`) take
 
 from __future__ import annotations
 
+from types import SimpleNamespace
 from typing import Optional, Tuple, Union
 
 import torch
@@ -113,10 +114,37 @@ def _project_short(attn, x: torch.Tensor, freqs: Freqs, requests: AdapterRequest
                  for t in (query, key, value))
 
 
+def _project_bare(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: Freqs):
+    """The one launch for a module with adapters that no request takes (no ``requests``), or None where there is none.
+    With a table, or no rotation, the call of the module without adapters; with positions the call of requests without
+    an adapter, whose results those are (rounded, where the plain producer truncates behind norm and rotation)."""
+    if isinstance(freqs, AxialPositions):
+        if not isinstance(hidden_states, torch.Tensor):
+            return None
+        nobody = AdapterRequests(torch.full((1,), -1, dtype=torch.int32, device=hidden_states.device))
+        arguments = fused_adapters_arguments(attn, hidden_states, freqs, nobody)
+        if arguments is None:
+            return None
+        x, weights, a, b, *more = arguments  # (the adapters take no part, in a gradient either)
+        return project_qkv_adapters((x, weights, [t.detach() for t in a], [t.detach() for t in b], *more))
+    to = [m.base if is_adapted(m) else m for m in (attn.to_q, attn.to_k, attn.to_v)]
+    nq, nk = _norms(attn)
+    bare = SimpleNamespace(heads=attn.heads, norm_q=nq, norm_k=nk, to_q=to[0], to_k=to[1], to_v=to[2])
+    if is_int8(bare):
+        return project_qkv(bare, hidden_states, freqs) if fused_int8_supported(bare, freqs) else None
+    if isinstance(hidden_states, torch.Tensor) and fused_supported(bare, hidden_states, freqs):
+        return project_qkv(bare, hidden_states, freqs)
+    return None
+
+
 def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: Freqs,
                      fused: bool, requests: Optional[AdapterRequests]
                      ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """project_qkv of a module with adapters."""
+    if fused and requests is None:
+        bare = _project_bare(attn, hidden_states, freqs)
+        if bare is not None:
+            return bare
     if fused and requests is not None:
         arguments = fused_adapters_arguments(attn, hidden_states, freqs, requests)
         if arguments is not None:
@@ -163,7 +191,10 @@ def project_qkv(attn: nn.Module, hidden_states: Union[torch.Tensor, Int8Rows], f
     (:class:`harp_amd.AxialPositions`): the one-launch forms read their table,
     otherwise :func:`harp_amd.qk_norm_axial_rope` norms and rotates q and k.
     ``requests``: which tokens take which of the module's adapters
-    (:func:`harp_amd.adapt_attention`); without it none is added."""
+    (:func:`harp_amd.adapt_attention`); without it none is added.  q and k of an
+    adapted module are rounded to nearest where ``requests`` or positions are
+    given; with a table and no requests they are the plain module's, which follow the
+    reference and truncate."""
     adapted = any(is_adapted(getattr(attn, n, None)) for n in ("to_q", "to_k", "to_v"))
     if requests is not None and not adapted and not _adapted_out(attn):
         raise ValueError("requests need an attention module with adapters (harp_amd.adapt_attention)")

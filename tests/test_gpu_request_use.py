@@ -567,3 +567,47 @@ def test_short_requests_without_a_token():
             for freqs in (pos, pos.table(), None):
                 for t in harp_amd.project_qkv(attn, x, freqs, requests=requests):
                     assert t.shape == (B, 2, S, 128) and t.dtype == B16
+
+
+def test_an_adapted_module_without_requests_keeps_the_one_launch(monkeypatch):
+    """No requests: with a table or no rotation the call of the module without adapters, bit for bit, with gradients
+    too; with positions the call of requests that take none.  No separate projection runs."""
+    g = _gen(79)
+    base = _attention(g, 192, 2)
+    names = ("to_q", "to_k", "to_v")
+    x, pos = _rand(g, 2, 70, 192), _positions(g, 2, 70, ROPE)
+    attn = harp_amd.adapt_attention(base, **{t: _low(g, 2, 16, 192, 256) for t in names})
+    some = harp_amd.adapt_attention(base, to_q=_low(g, 2, 8, 192, 256), to_v=_low(g, 2, 16, 192, 256))
+
+    def no_parts(*_):
+        raise AssertionError("a projection of its own")
+
+    for m in (base.to_q, base.to_k, base.to_v):
+        monkeypatch.setattr(m, "forward", no_parts)
+    with torch.no_grad():
+        for freqs in (pos.table(), ROPE.table(pos.positions[0]), None):
+            for module in (attn, some):
+                for a, b in zip(harp_amd.project_qkv(module, x, freqs), harp_amd.project_qkv(base, x, freqs)):
+                    assert torch.equal(a, b) and a.stride() == b.stride()
+        nobody = harp_amd.AdapterRequests(torch.tensor([-1, 7], device=DEV))
+        for a, b in zip(harp_amd.project_qkv(attn, x, pos), harp_amd.project_qkv(attn, x, pos, requests=nobody)):
+            assert torch.equal(a, b)
+    leaves = (x.requires_grad_(), base.norm_q.weight, base.norm_k.weight)
+    d = [_rand(g, 2, 70, 2, 128).transpose(1, 2) for _ in range(3)]
+    for freqs in (pos.table(), pos):
+        out = harp_amd.project_qkv(attn, x, freqs)
+        grads = torch.autograd.grad(out, leaves + (attn.to_q.a, attn.to_v.b), d, allow_unused=True)
+        assert grads[3] is None and grads[4] is None  # the adapters take no part
+        if freqs is pos:
+            same = harp_amd.project_qkv(attn, x, pos, requests=nobody)
+        else:
+            same = harp_amd.project_qkv(base, x, freqs)
+        for a, b in zip((*out, *grads[:3]), (*same, *torch.autograd.grad(same, leaves, d))):
+            assert torch.equal(a, b)
+    rows = harp_amd.quantize_attention(_attention(g, 192, 2))
+    low8 = harp_amd.adapt_attention(rows, **{t: _low(g, 2, 16, 192, 256) for t in names})
+    with torch.no_grad():
+        for freqs in (pos.table(), None):
+            for h in (x.detach(), harp_amd.quantize_int8(x.detach())):
+                for a, b in zip(harp_amd.project_qkv(low8, h, freqs), harp_amd.project_qkv(rows, h, freqs)):
+                    assert torch.equal(a, b)
