@@ -46,9 +46,6 @@ REQUEST_OPS_LIB = OUT / "libharp_request_ops.so"
 HIP_SOURCES = ["ra_kernels.hip", "fwd_asm.hip", "dq_asm.hip", "dkdv_asm.hip", "ra_abi.hip", "qk_kernels.hip", "qk_abi.hip", "proj_kernels.hip",
                "norm_kernels.hip", "prod8_kernels.hip", "blk_abi.hip", "rope_kernels.hip", "adapter_kernels.hip",
                "req_abi.hip"]
-HIP_HEADERS = ["ra_common.h", "ra_kernels.h", "qk_kernels.h", "proj_kernels.h", "blk_kernels.h", "req_kernels.h", "fwd_asm.inc", "fwd_asm_gen.py",
-               "dq_asm.inc", "dq_asm_gen.py", "dkdv_asm.inc",
-               "dkdv_asm_gen.py", "asm_sched.py", "torch_autograd_util.h"]
 OPS_SOURCE = "torch_ring_attention_ops.cpp"
 ASYNC_OPS_SOURCE = "torch_async_op.cpp"
 BLOCK_OPS_SOURCE = "torch_block_ops.cpp"
@@ -185,9 +182,8 @@ def sources_newer_than_libs() -> bool:
     if not all(p.exists() for p in libs):
         return True
     newest_lib = min(p.stat().st_mtime for p in libs)
-    srcs = [CSRC / s for s in HIP_SOURCES + HIP_HEADERS
-            + [OPS_SOURCE, ASYNC_OPS_SOURCE, BLOCK_OPS_SOURCE, REQUEST_OPS_SOURCE]]
-    srcs += [INCLUDE / h for h in ("harp_ring_attn.h", "harp_qk_norm_rope.h", "harp_block_ops.h", "harp_request_ops.h")]
+    # (sources, headers and generators: whatever lies there)
+    srcs = [p for d in (CSRC, INCLUDE) for p in d.iterdir() if p.is_file()]
     return any(s.stat().st_mtime > newest_lib for s in srcs)
 
 
