@@ -107,9 +107,10 @@ at::Tensor heads_of(const at::Tensor& t) {
   const at::Tensor c = r.contiguous();
   return readable(c) ? c : c.clone(at::MemoryFormat::Contiguous);  // (contiguous, from an odd address on)
 }
-at::Tensor like(const at::Tensor& x) {  // x's layout where it is one without holes
-  return x.is_non_overlapping_and_dense() ? at::empty_strided(x.sizes(), x.strides(), x.options())
-                                          : at::empty(x.sizes(), x.options());
+// x's layout, without the holes it may have; another where the kernels cannot write that
+at::Tensor like(const at::Tensor& x) {
+  const at::Tensor r = at::empty_like(x);
+  return r.numel() == 0 || readable(r) ? r : at::empty(x.sizes(), x.options());
 }
 void strides_of(const at::Tensor& t, int64_t (&st)[3]) {
   const int order[3] = {0, 1, 2};
@@ -178,7 +179,7 @@ std::tuple<at::Tensor, at::Tensor> rope_forward(const at::Tensor& q, const OptTe
   for (int i = 0; i < 2; ++i) {
     if (i && !given(k)) break;
     x[i] = heads_of(i ? *k : q);
-    y[i] = like(x[i]);
+    y[i] = like(i ? *k : q);
     w[i] = weight_of(i ? kw : qw, q, i ? "k_weight" : "q_weight");
     harp_req_heads_t& h = heads[i];
     h.x = x[i].const_data_ptr();

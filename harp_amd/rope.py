@@ -100,7 +100,8 @@ def qk_norm_axial_rope(q: torch.Tensor, k: Optional[torch.Tensor], positions: to
     strides; k may be None.  ``positions``: [S, axes] for all of the batch, or [B, S, axes].
     ``eps``: of the RMSNorms in front of the rotation, one number or one for q and one for k; None
     leaves the norm out.  The weights are bfloat16 or float32 [D] vectors, or None for a norm without one.
-    The results have q's and k's layouts.  Gradients of q, k and the weights, once and in reverse mode."""
+    The results have q's and k's layouts, without the holes these may have (features are neighbours
+    always).  Gradients of q, k and the weights, once and in reverse mode."""
     pair = tuple(eps) if isinstance(eps, (tuple, list)) else (eps, eps)
     if len(pair) != 2 or any(e is not None and not e >= 0 for e in pair):
         raise ValueError(f"eps must be None, a non-negative number, or two of these, got {eps}")

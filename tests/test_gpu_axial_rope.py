@@ -301,6 +301,35 @@ def test_contiguous_tensors_from_any_address_on(dtype, offset):
         assert torch.equal(a, b)
 
 
+def test_results_have_the_layout_of_q_and_k():
+    """Token-major, head-major, parts of one packed projection, rows that are no multiple of 16 bytes apart: the
+    order of q's and k's dimensions, without holes."""
+    g = _gen(23)
+    B, S, H, D = 2, 6, 3, 16
+    rope = harp_amd.AxialRope((4, 4, 8), 256.0)
+    pos = _grid(S, g).to(DEV)
+    token, head = (S * H * D, D, H * D, 1), (H * S * D, S * D, D, 1)
+    packed = _rand(g, B, S, 3, H, D).requires_grad_()
+    odd = _rand(g, B, S, H, D + 3)[..., 1:1 + D].transpose(1, 2)
+    forms = [(_heads(g, B, S, H, D, B16), token), (_rand(g, B, H, S, D), head), (odd, token),
+             *((packed[:, :, i].transpose(1, 2), token) for i in range(3)),
+             (_rand(g, B, S, 1, D).expand(-1, -1, H, -1).transpose(1, 2), None),
+             (_rand(g, B, H, D, S).transpose(2, 3), head)]
+    for x, strides in forms:
+        y, yk = harp_amd.qk_norm_axial_rope(x, x, pos, rope, eps=1e-5)
+        want, _ = harp_amd.qk_norm_axial_rope(x.detach().clone(memory_format=torch.contiguous_format), None, pos, rope, eps=1e-5)
+        assert torch.equal(y, want) and torch.equal(yk, want) and y.stride(3) == 1
+        assert strides is None or (y.stride() == strides and yk.stride() == strides)
+    q, k = (packed[:, :, i].transpose(1, 2) for i in (0, 1))
+    out = harp_amd.qk_norm_axial_rope(q, k, pos, rope, eps=1e-5)
+    (grad,) = torch.autograd.grad(out, packed, [torch.ones_like(t) for t in out])
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k)]
+    same = harp_amd.qk_norm_axial_rope(*leaves, pos, rope, eps=1e-5)
+    for i, d in enumerate(torch.autograd.grad(same, leaves, [torch.ones_like(t) for t in same])):
+        assert torch.equal(grad[:, :, i].transpose(1, 2), d)
+    assert not bool(grad[:, :, 2].any())
+
+
 def test_rows_that_are_empty_zero_or_not_finite():
     g = _gen(5)
     rope = harp_amd.AxialRope((32, 48, 48), 256.0)
