@@ -56,9 +56,10 @@
 // parts (zeros for the other requests' tokens) meets the same columns of B twice.
 // That is one tile per request up to rank 32 against K / 64 of the projection, and
 // no other pass over q, k and v; each result is then rounded once, to nearest,
-// behind the norm and the rotation, in fp32 until there.  768 tokens x 30 heads of
-// 3840 columns, rank 16, three requests: 90 us, as without an adapter; 32 requests of 8
-// tokens 65, one after the other in parts 93.
+// behind the norm and the rotation, in fp32 until there.  30 heads of 3840 columns,
+// rank 16, with adapters and without (calls of both in turn, with pauses): 768 tokens
+// of three requests 80 and 74 us, 8192 of two 630 and 612, 256 of 32 requests, whose
+// parts follow one another, 74 and 38.
 // Pipeline: one barrier per tile, in its last k-step, after which nobody
 // reads tile t's stage any more (its last fragments are in registers) and
 // tile t + 1 is complete; the copies of tile t + stages then go into tile t's
