@@ -39,7 +39,9 @@ def _freqs_table(freqs_cis: torch.Tensor, B: int, S: int) -> Tuple[torch.Tensor,
     """complex [S, 64] or [B or 1, S, 64] -> fp32 (cos, sin) pairs [.., S, 128]
     and its batch / row strides in floats (batch stride 0 when shared), as
     the async_op operators read it."""
-    r = torch.view_as_real(freqs_cis).flatten(-2) if freqs_cis.is_complex() else freqs_cis
+    # (a lazily conjugated or negated table as what it stands for: its memory is read)
+    r = freqs_cis.resolve_conj().resolve_neg()
+    r = torch.view_as_real(r).flatten(-2) if r.is_complex() else r
     if r.dtype != torch.float32:
         raise ValueError("freqs_cis must be complex64 [.., S, 64], or float32 (cos, sin) rows [.., S, 128]")
     r = r.contiguous()

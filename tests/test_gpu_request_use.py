@@ -611,3 +611,30 @@ def test_an_adapted_module_without_requests_keeps_the_one_launch(monkeypatch):
             for h in (x.detach(), harp_amd.quantize_int8(x.detach())):
                 for a, b in zip(harp_amd.project_qkv(low8, h, freqs), harp_amd.project_qkv(rows, h, freqs)):
                     assert torch.equal(a, b)
+
+
+def test_conjugated_and_negated_tables():
+    """A table that is a lazy conjugate (the rotation back) or a negated view, in the one launch and in parts."""
+    g = _gen(83)
+    base = _attention(g, 192, 2)
+    attn = harp_amd.adapt_attention(base, **{t: _low(g, 2, 16, 192, 256) for t in ("to_q", "to_k", "to_v")})
+    rows = harp_amd.quantize_attention(base)
+    x, pos = _rand(g, 2, 40, 192), _positions(g, 2, 40, ROPE)
+    requests = [harp_amd.AdapterRequests(torch.tensor([1, 0], device=DEV)),
+                harp_amd.AdapterRequests(torch.arange(16, device=DEV) % 2)]
+    table = pos.table()
+    for lazy in (table.conj(), torch._neg_view(table), torch._neg_view(table).conj()):
+        plain = lazy.clone().resolve_conj().resolve_neg().contiguous()
+        assert (lazy.is_conj() or lazy.is_neg()) and not (plain.is_conj() or plain.is_neg())
+        calls = [lambda f: harp_amd.project_qkv(base, x, f), lambda f: harp_amd.project_qkv(rows, x, f),
+                 lambda f: harp_amd.project_qkv(base, x, f, fused=False),
+                 *(lambda f, r=r: harp_amd.project_qkv(attn, x, f, requests=r) for r in (None, *requests))]
+        with torch.no_grad():
+            for call in calls:
+                for a, b in zip(call(lazy), call(plain)):
+                    assert torch.equal(a, b)
+        xg, grads = x.clone().requires_grad_(), []
+        for f in (lazy, plain):
+            out = harp_amd.project_qkv(base, xg, f)
+            grads.append(torch.autograd.grad(out, xg, [torch.ones_like(t) for t in out])[0])
+        assert torch.equal(*grads)
