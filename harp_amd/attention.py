@@ -149,7 +149,8 @@ def _project_adapted(attn, hidden_states: Union[torch.Tensor, Int8Rows], freqs: 
         arguments = fused_adapters_arguments(attn, hidden_states, freqs, requests)
         if arguments is not None:
             x, weights, a, b, _, _, _, norm_weights = arguments[:8]
-            if short_requests(x, requests) and not _records_gradient(x, *weights, *a, *b, *norm_weights):
+            table = freqs if isinstance(freqs, torch.Tensor) else None
+            if short_requests(x, requests) and not _records_gradient(x, *weights, *a, *b, *norm_weights, table):
                 return _project_short(attn, x, freqs, requests)
             return project_qkv_adapters(arguments)
     x, heads, rows = hidden_states, attn.heads, None

@@ -638,3 +638,15 @@ def test_conjugated_and_negated_tables():
             out = harp_amd.project_qkv(base, xg, f)
             grads.append(torch.autograd.grad(out, xg, [torch.ones_like(t) for t in out])[0])
         assert torch.equal(*grads)
+
+
+def test_a_table_with_a_gradient_is_refused_for_short_requests_too():
+    g = _gen(89)
+    base = _attention(g, 192, 2).requires_grad_(False)
+    low = [harp_amd.Adapters(_rand(g, 2, 16, 192), _rand(g, 2, 256, 16)) for _ in range(3)]
+    attn = harp_amd.adapt_attention(base, **dict(zip(("to_q", "to_k", "to_v"), low)))
+    x, table = _rand(g, 1, 16, 192), _positions(g, 1, 16, ROPE).table().requires_grad_()
+    for count in (1, 16):
+        requests = harp_amd.AdapterRequests(torch.zeros(count, dtype=torch.int32, device=DEV))
+        with pytest.raises(RuntimeError, match="rotation has no gradient"):
+            harp_amd.project_qkv(attn, x, table, requests=requests)
