@@ -50,7 +50,9 @@ from .rope import AxialPositions, AxialRope, qk_norm_axial_rope
 
 def _norm_rope(x: torch.Tensor, norm: Optional[nn.Module], freqs_cis: Optional[torch.Tensor]) -> torch.Tensor:
     """RMSNorm (when ``norm`` is set) then RoPE (when ``freqs_cis`` is set) of a
-    [B, H, S, D] view, on the async_op kernels."""
+    [B, H, S, D] view, on the async_op kernels (which take a token at least)."""
+    if x.numel() == 0:
+        return x
     if norm is not None:
         weight = getattr(norm, "weight", None)
         eps = float(norm.eps)

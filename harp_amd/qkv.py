@@ -107,7 +107,7 @@ def fused_supported(attn, hidden_states: torch.Tensor, freqs_cis: Optional[torch
             return False
         if not _aligned16(table):
             return False
-    return x.size(0) * x.size(1) < (1 << 31)
+    return 0 < x.size(0) * x.size(1) < (1 << 31)
 
 
 def qkv_project(hidden_states: torch.Tensor, weights: Sequence[torch.Tensor],

@@ -557,16 +557,29 @@ def test_short_requests_in_a_captured_graph():
                 assert torch.equal(a, b)
 
 
-def test_short_requests_without_a_token():
+def test_projections_without_a_token():
+    """No sample, or samples without a token: empty q, k and v from every form of the projections, and gradients."""
     g = _gen(73)
-    attn = harp_amd.adapt_attention(_attention(g, 192, 2), **{t: _low(g, 5, 16, 192, 256) for t in ("to_q", "to_k", "to_v")})
+    base = _attention(g, 192, 2)
+    rows = harp_amd.quantize_attention(base)
+    attn = harp_amd.adapt_attention(base, **{t: _low(g, 5, 16, 192, 256) for t in ("to_q", "to_k", "to_v")})
+    low8 = harp_amd.adapt_attention(rows, to_q=_low(g, 5, 16, 192, 256))
     requests = harp_amd.AdapterRequests(torch.zeros(9, dtype=torch.int32, device=DEV))
     for B, S in ((0, 4), (2, 0)):
         x, pos = _rand(g, B, S, 192), _positions(g, B, S, ROPE)
-        with torch.no_grad():
-            for freqs in (pos, pos.table(), None):
-                for t in harp_amd.project_qkv(attn, x, freqs, requests=requests):
-                    assert t.shape == (B, 2, S, 128) and t.dtype == B16
+        for freqs in (pos, pos.table(), None):
+            calls = [(m, fused, None) for m in (base, rows, attn, low8) for fused in (True, False)]
+            calls += [(m, fused, r) for m in (attn, low8) for fused in (True, False)
+                      for r in (requests, harp_amd.AdapterRequests(requests.index[:1]))]
+            for module, fused, r in calls:
+                with torch.no_grad():
+                    for t in harp_amd.project_qkv(module, x, freqs, fused=fused, requests=r):
+                        assert t.shape == (B, 2, S, 128) and t.dtype == B16
+                if module is base or module is attn:
+                    leaves = [x.clone().requires_grad_(), base.norm_q.weight] + ([attn.to_q.a, attn.to_v.b] if r else [])
+                    out = harp_amd.project_qkv(module, leaves[0], freqs, fused=fused, requests=r)
+                    for a, t in zip(torch.autograd.grad(out, leaves, out, allow_unused=True), leaves):
+                        assert a is None or (a.shape == t.shape and not bool(a.any()))
 
 
 def test_an_adapted_module_without_requests_keeps_the_one_launch(monkeypatch):
