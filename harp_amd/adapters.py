@@ -33,6 +33,9 @@ from .qkv import HEAD_DIM, fused_supported
 from .rope import AxialPositions, _ops
 
 
+MAX_TOKENS = 1 << 25  # of one call of the adapters' kernels
+
+
 class Adapters(NamedTuple):
     """n adapters of one rank (1 to 128) beside one projection: ``a`` bfloat16 [n, rank, in],
     ``b`` bfloat16 [n, out, rank], ``scales`` float32 [n] or None for ones.  Adapters of
@@ -143,15 +146,20 @@ def adapt_attention(attn, to_q: Optional[Adapters] = None, to_k: Optional[Adapte
     return AdaptedAttention(attn, to_q=to_q, to_k=to_k, to_v=to_v, to_out=to_out)
 
 
+def _tokens(hidden_states: torch.Tensor) -> int:
+    return hidden_states.numel() // max(hidden_states.size(-1), 1)
+
+
 def fused_adapters_arguments(attn, hidden_states: torch.Tensor, freqs, requests: AdapterRequests) -> Optional[tuple]:
     """What :func:`project_qkv_adapters` takes for this module and input, or None where it does not: adapters of one
     number and one rank, a multiple of 8, beside bfloat16 projections without a bias, heads of 128 features, norms of
-    both q and k with a rotation, and positions along interleaved axes where a gradient is recorded."""
+    both q and k with a rotation, positions along interleaved axes where a gradient is recorded, and 2^25 tokens at
+    most."""
     lins = (attn.to_q, attn.to_k, attn.to_v)
     if not all(is_adapted(m) for m in lins) or not isinstance(hidden_states, torch.Tensor):
         return None
     bases = [m.base for m in lins]
-    if any(isinstance(m, Int8Linear) for m in bases):
+    if any(isinstance(m, Int8Linear) for m in bases) or _tokens(hidden_states) > MAX_TOKENS:
         return None
     a, b = [m.a for m in lins], [m.b for m in lins]
     if a[1].shape != a[0].shape or a[2].shape != a[0].shape or a[0].size(1) % 8:
@@ -197,9 +205,8 @@ def short_requests(hidden_states: torch.Tensor, requests: AdapterRequests) -> bo
     than 8 tokens on the average.  The contraction takes a tile more for each request among a block's tokens, 128 or
     256 of them.  30 heads from 3840 features, one launch and parts: rank 16, 9 requests of one token 64 and 63 us, 32
     of one token 116 and 78, 64 of four 128 and 124; rank 128, 9 of one token 136 and 85, 64 of four 403 and 242."""
-    tokens = hidden_states.numel() // max(hidden_states.size(-1), 1)
     count = requests.index.numel()
-    return count > 8 and tokens < 8 * count
+    return count > 8 and _tokens(hidden_states) < 8 * count
 
 
 def is_adapted(module) -> bool:

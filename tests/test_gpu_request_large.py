@@ -3,6 +3,7 @@
 bytes, against 64 bits, and row strides beyond the 32-bit offsets of a tile."""
 
 import math
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -185,3 +186,28 @@ def test_rotation_of_many_rows(dtype, half, H, D):
     kd = k[0][:, rows].double()
     close(yk[0][:, rows], turn(kd, c, s), 2 * kd.abs().amax(-1, keepdim=True))
     assert math.isfinite(float(dx.float().abs().max() if dtype == F32 else dx.abs().max()))
+
+
+def test_projections_of_more_tokens_than_adapters_take():
+    """2^25 tokens and more: without requests the parts run; with them the adapters' limit is named."""
+    g = _gen(5)
+    S, dim = 2 ** 25 + 128, 64
+    attn = SimpleNamespace(heads=1)
+    for name in ("to_q", "to_k", "to_v"):
+        setattr(attn, name, torch.nn.Linear(dim, 128, bias=False, dtype=B16, device=DEV).requires_grad_(False))
+    attn.norm_q = attn.norm_k = SimpleNamespace(weight=torch.ones(128, dtype=B16, device=DEV), eps=1e-5)
+    low = {name: harp_amd.Adapters(_normal(g, 2, 8, dim), _normal(g, 2, 128, 8)) for name in ("to_q", "to_k", "to_v")}
+    attn = harp_amd.adapt_attention(attn, **low)
+    x = _normal(g, 1, S, dim)
+    rope = harp_amd.AxialRope((32, 48, 48), 256.0)
+    pos = torch.randint(0, 4000, (S, 3), device=DEV, generator=g, dtype=torch.int32)
+    with torch.no_grad():
+        q, _, v = harp_amd.project_qkv(attn, x, harp_amd.AxialPositions(pos, rope))
+        for at in (slice(0, 300), slice(S - 300, S)):
+            few = harp_amd.project_qkv(attn, x[:, at].contiguous(), harp_amd.AxialPositions(pos[at].contiguous(), rope))
+            # (parts round three times, the one launch once: 0.5 * 2^-8 of the norm each at most)
+            for a, b in ((q, few[0]), (v, few[2])):
+                assert float((a[:, :, at].double() - b.double()).norm() / b.double().norm()) <= 6e-3
+        with pytest.raises(RuntimeError, match="2\\^25"):
+            harp_amd.project_qkv(attn, x, harp_amd.AxialPositions(pos, rope),
+                                 requests=harp_amd.AdapterRequests(torch.zeros(1, dtype=torch.int32, device=DEV)))
